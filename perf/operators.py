@@ -137,11 +137,11 @@ class _Operands(object):
         return t
 
     def room(self, name, kind, *shape):
-        """Room for the output `name`. The plain forms make theirs themselves."""
+        """Room for the output `name`, zeros at first: what lies between the tensors stays so. The plain forms make theirs themselves."""
         if own:
             import cutorch_amd as thc
             self.handle[name] = thc.Tensor(kind).resize(shape)
-            self.tensor[name] = torch.as_tensor(_Alias(self.handle[name]), device="cuda")
+            self.tensor[name] = torch.as_tensor(_Alias(self.handle[name]), device="cuda").zero_()
 
     def normal(self, *shape, dtype=torch.float32):
         return torch.randn(shape, generator=self.g, device="cuda", dtype=dtype)
