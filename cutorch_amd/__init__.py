@@ -109,7 +109,7 @@ _COPY_SUFFIX = {"byte": "Byte", "char": "Char", "short": "Short", "int": "Int", 
 _FLOAT_KINDS = ("float", "half")
 _FUNCTIONS = {kind: {} for kind in _TYPES}      # method name -> foreign function, filled as they are used
 _CODES = {C.c_float: "f", C.c_double: "d", C.c_long: "l", C.c_int: "i", C.c_short: "h", C.c_byte: "b", C.c_ubyte: "B",
-          C.c_uint16: "e", C.POINTER(_Tensor): "t", None: "v"}
+          C.c_uint16: "e", C.POINTER(_Tensor): "t", C.c_void_p: "t", None: "v"}
 
 
 class _Calls(dict):
@@ -256,6 +256,16 @@ def _declare(l):
         for name in ("minall", "maxall"):
             opt(T + "_" + name, creal, P, TP)
         opt(T + "_renorm", None, P, TP, TP, creal, C.c_long, creal)
+        opt(T + "_embedding", None, P, TP, TP, TP, C.c_float)
+        opt(T + "_embeddingGrad", None, P, TP, TP, TP, C.c_float, C.c_long, C.c_int)
+        opt(T + "_tokenLogProb", None, P, TP, TP, TP)
+        opt(T + "_policyLoss", None, P, *([TP] * 9 + [C.c_double] * 4))
+        # lists of tensors (arrays of their addresses) and the step's numbers
+        masters = 1 if kind == "half" else 0
+        step = [C.c_double] * 5 + [C.c_long, C.c_double]
+        opt(T + "_adamW", None, P, C.c_int, *([P] * (4 + masters) + step))
+        opt(T + "_adamW8", None, P, C.c_int, *([P] * (6 + masters) + step))
+        opt(T + "_adamW8Moments", None, P, C.c_int, *([P] * 6))
     l.THCudaByteTensor_logicalall.argtypes = [P, TP]
     l.THCudaByteTensor_logicalany.argtypes = [P, TP]
     l.THCudaHalfTensor_copyCuda.argtypes = [P, TP, TP]
@@ -582,6 +592,32 @@ class Tensor(object):
         self._calls["min"](self.a, indices.a, src.a, dim, keepdim)
         return self
 
+    # ---------------------------------------- a language model's training step --
+    def embedding(self, weight, tokens, scale=1.0):
+        """self = scale * the rows of `weight` that the (1-based) tokens name."""
+        self._calls["embedding"](self.a, weight.a, tokens.a, scale)
+        return self
+
+    def embedding_grad(self, tokens, grad_output, scale=1.0, padding=0, accumulate=False):
+        """self, sized as the table, = scale * the rows of grad_output summed by token; added to with `accumulate`.
+        Positions of the token `padding` are left out."""
+        self._calls["embeddingGrad"](self.a, tokens.a, grad_output.a, scale, padding, accumulate)
+        return self
+
+    def token_log_prob(self, logits, tokens):
+        """self (float) = the log-probability of each row's token."""
+        logits._calls["tokenLogProb"](self.a, logits.a, tokens.a)
+        return self
+
+    def policy_loss(self, log_prob, grad_logits, logits, tokens, old, advantage, reference=None, weight=None, clip_low=0.2,
+                    clip_high=0.2, kl=0.0, grad_scale=1.0):
+        """self = each position's weighted clipped policy loss with its KL term, log_prob the tokens' log-probabilities,
+        grad_logits (None: not wanted; may be the logits) grad_scale times the gradient of the losses' sum."""
+        logits._calls["policyLoss"](self.a, log_prob.a, grad_logits.a if grad_logits is not None else 0, logits.a, tokens.a, old.a,
+                                    advantage.a, reference.a if reference is not None else 0, weight.a if weight is not None else 0,
+                                    clip_low, clip_high, kl, grad_scale)
+        return self
+
     def sumall(self):
         return self._calls["sumall"](self.a)
 
@@ -621,6 +657,73 @@ class Tensor(object):
 
     def maxall(self):
         return self._real_out(self._calls["maxall"](self.a))
+
+
+class AdamW(object):
+    """AdamW on a list of parameters, one call a step for all of them. `grads` are the tensors that the gradients are in at each
+    step. The moments are kept in floats, or with bits=8 in codes with a float for each 256 elements. Half parameters may
+    have float copies (`master`) that the steps go from. mean, square (and mean_scale, square_scale with 8 bits): the states
+    of an earlier run, as `step` is the number of steps it had made; zeros otherwise."""
+
+    def __init__(self, params, grads, master=None, lr=1e-3, beta1=0.9, beta2=0.999, eps=1e-8, weight_decay=0.01, bits=32, mean=None,
+                 square=None, mean_scale=None, square_scale=None, step=0):
+        if mean_scale is not None or square_scale is not None:
+            bits = 8
+        if bits not in (8, 32):
+            raise ValueError("states have 8 or 32 bits")
+        kinds = {p.kind for p in params}
+        if kinds - {"float", "half"} or len(kinds) > 1:
+            raise ValueError("parameters are all float or all half")
+        self.kind = kinds.pop() if kinds else "float"
+        if master is not None and self.kind != "half":
+            raise ValueError("float copies are of half parameters")
+        self.lr, self.beta1, self.beta2, self.eps, self.weight_decay, self.steps, self.bits = lr, beta1, beta2, eps, weight_decay, step, bits
+        self.params, self.grads, self.master = list(params), list(grads), list(master) if master is not None else None
+
+        def zeros(kind, shape):
+            return Tensor(kind).resize(shape).zero() if shape else Tensor(kind)
+
+        def state(given, kind, blocks=False):
+            if given is not None:
+                return list(given)
+            return [zeros(kind, (-(-p.numel() // 256),) if blocks and p.numel() else () if blocks else p.shape) for p in self.params]
+
+        self.mean = state(mean, "char" if bits == 8 else "float")
+        self.square = state(square, "byte" if bits == 8 else "float")
+        self.mean_scale = state(mean_scale, "float", True) if bits == 8 else None
+        self.square_scale = state(square_scale, "float", True) if bits == 8 else None
+        lists = [(self.params, self.kind)] + ([(self.master, "float")] if self.kind == "half" else []) + [(self.grads, self.kind)]
+        if bits == 8:
+            lists += [(self.mean, "char"), (self.mean_scale, "float"), (self.square, "byte"), (self.square_scale, "float")]
+        else:
+            lists += [(self.mean, "float"), (self.square, "float")]
+        self._arrays = [self._array(l, kind) for l, kind in lists]
+        self._args = [C.addressof(a) if a is not None else 0 for a in self._arrays]
+
+    def _array(self, tensors, kind):
+        if tensors is None:
+            return None
+        if len(tensors) != len(self.params):
+            raise ValueError("%d tensors for %d parameters" % (len(tensors), len(self.params)))
+        if any(t.kind != kind for t in tensors):
+            raise ValueError("a tensor of another type than %s" % kind)
+        return (C.c_void_p * max(1, len(tensors)))(*[t.a for t in tensors])
+
+    def step(self, grad_scale=1.0):
+        """One step from what the gradients hold, times grad_scale."""
+        _CALLS[self.kind]["adamW8" if self.bits == 8 else "adamW"](
+            len(self.params), *self._args, self.lr, self.beta1, self.beta2, self.eps, self.weight_decay, self.steps + 1, grad_scale)
+        self.steps += 1
+
+    def moments(self, mean=None, square=None):
+        """(mean, square): lists of float tensors with the moments, those given or new ones; of 32-bit states the states themselves."""
+        if self.bits == 32:
+            return self.mean, self.square
+        mean = [Tensor("float") for _ in self.params] if mean is None else mean
+        square = [Tensor("float") for _ in self.params] if square is None else square
+        arrays = [self._array(mean, "float"), self._array(square, "float")]
+        _CALLS["float"]["adamW8Moments"](len(self.params), *[C.addressof(a) for a in arrays], *self._args[-4:])
+        return mean, square
 
 
 def cached_memory():

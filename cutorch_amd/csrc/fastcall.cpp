@@ -201,6 +201,14 @@ void fill_registry() {
   add_result<signed char>("b");
   add_result<unsigned char>("B");
   add_result<uint16_t>("e");
+  // the operators of a training step: embedding takes an add_element<float> signature
+  add<void, T, T, T, float, long, int>("vtttfli");
+  add<void, T, T, T, T, T, T, T, T, T, double, double, double, double>("vtttttttttdddd");
+  add<void, int, T, T, T, T, double, double, double, double, double, long, double>("vittttdddddld");
+  add<void, int, T, T, T, T, T, double, double, double, double, double, long, double>("vitttttdddddld");
+  add<void, int, T, T, T, T, T, T, double, double, double, double, double, long, double>("vittttttdddddld");
+  add<void, int, T, T, T, T, T, T, T, double, double, double, double, double, long, double>("vitttttttdddddld");
+  add<void, int, T, T, T, T, T, T>("vitttttt");
   add<float, T, float>("ftf");
   add<float, T, Half>("fte");
   add<double, T, double>("dtd");

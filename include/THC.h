@@ -623,4 +623,104 @@ THC_AMD_DECLARE_MATH_API(THCudaHalfTensor, THHalf, float)
  *     them. */
 THC_API void THCudaTensor_sumallNoAlloc(THCState *state, THCudaTensor *self, float *result);
 
+/* ------------------------------------------------------------------------ */
+/* The two ends of a language model and its training step, for float and     */
+/* half tensors. No counterpart in the reference. Tokens are 1-based, as all */
+/* indices here. Every call is asynchronous on the current stream and gives  */
+/* the same bits for the same inputs; temporaries come from the state's      */
+/* allocator. Operands may be strided; those that a kernel does not take     */
+/* where they are go through dense copies (all but windows and batches of    */
+/* rows with unit stride along the last dim).                                */
+/* ------------------------------------------------------------------------ */
+#define THC_AMD_DECLARE_TOKEN_API(Tensor)                                      \
+  /* self[..., :] = scale * weight[token, :], rounded once. `weight` has two  \
+   * dims; self takes the tokens' sizes and the rows' length. A token outside \
+   * the table reads nothing, its row is NaN. */                               \
+  THC_API void Tensor##_embedding(THCState *, Tensor *self, Tensor *weight,    \
+                                  THCudaLongTensor *tokens, float scale);      \
+  /* The gradient of that: gradWeight[v, :] = scale * the sum of gradOutput's  \
+   * rows whose token is v, summed in float in the order of the positions and  \
+   * rounded once; rows of other tokens become 0. With `accumulate` the sums  \
+   * are added to what gradWeight holds and other rows keep it. Positions of   \
+   * `paddingToken` (0: none) and of tokens outside the table are left out.    \
+   * gradWeight keeps its sizes. */                                            \
+  THC_API void Tensor##_embeddingGrad(THCState *, Tensor *gradWeight,          \
+                                      THCudaLongTensor *tokens,                \
+                                      Tensor *gradOutput, float scale,         \
+                                      long paddingToken, int accumulate);      \
+  /* self = the log-probability of each row's token: x[token] - log(sum(       \
+   * exp(x))). Rows run along the logits' last dim, one token each; self takes \
+   * the tokens' sizes. NaN for a token outside the row. */                    \
+  THC_API void Tensor##_tokenLogProb(THCState *, THCudaTensor *self,           \
+                                     Tensor *logits,                           \
+                                     THCudaLongTensor *tokens);                \
+  /* Clipped policy loss with a KL term, and its gradient, in one pass:        \
+   *   lp = the token's log-probability, r = exp(lp - oldLogProb)              \
+   *   l = -min(r A, clip(r, 1 - clipLow, 1 + clipHigh) A)                     \
+   *       + klCoef (exp(refLogProb - lp) - (refLogProb - lp) - 1)             \
+   *   loss = weight * l, gradLogits = gradScale * d(sum of loss) / d(logits)  \
+   * loss and logProb take the tokens' sizes, gradLogits the logits' (it may   \
+   * be the logits themselves; null: losses alone). weight null: 1 / rows.     \
+   * A row of weight 0 is not read: its loss, log-probability and gradient     \
+   * are 0 whatever it holds. refLogProb null, or klCoef 0: no KL term.        \
+   * The loss of the batch is the sum of `loss`. */                            \
+  THC_API void Tensor##_policyLoss(                                            \
+      THCState *, THCudaTensor *loss, THCudaTensor *logProb,                   \
+      Tensor *gradLogits, Tensor *logits, THCudaLongTensor *tokens,            \
+      THCudaTensor *oldLogProb, THCudaTensor *advantage,                       \
+      THCudaTensor *refLogProb, THCudaTensor *weight, double clipLow,          \
+      double clipHigh, double klCoef, double gradScale);
+THC_AMD_DECLARE_TOKEN_API(THCudaTensor)
+THC_AMD_DECLARE_TOKEN_API(THCudaHalfTensor)
+
+/* One AdamW step of `count` tensors, in place:
+ *   g = gradScale grad;  m = beta1 m + (1 - beta1) g;
+ *   v = beta2 v + (1 - beta2) g^2
+ *   p = p (1 - lr weightDecay)
+ *       - lr / (1 - beta1^step) m / (sqrt(v / (1 - beta2^step)) + eps)
+ * in float, `step` counted from 1. The lists hold one tensor per parameter, of
+ * the parameter's sizes. Half parameters may have float copies (`master`, null
+ * for none): the step then goes from those and the parameters are their
+ * rounded values. No tensor may appear twice.
+ *
+ * adamW8 keeps the moments in 8 bits: codes of the parameter's sizes and one
+ * float (the largest magnitude) for each 256 elements of a tensor in its
+ * logical order, ceil(n / 256) of them:
+ *   m = meanScale (c / 127) |c / 127|,  v = squareScale (c / 255)^4
+ * with the nearest codes, v's at least 1 where v > 0. Zeros begin a run. A
+ * moment that is not finite makes its 256 elements' moments NaN.
+ * adamW8Moments writes the moments that such states hold as floats. */
+THC_API void THCudaTensor_adamW(THCState *state, int count, THCudaTensor **param,
+                                THCudaTensor **grad, THCudaTensor **mean,
+                                THCudaTensor **square, double lr, double beta1,
+                                double beta2, double eps, double weightDecay,
+                                long step, double gradScale);
+THC_API void THCudaHalfTensor_adamW(THCState *state, int count,
+                                    THCudaHalfTensor **param, THCudaTensor **master,
+                                    THCudaHalfTensor **grad, THCudaTensor **mean,
+                                    THCudaTensor **square, double lr, double beta1,
+                                    double beta2, double eps, double weightDecay,
+                                    long step, double gradScale);
+THC_API void THCudaTensor_adamW8(THCState *state, int count, THCudaTensor **param,
+                                 THCudaTensor **grad, THCudaCharTensor **mean,
+                                 THCudaTensor **meanScale, THCudaByteTensor **square,
+                                 THCudaTensor **squareScale, double lr, double beta1,
+                                 double beta2, double eps, double weightDecay,
+                                 long step, double gradScale);
+THC_API void THCudaHalfTensor_adamW8(THCState *state, int count,
+                                     THCudaHalfTensor **param, THCudaTensor **master,
+                                     THCudaHalfTensor **grad, THCudaCharTensor **mean,
+                                     THCudaTensor **meanScale,
+                                     THCudaByteTensor **square,
+                                     THCudaTensor **squareScale, double lr,
+                                     double beta1, double beta2, double eps,
+                                     double weightDecay, long step,
+                                     double gradScale);
+THC_API void THCudaTensor_adamW8Moments(THCState *state, int count,
+                                        THCudaTensor **mean, THCudaTensor **square,
+                                        THCudaCharTensor **meanCode,
+                                        THCudaTensor **meanScale,
+                                        THCudaByteTensor **squareCode,
+                                        THCudaTensor **squareScale);
+
 #endif /* THC_AMD_THC_H */
