@@ -14,6 +14,7 @@
 // (the growth of the moments in the first steps) is in the float and is not rounded to codes.
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 #include <vector>
 
 #include "training.hpp"
@@ -36,7 +37,7 @@ __device__ __forceinline__ float adamw_step(const Hyper& h, float p, float g, fl
   return p * h.keep - (m / root) * h.rate;
 }
 
-// The tensors of one launch, as kernel arguments.
+// The tensors of one launch travel as kernel arguments: no table has to reach the device first.
 struct Item {
   void* param;
   float* master;
@@ -45,23 +46,84 @@ struct Item {
   float *meanScale, *squareScale;
   int64_t size;
 };
+constexpr int kItems = 56;                            // 3.9 KiB of arguments
+constexpr int kPacks = 4;                             // of 4 elements, in flight per lane
+constexpr int kPart = kBlock * 4 * kPacks;            // elements a workgroup
+struct StepArgs {
+  Hyper h;
+  int32_t count;
+  uint32_t firstPart[kItems];                         // the workgroup that each tensor begins with
+  Item item[kItems];
+};
 
-template <typename T>
-__global__ __launch_bounds__(kBlock) void step_kernel(Item t, Hyper h) {
-  constexpr int V = 4;
-  const int64_t i0 = ((int64_t)blockIdx.x * kBlock + threadIdx.x) * V;
+// Which tensor this workgroup has: every lane looks at one.
+__device__ __forceinline__ int item_of(const StepArgs& a) {
+  const int lane = threadIdx.x & 63;
+  const uint32_t first = lane < a.count ? a.firstPart[lane] : ~0u;
+  return __builtin_amdgcn_readfirstlane(__popcll(__ballot(first <= blockIdx.x)) - 1);
+}
+
+// Four neighbours as floats, and back; `n` of them are the tensor's.
+template <bool NT, typename T>
+__device__ __forceinline__ void load4(float (&to)[4], const T* from, int n) {
+  using P = Pack<T, 4>;
+  if (n >= 4) {
+    const P p = load_pack_unaligned<NT, P>(from);
 #pragma unroll
-  for (int e = 0; e < V; ++e) {
-    const int64_t i = i0 + e;
-    if (i >= t.size) return;
-    T* param = static_cast<T*>(t.param);
-    float *mean = static_cast<float*>(t.mean), *square = static_cast<float*>(t.square);
-    float m = mean[i], v = square[i];
-    const float p = adamw_step(h, t.master ? t.master[i] : Cvt<T>::up(param[i]), Cvt<T>::up(static_cast<const T*>(t.grad)[i]), m, v);
-    mean[i] = m;
-    square[i] = v;
-    if (t.master) t.master[i] = p;
-    param[i] = rounded<T>(p);
+    for (int e = 0; e < 4; ++e) to[e] = Cvt<T>::up(p.v[e]);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) to[e] = e < n ? Cvt<T>::up(from[e]) : 0.f;
+  }
+}
+template <bool NT, typename T>
+__device__ __forceinline__ void store4(T* to, const float (&from)[4], int n) {
+  using P = Pack<T, 4>;
+  if (n >= 4) {
+    P p;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) p.v[e] = rounded<T>(from[e]);
+    store_pack_unaligned<NT>(to, p);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (e < n) to[e] = rounded<T>(from[e]);
+  }
+}
+
+// States in 32 bits: kPacks packs of each operand in flight, then the arithmetic, in place.
+template <typename T, bool MASTER, bool NT>
+__global__ __launch_bounds__(kBlock) void step_kernel(StepArgs a) {
+  const Item& t = a.item[item_of(a)];
+  const int64_t base = (int64_t)(blockIdx.x - a.firstPart[item_of(a)]) * kPart;
+  const int left = (int)min((int64_t)kPart, t.size - base);
+  T* param = static_cast<T*>(t.param) + base;
+  float* master = MASTER ? t.master + base : nullptr;
+  const T* grad = static_cast<const T*>(t.grad) + base;
+  float *mean = static_cast<float*>(t.mean) + base, *square = static_cast<float*>(t.square) + base;
+  float p[kPacks][4], g[kPacks][4], m[kPacks][4], v[kPacks][4];
+#pragma unroll
+  for (int u = 0; u < kPacks; ++u) {
+    const int i = (u * kBlock + threadIdx.x) * 4;
+    if (i < left) {
+      if constexpr (MASTER) load4<true>(p[u], master + i, left - i);
+      else load4<true>(p[u], param + i, left - i);
+      load4<true>(g[u], grad + i, left - i);
+      load4<true>(m[u], mean + i, left - i);
+      load4<true>(v[u], square + i, left - i);
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < kPacks; ++u) {
+    const int i = (u * kBlock + threadIdx.x) * 4;
+    if (i < left) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) p[u][e] = adamw_step(a.h, p[u][e], g[u][e], m[u][e], v[u][e]);
+      store4<NT>(mean + i, m[u], left - i);
+      store4<NT>(square + i, v[u], left - i);
+      if constexpr (MASTER) store4<NT>(master + i, p[u], left - i);
+      store4<NT>(param + i, p[u], left - i);
+    }
   }
 }
 
@@ -74,74 +136,163 @@ __device__ __forceinline__ float decode_square(uint8_t c, float top) {
   t = t * t;
   return (t * t) * top;
 }
-// The largest of a wave's magnitudes as bits: NaN is above infinity, so it is not lost.
+// The largest of a wave's magnitudes as bits: NaN is above infinity, so it is not lost. Each row of 16 lanes by shifts, then the rows.
 __device__ __forceinline__ float wave_top(uint32_t bits) {
-#pragma unroll
-  for (int d = 32; d >= 1; d >>= 1) bits = max(bits, (uint32_t)__shfl_xor((int)bits, d));
-  return __uint_as_float(bits);
+  int v = (int)bits;
+  auto step = [&](auto control, auto rows) {
+    const int o = __builtin_amdgcn_update_dpp(v, v, decltype(control)::value, decltype(rows)::value, 0xf, false);
+    v = (int)max((uint32_t)v, (uint32_t)o);
+  };
+  using std::integral_constant;
+  step(integral_constant<int, 0x111>{}, integral_constant<int, 0xf>{});   // row_shr 1, 2, 4, 8
+  step(integral_constant<int, 0x112>{}, integral_constant<int, 0xf>{});
+  step(integral_constant<int, 0x114>{}, integral_constant<int, 0xf>{});
+  step(integral_constant<int, 0x118>{}, integral_constant<int, 0xf>{});
+  step(integral_constant<int, 0x142>{}, integral_constant<int, 0xa>{});   // lane 15 of a row to the next one
+  step(integral_constant<int, 0x143>{}, integral_constant<int, 0xc>{});   // lane 31 to the last two rows
+  return __uint_as_float((uint32_t)__builtin_amdgcn_readlane(v, 63));
 }
 __device__ __forceinline__ float inverse_top(float& top) {
   if (top < kSmallestTop) top = 0.f;
   return top > 0.f ? 1.f / top : 0.f;
 }
-
-// A wave a block of states.
 template <typename T>
-__global__ __launch_bounds__(kBlock) void step8_kernel(Item t, Hyper h) {
-  constexpr int V = 4;
-  const int lane = threadIdx.x & 63;
-  const int64_t block = (int64_t)blockIdx.x * (kBlock / 64) + (threadIdx.x >> 6);
-  if (block * kStateBlock >= t.size) return;      // whole waves
-  T* param = static_cast<T*>(t.param);
-  int8_t* mean = static_cast<int8_t*>(t.mean);
-  uint8_t* square = static_cast<uint8_t*>(t.square);
-  const float oldMean = t.meanScale[block], oldSquare = t.squareScale[block];
-  float m[V], v[V];
-  uint32_t topMean = 0, topSquare = 0;
+__device__ __forceinline__ void load4_codes(T (&to)[4], const T* from, int n) {
+  using P = Pack<T, 4>;
+  if (n >= 4) {
+    const P p = load_pack_unaligned<true, P>(from);
 #pragma unroll
-  for (int e = 0; e < V; ++e) {
-    const int64_t i = block * kStateBlock + lane * V + e;
-    m[e] = v[e] = 0.f;
-    if (i < t.size) {
-      m[e] = decode_mean(mean[i], oldMean);
-      v[e] = decode_square(square[i], oldSquare);
-      const float p = adamw_step(h, t.master ? t.master[i] : Cvt<T>::up(param[i]), Cvt<T>::up(static_cast<const T*>(t.grad)[i]), m[e], v[e]);
-      if (t.master) t.master[i] = p;
-      param[i] = rounded<T>(p);
-      topMean = max(topMean, __float_as_uint(fabsf(m[e])));
-      topSquare = max(topSquare, __float_as_uint(v[e]));
-    }
-  }
-  float newMean = wave_top(topMean), newSquare = wave_top(topSquare);
-  const float inverseMean = inverse_top(newMean), inverseSquare = inverse_top(newSquare);
+    for (int e = 0; e < 4; ++e) to[e] = p.v[e];
+  } else {
 #pragma unroll
-  for (int e = 0; e < V; ++e) {
-    const int64_t i = block * kStateBlock + lane * V + e;
-    if (i < t.size) {
-      const float c = rintf(sqrtf(fabsf(m[e]) * inverseMean) * 127.f);
-      mean[i] = (int8_t)(int)(m[e] < 0.f ? -c : c);
-      const float share = v[e] * inverseSquare;
-      const float d = rintf(sqrtf(sqrtf(share)) * 255.f);
-      square[i] = (uint8_t)(int)(share > 0.f ? fmaxf(d, 1.f) : d);
-    }
+    for (int e = 0; e < 4; ++e) to[e] = e < n ? from[e] : T(0);
   }
-  if (lane == 0) {
-    t.meanScale[block] = newMean;
-    t.squareScale[block] = newSquare;
+}
+template <bool NT, typename T>
+__device__ __forceinline__ void store4_codes(T* to, const T (&from)[4], int n) {
+  using P = Pack<T, 4>;
+  if (n >= 4) {
+    P p;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) p.v[e] = from[e];
+    store_pack_unaligned<NT>(to, p);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (e < n) to[e] = from[e];
   }
 }
 
-// The moments that 8-bit states stand for.
-__global__ __launch_bounds__(kBlock) void decode_kernel(const int8_t* mean, const float* meanScale, const uint8_t* square, const float* squareScale,
-                                                        float* meanOut, float* squareOut, int64_t n) {
-  const int64_t i = (int64_t)blockIdx.x * kBlock + threadIdx.x;
-  if (i >= n) return;
-  meanOut[i] = decode_mean(mean[i], meanScale[i / kStateBlock]);
-  squareOut[i] = decode_square(square[i], squareScale[i / kStateBlock]);
+// States in 8 bits: a wave has kPacks blocks of states, 4 elements a lane of each. What is behind a tensor's end counts as zeros.
+template <typename T, bool MASTER, bool NT>
+__global__ __launch_bounds__(kBlock) void step8_kernel(StepArgs a) {
+  const Item& t = a.item[item_of(a)];
+  const int64_t base = (int64_t)(blockIdx.x - a.firstPart[item_of(a)]) * kPart;
+  const int left = (int)min((int64_t)kPart, t.size - base);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  T* param = static_cast<T*>(t.param) + base;
+  float* master = MASTER ? t.master + base : nullptr;
+  const T* grad = static_cast<const T*>(t.grad) + base;
+  int8_t* mean = static_cast<int8_t*>(t.mean) + base;
+  uint8_t* square = static_cast<uint8_t*>(t.square) + base;
+  float *meanScale = t.meanScale + base / kStateBlock, *squareScale = t.squareScale + base / kStateBlock;
+  float p[kPacks][4], g[kPacks][4], topMean[kPacks], topSquare[kPacks];
+  int8_t codeMean[kPacks][4];
+  uint8_t codeSquare[kPacks][4];
+#pragma unroll
+  for (int u = 0; u < kPacks; ++u) {
+    const int block = u * (kBlock / 64) + wave, i = block * kStateBlock + lane * 4;
+    if (block * kStateBlock < left) {      // whole waves
+      const int n = left - i;              // none for the lanes behind the end
+      topMean[u] = meanScale[block];
+      topSquare[u] = squareScale[block];
+      if constexpr (MASTER) load4<true>(p[u], master + i, n);
+      else load4<true>(p[u], param + i, n);
+      load4<true>(g[u], grad + i, n);
+      load4_codes(codeMean[u], mean + i, n);
+      load4_codes(codeSquare[u], square + i, n);
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < kPacks; ++u) {
+    const int block = u * (kBlock / 64) + wave, i = block * kStateBlock + lane * 4;
+    if (block * kStateBlock < left) {
+      const int n = left - i;
+      float m[4], v[4];
+      uint32_t maxMean = 0, maxSquare = 0;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        m[e] = decode_mean(codeMean[u][e], topMean[u]);
+        v[e] = decode_square(codeSquare[u][e], topSquare[u]);
+        p[u][e] = adamw_step(a.h, p[u][e], g[u][e], m[e], v[e]);
+        if (e < n) {          // (zeros behind the end may meet a factor that is not finite)
+          maxMean = max(maxMean, __float_as_uint(fabsf(m[e])));
+          maxSquare = max(maxSquare, __float_as_uint(v[e]));
+        }
+      }
+      if constexpr (MASTER) store4<NT>(master + i, p[u], n);
+      store4<NT>(param + i, p[u], n);
+      float newMean = wave_top(maxMean), newSquare = wave_top(maxSquare);
+      const float inverseMean = inverse_top(newMean), inverseSquare = inverse_top(newSquare);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float c = rintf(sqrtf(fabsf(m[e]) * inverseMean) * 127.f);
+        codeMean[u][e] = (int8_t)(int)(m[e] < 0.f ? -c : c);
+        const float share = v[e] * inverseSquare;
+        const float d = rintf(sqrtf(sqrtf(share)) * 255.f);
+        codeSquare[u][e] = (uint8_t)(int)(share > 0.f ? fmaxf(d, 1.f) : d);
+      }
+      store4_codes<NT>(mean + i, codeMean[u], n);
+      store4_codes<NT>(square + i, codeSquare[u], n);
+      if (lane == 0) {
+        meanScale[block] = newMean;
+        squareScale[block] = newSquare;
+      }
+    }
+  }
+}
+
+// The moments that 8-bit states stand for: the items' codes and scales, into `param` and `master`.
+template <bool NT>
+__global__ __launch_bounds__(kBlock) void decode_kernel(StepArgs a) {
+  const Item& t = a.item[item_of(a)];
+  const int64_t base = (int64_t)(blockIdx.x - a.firstPart[item_of(a)]) * kPart;
+  const int left = (int)min((int64_t)kPart, t.size - base);
+  const int8_t* mean = static_cast<const int8_t*>(t.mean) + base;
+  const uint8_t* square = static_cast<const uint8_t*>(t.square) + base;
+  const float *meanScale = t.meanScale + base / kStateBlock, *squareScale = t.squareScale + base / kStateBlock;
+  float *meanOut = static_cast<float*>(t.param) + base, *squareOut = t.master + base;
+  int8_t codeMean[kPacks][4];
+  uint8_t codeSquare[kPacks][4];
+  float topMean[kPacks], topSquare[kPacks];
+#pragma unroll
+  for (int u = 0; u < kPacks; ++u) {
+    const int i = (u * kBlock + threadIdx.x) * 4;
+    if (i < left) {
+      topMean[u] = meanScale[i / kStateBlock];
+      topSquare[u] = squareScale[i / kStateBlock];
+      load4_codes(codeMean[u], mean + i, left - i);
+      load4_codes(codeSquare[u], square + i, left - i);
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < kPacks; ++u) {
+    const int i = (u * kBlock + threadIdx.x) * 4;
+    if (i < left) {
+      float m[4], v[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        m[e] = decode_mean(codeMean[u][e], topMean[u]);
+        v[e] = decode_square(codeSquare[u][e], topSquare[u]);
+      }
+      store4<NT>(meanOut + i, m, left - i);
+      store4<NT>(squareOut + i, v, left - i);
+    }
+  }
 }
 
 // ------------------------------------------------------------------------- host --
-// Operands that are written where they are if they are dense, else through a copy.
+// Operands that are used where they are if they are dense, else through a copy.
 struct Held {
   THCState* s;
   struct One {
@@ -158,6 +309,7 @@ struct Held {
     for (One& o : all) tensor_free(s, o.dense);
   }
   void* add(AnyTensor* t, DType dt, bool written) {
+    if (tensor_is_contiguous(t)) return tensor_data(t, dt);
     all.reserve(all.size() + 1);
     AnyTensor* dense = tensor_new_contiguous(s, t, dt);
     all.push_back(One{t, dense, dt, written});
@@ -165,7 +317,28 @@ struct Held {
   }
   void write_back() {
     for (One& o : all)
-      if (o.written && o.dense != o.tensor) copy_tensor(s, o.dt, o.tensor, o.dense, false);
+      if (o.written) copy_tensor(s, o.dt, o.tensor, o.dense, false);
+  }
+};
+
+// Collects tensors and launches a kernel for as many as its arguments hold. NT: what the whole call writes is too much for the caches.
+template <typename Launch>
+struct Batch {
+  StepArgs a{};
+  uint32_t parts = 0;
+  Launch launch;
+  explicit Batch(Launch l) : launch(l) {}
+  void add(const Item& t) {
+    const int64_t n = (t.size + kPart - 1) / kPart;
+    if (a.count == kItems || (a.count && parts + n > (int64_t)1 << 31)) flush();
+    a.firstPart[a.count] = parts;
+    a.item[a.count++] = t;
+    parts += (uint32_t)n;
+  }
+  void flush() {
+    if (a.count) launch(a, dim3(parts));
+    a.count = 0;
+    parts = 0;
   }
 };
 
@@ -186,7 +359,7 @@ void check_list(THCState* s, const AnyTensor* t, const AnyTensor* like, int arg,
   check_same_gpu(s, 1, &t);
   THC_ARG_CHECK(t->nDimension <= kMaxDims, arg, "%s", kDimWarning);
   THC_ARG_CHECK(same_sizes(t, like), arg, "tensor %d has other sizes than its parameter", index + 1);
-  THC_ARG_CHECK(!written || !overlapping(tensor_layout(t)), arg, "elements of tensor %d overlap", index + 1);
+  THC_ARG_CHECK(!written || tensor_is_contiguous(t) || !overlapping(tensor_layout(t)), arg, "elements of tensor %d overlap", index + 1);
 }
 
 void adamw(THCState* s, DType dt, int count, const Lists& l, double lr, double beta1, double beta2, double eps, double weightDecay, long step,
@@ -222,7 +395,27 @@ void adamw(THCState* s, DType dt, int count, const Lists& l, double lr, double b
   h.keep = (float)(1 - lr * weightDecay);
   h.rate = (float)(lr / (1 - std::pow(beta1, (double)step)));
   h.gradScale = (float)gradScale;
+  int64_t elements = 0;
+  for (int i = 0; i < count; ++i) elements += tensor_numel(l.param[i]);
+  const bool nt = streaming_store("adamw.nt", elements * (int64_t)(eight ? 6 : 12));
   hipStream_t st = current_stream(s);
+  auto launch = [&](const StepArgs& a, dim3 grid) {
+    auto go = [&](auto type, auto master, auto stream) {
+      using T = decltype(type);
+      constexpr bool M = decltype(master)::value, NT = decltype(stream)::value;
+      if (eight) hipLaunchKernelGGL((step8_kernel<T, M, NT>), grid, dim3(kBlock), 0, st, a);
+      else hipLaunchKernelGGL((step_kernel<T, M, NT>), grid, dim3(kBlock), 0, st, a);
+    };
+    auto typed = [&](auto stream) {
+      if (!half) go(float{}, std::false_type{}, stream);
+      else if (!l.master) go(__half{}, std::false_type{}, stream);
+      else go(__half{}, std::true_type{}, stream);
+    };
+    if (nt) typed(std::true_type{});
+    else typed(std::false_type{});
+  };
+  Batch<decltype(launch)> batch(launch);
+  batch.a.h = h;
   Held held(s);
   for (int i = 0; i < count; ++i) {
     if (!has_elements(l.param[i])) continue;
@@ -239,15 +432,9 @@ void adamw(THCState* s, DType dt, int count, const Lists& l, double lr, double b
       t.meanScale = (float*)held.add(l.meanScale[i], DType::F32, true);
       t.squareScale = (float*)held.add(l.squareScale[i], DType::F32, true);
     }
-    const dim3 grid((unsigned)((t.size + 4 * kBlock - 1) / (4 * kBlock)));
-    if (eight) {
-      if (half) hipLaunchKernelGGL((step8_kernel<__half>), grid, dim3(kBlock), 0, st, t, h);
-      else hipLaunchKernelGGL((step8_kernel<float>), grid, dim3(kBlock), 0, st, t, h);
-    } else {
-      if (half) hipLaunchKernelGGL((step_kernel<__half>), grid, dim3(kBlock), 0, st, t, h);
-      else hipLaunchKernelGGL((step_kernel<float>), grid, dim3(kBlock), 0, st, t, h);
-    }
+    batch.add(t);
   }
+  batch.flush();
   THC_CHECK(hipGetLastError());
   note_kernel(eight ? "adamw8" : "adamw");
   held.write_back();
@@ -266,23 +453,32 @@ void moments(THCState* s, int count, AnyTensor** meanOut, AnyTensor** squareOut,
     THC_ARG_CHECK(meanOut[i], 3, "tensor %d is missing", i + 1);
     THC_ARG_CHECK(squareOut[i], 4, "tensor %d is missing", i + 1);
   }
+  int64_t elements = 0;
+  for (int i = 0; i < count; ++i) elements += tensor_numel(mean[i]);
+  const bool nt = streaming_store("adamw.nt", elements * 8);
   hipStream_t st = current_stream(s);
+  auto launch = [&](const StepArgs& a, dim3 grid) {
+    if (nt) hipLaunchKernelGGL((decode_kernel<true>), grid, dim3(kBlock), 0, st, a);
+    else hipLaunchKernelGGL((decode_kernel<false>), grid, dim3(kBlock), 0, st, a);
+  };
+  Batch<decltype(launch)> batch(launch);
   Held held(s);
   for (int i = 0; i < count; ++i) {
-    const int64_t n = tensor_numel(mean[i]);
     tensor_resize_as(s, meanOut[i], mean[i], DType::F32);
     tensor_resize_as(s, squareOut[i], mean[i], DType::F32);
-    if (n == 0) continue;
+    if (!has_elements(mean[i])) continue;
     note_stream_use(s, {meanOut[i], squareOut[i], mean[i], meanScale[i], square[i], squareScale[i]});
-    float* to = (float*)held.add(meanOut[i], DType::F32, true);
-    float* toSquare = (float*)held.add(squareOut[i], DType::F32, true);
-    const int8_t* from = (const int8_t*)held.add(mean[i], DType::I8, false);
-    const uint8_t* fromSquare = (const uint8_t*)held.add(square[i], DType::U8, false);
-    const float* scale = (const float*)held.add(meanScale[i], DType::F32, false);
-    const float* scaleSquare = (const float*)held.add(squareScale[i], DType::F32, false);
-    hipLaunchKernelGGL(decode_kernel, dim3((unsigned)((n + kBlock - 1) / kBlock)), dim3(kBlock), 0, st, from, scale, fromSquare, scaleSquare, to,
-                       toSquare, n);
+    Item t{};
+    t.size = tensor_numel(mean[i]);
+    t.param = held.add(meanOut[i], DType::F32, true);
+    t.master = (float*)held.add(squareOut[i], DType::F32, true);
+    t.mean = held.add(mean[i], DType::I8, false);
+    t.square = held.add(square[i], DType::U8, false);
+    t.meanScale = (float*)held.add(meanScale[i], DType::F32, false);
+    t.squareScale = (float*)held.add(squareScale[i], DType::F32, false);
+    batch.add(t);
   }
+  batch.flush();
   THC_CHECK(hipGetLastError());
   note_kernel("adamw8-moments");
   held.write_back();
