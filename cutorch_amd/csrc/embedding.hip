@@ -130,17 +130,26 @@ void embedding(THCState* s, DType dt, AnyTensor* self, AnyTensor* table, AnyTens
 //           edge leaves a partial sum. Rows of tokens that do not occur are zeroed by other workgroups of this launch.
 //   fold    the partial sums of each token that crosses edges, in the chunks' order
 
-// Grouping. Token k (0-based) belongs to owner k mod G; every owner reads all tokens and places its own. No owner waits for another:
-// it counts the tokens of the owners before it on the way, which is where its slots begin. A token's slots are side by side and
-// its positions in order; the order of the tokens does not matter to the sums.
+// Grouping. Token k (0-based) belongs to owner k mod G. An owner sweeps the tokens twice, counts its own and places them; the tokens of
+// the owners before it, which it counts on the way, say where its slots begin: no owner waits for another. A token's slots are side
+// by side and its positions in order; the order of the tokens does not matter to the sums.
+// Few positions are swept as they are, by every owner. Of many, each owner would look at all: they are first split, tile by tile, into
+// the owners' shares.
 struct Grouping {
   int32_t* position;   // of each slot
   int32_t* token;      // of each slot, 0-based
   int32_t* used;       // occurrences of each token
   int32_t* total;      // slots
 };
-constexpr int kGroupThreads = 512, kGroupWaves = kGroupThreads / 64;
-constexpr int kOwnTokens = 1024;     // tokens that one owner takes at most: 32 KiB of counts
+constexpr int kGroupThreads = 1024, kGroupWaves = kGroupThreads / 64;
+constexpr int kOwnTokens = 512;      // tokens that one owner takes at most: 32 KiB of counts
+constexpr int kFound = 512;          // positions that a wave remembers between its two sweeps: 64 KiB
+constexpr int kTile = 4096;          // positions that are split together, 4 a lane
+// Splitting costs a launch and saves every owner the sight of the others' positions. us of the whole gradient, swept and split: 1500 x 513
+// 15, 20; 32768 x 1024 47, 51; 49152 x 1024 62, 63; 65536 x 1024 75, 74; 131072 x 1024 167, 124; 300000 x 64 224, 108 (halves, added).
+constexpr int kSplitFrom = 57344;
+constexpr int kMostSplit = 1024;     // owners that they are split between
+constexpr int kAhead = 8;            // loads in flight
 
 __device__ __forceinline__ int wave_sum(int v) {
 #pragma unroll
@@ -148,42 +157,73 @@ __device__ __forceinline__ int wave_sum(int v) {
   return v;
 }
 
-__global__ __launch_bounds__(kGroupThreads) void group_kernel(Grouping g, const int64_t* __restrict__ tokens, int32_t n, int64_t vocab,
-                                                              int64_t padding, int shift) {
-  __shared__ int counts[kGroupWaves][kOwnTokens];
-  __shared__ int waveTotal[kGroupWaves], before[kGroupWaves];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const uint64_t mask = (uint64_t(1) << shift) - 1, me = blockIdx.x;
-  const int owned = (int)((vocab - 1 - (int64_t)me) >> shift) + 1;   // me < vocab
-  for (int i = threadIdx.x; i < kGroupWaves * kOwnTokens; i += kGroupThreads) (&counts[0][0])[i] = 0;
-  __syncthreads();
-  // a wave takes a run of positions, 64 at a time
-  const int32_t run = ((n + kGroupWaves - 1) / kGroupWaves + 63) & ~63;
-  const int32_t first = min(n, wave * run), last = min(n, first + run);
-  int lower = 0;
-  for (int32_t i = first + lane; i < last; i += 64) {
-    const uint64_t k = (uint64_t)(tokens[i] - 1);
-    if (k < (uint64_t)vocab && (int64_t)k != padding - 1) {
-      const uint64_t owner = k & mask;
-      lower += owner < me;
-      if (owner == me) atomicAdd(&counts[wave][k >> shift], 1);      // whole numbers: any order gives the same
+// Calls f(position, token, whether it is one of the table's and not padding) for positions [first, last), 64 side by side and in order.
+// Tokens are 0-based here and have 32 bits once their upper half has been looked at.
+template <typename F>
+__device__ __forceinline__ void each_token(const int64_t* __restrict__ tokens, int32_t first, int32_t last, uint32_t vocab, uint32_t padding,
+                                           const F& f) {
+  const int lane = threadIdx.x & 63;
+  for (int32_t i0 = first; i0 < last; i0 += 64 * kAhead) {
+    uint64_t k[kAhead];
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) k[u] = (uint64_t)tokens[min(i0 + u * 64 + lane, last - 1)];
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      const int32_t i = i0 + u * 64 + lane;
+      const uint32_t token = (uint32_t)k[u] - 1;
+      f(i, token, (k[u] >> 32) == 0 && token < vocab && token != padding && i < last);
     }
   }
-  lower = wave_sum(lower);
-  if (lane == 0) before[wave] = lower;
-  __syncthreads();
-  int start = 0;
-  for (int w = 0; w < kGroupWaves; ++w) start += before[w];
-  // the slots of each wave's occurrences of each token: tokens in order, each wave after the ones before it
-  constexpr int kPer = kOwnTokens / kGroupThreads;
-  int mine[kPer], sum = 0;
+}
+
+// A tile's positions by owner, in order within each: entries (position, token) and where each owner's begin; padding and tokens outside
+// the table are left out. Equal owners among a wave's lanes are found bit by bit.
+struct Split {
+  int2* entry;        // kTile per tile
+  int32_t* begin;     // owners + 1 per tile
+};
+__global__ __launch_bounds__(kGroupThreads) void split_kernel(Split to, const int64_t* __restrict__ tokens, int32_t n, uint32_t vocab,
+                                                              uint32_t padding, int shift) {
+  constexpr int kPer = kTile / kGroupThreads;
+  __shared__ int counts[kGroupWaves][kMostSplit];
+  __shared__ int waveTotal[kGroupWaves];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, owners = 1 << shift;
+  const uint64_t below = (uint64_t(1) << lane) - 1;
+  const uint32_t mask = (uint32_t)owners - 1;
+  const int32_t first = (int32_t)blockIdx.x * kTile + wave * (64 * kPer) + lane;
+  uint64_t k[kPer];
 #pragma unroll
-  for (int j = 0; j < kPer; ++j) {
-    const int r = threadIdx.x * kPer + j;
-    mine[j] = 0;
-    for (int w = 0; w < kGroupWaves; ++w) mine[j] += counts[w][r];
-    sum += mine[j];
-    if (r < owned) g.used[me + ((int64_t)r << shift)] = mine[j];
+  for (int u = 0; u < kPer; ++u) k[u] = (uint64_t)tokens[min(first + u * 64, n - 1)];
+  for (int b = lane; b < owners; b += 64) counts[wave][b] = 0;       // (each wave its own)
+  int rank[kPer];
+  bool valid[kPer];
+#pragma unroll
+  for (int u = 0; u < kPer; ++u) {
+    const uint32_t token = (uint32_t)k[u] - 1, owner = token & mask;
+    valid[u] = (k[u] >> 32) == 0 && token < vocab && token != padding && first + u * 64 < n;
+    uint64_t peers = __ballot(valid[u]);
+    for (int bit = 0; bit < shift; ++bit) {
+      const uint64_t set = __ballot((owner >> bit) & 1);
+      peers &= (owner >> bit) & 1 ? set : ~set;
+    }
+    if (valid[u]) {
+      const int at = counts[wave][owner];
+      rank[u] = at + __popcll(peers & below);
+      __builtin_amdgcn_wave_barrier();
+      if ((peers & below) == 0) counts[wave][owner] = at + __popcll(peers);
+    }
+    __builtin_amdgcn_wave_barrier();
+  }
+  __syncthreads();
+  // owners in order, a thread each; each wave's after those of the ones before it
+  const int b = threadIdx.x;
+  int count[kGroupWaves], sum = 0;
+  if (b < owners) {
+#pragma unroll
+    for (int w = 0; w < kGroupWaves; ++w) {
+      count[w] = counts[w][b];
+      sum += count[w];
+    }
   }
   int upto = sum;
 #pragma unroll
@@ -193,80 +233,197 @@ __global__ __launch_bounds__(kGroupThreads) void group_kernel(Grouping g, const 
   }
   if (lane == 63) waveTotal[wave] = upto;
   __syncthreads();
-  int at = start + upto - sum;
+  int at = upto - sum;
   for (int w = 0; w < wave; ++w) at += waveTotal[w];
+  int32_t* begin = to.begin + (int64_t)blockIdx.x * (owners + 1);
+  if (b < owners) {
+    begin[b] = at;
 #pragma unroll
-  for (int j = 0; j < kPer; ++j) {
-    int slot = at;
     for (int w = 0; w < kGroupWaves; ++w) {
-      const int c = counts[w][threadIdx.x * kPer + j];
-      counts[w][threadIdx.x * kPer + j] = slot;
-      slot += c;
+      counts[w][b] = at;
+      at += count[w];
     }
-    at += mine[j];
+    if (b == owners - 1) begin[owners] = at;
   }
-  if (me == mask && threadIdx.x == kGroupThreads - 1) *g.total = at;
   __syncthreads();
-  for (int32_t i0 = first; i0 < last; i0 += 64) {
-    const int32_t i = i0 + lane;
-    const uint64_t k = i < last ? (uint64_t)(tokens[i] - 1) : ~uint64_t(0);
-    uint64_t left = __ballot(k < (uint64_t)vocab && (int64_t)k != padding - 1 && (k & mask) == me);
-    const int r = (int)(k >> shift);
-    while (left) {        // the lanes that hold one token take its next slots, in order
+#pragma unroll
+  for (int u = 0; u < kPer; ++u) {
+    const uint32_t token = (uint32_t)k[u] - 1;
+    if (valid[u]) to.entry[(int64_t)blockIdx.x * kTile + counts[wave][token & mask] + rank[u]] = int2{first + u * 64, (int)token};
+  }
+}
+
+template <bool SPLIT>
+__global__ __launch_bounds__(kGroupThreads) void group_kernel(Grouping g, Split split, const int64_t* __restrict__ tokens, int32_t n, uint32_t vocab,
+                                                              uint32_t padding, int shift) {
+  __shared__ int counts[kGroupWaves][kOwnTokens];
+  __shared__ int2 found[kGroupWaves][kFound];
+  __shared__ int waveTotal[kGroupWaves], before[kGroupWaves];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const uint64_t below = (uint64_t(1) << lane) - 1;
+  const uint32_t mask = (1u << shift) - 1, me = blockIdx.x;
+  const int owned = (int)((vocab - 1 - me) >> shift) + 1;            // me < vocab
+  for (int r = lane; r < owned; r += 64) counts[wave][r] = 0;        // (each wave its own)
+  int lower = 0, mine = 0;
+  // The owner's positions, in order: f(position, token, whether it is the owner's). A wave takes a run of positions, or of tiles.
+  auto sweep = [&](const auto& f) {
+    if constexpr (SPLIT) {
+      const int tiles = (n + kTile - 1) / kTile, run = (tiles + kGroupWaves - 1) / kGroupWaves;
+      const int last = min(tiles, (wave + 1) * run);
+      for (int t = wave * run; t < last; ++t) {
+        const int32_t* begin = split.begin + (int64_t)t * (mask + 2) + me;
+        const int2* entry = split.entry + (int64_t)t * kTile;
+        const int from = begin[0], to = begin[1];
+        for (int j = from; j < to; j += 64) {
+          const int2 e = entry[min(j + lane, to - 1)];
+          f(e.x, (uint32_t)e.y, j + lane < to);
+        }
+      }
+    } else {
+      const int32_t run = ((n + kGroupWaves - 1) / kGroupWaves + 63) & ~63;
+      const int32_t first = min(n, wave * run), last = min(n, first + run);
+      each_token(tokens, first, last, vocab, padding, [&](int32_t i, uint32_t token, bool valid) {
+        const uint32_t owner = valid ? token & mask : ~0u;
+        lower += owner < me;
+        f(i, token, owner == me);
+      });
+    }
+  };
+  if constexpr (SPLIT) {       // a tile's share begins behind the owners before this one
+    const int tiles = (n + kTile - 1) / kTile;
+    for (int t = threadIdx.x; t < tiles; t += kGroupThreads) lower += split.begin[(int64_t)t * (mask + 2) + me];
+  }
+  sweep([&](int32_t i, uint32_t token, bool own) {
+    const uint64_t all = __ballot(own);
+    if (all) {
+      if (own) {
+        atomicAdd(&counts[wave][token >> shift], 1);      // whole numbers: any order gives the same
+        const int to = mine + __popcll(all & below);
+        if (to < kFound) found[wave][to] = int2{i, (int)(token >> shift)};
+      }
+      mine += __popcll(all);
+    }
+  });
+  lower = wave_sum(lower);
+  if (lane == 0) before[wave] = lower;
+  __syncthreads();
+  int start = 0;
+#pragma unroll
+  for (int w = 0; w < kGroupWaves; ++w) start += before[w];
+  // the slots of each wave's occurrences of each token: tokens in order, a thread each, each wave's after those of the ones before it
+  const int r = threadIdx.x;
+  int count[kGroupWaves], sum = 0;
+  if (r < owned) {
+#pragma unroll
+    for (int w = 0; w < kGroupWaves; ++w) {
+      count[w] = counts[w][r];
+      sum += count[w];
+    }
+    g.used[me + ((uint32_t)r << shift)] = sum;
+  }
+  int upto = sum;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int o = __shfl_up(upto, d);
+    if (lane >= d) upto += o;
+  }
+  if (lane == 63) waveTotal[wave] = upto;
+  __syncthreads();
+  int slot = start + upto - sum;
+  for (int w = 0; w < wave; ++w) slot += waveTotal[w];
+  if (r < owned) {
+#pragma unroll
+    for (int w = 0; w < kGroupWaves; ++w) {
+      counts[w][r] = slot;
+      slot += count[w];
+    }
+  }
+  if (me == mask && threadIdx.x == kGroupThreads - 1) *g.total = slot;
+  __syncthreads();
+  // up to 64 occurrences, in order: the lanes that hold one token take its next slots
+  auto place = [&](int32_t position, int which, bool own) {
+    uint64_t left = __ballot(own);
+    while (left) {
       const int leader = __ffsll((unsigned long long)left) - 1;
-      const int which = __shfl(r, leader);
-      const bool same = ((left >> lane) & 1) && r == which;
+      const int token = __shfl(which, leader);
+      const bool same = ((left >> lane) & 1) && which == token;
       const uint64_t peers = __ballot(same);
-      const int slot = counts[wave][which];
+      const int at = counts[wave][token];
       if (same) {
-        const int to = slot + __popcll(peers & ((uint64_t(1) << lane) - 1));
-        g.position[to] = i;
-        g.token[to] = (int32_t)k;
+        const int to = at + __popcll(peers & below);
+        g.position[to] = position;
+        g.token[to] = (int32_t)(me + ((uint32_t)token << shift));
       }
       __builtin_amdgcn_wave_barrier();
-      if (lane == leader) counts[wave][which] = slot + __popcll(peers);
+      if (lane == leader) counts[wave][token] = at + __popcll(peers);
       __builtin_amdgcn_wave_barrier();
       left &= ~peers;
     }
+  };
+  if (mine <= kFound) {
+    for (int i = lane; i - lane < mine; i += 64) {
+      const int2 f = found[wave][min(i, kFound - 1)];
+      place(f.x, f.y, i < mine);
+    }
+  } else {      // a common token's owner: its positions again
+    sweep([&](int32_t i, uint32_t token, bool own) { place(i, (int)(token >> shift), own); });
   }
 }
 
 struct GradArgs {
   Grouping g;
-  float* partial;        // per chunk: of the run that began before it, of the run that goes on behind it
+  float* partial;        // two rows per chunk: of the run that began before it, of the run that goes on behind it
   int64_t outRowStride;  // of the output's gradient (elements)
   int64_t gradStride;    // of the table's gradient
-  int32_t dim, chunk;    // slots a chunk
+  int32_t dim, partialStride, chunk;    // chunk: its slots
   int32_t lanes;         // that share a row
   int32_t chunks;
   float factor;
   bool add;
 };
 
+// The sums of V columns into the table's gradient, but for the first `skip` of them (another lane's).
 template <typename T, int V>
-__device__ __forceinline__ void finish_row(T* grad, const float (&acc)[V], float factor, bool add) {
+__device__ __forceinline__ void finish_row(T* grad, const float (&acc)[V], float factor, bool add, int skip, int end = V) {
   using P = Pack<T, V>;
-  P r;
-  if (add) {
-    const P old = load_pack_unaligned<false, P>(grad);
+  if (skip == 0 && end >= V) {
+    P r;
+    if (add) {
+      const P old = load_pack_unaligned<false, P>(grad);
 #pragma unroll
-    for (int e = 0; e < V; ++e) r.v[e] = rounded<T>(Cvt<T>::up(old.v[e]) + acc[e] * factor);
+      for (int e = 0; e < V; ++e) r.v[e] = rounded<T>(Cvt<T>::up(old.v[e]) + acc[e] * factor);
+    } else {
+#pragma unroll
+      for (int e = 0; e < V; ++e) r.v[e] = rounded<T>(acc[e] * factor);
+    }
+    store_pack_unaligned<false>(grad, r);
   } else {
 #pragma unroll
-    for (int e = 0; e < V; ++e) r.v[e] = rounded<T>(acc[e] * factor);
+    for (int e = 0; e < V; ++e)
+      if (e >= skip && e < end) grad[e] = rounded<T>((add ? Cvt<T>::up(grad[e]) : 0.f) + acc[e] * factor);
   }
-  store_pack_unaligned<false>(grad, r);
+}
+template <int V>
+__device__ __forceinline__ void write_partial(float* to, const float (&acc)[V]) {
+  if constexpr (V % 4 == 0) {
+#pragma unroll
+    for (int e = 0; e < V; e += 4) store_pack_unaligned<false>(to + e, Pack<float, 4>{{acc[e], acc[e + 1], acc[e + 2], acc[e + 3]}});
+  } else {
+#pragma unroll
+    for (int e = 0; e < V; ++e) to[e] = acc[e];
+  }
 }
 
-// V columns a lane (a row's last lane may be moved back when the gradient is written whole; added to, each column has one owner, so the
-// odd rest is left to lanes of one column: blockIdx.y counts slabs of packs, then of single columns).
+// V columns a lane; a row's last lane is moved back into the row and leaves the columns that it shares to the lane before it.
 template <typename T, int V, int U>
-__global__ __launch_bounds__(kBlock) void sum_kernel(GradArgs a, const T* __restrict__ out, T* __restrict__ grad, int32_t firstColumn,
-                                                     int32_t columns, int64_t vocab, int32_t chunkBlocks) {
+__global__ __launch_bounds__(kBlock) void sum_kernel(GradArgs a, const T* __restrict__ out, T* __restrict__ grad, int64_t vocab,
+                                                     int32_t chunkBlocks) {
   using P = Pack<T, V>;
   const int sub = threadIdx.x / a.lanes, lane = threadIdx.x % a.lanes, subs = blockDim.x / a.lanes;
-  const int32_t c0 = firstColumn + ((int32_t)blockIdx.y * a.lanes + lane) * V;
-  if (c0 >= firstColumn + columns) return;
+  const int32_t column = ((int32_t)blockIdx.y * a.lanes + lane) * V;
+  if (column >= a.dim) return;
+  const int32_t c0 = min(column, a.dim - V);
+  const int skip = column - c0;
   if ((int32_t)blockIdx.x >= chunkBlocks) {     // rows of tokens that do not occur
     P zero;
 #pragma unroll
@@ -288,7 +445,7 @@ __global__ __launch_bounds__(kBlock) void sum_kernel(GradArgs a, const T* __rest
   for (int e = 0; e < V; ++e) acc[e] = 0.f;
   int32_t token = a.g.token[s0];
   bool here = token != previous;       // the run began in this chunk
-  float* part = a.partial + (int64_t)c * 2 * a.dim + c0;
+  float* part = a.partial + (int64_t)c * 2 * a.partialStride + c0;
   for (int32_t s = s0; s < s1; s += U) {
     int32_t at[U], tok[U];
     P v[U];
@@ -304,12 +461,8 @@ __global__ __launch_bounds__(kBlock) void sum_kernel(GradArgs a, const T* __rest
     for (int u = 0; u < U; ++u) {
       if (s + u < s1) {
         if (tok[u] != token) {
-          if (here) {
-            finish_row<T, V>(grad + (int64_t)token * a.gradStride + c0, acc, a.factor, a.add);
-          } else {
-#pragma unroll
-            for (int e = 0; e < V; ++e) part[e] = acc[e];
-          }
+          if (here) finish_row<T, V>(grad + (int64_t)token * a.gradStride + c0, acc, a.factor, a.add, skip);
+          else write_partial(part, acc);
           token = tok[u];
           here = true;
 #pragma unroll
@@ -320,33 +473,171 @@ __global__ __launch_bounds__(kBlock) void sum_kernel(GradArgs a, const T* __rest
       }
     }
   }
-  if (here && token != next) {
-    finish_row<T, V>(grad + (int64_t)token * a.gradStride + c0, acc, a.factor, a.add);
-  } else {
-    if (here) part += a.dim;
-#pragma unroll
-    for (int e = 0; e < V; ++e) part[e] = acc[e];
-  }
+  if (here && token != next) finish_row<T, V>(grad + (int64_t)token * a.gradStride + c0, acc, a.factor, a.add, skip);
+  else write_partial(here ? part + a.partialStride : part, acc);
 }
 
-// The token whose run begins in chunk c and goes on behind it: its partial sums, chunk by chunk.
+// The token whose run begins in chunk c and goes on behind it: its partial sums. The workgroup's waves take them in turn, four columns
+// a lane, and their sums meet in LDS.
 template <typename T>
 __global__ __launch_bounds__(kBlock) void fold_kernel(GradArgs a, T* __restrict__ grad) {
+  constexpr int W = kBlock / 64, U = 4;
+  __shared__ float meet[W][4][64];
   const int32_t c = blockIdx.x, total = *a.g.total;
-  const int32_t s0 = c * a.chunk, s1 = s0 + a.chunk;
+  const int64_t s0 = (int64_t)c * a.chunk, s1 = s0 + a.chunk;
   if (s1 >= total) return;
   const int32_t token = a.g.token[s1];
   if (a.g.token[s1 - 1] != token) return;
   if (a.g.token[s0] == token && s0 > 0 && a.g.token[s0 - 1] == token) return;    // began before
-  const int32_t column = (int32_t)blockIdx.y * kBlock + threadIdx.x;
-  if (column >= a.dim) return;
-  float acc[1] = {a.partial[((int64_t)c * 2 + 1) * a.dim + column]};
-  for (int32_t d = c + 1;; ++d) {
-    acc[0] += a.partial[(int64_t)d * 2 * a.dim + column];
-    const int64_t behind = (int64_t)(d + 1) * a.chunk;
-    if (behind >= total || a.g.token[behind] != token) break;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  // the chunk that the run ends in
+  int32_t end = c + 1;
+  for (;;) {
+    const int64_t behind = ((int64_t)end + lane + 1) * a.chunk;
+    const uint64_t over = __ballot(behind >= total || a.g.token[min(behind, (int64_t)total - 1)] != token);
+    if (over) {
+      end += __ffsll((unsigned long long)over) - 1;
+      break;
+    }
+    end += 64;
   }
-  finish_row<T, 1>(grad + (int64_t)token * a.gradStride + column, acc, a.factor, a.add);
+  const int32_t column = ((int32_t)blockIdx.y * 64 + lane) * 4;
+  float acc[4] = {0.f, 0.f, 0.f, 0.f};
+  using P = Pack<float, 4>;
+  if (column < a.dim) {
+    // chunk c's second row, then the first rows of the chunks behind it
+    for (int32_t j0 = c + wave; j0 <= end; j0 += W * U) {
+      P v[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int32_t j = j0 + u * W;
+        if (j <= end) v[u] = *reinterpret_cast<const P*>(a.partial + ((int64_t)j * 2 + (j == c)) * a.partialStride + column);
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (j0 + u * W <= end) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[e] += v[u].v[e];
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < 4; ++e) meet[wave][e][lane] = acc[e];
+  __syncthreads();
+  if (wave != 0 || column >= a.dim) return;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+#pragma unroll
+    for (int w = 1; w < W; ++w) acc[e] += meet[w][e][lane];
+  }
+  finish_row<T, 4>(grad + (int64_t)token * a.gradStride + column, acc, a.factor, a.add, 0, a.dim - column);
+}
+
+// Few positions: one launch. A workgroup has one position and 64 lanes of columns; where its token has no earlier position, it lists the later
+// ones and sums their rows, its waves in turn. Every workgroup looks at all tokens, which is what bounds the number of positions.
+// Workgroups behind the positions zero the rows, kFewRows each, of tokens that do not occur.
+constexpr int kFew = 2048, kFewRows = 64;
+template <typename T, int V>
+__global__ __launch_bounds__(kBlock) void few_kernel(T* __restrict__ grad, int64_t gradStride, const int64_t* __restrict__ tokens, int32_t n,
+                                                     uint32_t vocab, uint32_t padding, const T* __restrict__ out, int64_t outStride, int32_t dim,
+                                                     float factor, bool add) {
+  using P = Pack<T, V>;
+  constexpr int W = kBlock / 64, U = 8;
+  __shared__ uint64_t same[kFew / 64];
+  __shared__ uint16_t list[kFew];
+  __shared__ float meet[W][V][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int32_t column = ((int32_t)blockIdx.y * 64 + lane) * V, c0 = min(column, dim - V);
+  const int skip = column - c0;
+  auto token_at = [&](int32_t i) -> uint32_t {      // 0-based; ~0 for one that has no row
+    const uint64_t k = (uint64_t)tokens[i];
+    const uint32_t token = (uint32_t)k - 1;
+    return (k >> 32) == 0 && token < vocab && token != padding ? token : ~0u;
+  };
+  if ((int32_t)blockIdx.x >= n) {
+    const uint32_t row0 = (uint32_t)((int32_t)blockIdx.x - n) * kFewRows;
+    if (threadIdx.x == 0) same[0] = 0;
+    __syncthreads();
+    for (int32_t i = threadIdx.x; i < n; i += kBlock) {
+      const uint32_t token = token_at(i);
+      if (token - row0 < (uint32_t)kFewRows) atomicOr((unsigned long long*)&same[0], 1ull << (token - row0));
+    }
+    __syncthreads();
+    const uint64_t used = same[0];
+    if (column >= dim) return;
+    P zero;
+#pragma unroll
+    for (int e = 0; e < V; ++e) zero.v[e] = Cvt<T>::down(0.f);
+    for (int r = wave; r < kFewRows && row0 + r < vocab; r += W)
+      if (!((used >> r) & 1)) store_pack_unaligned<false>(grad + (int64_t)(row0 + r) * gradStride + c0, zero);
+    return;
+  }
+  const uint32_t me = token_at(blockIdx.x);
+  if (me == ~0u) return;
+  // wave w looks at the words w, w + 4, ... of 64 positions, all loads in flight
+  constexpr int kWords = kFew / 64 / W;
+  const int64_t mine = (int64_t)me + 1;
+  int64_t seen[kWords];
+#pragma unroll
+  for (int j = 0; j < kWords; ++j) {
+    const int32_t i = (j * W + wave) * 64 + lane;
+    seen[j] = i < n ? tokens[i] : 0;
+  }
+#pragma unroll
+  for (int j = 0; j < kWords; ++j) {
+    const uint64_t m = __ballot(seen[j] == mine);
+    if (lane == 0) same[j * W + wave] = m;
+  }
+  __syncthreads();
+  // a lane a word: how many positions lie before it, and whether an earlier position's workgroup has the token
+  const uint64_t word = lane < kFew / 64 ? same[lane] : 0;
+  int upto = __popcll(word);
+#pragma unroll
+  for (int d = 1; d < kFew / 64; d <<= 1) {
+    const int o = __shfl_up(upto, d);
+    if (lane >= d) upto += o;
+  }
+  const int count = __shfl(upto, kFew / 64 - 1), before = upto - __popcll(word);
+  const int32_t here = blockIdx.x;
+  const uint64_t earlier = lane * 64 + 64 <= here ? word : lane * 64 < here ? word & ((uint64_t(1) << (here & 63)) - 1) : 0;
+  if (__ballot(earlier != 0)) return;      // the same for all
+#pragma unroll
+  for (int j = 0; j < kWords; ++j) {
+    const int w = j * W + wave, base = __shfl(before, w);
+    if (seen[j] == mine) list[base + __popcll(same[w] & ((uint64_t(1) << lane) - 1))] = (uint16_t)(w * 64 + lane);
+  }
+  __syncthreads();
+  float acc[V];
+#pragma unroll
+  for (int e = 0; e < V; ++e) acc[e] = 0.f;
+  if (column < dim) {
+    for (int k = wave; k < count; k += W * U) {
+      P v[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (k + u * W < count) v[u] = load_pack_unaligned<true, P>(out + (int64_t)list[k + u * W] * outStride + c0);
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (k + u * W < count) {
+#pragma unroll
+          for (int e = 0; e < V; ++e) acc[e] += Cvt<T>::up(v[u].v[e]);
+        }
+      }
+    }
+  }
+  if (count > 1) {
+#pragma unroll
+    for (int e = 0; e < V; ++e) meet[wave][e][lane] = acc[e];
+    __syncthreads();
+    if (wave != 0) return;
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+#pragma unroll
+      for (int w = 1; w < W; ++w) acc[e] += meet[w][e][lane];
+    }
+  }
+  if (wave == 0 && column < dim) finish_row<T, V>(grad + (int64_t)me * gradStride + c0, acc, factor, add, skip);
 }
 
 template <typename T>
@@ -354,44 +645,72 @@ void launch_grad(THCState* s, T* grad, int64_t vocab, int64_t gradStride, const 
                  int32_t dim, float factor, int64_t padding, bool add) {
   hipStream_t st = current_stream(s);
   constexpr int kPack = 16 / sizeof(T);
+  const int V = dim >= kPack ? kPack : 1;
+  const int32_t fewSlabs = (dim + 64 * V - 1) / (64 * V);
+  // us in three launches and in one (halves, added): 16 positions of 513 9.7, 3.9; 512 x 2048 12.4, 7.5; 1024 x 513 13.6, 9.4; 1500 x 64 12.9,
+  // 10.0; 1024 x 2048 14.5, 14.0; 1500 x 2048 15.3, 20.4; 512 x 8192 15.8, 16.9: the one launch's time goes with the workgroups times what
+  // each looks at.
+  if (n <= kFew && (int64_t)n * n * fewSlabs <= tuning("embedding.few", 3 << 20)) {
+    const dim3 grid((unsigned)(n + (add ? 0 : (vocab + kFewRows - 1) / kFewRows)), fewSlabs);
+    const uint32_t left = (uint32_t)(padding - 1);
+    if (V == 1)
+      hipLaunchKernelGGL((few_kernel<T, 1>), grid, dim3(kBlock), 0, st, grad, gradStride, tokens, n, (uint32_t)vocab, left, out, outStride, dim,
+                         factor, add);
+    else
+      hipLaunchKernelGGL((few_kernel<T, kPack>), grid, dim3(kBlock), 0, st, grad, gradStride, tokens, n, (uint32_t)vocab, left, out, outStride,
+                         dim, factor, add);
+    return;
+  }
   GradArgs a{};
   a.dim = dim;
-  a.chunk = 16;
+  a.partialStride = (dim + 3) & ~3;
   a.outRowStride = outStride;
   a.gradStride = gradStride;
   a.factor = factor;
   a.add = add;
+  // a power of two of lanes for a short row, several chunks to a workgroup; whole waves for a long one
+  const int32_t packs = (dim + V - 1) / V;
+  int lanes = 1;
+  while (lanes < 64 && lanes < packs) lanes *= 2;
+  const int slabs = (packs + kBlock - 1) / kBlock;
+  if (packs > 64) lanes = ((packs + slabs - 1) / slabs + 63) / 64 * 64;
+  a.lanes = lanes;
+  const int subs = std::max(1, kBlock / lanes);
+  // Chunks that leave four workgroups to a CU, but no more than 4096 of them: each leaves partial sums. us with chunks of 4, 8, 16, 32, 64:
+  // 1500 x 513 fp32 15.0, 15.5, 17.9, 23, 33; 8192 x 4096 half 54, 45, 40, 43, 53; 32768 x 2048 half 116, 94, 86, 84, 87; 131072 x 64 fp32
+  // 180, 139, 118, 115, 123.
+  const int64_t want = (int64_t)num_compute_units(s) * 4 * kBlock;
+  a.chunk = (int32_t)std::min<int64_t>(64, std::max<int64_t>(std::max(4, std::min(32, n / 4096)), (int64_t)n * lanes * slabs / want));
   a.chunks = (n + a.chunk - 1) / a.chunk;
   // owners: a power of two, none of which has more tokens than it has room to count
   int shift = 0;
   while ((int64_t(1) << shift) < std::min<int64_t>(vocab, 256) || ((vocab - 1) >> shift) + 1 > kOwnTokens) ++shift;
   while ((int64_t(1) << shift) > vocab) --shift;
-  const int64_t slots = (n + 3) & ~3, words = (vocab + 3) & ~int64_t(3);
-  Workspace w(s, (slots * 2 + words + 4) * 4 + (int64_t)a.chunks * 2 * dim * 4);
+  const bool apart = n > tuning("embedding.split", kSplitFrom) && (1 << shift) <= kMostSplit;
+  const int64_t tiles = apart ? (n + kTile - 1) / kTile : 0;
+  const int64_t slots = (n + 3) & ~3, words = (vocab + 3) & ~int64_t(3), partials = (int64_t)a.chunks * 2 * a.partialStride;
+  Workspace w(s, (slots * 2 + words + 4 + partials) * 4 + tiles * (kTile * 8 + ((1 << shift) + 1) * 4));
   a.g.position = reinterpret_cast<int32_t*>(w.data());
   a.g.token = a.g.position + slots;
   a.g.used = a.g.token + slots;
   a.g.total = a.g.used + words;
   a.partial = reinterpret_cast<float*>(a.g.total + 4);
-  hipLaunchKernelGGL(group_kernel, dim3(1u << shift), dim3(kGroupThreads), 0, st, a.g, tokens, n, vocab, padding, shift);
-  auto sum = [&](auto vTag, int32_t first, int32_t columns) {
-    constexpr int V = decltype(vTag)::value;
-    if (columns <= 0) return;
-    const int32_t packs = columns / V;
-    int lanes = 1;
-    while (lanes < 64 && lanes < packs) lanes *= 2;
-    if (packs > 64) lanes = std::min(kBlock, (packs + 63) / 64 * 64);
-    a.lanes = lanes;
-    const int subs = std::max(1, kBlock / lanes);
-    const int32_t chunkBlocks = (a.chunks + subs - 1) / subs;
-    const int64_t zeroBlocks = add ? 0 : (vocab + subs * 16 - 1) / (subs * 16);
-    hipLaunchKernelGGL((sum_kernel<T, V, 8>), dim3((unsigned)(chunkBlocks + zeroBlocks), (packs + lanes - 1) / lanes), dim3(subs * lanes), 0, st,
-                       a, out, grad, first, columns, vocab, chunkBlocks);
-  };
-  const int32_t whole = dim / kPack * kPack;
-  sum(std::integral_constant<int, kPack>{}, 0, whole);
-  sum(std::integral_constant<int, 1>{}, whole, dim - whole);
-  hipLaunchKernelGGL((fold_kernel<T>), dim3(a.chunks, (dim + kBlock - 1) / kBlock), dim3(kBlock), 0, st, a, grad);
+  Split split;
+  split.entry = reinterpret_cast<int2*>(a.partial + partials);
+  split.begin = reinterpret_cast<int32_t*>(split.entry + tiles * kTile);
+  const uint32_t left = (uint32_t)(padding - 1);
+  if (apart) {
+    hipLaunchKernelGGL(split_kernel, dim3((unsigned)tiles), dim3(kGroupThreads), 0, st, split, tokens, n, (uint32_t)vocab, left, shift);
+    hipLaunchKernelGGL(group_kernel<true>, dim3(1u << shift), dim3(kGroupThreads), 0, st, a.g, split, tokens, n, (uint32_t)vocab, left, shift);
+  } else {
+    hipLaunchKernelGGL(group_kernel<false>, dim3(1u << shift), dim3(kGroupThreads), 0, st, a.g, split, tokens, n, (uint32_t)vocab, left, shift);
+  }
+  const int32_t chunkBlocks = (a.chunks + subs - 1) / subs;
+  const int64_t zeroBlocks = add ? 0 : (vocab + subs * 16 - 1) / (subs * 16);
+  const dim3 grid((unsigned)(chunkBlocks + zeroBlocks), slabs), block(subs * lanes);
+  if (V == 1) hipLaunchKernelGGL((sum_kernel<T, 1, 8>), grid, block, 0, st, a, out, grad, vocab, chunkBlocks);
+  else hipLaunchKernelGGL((sum_kernel<T, kPack, 8>), grid, block, 0, st, a, out, grad, vocab, chunkBlocks);
+  hipLaunchKernelGGL((fold_kernel<T>), dim3(a.chunks, (dim + 255) / 256), dim3(kBlock), 0, st, a, grad);
 }
 
 void embedding_grad(THCState* s, DType dt, AnyTensor* grad, AnyTensor* tokens, AnyTensor* out, float factor, long padding, int accumulate) {

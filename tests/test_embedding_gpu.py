@@ -136,6 +136,39 @@ def test_gradient(thc, kind, how, vocab, dim, count, add):
     again = _tensor(thc, start)
     again.embedding_grad(_tensor(thc, tokens), _tensor(thc, out), 0.75, accumulate=add)
     assert_bit_equal(again.numpy(), got)
+    thc.set_tuning("embedding.few", 0)       # as many positions are summed
+    try:
+        again = _tensor(thc, start)
+        again.embedding_grad(_tensor(thc, tokens), _tensor(thc, out), 0.75, accumulate=add)
+    finally:
+        thc.set_tuning("embedding.few", 3 << 20)
+    _near(again.numpy(), want, mass, n, kind)
+
+
+@pytest.fixture
+def split(thc):
+    """Positions are split between their owners first, as those of many tokens are."""
+    thc.set_tuning("embedding.split", 0)
+    thc.set_tuning("embedding.few", 0)
+    yield
+    thc.set_tuning("embedding.split", 57344)
+    thc.set_tuning("embedding.few", 3 << 20)
+
+
+@pytest.mark.parametrize("how", ["text", "one", "two", "each"])
+@pytest.mark.parametrize("vocab,dim,count", [(1, 1, 1), (2, 3, 4096), (7, 5, 64), (300, 17, 1000), (5003, 64, 4097), (255, 9, 8191),
+                                             (131073, 4, 12289), (262144, 3, 9000), (524288, 2, 20000), (524289, 2, 5000), (300, 5, 70000)])
+def test_gradient_of_split_positions(thc, split, how, vocab, dim, count):
+    rng = np.random.default_rng(vocab + count)
+    tokens = _tokens(rng, how, vocab, count)
+    tokens[rng.random(count) < 0.02] = 0
+    out = rng.standard_normal((count, dim)).astype(np.float32)
+    start = _table(rng, vocab, dim, "float")
+    for add in (False, True):
+        grad = _tensor(thc, start)
+        grad.embedding_grad(_tensor(thc, tokens), _tensor(thc, out), 0.5, padding=vocab // 2, accumulate=add)
+        want, mass, n = _sums((vocab, dim), tokens, out, 0.5, vocab // 2, start.astype(np.float64) if add else None)
+        _near(grad.numpy(), want, mass, n, "float")
 
 
 @pytest.mark.parametrize("vocab,count", [(262143, 5000), (300001, 4099), (1 << 20, 1000)])
@@ -158,6 +191,18 @@ def test_gradient_of_many_tokens(thc, count):
     grad.embedding_grad(_tensor(thc, tokens), _tensor(thc, out), 0.01, padding=2)
     want, mass, n = _sums((2000, 40), tokens, out, 0.01, 2)
     _near(grad.numpy(), want, mass, n, "half")
+
+
+@pytest.mark.parametrize("how", ["one", "two"])
+def test_gradient_of_one_common_token(thc, how):
+    """Its positions are more than a workgroup keeps between its sweeps, its run crosses hundreds of chunks."""
+    rng = np.random.default_rng(13)
+    tokens = _tokens(rng, how, 3000, 30011)
+    out = rng.standard_normal((30011, 9)).astype(np.float32)
+    grad = _tensor(thc, np.ones((3000, 9), np.float32))
+    grad.embedding_grad(_tensor(thc, tokens), _tensor(thc, out))
+    want, mass, n = _sums((3000, 9), tokens, out, 1, 0)
+    _near(grad.numpy(), want, mass, n, "float")
 
 
 @pytest.mark.parametrize("kind", ["float", "half"])
