@@ -29,11 +29,25 @@ struct Hyper {
   float beta1, oneMinusBeta1, beta2, oneMinusBeta2, rootScale, eps, keep, rate, gradScale;
 };
 
+// The square root of a share (0 to 1), from the reciprocal root r: with y = x r, y + (x - y y) r / 2 is the root's nearest float
+// for every float from 2^-97 on (compared with sqrtf for each of them), 0 for 0, and off by one place at most below, where shares have code
+// 0 or 1 either way. sqrtf looks after every range of its argument and takes 16 instructions, this 6, of which a step makes four: 8-bit
+// steps are bound by arithmetic.
+__device__ __forceinline__ float share_root(float x) {
+  const float r = __builtin_amdgcn_rsqf(fmaxf(x, 0x1p-126f)), y = x * r;
+  return __builtin_fmaf(__builtin_fmaf(-y, y, x), 0.5f * r, y);
+}
+// The same for a second moment, which may be infinite.
+__device__ __forceinline__ float moment_root(float v) {
+  const float y = share_root(v);
+  return v == __builtin_inff() ? v : y;
+}
+
 __device__ __forceinline__ float adamw_step(const Hyper& h, float p, float g, float& m, float& v) {
   g = g * h.gradScale;
   m = m * h.beta1 + g * h.oneMinusBeta1;
   v = v * h.beta2 + (g * g) * h.oneMinusBeta2;
-  const float root = sqrtf(v) * h.rootScale + h.eps;
+  const float root = moment_root(v) * h.rootScale + h.eps;
   return p * h.keep - (m / root) * h.rate;
 }
 
@@ -92,11 +106,9 @@ __device__ __forceinline__ void store4(T* to, const float (&from)[4], int n) {
 }
 
 // States in 32 bits: kPacks packs of each operand in flight, then the arithmetic, in place.
-template <typename T, bool MASTER, bool NT>
-__global__ __launch_bounds__(kBlock) void step_kernel(StepArgs a) {
-  const Item& t = a.item[item_of(a)];
-  const int64_t base = (int64_t)(blockIdx.x - a.firstPart[item_of(a)]) * kPart;
-  const int left = (int)min((int64_t)kPart, t.size - base);
+// FULL: the tensor does not end in this part.
+template <typename T, bool MASTER, bool NT, bool FULL>
+__device__ __forceinline__ void step_part(const Hyper& h, const Item& t, int64_t base, int left) {
   T* param = static_cast<T*>(t.param) + base;
   float* master = MASTER ? t.master + base : nullptr;
   const T* grad = static_cast<const T*>(t.grad) + base;
@@ -105,26 +117,36 @@ __global__ __launch_bounds__(kBlock) void step_kernel(StepArgs a) {
 #pragma unroll
   for (int u = 0; u < kPacks; ++u) {
     const int i = (u * kBlock + threadIdx.x) * 4;
-    if (i < left) {
-      if constexpr (MASTER) load4<true>(p[u], master + i, left - i);
-      else load4<true>(p[u], param + i, left - i);
-      load4<true>(g[u], grad + i, left - i);
-      load4<true>(m[u], mean + i, left - i);
-      load4<true>(v[u], square + i, left - i);
+    if (FULL || i < left) {
+      const int n = FULL ? 4 : left - i;
+      if constexpr (MASTER) load4<true>(p[u], master + i, n);
+      else load4<true>(p[u], param + i, n);
+      load4<true>(g[u], grad + i, n);
+      load4<true>(m[u], mean + i, n);
+      load4<true>(v[u], square + i, n);
     }
   }
 #pragma unroll
   for (int u = 0; u < kPacks; ++u) {
     const int i = (u * kBlock + threadIdx.x) * 4;
-    if (i < left) {
+    if (FULL || i < left) {
+      const int n = FULL ? 4 : left - i;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) p[u][e] = adamw_step(a.h, p[u][e], g[u][e], m[u][e], v[u][e]);
-      store4<NT>(mean + i, m[u], left - i);
-      store4<NT>(square + i, v[u], left - i);
-      if constexpr (MASTER) store4<NT>(master + i, p[u], left - i);
-      store4<NT>(param + i, p[u], left - i);
+      for (int e = 0; e < 4; ++e) p[u][e] = adamw_step(h, p[u][e], g[u][e], m[u][e], v[u][e]);
+      store4<NT>(mean + i, m[u], n);
+      store4<NT>(square + i, v[u], n);
+      if constexpr (MASTER) store4<NT>(master + i, p[u], n);
+      store4<NT>(param + i, p[u], n);
     }
   }
+}
+template <typename T, bool MASTER, bool NT>
+__global__ __launch_bounds__(kBlock) void step_kernel(StepArgs a) {
+  const int i = item_of(a);
+  const Item& t = a.item[i];
+  const int64_t base = (int64_t)(blockIdx.x - a.firstPart[i]) * kPart, left = t.size - base;
+  if (left >= kPart) step_part<T, MASTER, NT, true>(a.h, t, base, kPart);
+  else step_part<T, MASTER, NT, false>(a.h, t, base, (int)left);
 }
 
 __device__ __forceinline__ float decode_mean(int8_t c, float top) {
@@ -184,11 +206,9 @@ __device__ __forceinline__ void store4_codes(T* to, const T (&from)[4], int n) {
 }
 
 // States in 8 bits: a wave has kPacks blocks of states, 4 elements a lane of each. What is behind a tensor's end counts as zeros.
-template <typename T, bool MASTER, bool NT>
-__global__ __launch_bounds__(kBlock) void step8_kernel(StepArgs a) {
-  const Item& t = a.item[item_of(a)];
-  const int64_t base = (int64_t)(blockIdx.x - a.firstPart[item_of(a)]) * kPart;
-  const int left = (int)min((int64_t)kPart, t.size - base);
+// FULL: the tensor does not end in this part.
+template <typename T, bool MASTER, bool NT, bool FULL>
+__device__ __forceinline__ void step8_part(const Hyper& h, const Item& t, int64_t base, int left) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   T* param = static_cast<T*>(t.param) + base;
   float* master = MASTER ? t.master + base : nullptr;
@@ -202,8 +222,8 @@ __global__ __launch_bounds__(kBlock) void step8_kernel(StepArgs a) {
 #pragma unroll
   for (int u = 0; u < kPacks; ++u) {
     const int block = u * (kBlock / 64) + wave, i = block * kStateBlock + lane * 4;
-    if (block * kStateBlock < left) {      // whole waves
-      const int n = left - i;              // none for the lanes behind the end
+    if (FULL || block * kStateBlock < left) {      // whole waves
+      const int n = FULL ? 4 : left - i;           // none for the lanes behind the end
       topMean[u] = meanScale[block];
       topSquare[u] = squareScale[block];
       if constexpr (MASTER) load4<true>(p[u], master + i, n);
@@ -216,16 +236,16 @@ __global__ __launch_bounds__(kBlock) void step8_kernel(StepArgs a) {
 #pragma unroll
   for (int u = 0; u < kPacks; ++u) {
     const int block = u * (kBlock / 64) + wave, i = block * kStateBlock + lane * 4;
-    if (block * kStateBlock < left) {
-      const int n = left - i;
+    if (FULL || block * kStateBlock < left) {
+      const int n = FULL ? 4 : left - i;
       float m[4], v[4];
       uint32_t maxMean = 0, maxSquare = 0;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         m[e] = decode_mean(codeMean[u][e], topMean[u]);
         v[e] = decode_square(codeSquare[u][e], topSquare[u]);
-        p[u][e] = adamw_step(a.h, p[u][e], g[u][e], m[e], v[e]);
-        if (e < n) {          // (zeros behind the end may meet a factor that is not finite)
+        p[u][e] = adamw_step(h, p[u][e], g[u][e], m[e], v[e]);
+        if (FULL || e < n) {          // (zeros behind the end may meet a factor that is not finite)
           maxMean = max(maxMean, __float_as_uint(fabsf(m[e])));
           maxSquare = max(maxSquare, __float_as_uint(v[e]));
         }
@@ -236,10 +256,10 @@ __global__ __launch_bounds__(kBlock) void step8_kernel(StepArgs a) {
       const float inverseMean = inverse_top(newMean), inverseSquare = inverse_top(newSquare);
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const float c = rintf(sqrtf(fabsf(m[e]) * inverseMean) * 127.f);
+        const float c = rintf(share_root(fabsf(m[e]) * inverseMean) * 127.f);
         codeMean[u][e] = (int8_t)(int)(m[e] < 0.f ? -c : c);
         const float share = v[e] * inverseSquare;
-        const float d = rintf(sqrtf(sqrtf(share)) * 255.f);
+        const float d = rintf(share_root(share_root(share)) * 255.f);
         codeSquare[u][e] = (uint8_t)(int)(share > 0.f ? fmaxf(d, 1.f) : d);
       }
       store4_codes<NT>(mean + i, codeMean[u], n);
@@ -250,6 +270,14 @@ __global__ __launch_bounds__(kBlock) void step8_kernel(StepArgs a) {
       }
     }
   }
+}
+template <typename T, bool MASTER, bool NT>
+__global__ __launch_bounds__(kBlock) void step8_kernel(StepArgs a) {
+  const int i = item_of(a);
+  const Item& t = a.item[i];
+  const int64_t base = (int64_t)(blockIdx.x - a.firstPart[i]) * kPart, left = t.size - base;
+  if (left >= kPart) step8_part<T, MASTER, NT, true>(a.h, t, base, kPart);
+  else step8_part<T, MASTER, NT, false>(a.h, t, base, (int)left);
 }
 
 // The moments that 8-bit states stand for: the items' codes and scales, into `param` and `master`.
@@ -397,7 +425,11 @@ void adamw(THCState* s, DType dt, int count, const Lists& l, double lr, double b
   h.gradScale = (float)gradScale;
   int64_t elements = 0;
   for (int i = 0; i < count; ++i) elements += tensor_numel(l.param[i]);
-  const bool nt = streaming_store("adamw.nt", elements * (int64_t)(eight ? 6 : 12));
+  // Streaming stores where the whole call's operands do not stay in the 256 MiB memory-side cache until the next step. us, plain and
+  // streaming: 4.4 M floats (70 MB) 25.4, 26.6; 17.7 M halves with float copies 100, 95, with 8-bit states (177 MB) 112, 118; 161 M floats
+  // with 8-bit states 891, 868.
+  const int64_t touched = elements * (2 * (int64_t)dtype_size(dt) + (l.master ? 4 : 0) + (eight ? 2 : 8));
+  const bool nt = tuning("adamw.nt", touched >= (int64_t(256) << 20)) != 0;
   hipStream_t st = current_stream(s);
   auto launch = [&](const StepArgs& a, dim3 grid) {
     auto go = [&](auto type, auto master, auto stream) {

@@ -16,8 +16,10 @@ namespace {
 // ------------------------------------------------------------------ lookup --
 // One 16-byte pack of the output per item, U items in flight per lane; items are counted over (row, pack), so that short rows share a
 // workgroup. Packs lie at element-aligned addresses (rows of any length), a row's last one is moved back into the row and
-// repeats elements of the one before it: the same values are written twice, nothing needs a tail.
-template <typename T, int V, int U, bool NT, typename I>
+// repeats elements of the one before it: the same values are written twice, nothing needs a tail. Stores are streaming ones at every
+// size (us with plain ones and so: 2048 rows of 2048 halves 4.9, 4.8, 8192 x 1024 6.5, 5.5, 65536 x 1024 43.5, 29.0); table rows may
+// come again and are read plainly.
+template <typename T, int V, int U, typename I>
 __global__ __launch_bounds__(kBlock) void lookup_kernel(T* __restrict__ out, const T* __restrict__ table, const int64_t* __restrict__ tokens,
                                                         int64_t vocab, int64_t tableStride, int32_t dim, I items, Divisor<I> packs, float factor) {
   using P = Pack<T, V>;
@@ -48,7 +50,7 @@ __global__ __launch_bounds__(kBlock) void lookup_kernel(T* __restrict__ out, con
     if (base + (I)u * kBlock < items) {
 #pragma unroll
       for (int e = 0; e < V; ++e) v[u].v[e] = rounded<T>(Cvt<T>::up(v[u].v[e]) * factor);
-      store_pack_unaligned<NT>(out + (int64_t)row[u] * dim + at[u], v[u]);
+      store_pack_unaligned<true>(out + (int64_t)row[u] * dim + at[u], v[u]);
     }
   }
 }
@@ -64,12 +66,8 @@ void launch_lookup(THCState* s, T* out, const T* table, const int64_t* tokens, i
     Divisor<I> d;
     d.set((uint64_t)packs);
     const dim3 grid((unsigned)((items + kBlock * U - 1) / (kBlock * U)));
-    if (streaming_store("embedding.nt", count * dim * (int64_t)sizeof(T)))
-      hipLaunchKernelGGL((lookup_kernel<T, V, U, true, I>), grid, dim3(kBlock), 0, st, out, table, tokens, vocab, tableStride, (int32_t)dim,
-                         (I)items, d, factor);
-    else
-      hipLaunchKernelGGL((lookup_kernel<T, V, U, false, I>), grid, dim3(kBlock), 0, st, out, table, tokens, vocab, tableStride, (int32_t)dim,
-                         (I)items, d, factor);
+    hipLaunchKernelGGL((lookup_kernel<T, V, U, I>), grid, dim3(kBlock), 0, st, out, table, tokens, vocab, tableStride, (int32_t)dim, (I)items, d,
+                       factor);
   };
   constexpr int kPack = 16 / sizeof(T);
   auto width = [&](auto uTag, auto idxTag) {

@@ -8,24 +8,28 @@
 // A row is read once. Maxima, sums and the loss are in float; the gradient is rounded once. A row of weight 0 is not read: its loss,
 // log-probability and gradient are 0, whatever its logits, token and other inputs hold. A token outside 1..V makes its row NaN.
 #include <algorithm>
+#include <type_traits>
 
 #include "training.hpp"
 
 namespace thc {
 namespace {
 
-constexpr float kLog2e = 1.44269504088896340736f;
+constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
 __device__ __forceinline__ float minus_infinity() { return -__builtin_inff(); }
 
-// A running maximum and the sum of exp(x - max) below it. The empty one has -inf and 0; a part all of whose values are -inf too.
+// A running maximum, times log2(e) and rounded, and the sum of 2^(x log2(e) - m) below it. What the rounding moved cancels: the chosen
+// logit and the gradient's exponentials are measured from the same m. x log2(e) - m is one operation and rounds once, near 0 for the
+// values that count. The empty part has -inf and 0; so has one all of whose values are -inf.
 struct Soft {
   float m, s;
 };
-__device__ __forceinline__ float exp_below(float x, float m) { return __builtin_amdgcn_exp2f((x - m) * kLog2e); }
+__device__ __forceinline__ float below(float x, float m) { return __builtin_fmaf(x, kLog2e, -m); }
+__device__ __forceinline__ float exp_below(float x, float m) { return __builtin_amdgcn_exp2f(below(x, m)); }
+__device__ __forceinline__ float finite_or_zero(float m) { return m == minus_infinity() ? 0.f : m; }
 __device__ __forceinline__ Soft join(Soft a, Soft b) {
-  const float m = fmaxf(a.m, b.m);
-  const float safe = m == minus_infinity() ? 0.f : m;
-  return Soft{m, a.s * exp_below(a.m, safe) + b.s * exp_below(b.m, safe)};
+  const float m = fmaxf(a.m, b.m), safe = finite_or_zero(m);
+  return Soft{m, a.s * __builtin_amdgcn_exp2f(a.m - safe) + b.s * __builtin_amdgcn_exp2f(b.m - safe)};
 }
 __device__ __forceinline__ Soft wave_join(Soft a) {
 #pragma unroll
@@ -35,42 +39,42 @@ __device__ __forceinline__ Soft wave_join(Soft a) {
 template <int W>
 __device__ __forceinline__ Soft block_join(Soft a, Soft* lds) {
   a = wave_join(a);
-  if constexpr (W == 1) return a;
-  if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = a;
-  __syncthreads();
-  a = lds[0];
+  if constexpr (W > 1) {
+    const int lane = threadIdx.x & 63;
+    if (lane == 0) lds[threadIdx.x >> 6] = a;
+    lds_barrier();
+    a = lds[lane & (W - 1)];
 #pragma unroll
-  for (int w = 1; w < W; ++w) a = join(a, lds[w]);
+    for (int d = W / 2; d >= 1; d >>= 1) a = join(a, Soft{__shfl_xor(a.m, d), __shfl_xor(a.s, d)});
+  }
   return a;
 }
 
-// The row's aligned 16-byte packs: the first begins at or below the row's first element, so it and the last may hold neighbours'
-// elements, which count as -inf. Every pack holds an element of the row, so no access leaves a 16-byte unit the row owns part of.
+// A row as its aligned 16-byte packs and the elements before and behind them, of which lanes 0 to 15 of the first wave hold one each.
 template <typename T>
-struct RowPacks {
+struct RowParts {
   static constexpr int V = 16 / sizeof(T);
   using P = Pack<T, V>;
+  const T* row;
   const P* first;
-  int32_t before, length, packs;
-  __device__ __forceinline__ RowPacks(const T* row, int32_t n) {
-    before = (int32_t)((reinterpret_cast<uintptr_t>(row) / sizeof(T)) & (V - 1));
-    first = reinterpret_cast<const P*>(row - before);
-    length = n;
-    packs = (before + n + V - 1) / V;
+  int32_t head, packs, tail;
+  int32_t lane0;      // the pack that thread 0 has first: it lies where a 128-byte line begins, so that no two waves write into one line
+  __device__ __forceinline__ RowParts(const T* x, int32_t n) {
+    row = x;
+    head = min(n, (int32_t)((-reinterpret_cast<uintptr_t>(x) / sizeof(T)) & (V - 1)));
+    first = reinterpret_cast<const P*>(x + head);
+    packs = (n - head) / V;
+    tail = n - head - packs * V;
+    lane0 = -(int32_t)((reinterpret_cast<uintptr_t>(first) / 16) & 7);
   }
-  __device__ __forceinline__ bool whole(int32_t k) const { return k * V >= before && (k + 1) * V <= before + length; }
-  // Pack k with -inf in the place of what is not the row's.
-  __device__ __forceinline__ P load(int32_t k) const {
-    P p = load_pack<true>(first + k);
-    if (!whole(k)) {
-#pragma unroll
-      for (int e = 0; e < V; ++e) {
-        const int32_t i = k * V + e - before;
-        if (i < 0 || i >= length) p.v[e] = Cvt<T>::down(minus_infinity());
-      }
-    }
-    return p;
+  __device__ __forceinline__ bool has(int32_t k) const { return (uint32_t)k < (uint32_t)packs; }
+  // The element that this lane holds besides its packs, or -1.
+  __device__ __forceinline__ int32_t edge() const {
+    const int32_t t = threadIdx.x;
+    return t < V ? (t < head ? t : -1) : t < 2 * V && t - V < tail ? head + packs * V + t - V : -1;
   }
+  __device__ __forceinline__ P load(int32_t k) const { return load_pack<true>(first + k); }
+  __device__ __forceinline__ float load_edge(int32_t i) const { return i >= 0 ? Cvt<T>::up(row[i]) : minus_infinity(); }
 };
 
 struct RowOffsets {
@@ -91,90 +95,339 @@ struct PolicyArgs {
   float low, high, kl, gradScale, evenWeight;
 };
 
-__device__ __forceinline__ float weight_of(const PolicyArgs& a, uint32_t row) { return a.weight ? a.weight[row] : a.evenWeight; }
+// A position's numbers, asked for before its row is.
+struct Position {
+  int64_t token;      // 0-based
+  float weight, old, advantage, reference;
+};
+__device__ __forceinline__ Position position_of(const PolicyArgs& a, uint32_t row) {
+  Position p{};
+  p.token = a.token[row] - 1;
+  p.weight = a.weight ? a.weight[row] : a.evenWeight;
+  if (a.loss) {
+    p.old = a.old[row];
+    p.advantage = a.advantage[row];
+    if (a.reference) p.reference = a.reference[row];
+  }
+  return p;
+}
 
 // Loss and log-probability of a row, by its first lane; returns the slope f w dl/dlp.
-__device__ __forceinline__ float policy_row(const PolicyArgs& a, uint32_t row, float chosen, Soft soft, float w, bool write) {
-  const float lp = (chosen - soft.m) - logf(soft.s);
+__device__ __forceinline__ float policy_row(const PolicyArgs& a, uint32_t row, const Position& p, float chosen, Soft soft, bool write) {
+  const float lp = (below(chosen, soft.m) - log2f(soft.s)) * kLn2;
   if (!a.loss) {
     if (write) a.logProb[row] = lp;
     return 0.f;
   }
-  const float advantage = a.advantage[row];
-  const float ratio = expf(lp - a.old[row]);
-  const float free = ratio * advantage, held = fminf(fmaxf(ratio, a.low), a.high) * advantage;
+  const float ratio = expf(lp - p.old);
+  const float free = ratio * p.advantage, held = fminf(fmaxf(ratio, a.low), a.high) * p.advantage;
   // (neither below nor above: a NaN, which fmin would drop)
   float loss = free <= held ? -free : free > held ? -held : free + held;
   float slope = free <= held ? -free : free > held ? 0.f : free + held;
   if (a.reference) {
-    const float away = a.reference[row] - lp, e = expf(away);
+    const float away = p.reference - lp, e = expf(away);
     loss += a.kl * (e - away - 1.f);
     slope += a.kl * (1.f - e);
   }
   if (write) {
-    a.loss[row] = w * loss;
+    a.loss[row] = p.weight * loss;
     a.logProb[row] = lp;
   }
-  return w * slope * a.gradScale;
+  return p.weight * slope * a.gradScale;
 }
 
-// One workgroup a row; the row is read twice, the second time for the gradient.
+template <typename T>
+__device__ __forceinline__ float top_of(const Pack<T, 16 / sizeof(T)>& p) {
+  if constexpr (sizeof(T) == 2) {
+    typedef _Float16 Two __attribute__((ext_vector_type(2)));
+    Two h[4];
+    __builtin_memcpy(h, &p, 16);
+    const Two m = __builtin_elementwise_max(__builtin_elementwise_max(h[0], h[1]), __builtin_elementwise_max(h[2], h[3]));
+    return fmaxf((float)m[0], (float)m[1]);
+  } else {
+    return fmaxf(fmaxf(p.v[0], p.v[1]), fmaxf(p.v[2], p.v[3]));
+  }
+}
+template <typename T>
+__device__ __forceinline__ float sum_below(const Pack<T, 16 / sizeof(T)>& p, float m) {
+  constexpr int V = 16 / sizeof(T);
+  float s[V];
+#pragma unroll
+  for (int e = 0; e < V; ++e) s[e] = exp_below(Cvt<T>::up(p.v[e]), m);
+#pragma unroll
+  for (int w = V / 2; w >= 1; w /= 2) {
+#pragma unroll
+    for (int e = 0; e < w; ++e) s[e] += s[e + w];
+  }
+  return s[0];
+}
+
+// What a row's gradient is made from: c 2^(x log2(e) - m), and `slope` more at the token, element `hit` of the row.
+struct RowSlope {
+  float c, slope, m;
+  int32_t hit;
+};
+// A pack of the gradient; its first element is element i0 of the row. The stores are streaming ones at every size: with plain ones 4096 x
+// 100001 halves take 305 us instead of 285, 512 x 32000 16.5 instead of 13.9, 1000 x 8000 11.6 instead of 9.2.
+template <typename T>
+__device__ __forceinline__ void store_gradient(T* out, int32_t i0, const Pack<T, 16 / sizeof(T)>& p, const RowSlope& r) {
+  constexpr int V = 16 / sizeof(T);
+  float g[V];
+#pragma unroll
+  for (int e = 0; e < V; ++e) g[e] = r.c * exp_below(Cvt<T>::up(p.v[e]), r.m);
+  if ((uint32_t)(r.hit - i0) < (uint32_t)V) {
+#pragma unroll
+    for (int e = 0; e < V; ++e)
+      if (i0 + e == r.hit) g[e] += r.slope;
+  }
+  Pack<T, V> q;
+  if constexpr (sizeof(T) == 2) {
+    typedef _Float16 Half2 __attribute__((ext_vector_type(2)));
+    typedef float Float2 __attribute__((ext_vector_type(2)));
+    Half2 h[V / 2];
+#pragma unroll
+    for (int e = 0; e < V / 2; ++e) h[e] = __builtin_convertvector((Float2{g[2 * e], g[2 * e + 1]}), Half2);
+    __builtin_memcpy(&q, h, 16);
+  } else {
+#pragma unroll
+    for (int e = 0; e < V; ++e) q.v[e] = g[e];
+  }
+  store_pack_unaligned<true>(out + i0, q);
+}
+template <typename T>
+__device__ __forceinline__ void store_edge(T* out, int32_t i, float x, const RowSlope& r) {
+  if (i >= 0) out[i] = rounded<T>(r.c * exp_below(x, r.m) + (i == r.hit ? r.slope : 0.f));
+}
+template <typename T, int W>
+__device__ __forceinline__ void store_zeros(T* out, int32_t n) {
+  constexpr int V = 16 / sizeof(T);
+  Pack<T, V> zero;
+#pragma unroll
+  for (int e = 0; e < V; ++e) zero.v[e] = Cvt<T>::down(0.f);
+  for (int32_t i = threadIdx.x * V; i < n; i += W * 64 * V) {
+    if (i + V <= n) store_pack_unaligned<false>(out + i, zero);
+    else
+      for (int32_t j = i; j < n; ++j) out[j] = Cvt<T>::down(0.f);
+  }
+}
+
+// A row without a weight: its outputs are 0. (A NaN weight is one.)
 template <typename T, int W, bool GRAD>
-__global__ __launch_bounds__(W * 64) void row_kernel(PolicyArgs a, const T* logits, RowOffsets lo, T* grad, RowOffsets go,
-                                                     int32_t vocab) {
-  constexpr int V = RowPacks<T>::V;
+__device__ __forceinline__ void skip_row(const PolicyArgs& a, uint32_t row, T* out, int32_t vocab) {
+  if (threadIdx.x == 0) {
+    if (a.loss) a.loss[row] = 0.f;
+    a.logProb[row] = 0.f;
+  }
+  if constexpr (GRAD) store_zeros<T, W>(out, vocab);
+}
+template <typename T>
+__device__ __forceinline__ float chosen_of(const T* x, int64_t token, int32_t vocab) {
+  return (uint64_t)token < (uint64_t)vocab ? Cvt<T>::up(x[token]) : __builtin_nanf("");
+}
+
+// Takes the packs at k, k + step, ... (U of them; those behind `end` are not there) into a running maximum and sum.
+template <typename T, int U>
+__device__ __forceinline__ Soft take(Soft soft, const Pack<T, 16 / sizeof(T)>* v, int32_t k, int32_t step, int32_t end) {
+  float m = soft.m;
+#pragma unroll
+  for (int u = 0; u < U; ++u)
+    if ((uint32_t)(k + u * step) < (uint32_t)end) m = fmaxf(m, top_of<T>(v[u]) * kLog2e);
+  const float safe = finite_or_zero(m);
+  float s = soft.s * __builtin_amdgcn_exp2f(soft.m - safe);
+#pragma unroll
+  for (int u = 0; u < U; ++u)
+    if ((uint32_t)(k + u * step) < (uint32_t)end) s += sum_below<T>(v[u], safe);
+  return Soft{m, s};
+}
+__device__ __forceinline__ Soft take_edge(float x) {
+  const float m = x * kLog2e;
+  return Soft{m, m == minus_infinity() ? 0.f : exp_below(x, m)};
+}
+
+// Direct load of one pack a lane into LDS: lane i's 16 bytes go to `to` + 16 i of the wave's part.
+__device__ __forceinline__ void load_to_lds(const void* from, void* to) {
+  typedef const __attribute__((address_space(1))) void* Global;
+  typedef __attribute__((address_space(3))) void* Local;
+  __builtin_amdgcn_global_load_lds((Global)from, (Local)to, 16, 0, /*nt*/ 2);
+}
+
+// A workgroup has a row, a lane R packs of it in registers and L in LDS from the first read to the gradient: the row crosses the memory
+// once each way. What is longer than that is read again for the gradient (REST). E: waves a SIMD that the registers leave room for.
+template <typename T, int W, int R, int L, int E, bool REST>
+__global__ __launch_bounds__(W * 64) __attribute__((amdgpu_waves_per_eu(E, E))) void held_row_kernel(PolicyArgs a, const T* logits, RowOffsets lo, T* grad,
+                                                                                               RowOffsets go, int32_t vocab) {
+  constexpr int U = R < 4 ? R : 4, kStep = W * 64, V = 16 / sizeof(T);
+  using P = Pack<T, V>;
+  __shared__ Soft lds[W];
+  extern __shared__ __attribute__((aligned(16))) char room[];      // L packs a lane
+  P(*more)[W][64] = reinterpret_cast<P(*)[W][64]>(room);
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const uint32_t row = blockIdx.x;
+  const Position at = position_of(a, row);
+  T* out = grad + go.at(row);
+  if (at.weight == 0.f) {
+    skip_row<T, W, true>(a, row, out, vocab);
+    return;
+  }
+  const RowParts<T> x(logits + lo.at(row), vocab);
+  P v[R];
+#pragma unroll
+  for (int u = 0; u < R; ++u) {
+    const int32_t k = x.lane0 + (int32_t)threadIdx.x + u * kStep;
+    if (x.has(k)) v[u] = x.load(k);
+  }
+#pragma unroll
+  for (int u = 0; u < L; ++u) {
+    const int32_t k = x.lane0 + (int32_t)threadIdx.x + (R + u) * kStep;
+    if (x.has(k)) load_to_lds(x.first + k, &more[u][wave][0]);
+  }
+  const float chosen = chosen_of(x.row, at.token, vocab), edge = x.load_edge(x.edge());
+  Soft soft{minus_infinity(), 0.f};
+#pragma unroll
+  for (int u = 0; u < R; u += U) soft = take<T, U>(soft, v + u, x.lane0 + (int32_t)threadIdx.x + u * kStep, kStep, x.packs);
+  if constexpr (L > 0) {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+#pragma unroll
+    for (int u = 0; u < L; ++u) {
+      const int32_t k = x.lane0 + (int32_t)threadIdx.x + (R + u) * kStep;
+      const P p = more[u][wave][lane];
+      soft = take<T, 1>(soft, &p, k, kStep, x.packs);
+    }
+  }
+  if constexpr (REST) {
+    for (int32_t k = x.lane0 + (int32_t)threadIdx.x + (R + L) * kStep; k < x.packs; k += U * kStep) {
+      P q[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (x.has(k + u * kStep)) q[u] = x.load(k + u * kStep);
+      soft = take<T, U>(soft, q, k, kStep, x.packs);
+    }
+  }
+  soft = block_join<W>(join(soft, take_edge(edge)), lds);
+  const float slope = policy_row(a, row, at, chosen, soft, threadIdx.x == 0);
+  const RowSlope r{-slope / soft.s, slope, soft.m, (int32_t)at.token};
+  store_edge(out, x.edge(), edge, r);
+#pragma unroll
+  for (int u = 0; u < R; ++u) {
+    const int32_t k = x.lane0 + (int32_t)threadIdx.x + u * kStep;
+    if (x.has(k)) store_gradient<T>(out, x.head + k * V, v[u], r);
+  }
+#pragma unroll
+  for (int u = 0; u < L; ++u) {
+    const int32_t k = x.lane0 + (int32_t)threadIdx.x + (R + u) * kStep;
+    if (x.has(k)) store_gradient<T>(out, x.head + k * V, more[u][wave][lane], r);
+  }
+  if constexpr (REST) {
+    for (int32_t k = x.lane0 + (int32_t)threadIdx.x + (R + L) * kStep; k < x.packs; k += U * kStep) {
+      P q[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (x.has(k + u * kStep)) q[u] = x.load(k + u * kStep);
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (x.has(k + u * kStep)) store_gradient<T>(out, x.head + (k + u * kStep) * V, q[u], r);
+    }
+  }
+}
+
+// Losses and log-probabilities alone: a workgroup has a row.
+template <typename T, int W>
+__global__ __launch_bounds__(W * 64) void row_kernel(PolicyArgs a, const T* __restrict__ logits, RowOffsets lo, int32_t vocab) {
+  constexpr int U = 4, kStep = W * 64, V = 16 / sizeof(T);
   using P = Pack<T, V>;
   __shared__ Soft lds[W];
   const uint32_t row = blockIdx.x;
-  const float w = weight_of(a, row);
-  T* out = GRAD ? grad + go.at(row) : nullptr;
-  if (w == 0.f) {
-    if (threadIdx.x == 0) {
-      if (a.loss) a.loss[row] = 0.f;
-      a.logProb[row] = 0.f;
-    }
-    if constexpr (GRAD)
-      for (int32_t i = threadIdx.x; i < vocab; i += W * 64) out[i] = Cvt<T>::down(0.f);
+  const Position at = position_of(a, row);
+  if (at.weight == 0.f) {
+    skip_row<T, W, false>(a, row, (T*)nullptr, vocab);
     return;
   }
-  const T* x = logits + lo.at(row);
-  const int64_t token = a.token[row] - 1;
-  const float chosen = (uint64_t)token < (uint64_t)vocab ? Cvt<T>::up(x[token]) : __builtin_nanf("");
-  const RowPacks<T> packs(x, vocab);
-  Soft soft{minus_infinity(), 0.f};
-  for (int32_t k = threadIdx.x; k < packs.packs; k += W * 64) {
-    const P p = packs.load(k);
-    float m = Cvt<T>::up(p.v[0]);
+  const RowParts<T> x(logits + lo.at(row), vocab);
+  const float chosen = chosen_of(x.row, at.token, vocab);
+  Soft soft = take_edge(x.load_edge(x.edge()));
+  for (int32_t k = x.lane0 + (int32_t)threadIdx.x; k < x.packs; k += U * kStep) {
+    P v[U];
 #pragma unroll
-    for (int e = 1; e < V; ++e) m = fmaxf(m, Cvt<T>::up(p.v[e]));
-    const float top = fmaxf(m, soft.m), safe = top == minus_infinity() ? 0.f : top;
-    float s = soft.s * exp_below(soft.m, safe);
-#pragma unroll
-    for (int e = 0; e < V; ++e) s += exp_below(Cvt<T>::up(p.v[e]), safe);
-    soft = Soft{top, s};
+    for (int u = 0; u < U; ++u)
+      if (x.has(k + u * kStep)) v[u] = x.load(k + u * kStep);
+    soft = take<T, U>(soft, v, k, kStep, x.packs);
   }
   soft = block_join<W>(soft, lds);
-  const float slope = policy_row(a, row, chosen, soft, w, threadIdx.x == 0);
+  policy_row(a, row, at, chosen, soft, threadIdx.x == 0);
+}
+
+// Few long rows: each is cut into `parts` (at most 64) of `per` packs, a workgroup each, and a second launch joins their maxima and sums;
+// with a gradient every part joins them for itself and reads its packs again, from the caches.
+struct Parts {
+  Soft* soft;       // of each row, side by side
+  int32_t parts, per;
+};
+template <typename T, int W>
+__global__ __launch_bounds__(W * 64) void part_kernel(PolicyArgs a, const T* __restrict__ logits, RowOffsets lo, int32_t vocab, Parts p) {
+  constexpr int U = 4, kStep = W * 64, V = 16 / sizeof(T);
+  using P = Pack<T, V>;
+  __shared__ Soft lds[W];
+  const uint32_t row = blockIdx.y, part = blockIdx.x;
+  if (a.weight && a.weight[row] == 0.f) return;
+  const RowParts<T> x(logits + lo.at(row), vocab);
+  Soft soft = take_edge(part == 0 ? x.load_edge(x.edge()) : minus_infinity());
+  const int32_t begin = x.lane0 + (int32_t)part * p.per, end = min(x.packs, begin + p.per);
+  for (int32_t k = begin + (int32_t)threadIdx.x; k < end; k += U * kStep) {
+    P v[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (k + u * kStep < end && x.has(k + u * kStep)) v[u] = x.load(k + u * kStep);
+    soft = take<T, U>(soft, v, k, kStep, end);
+  }
+  soft = block_join<W>(soft, lds);
+  if (threadIdx.x == 0) p.soft[(int64_t)row * p.parts + part] = soft;
+}
+template <typename T, int W, bool GRAD>
+__global__ __launch_bounds__(W * 64) void join_kernel(PolicyArgs a, const T* logits, RowOffsets lo, T* grad, RowOffsets go, int32_t vocab, Parts p) {
+  constexpr int U = 4, kStep = W * 64, V = 16 / sizeof(T);
+  using P = Pack<T, V>;
+  const uint32_t row = blockIdx.y, part = blockIdx.x;
+  const int lane = threadIdx.x & 63;
+  const Position at = position_of(a, row);
+  const RowParts<T> x(logits + lo.at(row), vocab);
+  T* out = GRAD ? grad + go.at(row) : nullptr;
+  const int32_t begin = x.lane0 + (int32_t)part * p.per, end = min(x.packs, begin + p.per);
+  const bool first = part == 0 && threadIdx.x == 0;
+  Soft soft{minus_infinity(), 0.f};
+  RowSlope r{0.f, 0.f, 0.f, -1};
+  if (at.weight != 0.f) {
+    if (lane < p.parts) soft = p.soft[(int64_t)row * p.parts + lane];
+    const float chosen = chosen_of(x.row, at.token, vocab);
+    soft = wave_join(soft);
+    const float slope = policy_row(a, row, at, chosen, soft, first);
+    r = RowSlope{-slope / soft.s, slope, soft.m, (int32_t)at.token};
+  } else if (first) {
+    if (a.loss) a.loss[row] = 0.f;
+    a.logProb[row] = 0.f;
+  }
   if constexpr (GRAD) {
-    const float c = -slope / soft.s;
-    const int32_t hit = (int32_t)token;
-    for (int32_t k = threadIdx.x; k < packs.packs; k += W * 64) {
-      const P p = packs.load(k);
-      P g;
+    const bool used = at.weight != 0.f;
+    if (part == 0) {
+      const int32_t i = x.edge();
+      if (used) store_edge(out, i, x.load_edge(i), r);
+      else if (i >= 0) out[i] = Cvt<T>::down(0.f);
+    }
+    for (int32_t k = begin + (int32_t)threadIdx.x; k < end; k += U * kStep) {
+      P v[U];
 #pragma unroll
-      for (int e = 0; e < V; ++e) {
-        float d = c * exp_below(Cvt<T>::up(p.v[e]), soft.m);
-        if (k * V + e - packs.before == hit) d += slope;
-        g.v[e] = rounded<T>(d);
-      }
-      const int32_t i0 = k * V - packs.before;
-      if (packs.whole(k)) {
-        store_pack_unaligned<false>(out + i0, g);
-      } else {
+      for (int u = 0; u < U; ++u) {
+        if (k + u * kStep < end && x.has(k + u * kStep)) {
+          if (used) {
+            v[u] = x.load(k + u * kStep);
+          } else {
 #pragma unroll
-        for (int e = 0; e < V; ++e)
-          if (i0 + e >= 0 && i0 + e < vocab) out[i0 + e] = g.v[e];
+            for (int e = 0; e < V; ++e) v[u].v[e] = Cvt<T>::down(0.f);
+          }
+        }
       }
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (k + u * kStep < end && x.has(k + u * kStep)) store_gradient<T>(out, x.head + (k + u * kStep) * V, v[u], r);
     }
   }
 }
@@ -191,10 +444,66 @@ template <typename T>
 void launch_rows(THCState* s, const PolicyArgs& a, const T* logits, const Rows& lr, T* grad, const Rows& gr) {
   hipStream_t st = current_stream(s);
   const dim3 grid((unsigned)lr.count);
-  if (grad)
-    hipLaunchKernelGGL((row_kernel<T, 4, true>), grid, dim3(256), 0, st, a, logits, offsets_of(lr), grad, offsets_of(gr), (int32_t)lr.length);
-  else
-    hipLaunchKernelGGL((row_kernel<T, 4, false>), grid, dim3(256), 0, st, a, logits, offsets_of(lr), grad, offsets_of(lr), (int32_t)lr.length);
+  const int32_t vocab = (int32_t)lr.length;
+  constexpr int V = 16 / sizeof(T);
+  const int32_t packs = vocab / V + 7;      // at most, with those that a line's begin is before the row
+  const RowOffsets lo = offsets_of(lr), go = grad ? offsets_of(gr) : lo;
+  // Few long rows are split. us with a workgroup a row and split: log-probabilities of 24 rows of 32000 halves 6.5, 6.4, of 128000 13.3, 7.6;
+  // 128 x 128000 15.2, 13.0; 256 x 128000 16.5, 18.7; 1 x 262144 22, 6. Losses with gradients, whose rows are then read twice: 24 x 32000
+  // 8.4, 8.7; 24 x 128000 18.5, 11.1; 64 x 128000 19.2, 16.7; 128 x 128000 20.4, 25.7.
+  const int64_t perRow = tuning("loss.split", 100);
+  if (lr.count <= 128 && packs >= (grad ? 10240 : 6144) && packs >= lr.count * perRow * (grad ? 2 : 1)) {
+    constexpr int W = 4;
+    Parts p;
+    p.parts = (int32_t)std::max<int64_t>(1, std::min<int64_t>(64, 4096 / (lr.count * W)));
+    p.per = ((packs + p.parts - 1) / p.parts + W * 64 - 1) / (W * 64) * (W * 64);
+    p.parts = (packs + p.per - 1) / p.per;
+    Workspace w(s, lr.count * p.parts * (int64_t)sizeof(Soft));
+    p.soft = reinterpret_cast<Soft*>(w.data());
+    const dim3 cut((unsigned)p.parts, (unsigned)lr.count);
+    hipLaunchKernelGGL((part_kernel<T, W>), cut, dim3(W * 64), 0, st, a, logits, lo, vocab, p);
+    if (grad) hipLaunchKernelGGL((join_kernel<T, W, true>), cut, dim3(W * 64), 0, st, a, logits, lo, grad, go, vocab, p);
+    else hipLaunchKernelGGL((join_kernel<T, 1, false>), dim3(1, (unsigned)lr.count), dim3(64), 0, st, a, logits, lo, grad, go, vocab, p);
+    return;
+  }
+  using std::integral_constant;
+  if (!grad) {
+    // Waves a row: as many as leave about 16 to a CU, but two packs a lane. us with 1, 2, 4, 8, 16: 16384 rows of 4000 halves 23.5, 23.6, 34,
+    // 56, 88; 1000 x 32000 22, 14.5, 16, 15, 18.5; 600 x 128000 72, 42, 45, 31, 35; 256 x 16000 fp32 with 4 and 16 11.4, 6.9.
+    auto go = [&](auto wTag) {
+      constexpr int W = decltype(wTag)::value;
+      hipLaunchKernelGGL((row_kernel<T, W>), grid, dim3(W * 64), 0, st, a, logits, lo, vocab);
+    };
+    const int64_t want = 4800;
+    if (lr.count >= want || packs < 256) go(integral_constant<int, 1>{});
+    else if (lr.count * 2 >= want || packs < 512) go(integral_constant<int, 2>{});
+    else if (lr.count * 4 >= want || packs < 1024) go(integral_constant<int, 4>{});
+    else if (lr.count * 8 >= want || packs < 2048) go(integral_constant<int, 8>{});
+    else go(integral_constant<int, 16>{});
+    return;
+  }
+  auto held = [&](auto waves, auto registers, auto shared, auto perSimd, auto rest) {
+    constexpr int W = decltype(waves)::value, R = decltype(registers)::value, L = decltype(shared)::value;
+    hipLaunchKernelGGL((held_row_kernel<T, W, R, L, decltype(perSimd)::value, decltype(rest)::value>), grid, dim3(W * 64), L * W * 64 * 16, st, a,
+                       logits, lo, grad, go, vocab);
+  };
+#define HELD(W, R, L, E, REST)                                                                                            \
+  held(integral_constant<int, W>{}, integral_constant<int, R>{}, integral_constant<int, L>{}, integral_constant<int, E>{}, \
+       integral_constant<bool, REST>{})
+  // The least that hold a row, so that a CU has several: one loads while another computes and a third stores. us, halves with gradients:
+  // 16384 x 8000 with 4 waves of 4, 8 and 16 packs 82, 84, 100; 8192 x 16000 with 8 waves of 4 and 8, 16 of 8 84, 88, 111; 8192 x 32000
+  // with 8 of 8, 16 of 8 and 16 of 16 168, 170, 256; 4096 x 65000 with 16 of 8 and 16 of 16 173, 215; 4096 x 100001 with 8 waves of 16
+  // and 9 more in LDS (two workgroups a CU) and 16 of 16 285, 312; 2048 x 262144 with its end read again 478 (floor 314).
+  if (packs <= 64) HELD(1, 1, 0, 8, false);
+  else if (packs <= 256) HELD(1, 4, 0, 8, false);
+  else if (packs <= 1024) HELD(4, 4, 0, 8, false);
+  else if (packs <= 2048) HELD(8, 4, 0, 8, false);
+  else if (packs <= 4096) HELD(8, 8, 0, 6, false);
+  else if (packs <= 8192) HELD(16, 8, 0, 8, false);
+  else if (packs <= 12800) HELD(8, 16, 9, 4, false);
+  else if (packs <= 25600) HELD(16, 16, 9, 4, false);
+  else HELD(16, 12, 9, 4, true);
+#undef HELD
 }
 
 // A per-position operand: float, as many elements as there are rows.

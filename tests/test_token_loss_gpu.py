@@ -30,6 +30,25 @@ def _lp_bound(x, tokens, want):
     return EPS * (x.shape[1] / 64 + 24 + 3 + 4 * span + 4 * np.abs(want))
 
 
+@pytest.fixture(params=["split", "whole"])
+def rows_are(thc, request):
+    """Few long rows are split between workgroups, or not, as many are not."""
+    thc.set_tuning("loss.split", 100 if request.param == "split" else 1 << 30)
+    yield request.param
+    thc.set_tuning("loss.split", 100)
+
+
+@pytest.mark.parametrize("kind", ["float", "half"])
+@pytest.mark.parametrize("vocab", [40001, 81913, 120000, 160011, 262145])
+def test_log_prob_of_long_rows(thc, rows_are, kind, vocab):
+    rng = np.random.default_rng(vocab)
+    for rows in (2, 70):
+        x, tokens = _logits(rng, rows, vocab, kind), rng.integers(1, vocab + 1, rows)
+        want = _log_prob(x, tokens)
+        off = np.abs(thc.Tensor("float").token_log_prob(thc.Tensor.from_numpy(x), thc.Tensor.from_numpy(tokens)).numpy() - want)
+        assert np.all(off <= _lp_bound(x, tokens, want)), (rows, off.max())
+
+
 @pytest.mark.parametrize("kind", ["float", "half"])
 @pytest.mark.parametrize("vocab", LENGTHS + LONG)
 def test_log_prob(thc, kind, vocab):
@@ -130,9 +149,11 @@ def test_policy_loss(thc, kind, vocab, reference):
 
 
 @pytest.mark.parametrize("kind", ["float", "half"])
-@pytest.mark.parametrize("vocab", LONG)
-def test_policy_loss_of_long_rows(thc, kind, vocab):
-    _check(thc, np.random.default_rng(vocab), 3, vocab, kind, True, masked=False, scale=512.0)
+@pytest.mark.parametrize("vocab", LONG + [81850, 102400, 204700, 210001])
+def test_policy_loss_of_long_rows(thc, rows_are, kind, vocab):
+    rng = np.random.default_rng(vocab)
+    _check(thc, rng, 3, vocab, kind, True, masked=False, scale=512.0)
+    _check(thc, rng, 11, vocab, kind, False, masked=True, scale=512.0)
 
 
 @pytest.mark.parametrize("kind", ["float", "half"])
@@ -142,8 +163,8 @@ def test_policy_loss_of_many_rows(thc, kind, rows, vocab):
 
 
 @pytest.mark.parametrize("kind", ["float", "half"])
-@pytest.mark.parametrize("vocab", [5, 1000, 1001, 33001, 140001])
-def test_gradient_in_the_logits_place(thc, kind, vocab):
+@pytest.mark.parametrize("vocab", [5, 1000, 1001, 33001, 140001, 210001])
+def test_gradient_in_the_logits_place(thc, rows_are, kind, vocab):
     rng = np.random.default_rng(vocab)
     case = _case(rng, 40 if vocab < 2000 else 4, vocab, kind, True, True)
     apart, place = _run(thc, case, scale=8.0), _run(thc, case, scale=8.0, into="logits")
@@ -191,7 +212,7 @@ def test_views(thc, kind):
 
 @pytest.mark.parametrize("kind", ["float", "half"])
 @pytest.mark.parametrize("vocab", [6, 1000, 9001, 140001])
-def test_rows_that_hold_nothing_to_learn_from(thc, kind, vocab):
+def test_rows_that_hold_nothing_to_learn_from(thc, rows_are, kind, vocab):
     """Masked logits (-inf and the type's lowest value), rows of weight 0 that hold anything, a token that the mask has taken away."""
     rng = np.random.default_rng(vocab)
     x, tokens, old, advantage, ref, weight = _case(rng, 8, vocab, kind, True, False)
