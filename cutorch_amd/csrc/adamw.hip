@@ -51,31 +51,55 @@ __device__ __forceinline__ float adamw_step(const Hyper& h, float p, float g, fl
   return p * h.keep - (m / root) * h.rate;
 }
 
-// The tensors of one launch travel as kernel arguments: no table has to reach the device first.
-struct Item {
-  void* param;
-  float* master;
-  const void* grad;
-  void *mean, *square;
-  float *meanScale, *squareScale;
-  int64_t size;
-};
-constexpr int kItems = 56;                            // 3.9 KiB of arguments
-constexpr int kPacks = 4;                             // of 4 elements, in flight per lane
-constexpr int kPart = kBlock * 4 * kPacks;            // elements a workgroup
-struct StepArgs {
+// The tensors of one launch travel as kernel arguments, so that no table has to reach the device first: the parameter, the gradient, the
+// moments, with 8-bit states their scales, and the float copies if there are any. A launch costs the host more the more arguments
+// it has (2.4 us for few, about 4 for 4 KiB), so there is a form for few tensors and one for as many as 4 KiB hold (147 tensors of a few
+// thousand floats in two launches 11.0 us, in three of 64 15.2). Large ones take 56 a launch: their workgroups find theirs with one load
+// (202 M halves with float copies 962 us, with up to 77 a launch 975).
+enum { kParam, kGrad, kMean, kSquare, kMeanScale, kSquareScale };
+template <int POINTERS, int N>
+struct Args {
+  static constexpr int kPointers = POINTERS, kItems = N;
   Hyper h;
   int32_t count;
-  uint32_t firstPart[kItems];                         // the workgroup that each tensor begins with
-  Item item[kItems];
+  uint32_t firstPart[N];                // the workgroup that each tensor begins with
+  struct {
+    void* p[POINTERS];
+    int64_t size;
+  } item[N];
+};
+constexpr int kFewItems = 32, kLargeItems = 56;
+template <int POINTERS>
+constexpr int kManyItems = (4096 - 48) / (8 * POINTERS + 12);
+
+// What this workgroup has: a tensor, found by every lane looking at one or two, and the place in it. All that the arguments say of it is
+// asked for at once.
+template <typename A>
+struct Part {
+  void* p[A::kPointers];
+  int64_t base, left;
+  __device__ __forceinline__ Part(const A& a, int part) {
+    constexpr int J = (A::kItems + 63) / 64;
+    const int lane = threadIdx.x & 63;
+    uint32_t first[J];
+#pragma unroll
+    for (int j = 0; j < J; ++j) first[j] = a.firstPart[min(j * 64 + lane, A::kItems - 1)];
+    int n = 0;
+#pragma unroll
+    for (int j = 0; j < J; ++j) n += __popcll(__ballot(j * 64 + lane < a.count && first[j] <= blockIdx.x));
+    const int i = __builtin_amdgcn_readfirstlane(n - 1);
+#pragma unroll
+    for (int k = 0; k < A::kPointers; ++k) p[k] = a.item[i].p[k];
+    base = (int64_t)(blockIdx.x - a.firstPart[i]) * part;
+    left = a.item[i].size - base;
+  }
 };
 
-// Which tensor this workgroup has: every lane looks at one.
-__device__ __forceinline__ int item_of(const StepArgs& a) {
-  const int lane = threadIdx.x & 63;
-  const uint32_t first = lane < a.count ? a.firstPart[lane] : ~0u;
-  return __builtin_amdgcn_readfirstlane(__popcll(__ballot(first <= blockIdx.x)) - 1);
-}
+// Packs of 4 elements of every operand that a lane has in flight, by kernel, and so the elements of a workgroup. us with 1, 2, 4: 4.4 M floats
+// 25.5, 22.5, 27.0, 202 M halves with float copies 959, 953, 962; 8-bit states: 0.9 M halves 12.2, 14.9, 13.7, 184 M floats with the
+// moments as floats 805, 829, 840.
+constexpr int kStepPacks = 2, kStep8Packs = 1, kDecodePacks = 1;
+constexpr int part_size(int packs) { return kBlock * 4 * packs; }
 
 // Four neighbours as floats, and back; `n` of them are the tensor's.
 template <bool NT, typename T>
@@ -105,17 +129,17 @@ __device__ __forceinline__ void store4(T* to, const float (&from)[4], int n) {
   }
 }
 
-// States in 32 bits: kPacks packs of each operand in flight, then the arithmetic, in place.
-// FULL: the tensor does not end in this part.
+// States in 32 bits, in place. FULL: the tensor does not end in this part.
 template <typename T, bool MASTER, bool NT, bool FULL>
-__device__ __forceinline__ void step_part(const Hyper& h, const Item& t, int64_t base, int left) {
-  T* param = static_cast<T*>(t.param) + base;
-  float* master = MASTER ? t.master + base : nullptr;
-  const T* grad = static_cast<const T*>(t.grad) + base;
-  float *mean = static_cast<float*>(t.mean) + base, *square = static_cast<float*>(t.square) + base;
-  float p[kPacks][4], g[kPacks][4], m[kPacks][4], v[kPacks][4];
+__device__ __forceinline__ void step_part(const Hyper& h, void* const* pointers, int64_t base, int left) {
+  constexpr int U = kStepPacks;
+  T* param = static_cast<T*>(pointers[kParam]) + base;
+  const T* grad = static_cast<const T*>(pointers[kGrad]) + base;
+  float *mean = static_cast<float*>(pointers[kMean]) + base, *square = static_cast<float*>(pointers[kSquare]) + base;
+  float* master = MASTER ? static_cast<float*>(pointers[kSquare + 1]) + base : nullptr;
+  float p[U][4], g[U][4], m[U][4], v[U][4];
 #pragma unroll
-  for (int u = 0; u < kPacks; ++u) {
+  for (int u = 0; u < U; ++u) {
     const int i = (u * kBlock + threadIdx.x) * 4;
     if (FULL || i < left) {
       const int n = FULL ? 4 : left - i;
@@ -127,7 +151,7 @@ __device__ __forceinline__ void step_part(const Hyper& h, const Item& t, int64_t
     }
   }
 #pragma unroll
-  for (int u = 0; u < kPacks; ++u) {
+  for (int u = 0; u < U; ++u) {
     const int i = (u * kBlock + threadIdx.x) * 4;
     if (FULL || i < left) {
       const int n = FULL ? 4 : left - i;
@@ -140,13 +164,12 @@ __device__ __forceinline__ void step_part(const Hyper& h, const Item& t, int64_t
     }
   }
 }
-template <typename T, bool MASTER, bool NT>
-__global__ __launch_bounds__(kBlock) void step_kernel(StepArgs a) {
-  const int i = item_of(a);
-  const Item& t = a.item[i];
-  const int64_t base = (int64_t)(blockIdx.x - a.firstPart[i]) * kPart, left = t.size - base;
-  if (left >= kPart) step_part<T, MASTER, NT, true>(a.h, t, base, kPart);
-  else step_part<T, MASTER, NT, false>(a.h, t, base, (int)left);
+template <typename T, bool MASTER, bool NT, typename A>
+__global__ __launch_bounds__(kBlock) void step_kernel(A a) {
+  constexpr int kPart = part_size(kStepPacks);
+  const Part<A> t(a, kPart);
+  if (t.left >= kPart) step_part<T, MASTER, NT, true>(a.h, t.p, t.base, kPart);
+  else step_part<T, MASTER, NT, false>(a.h, t.p, t.base, (int)t.left);
 }
 
 __device__ __forceinline__ float decode_mean(int8_t c, float top) {
@@ -205,22 +228,24 @@ __device__ __forceinline__ void store4_codes(T* to, const T (&from)[4], int n) {
   }
 }
 
-// States in 8 bits: a wave has kPacks blocks of states, 4 elements a lane of each. What is behind a tensor's end counts as zeros.
+// States in 8 bits: a wave has a block of states per pack, 4 elements a lane. What is behind a tensor's end counts as zeros.
 // FULL: the tensor does not end in this part.
 template <typename T, bool MASTER, bool NT, bool FULL>
-__device__ __forceinline__ void step8_part(const Hyper& h, const Item& t, int64_t base, int left) {
+__device__ __forceinline__ void step8_part(const Hyper& h, void* const* pointers, int64_t base, int left) {
+  constexpr int U = kStep8Packs;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  T* param = static_cast<T*>(t.param) + base;
-  float* master = MASTER ? t.master + base : nullptr;
-  const T* grad = static_cast<const T*>(t.grad) + base;
-  int8_t* mean = static_cast<int8_t*>(t.mean) + base;
-  uint8_t* square = static_cast<uint8_t*>(t.square) + base;
-  float *meanScale = t.meanScale + base / kStateBlock, *squareScale = t.squareScale + base / kStateBlock;
-  float p[kPacks][4], g[kPacks][4], topMean[kPacks], topSquare[kPacks];
-  int8_t codeMean[kPacks][4];
-  uint8_t codeSquare[kPacks][4];
+  T* param = static_cast<T*>(pointers[kParam]) + base;
+  const T* grad = static_cast<const T*>(pointers[kGrad]) + base;
+  int8_t* mean = static_cast<int8_t*>(pointers[kMean]) + base;
+  uint8_t* square = static_cast<uint8_t*>(pointers[kSquare]) + base;
+  float* meanScale = static_cast<float*>(pointers[kMeanScale]) + base / kStateBlock;
+  float* squareScale = static_cast<float*>(pointers[kSquareScale]) + base / kStateBlock;
+  float* master = MASTER ? static_cast<float*>(pointers[kSquareScale + 1]) + base : nullptr;
+  float p[U][4], g[U][4], topMean[U], topSquare[U];
+  int8_t codeMean[U][4];
+  uint8_t codeSquare[U][4];
 #pragma unroll
-  for (int u = 0; u < kPacks; ++u) {
+  for (int u = 0; u < U; ++u) {
     const int block = u * (kBlock / 64) + wave, i = block * kStateBlock + lane * 4;
     if (FULL || block * kStateBlock < left) {      // whole waves
       const int n = FULL ? 4 : left - i;           // none for the lanes behind the end
@@ -234,7 +259,7 @@ __device__ __forceinline__ void step8_part(const Hyper& h, const Item& t, int64_
     }
   }
 #pragma unroll
-  for (int u = 0; u < kPacks; ++u) {
+  for (int u = 0; u < U; ++u) {
     const int block = u * (kBlock / 64) + wave, i = block * kStateBlock + lane * 4;
     if (FULL || block * kStateBlock < left) {
       const int n = FULL ? 4 : left - i;
@@ -271,52 +296,59 @@ __device__ __forceinline__ void step8_part(const Hyper& h, const Item& t, int64_
     }
   }
 }
-template <typename T, bool MASTER, bool NT>
-__global__ __launch_bounds__(kBlock) void step8_kernel(StepArgs a) {
-  const int i = item_of(a);
-  const Item& t = a.item[i];
-  const int64_t base = (int64_t)(blockIdx.x - a.firstPart[i]) * kPart, left = t.size - base;
-  if (left >= kPart) step8_part<T, MASTER, NT, true>(a.h, t, base, kPart);
-  else step8_part<T, MASTER, NT, false>(a.h, t, base, (int)left);
+template <typename T, bool MASTER, bool NT, typename A>
+__global__ __launch_bounds__(kBlock) void step8_kernel(A a) {
+  constexpr int kPart = part_size(kStep8Packs);
+  const Part<A> t(a, kPart);
+  if (t.left >= kPart) step8_part<T, MASTER, NT, true>(a.h, t.p, t.base, kPart);
+  else step8_part<T, MASTER, NT, false>(a.h, t.p, t.base, (int)t.left);
 }
 
-// The moments that 8-bit states stand for: the items' codes and scales, into `param` and `master`.
-template <bool NT>
-__global__ __launch_bounds__(kBlock) void decode_kernel(StepArgs a) {
-  const Item& t = a.item[item_of(a)];
-  const int64_t base = (int64_t)(blockIdx.x - a.firstPart[item_of(a)]) * kPart;
-  const int left = (int)min((int64_t)kPart, t.size - base);
-  const int8_t* mean = static_cast<const int8_t*>(t.mean) + base;
-  const uint8_t* square = static_cast<const uint8_t*>(t.square) + base;
-  const float *meanScale = t.meanScale + base / kStateBlock, *squareScale = t.squareScale + base / kStateBlock;
-  float *meanOut = static_cast<float*>(t.param) + base, *squareOut = t.master + base;
-  int8_t codeMean[kPacks][4];
-  uint8_t codeSquare[kPacks][4];
-  float topMean[kPacks], topSquare[kPacks];
+// The moments that 8-bit states stand for: from codes and scales, the mean into kParam and the square into kGrad.
+template <bool FULL>
+__device__ __forceinline__ void decode_part(void* const* pointers, int64_t base, int left) {
+  constexpr int U = kDecodePacks;
+  const int8_t* mean = static_cast<const int8_t*>(pointers[kMean]) + base;
+  const uint8_t* square = static_cast<const uint8_t*>(pointers[kSquare]) + base;
+  const float* meanScale = static_cast<const float*>(pointers[kMeanScale]) + base / kStateBlock;
+  const float* squareScale = static_cast<const float*>(pointers[kSquareScale]) + base / kStateBlock;
+  float *meanOut = static_cast<float*>(pointers[kParam]) + base, *squareOut = static_cast<float*>(pointers[kGrad]) + base;
+  int8_t codeMean[U][4];
+  uint8_t codeSquare[U][4];
+  float topMean[U], topSquare[U];
 #pragma unroll
-  for (int u = 0; u < kPacks; ++u) {
+  for (int u = 0; u < U; ++u) {
     const int i = (u * kBlock + threadIdx.x) * 4;
-    if (i < left) {
+    if (FULL || i < left) {
+      const int n = FULL ? 4 : left - i;
       topMean[u] = meanScale[i / kStateBlock];
       topSquare[u] = squareScale[i / kStateBlock];
-      load4_codes(codeMean[u], mean + i, left - i);
-      load4_codes(codeSquare[u], square + i, left - i);
+      load4_codes(codeMean[u], mean + i, n);
+      load4_codes(codeSquare[u], square + i, n);
     }
   }
 #pragma unroll
-  for (int u = 0; u < kPacks; ++u) {
+  for (int u = 0; u < U; ++u) {
     const int i = (u * kBlock + threadIdx.x) * 4;
-    if (i < left) {
+    if (FULL || i < left) {
+      const int n = FULL ? 4 : left - i;
       float m[4], v[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         m[e] = decode_mean(codeMean[u][e], topMean[u]);
         v[e] = decode_square(codeSquare[u][e], topSquare[u]);
       }
-      store4<NT>(meanOut + i, m, left - i);
-      store4<NT>(squareOut + i, v, left - i);
+      store4<true>(meanOut + i, m, n);
+      store4<true>(squareOut + i, v, n);
     }
   }
+}
+template <typename A>
+__global__ __launch_bounds__(kBlock) void decode_kernel(A a) {
+  constexpr int kPart = part_size(kDecodePacks);
+  const Part<A> t(a, kPart);
+  if (t.left >= kPart) decode_part<true>(t.p, t.base, kPart);
+  else decode_part<false>(t.p, t.base, (int)t.left);
 }
 
 // ------------------------------------------------------------------------- host --
@@ -349,19 +381,28 @@ struct Held {
   }
 };
 
-// Collects tensors and launches a kernel for as many as its arguments hold. NT: what the whole call writes is too much for the caches.
-template <typename Launch>
+// Collects tensors of elements of these sizes and launches a kernel (by launch(args, grid)) for as many as its arguments hold.
+template <typename A, typename Launch>
 struct Batch {
-  StepArgs a{};
+  A a{};
+  int part;
+  const int* elementSize;      // of each pointer; 0: a scale for each block
   uint32_t parts = 0;
   Launch launch;
-  explicit Batch(Launch l) : launch(l) {}
-  void add(const Item& t) {
-    const int64_t n = (t.size + kPart - 1) / kPart;
-    if (a.count == kItems || (a.count && parts + n > (int64_t)1 << 31)) flush();
-    a.firstPart[a.count] = parts;
-    a.item[a.count++] = t;
-    parts += (uint32_t)n;
+  Batch(const Hyper& h, int partSize, const int* sizes, Launch l) : part(partSize), elementSize(sizes), launch(l) { a.h = h; }
+  void add(void* const* pointers, int64_t size) {
+    // (a launch has less than 2^32 threads: a larger tensor goes in pieces)
+    const int64_t most = (int64_t)part << 22;
+    for (int64_t at = 0; at < size; at += most) {
+      const int64_t n = std::min(most, size - at), count = (n + part - 1) / part;
+      if (a.count == A::kItems || parts + count > (int64_t)1 << 23) flush();
+      a.firstPart[a.count] = parts;
+      a.item[a.count].size = n;
+      for (int k = 0; k < A::kPointers; ++k)
+        a.item[a.count].p[k] = static_cast<char*>(pointers[k]) + (elementSize[k] ? at * elementSize[k] : at / kStateBlock * 4);
+      ++a.count;
+      parts += (uint32_t)count;
+    }
   }
   void flush() {
     if (a.count) launch(a, dim3(parts));
@@ -431,42 +472,54 @@ void adamw(THCState* s, DType dt, int count, const Lists& l, double lr, double b
   const int64_t touched = elements * (2 * (int64_t)dtype_size(dt) + (l.master ? 4 : 0) + (eight ? 2 : 8));
   const bool nt = tuning("adamw.nt", touched >= (int64_t(256) << 20)) != 0;
   hipStream_t st = current_stream(s);
-  auto launch = [&](const StepArgs& a, dim3 grid) {
-    auto go = [&](auto type, auto master, auto stream) {
-      using T = decltype(type);
-      constexpr bool M = decltype(master)::value, NT = decltype(stream)::value;
-      if (eight) hipLaunchKernelGGL((step8_kernel<T, M, NT>), grid, dim3(kBlock), 0, st, a);
-      else hipLaunchKernelGGL((step_kernel<T, M, NT>), grid, dim3(kBlock), 0, st, a);
-    };
-    auto typed = [&](auto stream) {
-      if (!half) go(float{}, std::false_type{}, stream);
-      else if (!l.master) go(__half{}, std::false_type{}, stream);
-      else go(__half{}, std::true_type{}, stream);
-    };
-    if (nt) typed(std::true_type{});
-    else typed(std::false_type{});
-  };
-  Batch<decltype(launch)> batch(launch);
-  batch.a.h = h;
   Held held(s);
-  for (int i = 0; i < count; ++i) {
-    if (!has_elements(l.param[i])) continue;
-    note_stream_use(s, {l.param[i], l.master ? l.master[i] : nullptr, l.grad[i], l.mean[i], l.square[i], eight ? l.meanScale[i] : nullptr,
-                        eight ? l.squareScale[i] : nullptr});
-    Item t{};
-    t.size = tensor_numel(l.param[i]);
-    t.param = held.add(l.param[i], dt, true);
-    if (l.master) t.master = (float*)held.add(l.master[i], DType::F32, true);
-    t.grad = held.add(l.grad[i], dt, false);
-    t.mean = held.add(l.mean[i], meanType, true);
-    t.square = held.add(l.square[i], squareType, true);
-    if (eight) {
-      t.meanScale = (float*)held.add(l.meanScale[i], DType::F32, true);
-      t.squareScale = (float*)held.add(l.squareScale[i], DType::F32, true);
+  auto run = [&](auto type, auto withMaster, auto withEight, auto streaming, auto items) {
+    using T = decltype(type);
+    constexpr bool M = decltype(withMaster)::value, E = decltype(withEight)::value, NT = decltype(streaming)::value;
+    constexpr int P = (E ? 6 : 4) + M;
+    constexpr int N = decltype(items)::value;
+    using A = Args<P, N ? N : kManyItems<P>>;
+    static_assert(sizeof(A) <= 4096, "kernel arguments");
+    auto launch = [&](const A& a, dim3 grid) {
+      if constexpr (E) hipLaunchKernelGGL((step8_kernel<T, M, NT, A>), grid, dim3(kBlock), 0, st, a);
+      else hipLaunchKernelGGL((step_kernel<T, M, NT, A>), grid, dim3(kBlock), 0, st, a);
+    };
+    constexpr int kSize = sizeof(T), kState = E ? 1 : 4;
+    const int sizes[7] = {kSize, kSize, kState, kState, E ? 0 : 4, 0, 4};
+    Batch<A, decltype(launch)> batch(h, part_size(E ? kStep8Packs : kStepPacks), sizes, launch);
+    for (int i = 0; i < count; ++i) {
+      if (!has_elements(l.param[i])) continue;
+      note_stream_use(s, {l.param[i], M ? l.master[i] : nullptr, l.grad[i], l.mean[i], l.square[i], E ? l.meanScale[i] : nullptr,
+                          E ? l.squareScale[i] : nullptr});
+      void* p[7];
+      p[kParam] = held.add(l.param[i], dt, true);
+      p[kGrad] = held.add(l.grad[i], dt, false);
+      p[kMean] = held.add(l.mean[i], meanType, true);
+      p[kSquare] = held.add(l.square[i], squareType, true);
+      if constexpr (E) {
+        p[kMeanScale] = held.add(l.meanScale[i], DType::F32, true);
+        p[kSquareScale] = held.add(l.squareScale[i], DType::F32, true);
+      }
+      if constexpr (M) p[P - 1] = held.add(l.master[i], DType::F32, true);
+      batch.add(p, tensor_numel(l.param[i]));
     }
-    batch.add(t);
-  }
-  batch.flush();
+    batch.flush();
+  };
+  using std::false_type;
+  using std::true_type;
+  auto typed = [&](auto type, auto master, auto bits) {
+    using std::integral_constant;
+    if (nt) run(type, master, bits, true_type{}, integral_constant<int, kLargeItems>{});
+    else if (count <= kFewItems) run(type, master, bits, false_type{}, integral_constant<int, kFewItems>{});
+    else run(type, master, bits, false_type{}, integral_constant<int, 0>{});      // as many as fit
+  };
+  auto states = [&](auto bits) {
+    if (!half) typed(float{}, false_type{}, bits);
+    else if (!l.master) typed(__half{}, false_type{}, bits);
+    else typed(__half{}, true_type{}, bits);
+  };
+  if (eight) states(true_type{});
+  else states(false_type{});
   THC_CHECK(hipGetLastError());
   note_kernel(eight ? "adamw8" : "adamw");
   held.write_back();
@@ -485,30 +538,25 @@ void moments(THCState* s, int count, AnyTensor** meanOut, AnyTensor** squareOut,
     THC_ARG_CHECK(meanOut[i], 3, "tensor %d is missing", i + 1);
     THC_ARG_CHECK(squareOut[i], 4, "tensor %d is missing", i + 1);
   }
-  int64_t elements = 0;
-  for (int i = 0; i < count; ++i) elements += tensor_numel(mean[i]);
-  const bool nt = streaming_store("adamw.nt", elements * 8);
   hipStream_t st = current_stream(s);
-  auto launch = [&](const StepArgs& a, dim3 grid) {
-    if (nt) hipLaunchKernelGGL((decode_kernel<true>), grid, dim3(kBlock), 0, st, a);
-    else hipLaunchKernelGGL((decode_kernel<false>), grid, dim3(kBlock), 0, st, a);
-  };
-  Batch<decltype(launch)> batch(launch);
+  using A = Args<6, kManyItems<6>>;
+  auto launch = [&](const A& a, dim3 grid) { hipLaunchKernelGGL((decode_kernel<A>), grid, dim3(kBlock), 0, st, a); };
+  const int sizes[6] = {4, 4, 1, 1, 0, 0};
+  Batch<A, decltype(launch)> batch(Hyper{}, part_size(kDecodePacks), sizes, launch);
   Held held(s);
   for (int i = 0; i < count; ++i) {
     tensor_resize_as(s, meanOut[i], mean[i], DType::F32);
     tensor_resize_as(s, squareOut[i], mean[i], DType::F32);
     if (!has_elements(mean[i])) continue;
     note_stream_use(s, {meanOut[i], squareOut[i], mean[i], meanScale[i], square[i], squareScale[i]});
-    Item t{};
-    t.size = tensor_numel(mean[i]);
-    t.param = held.add(meanOut[i], DType::F32, true);
-    t.master = (float*)held.add(squareOut[i], DType::F32, true);
-    t.mean = held.add(mean[i], DType::I8, false);
-    t.square = held.add(square[i], DType::U8, false);
-    t.meanScale = (float*)held.add(meanScale[i], DType::F32, false);
-    t.squareScale = (float*)held.add(squareScale[i], DType::F32, false);
-    batch.add(t);
+    void* p[6];
+    p[kParam] = held.add(meanOut[i], DType::F32, true);
+    p[kGrad] = held.add(squareOut[i], DType::F32, true);
+    p[kMean] = held.add(mean[i], DType::I8, false);
+    p[kSquare] = held.add(square[i], DType::U8, false);
+    p[kMeanScale] = held.add(meanScale[i], DType::F32, false);
+    p[kSquareScale] = held.add(squareScale[i], DType::F32, false);
+    batch.add(p, tensor_numel(mean[i]));
   }
   batch.flush();
   THC_CHECK(hipGetLastError());

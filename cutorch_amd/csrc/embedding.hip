@@ -19,18 +19,19 @@ namespace {
 // repeats elements of the one before it: the same values are written twice, nothing needs a tail. Stores are streaming ones at every
 // size (us with plain ones and so: 2048 rows of 2048 halves 4.9, 4.8, 8192 x 1024 6.5, 5.5, 65536 x 1024 43.5, 29.0); table rows may
 // come again and are read plainly.
-template <typename T, int V, int U, typename I>
+template <typename T, int V, int U>
 __global__ __launch_bounds__(kBlock) void lookup_kernel(T* __restrict__ out, const T* __restrict__ table, const int64_t* __restrict__ tokens,
-                                                        int64_t vocab, int64_t tableStride, int32_t dim, I items, Divisor<I> packs, float factor) {
+                                                        int64_t vocab, int64_t tableStride, int32_t dim, uint32_t items,
+                                                        Divisor<uint32_t> packs, float factor) {
   using P = Pack<T, V>;
-  const I base = (I)blockIdx.x * (kBlock * U) + threadIdx.x;
-  I row[U];
+  const uint32_t base = blockIdx.x * (kBlock * U) + threadIdx.x;
+  uint32_t row[U];
   int32_t at[U];
   int64_t token[U];
 #pragma unroll
   for (int u = 0; u < U; ++u) {
-    const I i = base + (I)u * kBlock;
-    I r;
+    const uint32_t i = base + u * kBlock;
+    uint32_t r;
     packs.divmod(i < items ? i : 0, row[u], r);
     at[u] = min((int32_t)r * V, dim - V);
     token[u] = tokens[row[u]] - 1;
@@ -47,7 +48,7 @@ __global__ __launch_bounds__(kBlock) void lookup_kernel(T* __restrict__ out, con
   }
 #pragma unroll
   for (int u = 0; u < U; ++u) {
-    if (base + (I)u * kBlock < items) {
+    if (base + u * kBlock < items) {
 #pragma unroll
       for (int e = 0; e < V; ++e) v[u].v[e] = rounded<T>(Cvt<T>::up(v[u].v[e]) * factor);
       store_pack_unaligned<true>(out + (int64_t)row[u] * dim + at[u], v[u]);
@@ -58,25 +59,23 @@ __global__ __launch_bounds__(kBlock) void lookup_kernel(T* __restrict__ out, con
 template <typename T>
 void launch_lookup(THCState* s, T* out, const T* table, const int64_t* tokens, int64_t count, int64_t vocab, int64_t tableStride, int64_t dim,
                    float factor) {
-  hipStream_t st = current_stream(s);
-  auto go = [&](auto vTag, auto uTag, auto idxTag) {
-    using I = decltype(idxTag);
-    constexpr int V = decltype(vTag)::value, U = decltype(uTag)::value;
-    const int64_t packs = (dim + V - 1) / V, items = count * packs;
-    Divisor<I> d;
-    d.set((uint64_t)packs);
-    const dim3 grid((unsigned)((items + kBlock * U - 1) / (kBlock * U)));
-    hipLaunchKernelGGL((lookup_kernel<T, V, U, I>), grid, dim3(kBlock), 0, st, out, table, tokens, vocab, tableStride, (int32_t)dim, (I)items, d,
-                       factor);
-  };
-  constexpr int kPack = 16 / sizeof(T);
-  auto width = [&](auto uTag, auto idxTag) {
-    if (dim >= kPack) go(std::integral_constant<int, kPack>{}, uTag, idxTag);
-    else go(std::integral_constant<int, 1>{}, uTag, idxTag);
-  };
-  const int64_t items = count * (dim >= kPack ? (dim + kPack - 1) / kPack : dim);
-  if (force_64bit_index() || items + 4 * kBlock >= kIndex32Limit) width(std::integral_constant<int, 4>{}, uint64_t{});
-  else width(std::integral_constant<int, 4>{}, uint32_t{});
+  constexpr int kPack = 16 / sizeof(T), U = 4;
+  const int V = dim >= kPack ? kPack : 1;
+  const int64_t packs = (dim + V - 1) / V;
+  Divisor<uint32_t> d;
+  d.set((uint64_t)packs);
+  // rows by the 2^30 items: a launch counts them in 32 bits
+  const int64_t most = std::max<int64_t>(1, tuning("embedding.items", 1 << 30) / packs);
+  for (int64_t first = 0; first < count; first += most) {
+    const uint32_t items = (uint32_t)(std::min(most, count - first) * packs);
+    const dim3 grid((items + kBlock * U - 1) / (kBlock * U));
+    if (V == 1)
+      hipLaunchKernelGGL((lookup_kernel<T, 1, U>), grid, dim3(kBlock), 0, current_stream(s), out + first * dim, table, tokens + first, vocab,
+                         tableStride, (int32_t)dim, items, d, factor);
+    else
+      hipLaunchKernelGGL((lookup_kernel<T, kPack, U>), grid, dim3(kBlock), 0, current_stream(s), out + first * dim, table, tokens + first,
+                         vocab, tableStride, (int32_t)dim, items, d, factor);
+  }
 }
 
 void check_table(const AnyTensor* table, int arg) {
@@ -648,7 +647,7 @@ void launch_grad(THCState* s, T* grad, int64_t vocab, int64_t gradStride, const 
   // us in three launches and in one (halves, added): 16 positions of 513 9.7, 3.9; 512 x 2048 12.4, 7.5; 1024 x 513 13.6, 9.4; 1500 x 64 12.9,
   // 10.0; 1024 x 2048 14.5, 14.0; 1500 x 2048 15.3, 20.4; 512 x 8192 15.8, 16.9: the one launch's time goes with the workgroups times what
   // each looks at.
-  if (n <= kFew && (int64_t)n * n * fewSlabs <= tuning("embedding.few", 3 << 20)) {
+  if (n <= kFew && vocab <= int64_t(1) << 28 && (int64_t)n * n * fewSlabs <= tuning("embedding.few", 3 << 20)) {
     const dim3 grid((unsigned)(n + (add ? 0 : (vocab + kFewRows - 1) / kFewRows)), fewSlabs);
     const uint32_t left = (uint32_t)(padding - 1);
     if (V == 1)
@@ -719,7 +718,7 @@ void embedding_grad(THCState* s, DType dt, AnyTensor* grad, AnyTensor* tokens, A
   const int64_t count = tensor_numel(tokens), vocab = grad->size[0], dim = grad->size[1];
   THC_ARG_CHECK(tensor_numel(out) == count * dim, 4, "%ld elements of the output's gradient for %ld tokens of %ld",
                 (long)tensor_numel(out), (long)count, (long)dim);
-  THC_ARG_CHECK(count <= int64_t(1) << 30, 3, "too many tokens");
+  THC_ARG_CHECK(count <= int64_t(1) << 29, 3, "too many tokens");
   THC_ARG_CHECK(vocab < kIndex32Limit, 2, "the table has too many rows");
   THC_ARG_CHECK(padding >= 0 && padding <= vocab, 6, "the padding token is outside the table");
   if (count == 0) {

@@ -77,6 +77,10 @@ struct RowParts {
   __device__ __forceinline__ float load_edge(int32_t i) const { return i >= 0 ? Cvt<T>::up(row[i]) : minus_infinity(); }
 };
 
+// Rows go along the grid's x and, behind the first 2^21 of them, y (a launch has less than 2^32 threads in a dim).
+constexpr int kRowsAcross = 21;
+__device__ __forceinline__ uint32_t grid_row() { return blockIdx.x + (blockIdx.y << kRowsAcross); }
+
 struct RowOffsets {
   int64_t stride, outerStride;
   Divisor<uint32_t> inner;
@@ -255,14 +259,15 @@ __device__ __forceinline__ void load_to_lds(const void* from, void* to) {
 // once each way. What is longer than that is read again for the gradient (REST). E: waves a SIMD that the registers leave room for.
 template <typename T, int W, int R, int L, int E, bool REST>
 __global__ __launch_bounds__(W * 64) __attribute__((amdgpu_waves_per_eu(E, E))) void held_row_kernel(PolicyArgs a, const T* logits, RowOffsets lo, T* grad,
-                                                                                               RowOffsets go, int32_t vocab) {
+                                                                                               RowOffsets go, int32_t vocab, uint32_t rows) {
   constexpr int U = R < 4 ? R : 4, kStep = W * 64, V = 16 / sizeof(T);
   using P = Pack<T, V>;
   __shared__ Soft lds[W];
   extern __shared__ __attribute__((aligned(16))) char room[];      // L packs a lane
   P(*more)[W][64] = reinterpret_cast<P(*)[W][64]>(room);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const uint32_t row = blockIdx.x;
+  const uint32_t row = grid_row();
+  if (row >= rows) return;
   const Position at = position_of(a, row);
   T* out = grad + go.at(row);
   if (at.weight == 0.f) {
@@ -332,11 +337,12 @@ __global__ __launch_bounds__(W * 64) __attribute__((amdgpu_waves_per_eu(E, E))) 
 
 // Losses and log-probabilities alone: a workgroup has a row.
 template <typename T, int W>
-__global__ __launch_bounds__(W * 64) void row_kernel(PolicyArgs a, const T* __restrict__ logits, RowOffsets lo, int32_t vocab) {
+__global__ __launch_bounds__(W * 64) void row_kernel(PolicyArgs a, const T* __restrict__ logits, RowOffsets lo, int32_t vocab, uint32_t rows) {
   constexpr int U = 4, kStep = W * 64, V = 16 / sizeof(T);
   using P = Pack<T, V>;
   __shared__ Soft lds[W];
-  const uint32_t row = blockIdx.x;
+  const uint32_t row = grid_row();
+  if (row >= rows) return;
   const Position at = position_of(a, row);
   if (at.weight == 0.f) {
     skip_row<T, W, false>(a, row, (T*)nullptr, vocab);
@@ -443,7 +449,8 @@ RowOffsets offsets_of(const Rows& r) {
 template <typename T>
 void launch_rows(THCState* s, const PolicyArgs& a, const T* logits, const Rows& lr, T* grad, const Rows& gr) {
   hipStream_t st = current_stream(s);
-  const dim3 grid((unsigned)lr.count);
+  const uint32_t rows = (uint32_t)lr.count;
+  const dim3 grid(std::min(rows, 1u << kRowsAcross), (rows + (1u << kRowsAcross) - 1) >> kRowsAcross);
   const int32_t vocab = (int32_t)lr.length;
   constexpr int V = 16 / sizeof(T);
   const int32_t packs = vocab / V + 7;      // at most, with those that a line's begin is before the row
@@ -472,7 +479,7 @@ void launch_rows(THCState* s, const PolicyArgs& a, const T* logits, const Rows& 
     // 56, 88; 1000 x 32000 22, 14.5, 16, 15, 18.5; 600 x 128000 72, 42, 45, 31, 35; 256 x 16000 fp32 with 4 and 16 11.4, 6.9.
     auto go = [&](auto wTag) {
       constexpr int W = decltype(wTag)::value;
-      hipLaunchKernelGGL((row_kernel<T, W>), grid, dim3(W * 64), 0, st, a, logits, lo, vocab);
+      hipLaunchKernelGGL((row_kernel<T, W>), grid, dim3(W * 64), 0, st, a, logits, lo, vocab, rows);
     };
     const int64_t want = 4800;
     if (lr.count >= want || packs < 256) go(integral_constant<int, 1>{});
@@ -485,7 +492,7 @@ void launch_rows(THCState* s, const PolicyArgs& a, const T* logits, const Rows& 
   auto held = [&](auto waves, auto registers, auto shared, auto perSimd, auto rest) {
     constexpr int W = decltype(waves)::value, R = decltype(registers)::value, L = decltype(shared)::value;
     hipLaunchKernelGGL((held_row_kernel<T, W, R, L, decltype(perSimd)::value, decltype(rest)::value>), grid, dim3(W * 64), L * W * 64 * 16, st, a,
-                       logits, lo, grad, go, vocab);
+                       logits, lo, grad, go, vocab, rows);
   };
 #define HELD(W, R, L, E, REST)                                                                                            \
   held(integral_constant<int, W>{}, integral_constant<int, R>{}, integral_constant<int, L>{}, integral_constant<int, E>{}, \

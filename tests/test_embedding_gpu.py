@@ -63,16 +63,16 @@ def test_lookup_views(thc, kind):
 
 
 @pytest.mark.parametrize("kind", ["float", "half"])
-def test_lookup_outside_and_wide_index(thc, kind):
+def test_lookup_outside_and_in_pieces(thc, kind):
     rng = np.random.default_rng(6)
     table = _table(rng, 9, 33, kind)
     tokens = np.array([1, 0, 9, 10, -1, 5, 2 ** 40, -2 ** 62, 3])
-    for wide in (False, True):
-        thc.force_64bit_index(wide)
+    for items in (1 << 30, 20, 1):      # as much as one launch takes
+        thc.set_tuning("embedding.items", items)
         try:
             got = thc.Tensor(kind).embedding(_tensor(thc, table), _tensor(thc, tokens), 3.0).numpy()
         finally:
-            thc.force_64bit_index(False)
+            thc.set_tuning("embedding.items", 1 << 30)
         want = _lookup(table, tokens, 3.0)
         assert np.array_equal(np.isnan(got), np.isnan(want))
         assert np.array_equal(got[~np.isnan(got)], want[~np.isnan(want)])

@@ -249,6 +249,20 @@ def test_rows_that_hold_nothing_to_learn_from(thc, rows_are, kind, vocab):
     assert got[6] == -np.inf and loss[6] == 0 and not grad[6].any()
 
 
+def test_more_rows_than_a_grid_has_across(thc):
+    """2^21 rows and some, of three logits."""
+    rng = np.random.default_rng(3)
+    rows = (1 << 21) + 1000
+    case = _case(rng, rows, 3, "half", False, True)
+    x, tokens, old, advantage, _, weight = case
+    want = _policy(x, tokens, old.astype(np.float64), advantage.astype(np.float64), None, weight.astype(np.float64), 0.2, 0.25, 0, 1.0)
+    b_loss, b_lp, b_grad = _bounds(x, tokens, old, advantage, None, weight, 0, 1.0, want, "half")
+    loss, lp, grad = _run(thc, case)
+    assert np.all(np.abs(loss - want[0]) <= b_loss) and np.all(np.abs(grad - want[2]) <= b_grad)
+    got = thc.Tensor("float").token_log_prob(thc.Tensor.from_numpy(x), thc.Tensor.from_numpy(tokens)).numpy()
+    assert np.all(np.abs(got - want[1]) <= b_lp) and np.all(np.abs(lp - want[1])[weight != 0] <= b_lp[weight != 0])
+
+
 def test_gradient_against_differences(thc):
     """Central differences of the losses themselves, at logits that move one at a time by 2^-6: they are off by h^2/6 times the third
     derivative (some units here) and by the losses' own rounding over h."""
