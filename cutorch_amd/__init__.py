@@ -7,6 +7,7 @@ and the benchmark. Every method is one call into the C ABI declared in
 include/THC.h; nothing here computes. Loading fails loudly if the library has
 not been built (`python -m cutorch_amd.build`): there is no fallback path.
 """
+import array
 import ctypes as C
 import os
 import struct
@@ -698,16 +699,16 @@ class AdamW(object):
         else:
             lists += [(self.mean, "float"), (self.square, "float")]
         self._arrays = [self._array(l, kind) for l, kind in lists]
-        self._args = [C.addressof(a) if a is not None else 0 for a in self._arrays]
+        self._args = [a.buffer_info()[0] if a is not None else 0 for a in self._arrays]
 
     def _array(self, tensors, kind):
         if tensors is None:
             return None
         if len(tensors) != len(self.params):
             raise ValueError("%d tensors for %d parameters" % (len(tensors), len(self.params)))
-        if any(t.kind != kind for t in tensors):
+        if any([t.kind != kind for t in tensors]):
             raise ValueError("a tensor of another type than %s" % kind)
-        return (C.c_void_p * max(1, len(tensors)))(*[t.a for t in tensors])
+        return array.array("Q", [t.a for t in tensors])
 
     def step(self, grad_scale=1.0):
         """One step from what the gradients hold, times grad_scale."""
@@ -722,7 +723,7 @@ class AdamW(object):
         mean = [Tensor("float") for _ in self.params] if mean is None else mean
         square = [Tensor("float") for _ in self.params] if square is None else square
         arrays = [self._array(mean, "float"), self._array(square, "float")]
-        _CALLS["float"]["adamW8Moments"](len(self.params), *[C.addressof(a) for a in arrays], *self._args[-4:])
+        _CALLS["float"]["adamW8Moments"](len(self.params), *[a.buffer_info()[0] for a in arrays], *self._args[-4:])
         return mean, square
 
 
