@@ -4,9 +4,9 @@
 //   embeddingGrad   dW[v, :] = f sum over the i with t_i = v of dY[i, :]      (or dW += that)
 //
 // Tokens are 1-based as all indices of this library are. A token outside the table reads nothing: its output row is NaN and its
-// gradient goes nowhere. Sums are in float, in the order of the positions, and are rounded once: the same call gives the same bits.
+// gradient goes nowhere. Sums are in float and in an order that the sizes and tokens alone decide; the product with f and what it is
+// added to round in float, the result once more to its type.
 #include <algorithm>
-#include <limits>
 
 #include "training.hpp"
 
@@ -80,7 +80,7 @@ void launch_lookup(THCState* s, T* out, const T* table, const int64_t* tokens, i
 
 void check_table(const AnyTensor* table, int arg) {
   THC_ARG_CHECK(table->nDimension == 2, arg, "the table must have two dims, has %d", table->nDimension);
-  THC_ARG_CHECK(table->size[1] < (int64_t(1) << 30), arg, "rows of the table are too long");
+  THC_ARG_CHECK(table->size[1] <= (int64_t(1) << 23), arg, "rows of the table are too long");      // (256 columns a workgroup along a grid's y)
 }
 
 void embedding(THCState* s, DType dt, AnyTensor* self, AnyTensor* table, AnyTensor* tokens, float factor) {
@@ -125,7 +125,7 @@ void embedding(THCState* s, DType dt, AnyTensor* self, AnyTensor* table, AnyTens
 //   group   the positions of each token side by side, in their order: slot -> position and token
 //   sum     chunks of slots are summed in registers; a token whose slots lie in one chunk is done, one that crosses a chunk's
 //           edge leaves a partial sum. Rows of tokens that do not occur are zeroed by other workgroups of this launch.
-//   fold    the partial sums of each token that crosses edges, in the chunks' order
+//   fold    the partial sums of each token that crosses edges
 
 // Grouping. Token k (0-based) belongs to owner k mod G. An owner sweeps the tokens twice, counts its own and places them; the tokens of
 // the owners before it, which it counts on the way, say where its slots begin: no owner waits for another. A token's slots are side
@@ -719,7 +719,7 @@ void embedding_grad(THCState* s, DType dt, AnyTensor* grad, AnyTensor* tokens, A
   THC_ARG_CHECK(tensor_numel(out) == count * dim, 4, "%ld elements of the output's gradient for %ld tokens of %ld",
                 (long)tensor_numel(out), (long)count, (long)dim);
   THC_ARG_CHECK(count <= int64_t(1) << 29, 3, "too many tokens");
-  THC_ARG_CHECK(vocab < kIndex32Limit, 2, "the table has too many rows");
+  THC_ARG_CHECK(vocab <= int64_t(1) << 30, 2, "the table has too many rows");
   THC_ARG_CHECK(padding >= 0 && padding <= vocab, 6, "the padding token is outside the table");
   if (count == 0) {
     if (!accumulate && !pointwise_apply(s, dt, PointOp::Fill, 0.f, grad, nullptr, nullptr, nullptr)) raise_arg_error(2, "%s", kDimWarning);

@@ -18,36 +18,63 @@ namespace {
 constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
 __device__ __forceinline__ float minus_infinity() { return -__builtin_inff(); }
 
-// A running maximum, times log2(e) and rounded, and the sum of 2^(x log2(e) - m) below it. What the rounding moved cancels: the chosen
-// logit and the gradient's exponentials are measured from the same m. x log2(e) - m is one operation and rounds once, near 0 for the
-// values that count. The empty part has -inf and 0; so has one all of whose values are -inf.
+// A running maximum and the sum of 2^(distance below it), distances in powers of two. The empty part has -inf and 0; so has one all of
+// whose values are -inf.
+//   half   m is the maximum times log2(e), rounded; x log2(e) - m is one operation, which takes x as it is, and rounds once, near 0 for the
+//          values that count. What m's rounding moved cancels: the chosen logit and the gradient are measured from the same m.
+//   float  m is the maximum itself and (x - m) log2(e) two operations: the product with m overflows where a whole row holds the type's
+//          lowest value.
 struct Soft {
   float m, s;
 };
-__device__ __forceinline__ float below(float x, float m) { return __builtin_fmaf(x, kLog2e, -m); }
-__device__ __forceinline__ float exp_below(float x, float m) { return __builtin_amdgcn_exp2f(below(x, m)); }
+template <typename T>
+__device__ __forceinline__ float scaled(float x) {
+  return sizeof(T) == 2 ? x * kLog2e : x;
+}
+template <typename T>
+__device__ __forceinline__ float below(float x, float m) {
+  if constexpr (sizeof(T) == 2) return __builtin_fmaf(x, kLog2e, -m);
+  else return (x - m) * kLog2e;
+}
+template <typename T>
+__device__ __forceinline__ float exp_below(float x, float m) {
+  return __builtin_amdgcn_exp2f(below<T>(x, m));
+}
+// What a sum below m becomes below `top`.
+template <typename T>
+__device__ __forceinline__ float lowered(float m, float top) {
+  return __builtin_amdgcn_exp2f(sizeof(T) == 2 ? m - top : (m - top) * kLog2e);
+}
 __device__ __forceinline__ float finite_or_zero(float m) { return m == minus_infinity() ? 0.f : m; }
+template <typename T>
 __device__ __forceinline__ Soft join(Soft a, Soft b) {
   const float m = fmaxf(a.m, b.m), safe = finite_or_zero(m);
-  return Soft{m, a.s * __builtin_amdgcn_exp2f(a.m - safe) + b.s * __builtin_amdgcn_exp2f(b.m - safe)};
+  return Soft{m, a.s * lowered<T>(a.m, safe) + b.s * lowered<T>(b.m, safe)};
 }
+template <typename T>
 __device__ __forceinline__ Soft wave_join(Soft a) {
 #pragma unroll
-  for (int d = 32; d >= 1; d >>= 1) a = join(a, Soft{__shfl_xor(a.m, d), __shfl_xor(a.s, d)});
+  for (int d = 32; d >= 1; d >>= 1) a = join<T>(a, Soft{__shfl_xor(a.m, d), __shfl_xor(a.s, d)});
   return a;
 }
-template <int W>
+template <typename T, int W>
 __device__ __forceinline__ Soft block_join(Soft a, Soft* lds) {
-  a = wave_join(a);
+  a = wave_join<T>(a);
   if constexpr (W > 1) {
     const int lane = threadIdx.x & 63;
     if (lane == 0) lds[threadIdx.x >> 6] = a;
     lds_barrier();
     a = lds[lane & (W - 1)];
 #pragma unroll
-    for (int d = W / 2; d >= 1; d >>= 1) a = join(a, Soft{__shfl_xor(a.m, d), __shfl_xor(a.s, d)});
+    for (int d = W / 2; d >= 1; d >>= 1) a = join<T>(a, Soft{__shfl_xor(a.m, d), __shfl_xor(a.s, d)});
   }
   return a;
+}
+// log(2^(x's distance below m) / s)
+template <typename T>
+__device__ __forceinline__ float log_share(float x, Soft soft) {
+  if constexpr (sizeof(T) == 2) return (below<T>(x, soft.m) - log2f(soft.s)) * kLn2;
+  else return (x - soft.m) - log2f(soft.s) * kLn2;
 }
 
 // A row as its aligned 16-byte packs and the elements before and behind them, of which lanes 0 to 15 of the first wave hold one each.
@@ -117,8 +144,9 @@ __device__ __forceinline__ Position position_of(const PolicyArgs& a, uint32_t ro
 }
 
 // Loss and log-probability of a row, by its first lane; returns the slope f w dl/dlp.
+template <typename T>
 __device__ __forceinline__ float policy_row(const PolicyArgs& a, uint32_t row, const Position& p, float chosen, Soft soft, bool write) {
-  const float lp = (below(chosen, soft.m) - log2f(soft.s)) * kLn2;
+  const float lp = log_share<T>(chosen, soft);
   if (!a.loss) {
     if (write) a.logProb[row] = lp;
     return 0.f;
@@ -157,7 +185,7 @@ __device__ __forceinline__ float sum_below(const Pack<T, 16 / sizeof(T)>& p, flo
   constexpr int V = 16 / sizeof(T);
   float s[V];
 #pragma unroll
-  for (int e = 0; e < V; ++e) s[e] = exp_below(Cvt<T>::up(p.v[e]), m);
+  for (int e = 0; e < V; ++e) s[e] = exp_below<T>(Cvt<T>::up(p.v[e]), m);
 #pragma unroll
   for (int w = V / 2; w >= 1; w /= 2) {
 #pragma unroll
@@ -178,7 +206,7 @@ __device__ __forceinline__ void store_gradient(T* out, int32_t i0, const Pack<T,
   constexpr int V = 16 / sizeof(T);
   float g[V];
 #pragma unroll
-  for (int e = 0; e < V; ++e) g[e] = r.c * exp_below(Cvt<T>::up(p.v[e]), r.m);
+  for (int e = 0; e < V; ++e) g[e] = r.c * exp_below<T>(Cvt<T>::up(p.v[e]), r.m);
   if ((uint32_t)(r.hit - i0) < (uint32_t)V) {
 #pragma unroll
     for (int e = 0; e < V; ++e)
@@ -200,19 +228,20 @@ __device__ __forceinline__ void store_gradient(T* out, int32_t i0, const Pack<T,
 }
 template <typename T>
 __device__ __forceinline__ void store_edge(T* out, int32_t i, float x, const RowSlope& r) {
-  if (i >= 0) out[i] = rounded<T>(r.c * exp_below(x, r.m) + (i == r.hit ? r.slope : 0.f));
+  if (i >= 0) out[i] = rounded<T>(r.c * exp_below<T>(x, r.m) + (i == r.hit ? r.slope : 0.f));
 }
+// Streaming stores for short rows, plain ones for long ones, whose workgroups are done when the caches have them (a tenth of the rows; us
+// with plain and with streaming ones: 16384 x 1000 halves 19.5, 18.5, 8192 x 32000 169, 178, 4096 x 100001 288, 293).
 template <typename T, int W>
 __device__ __forceinline__ void store_zeros(T* out, int32_t n) {
   constexpr int V = 16 / sizeof(T);
+  const RowParts<T> x(out, n);
   Pack<T, V> zero;
 #pragma unroll
   for (int e = 0; e < V; ++e) zero.v[e] = Cvt<T>::down(0.f);
-  for (int32_t i = threadIdx.x * V; i < n; i += W * 64 * V) {
-    if (i + V <= n) store_pack_unaligned<false>(out + i, zero);
-    else
-      for (int32_t j = i; j < n; ++j) out[j] = Cvt<T>::down(0.f);
-  }
+  if (x.edge() >= 0) out[x.edge()] = zero.v[0];
+  for (int32_t k = x.lane0 + (int32_t)threadIdx.x; k < x.packs; k += W * 64)
+    if (x.has(k)) store_pack_unaligned<W == 1>(out + x.head + k * V, zero);
 }
 
 // A row without a weight: its outputs are 0. (A NaN weight is one.)
@@ -235,17 +264,18 @@ __device__ __forceinline__ Soft take(Soft soft, const Pack<T, 16 / sizeof(T)>* v
   float m = soft.m;
 #pragma unroll
   for (int u = 0; u < U; ++u)
-    if ((uint32_t)(k + u * step) < (uint32_t)end) m = fmaxf(m, top_of<T>(v[u]) * kLog2e);
+    if ((uint32_t)(k + u * step) < (uint32_t)end) m = fmaxf(m, scaled<T>(top_of<T>(v[u])));
   const float safe = finite_or_zero(m);
-  float s = soft.s * __builtin_amdgcn_exp2f(soft.m - safe);
+  float s = soft.s * lowered<T>(soft.m, safe);
 #pragma unroll
   for (int u = 0; u < U; ++u)
     if ((uint32_t)(k + u * step) < (uint32_t)end) s += sum_below<T>(v[u], safe);
   return Soft{m, s};
 }
+template <typename T>
 __device__ __forceinline__ Soft take_edge(float x) {
-  const float m = x * kLog2e;
-  return Soft{m, m == minus_infinity() ? 0.f : exp_below(x, m)};
+  const float m = scaled<T>(x);
+  return Soft{m, m == minus_infinity() ? 0.f : exp_below<T>(x, m)};
 }
 
 // Direct load of one pack a lane into LDS: lane i's 16 bytes go to `to` + 16 i of the wave's part.
@@ -286,7 +316,8 @@ __global__ __launch_bounds__(W * 64) __attribute__((amdgpu_waves_per_eu(E, E))) 
     const int32_t k = x.lane0 + (int32_t)threadIdx.x + (R + u) * kStep;
     if (x.has(k)) load_to_lds(x.first + k, &more[u][wave][0]);
   }
-  const float chosen = chosen_of(x.row, at.token, vocab), edge = x.load_edge(x.edge());
+  float chosen = chosen_of(x.row, at.token, vocab);
+  const float edge = x.load_edge(x.edge());
   Soft soft{minus_infinity(), 0.f};
 #pragma unroll
   for (int u = 0; u < R; u += U) soft = take<T, U>(soft, v + u, x.lane0 + (int32_t)threadIdx.x + u * kStep, kStep, x.packs);
@@ -308,8 +339,10 @@ __global__ __launch_bounds__(W * 64) __attribute__((amdgpu_waves_per_eu(E, E))) 
       soft = take<T, U>(soft, q, k, kStep, x.packs);
     }
   }
-  soft = block_join<W>(join(soft, take_edge(edge)), lds);
-  const float slope = policy_row(a, row, at, chosen, soft, threadIdx.x == 0);
+  // (the barrier does not wait for loads, and behind it another wave may write where the chosen logit was)
+  asm volatile("" : "+v"(chosen));
+  soft = block_join<T, W>(join<T>(soft, take_edge<T>(edge)), lds);
+  const float slope = policy_row<T>(a, row, at, chosen, soft, threadIdx.x == 0);
   const RowSlope r{-slope / soft.s, slope, soft.m, (int32_t)at.token};
   store_edge(out, x.edge(), edge, r);
 #pragma unroll
@@ -350,7 +383,7 @@ __global__ __launch_bounds__(W * 64) void row_kernel(PolicyArgs a, const T* __re
   }
   const RowParts<T> x(logits + lo.at(row), vocab);
   const float chosen = chosen_of(x.row, at.token, vocab);
-  Soft soft = take_edge(x.load_edge(x.edge()));
+  Soft soft = take_edge<T>(x.load_edge(x.edge()));
   for (int32_t k = x.lane0 + (int32_t)threadIdx.x; k < x.packs; k += U * kStep) {
     P v[U];
 #pragma unroll
@@ -358,14 +391,15 @@ __global__ __launch_bounds__(W * 64) void row_kernel(PolicyArgs a, const T* __re
       if (x.has(k + u * kStep)) v[u] = x.load(k + u * kStep);
     soft = take<T, U>(soft, v, k, kStep, x.packs);
   }
-  soft = block_join<W>(soft, lds);
-  policy_row(a, row, at, chosen, soft, threadIdx.x == 0);
+  soft = block_join<T, W>(soft, lds);
+  policy_row<T>(a, row, at, chosen, soft, threadIdx.x == 0);
 }
 
 // Few long rows: each is cut into `parts` (at most 64) of `per` packs, a workgroup each, and a second launch joins their maxima and sums;
 // with a gradient every part joins them for itself and reads its packs again, from the caches.
 struct Parts {
   Soft* soft;       // of each row, side by side
+  float* chosen;    // of each row: the second launch may write the gradient over it
   int32_t parts, per;
 };
 template <typename T, int W>
@@ -376,7 +410,7 @@ __global__ __launch_bounds__(W * 64) void part_kernel(PolicyArgs a, const T* __r
   const uint32_t row = blockIdx.y, part = blockIdx.x;
   if (a.weight && a.weight[row] == 0.f) return;
   const RowParts<T> x(logits + lo.at(row), vocab);
-  Soft soft = take_edge(part == 0 ? x.load_edge(x.edge()) : minus_infinity());
+  Soft soft = take_edge<T>(part == 0 ? x.load_edge(x.edge()) : minus_infinity());
   const int32_t begin = x.lane0 + (int32_t)part * p.per, end = min(x.packs, begin + p.per);
   for (int32_t k = begin + (int32_t)threadIdx.x; k < end; k += U * kStep) {
     P v[U];
@@ -385,8 +419,11 @@ __global__ __launch_bounds__(W * 64) void part_kernel(PolicyArgs a, const T* __r
       if (k + u * kStep < end && x.has(k + u * kStep)) v[u] = x.load(k + u * kStep);
     soft = take<T, U>(soft, v, k, kStep, end);
   }
-  soft = block_join<W>(soft, lds);
-  if (threadIdx.x == 0) p.soft[(int64_t)row * p.parts + part] = soft;
+  soft = block_join<T, W>(soft, lds);
+  if (threadIdx.x == 0) {
+    p.soft[(int64_t)row * p.parts + part] = soft;
+    if (part == 0) p.chosen[row] = chosen_of(x.row, a.token[row] - 1, vocab);
+  }
 }
 template <typename T, int W, bool GRAD>
 __global__ __launch_bounds__(W * 64) void join_kernel(PolicyArgs a, const T* logits, RowOffsets lo, T* grad, RowOffsets go, int32_t vocab, Parts p) {
@@ -403,9 +440,9 @@ __global__ __launch_bounds__(W * 64) void join_kernel(PolicyArgs a, const T* log
   RowSlope r{0.f, 0.f, 0.f, -1};
   if (at.weight != 0.f) {
     if (lane < p.parts) soft = p.soft[(int64_t)row * p.parts + lane];
-    const float chosen = chosen_of(x.row, at.token, vocab);
-    soft = wave_join(soft);
-    const float slope = policy_row(a, row, at, chosen, soft, first);
+    const float chosen = p.chosen[row];
+    soft = wave_join<T>(soft);
+    const float slope = policy_row<T>(a, row, at, chosen, soft, first);
     r = RowSlope{-slope / soft.s, slope, soft.m, (int32_t)at.token};
   } else if (first) {
     if (a.loss) a.loss[row] = 0.f;
@@ -465,8 +502,9 @@ void launch_rows(THCState* s, const PolicyArgs& a, const T* logits, const Rows& 
     p.parts = (int32_t)std::max<int64_t>(1, std::min<int64_t>(64, 4096 / (lr.count * W)));
     p.per = ((packs + p.parts - 1) / p.parts + W * 64 - 1) / (W * 64) * (W * 64);
     p.parts = (packs + p.per - 1) / p.per;
-    Workspace w(s, lr.count * p.parts * (int64_t)sizeof(Soft));
+    Workspace w(s, lr.count * (p.parts * (int64_t)sizeof(Soft) + 4));
     p.soft = reinterpret_cast<Soft*>(w.data());
+    p.chosen = reinterpret_cast<float*>(p.soft + lr.count * p.parts);
     const dim3 cut((unsigned)p.parts, (unsigned)lr.count);
     hipLaunchKernelGGL((part_kernel<T, W>), cut, dim3(W * 64), 0, st, a, logits, lo, vocab, p);
     if (grad) hipLaunchKernelGGL((join_kernel<T, W, true>), cut, dim3(W * 64), 0, st, a, logits, lo, grad, go, vocab, p);

@@ -249,6 +249,29 @@ def test_rows_that_hold_nothing_to_learn_from(thc, rows_are, kind, vocab):
     assert got[6] == -np.inf and loss[6] == 0 and not grad[6].any()
 
 
+@pytest.mark.parametrize("kind", ["float", "half"])
+@pytest.mark.parametrize("vocab", [3, 700, 5000, 90001])
+def test_rows_of_one_extreme_value(thc, rows_are, kind, vocab):
+    """A mask of the type's lowest value over all of a row leaves every token as likely, whatever the value; so does its highest."""
+    low, high = np.finfo(NP[kind]).min, np.finfo(NP[kind]).max
+    x = np.stack([np.full(vocab, v, NP[kind]) for v in (low, high, low / 2, NP[kind](1))])
+    x[2, 1] = low            # one that is lower still has no chance
+    tokens = np.array([1, vocab, 1, 2])
+    got = thc.Tensor("float").token_log_prob(thc.Tensor.from_numpy(x), thc.Tensor.from_numpy(tokens)).numpy()
+    want = -np.log([vocab, vocab, vocab - 1, vocab])
+    assert np.all(np.abs(got - want) <= EPS * (vocab / 64 + 40 + 4 * np.abs(want)))
+    old, advantage = want.astype(np.float32), -np.ones(4, np.float32)
+    loss, lp, grad = _run(thc, (x, tokens, old, advantage, None, np.ones(4, np.float32)))
+    share = np.full((4, vocab), 1.0 / vocab)
+    share[2] = 1.0 / (vocab - 1)
+    share[2, 1] = 0
+    hot = np.zeros((4, vocab))
+    hot[np.arange(4), tokens - 1] = 1
+    # the ratios are 1 but for roundings, so are the slopes
+    bound = (EPS * (vocab / 32 + 200)) + (2.0 ** -11 * np.abs(hot - share) + 2.0 ** -25 if kind == "half" else 0)
+    assert np.all(np.abs(loss - 1) <= EPS * (vocab / 64 + 100)) and np.all(np.abs(grad - (hot - share)) <= bound)
+
+
 def test_more_rows_than_a_grid_has_across(thc):
     """2^21 rows and some, of three logits."""
     rng = np.random.default_rng(3)
