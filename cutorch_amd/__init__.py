@@ -596,17 +596,23 @@ class Tensor(object):
     # ---------------------------------------- a language model's training step --
     def embedding(self, weight, tokens, scale=1.0):
         """self = scale * the rows of `weight` that the (1-based) tokens name."""
+        if weight.kind != self.kind or tokens.kind != "long":
+            raise ValueError("rows of the table's type for long tokens")
         self._calls["embedding"](self.a, weight.a, tokens.a, scale)
         return self
 
     def embedding_grad(self, tokens, grad_output, scale=1.0, padding=0, accumulate=False):
         """self, sized as the table, = scale * the rows of grad_output summed by token; added to with `accumulate`.
         Positions of the token `padding` are left out."""
+        if grad_output.kind != self.kind or tokens.kind != "long":
+            raise ValueError("a gradient of the table's type for long tokens")
         self._calls["embeddingGrad"](self.a, tokens.a, grad_output.a, scale, padding, accumulate)
         return self
 
     def token_log_prob(self, logits, tokens):
         """self (float) = the log-probability of each row's token."""
+        if self.kind != "float" or tokens.kind != "long":
+            raise ValueError("float log-probabilities of long tokens")
         logits._calls["tokenLogProb"](self.a, logits.a, tokens.a)
         return self
 
@@ -614,6 +620,11 @@ class Tensor(object):
                     clip_high=0.2, kl=0.0, grad_scale=1.0):
         """self = each position's weighted clipped policy loss with its KL term, log_prob the tokens' log-probabilities,
         grad_logits (None: not wanted; may be the logits) grad_scale times the gradient of the losses' sum."""
+        for t in (self, log_prob, old, advantage, reference, weight):
+            if t is not None and t.kind != "float":
+                raise ValueError("losses, log-probabilities, advantages and weights are float")
+        if tokens.kind != "long" or (grad_logits is not None and grad_logits.kind != logits.kind):
+            raise ValueError("tokens are long, the gradient has the logits' type")
         logits._calls["policyLoss"](self.a, log_prob.a, grad_logits.a if grad_logits is not None else 0, logits.a, tokens.a, old.a,
                                     advantage.a, reference.a if reference is not None else 0, weight.a if weight is not None else 0,
                                     clip_low, clip_high, kl, grad_scale)

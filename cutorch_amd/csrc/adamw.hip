@@ -370,7 +370,7 @@ struct Held {
   }
   void* add(AnyTensor* t, DType dt, bool written) {
     if (tensor_is_contiguous(t)) return tensor_data(t, dt);
-    all.reserve(all.size() + 1);
+    if (all.size() == all.capacity()) all.reserve(2 * all.size() + 8);
     AnyTensor* dense = tensor_new_contiguous(s, t, dt);
     all.push_back(One{t, dense, dt, written});
     return tensor_data(dense, dt);
@@ -379,6 +379,12 @@ struct Held {
     for (One& o : all)
       if (o.written) copy_tensor(s, o.dt, o.tensor, o.dense, false);
   }
+};
+
+template <int POINTERS>
+struct Operands {
+  void* p[POINTERS];
+  int64_t size;
 };
 
 // Collects tensors of elements of these sizes and launches a kernel (by launch(args, grid)) for as many as its arguments hold.
@@ -417,8 +423,9 @@ struct Lists {
 
 int64_t state_blocks(int64_t n) { return (n + kStateBlock - 1) / kStateBlock; }
 
-void check_scales(const AnyTensor* scale, int64_t n, int arg, int index) {
+void check_scales(THCState* s, const AnyTensor* scale, int64_t n, int arg, int index) {
   THC_ARG_CHECK(scale, arg, "no scales of tensor %d's states", index + 1);
+  check_same_gpu(s, 1, &scale);
   THC_ARG_CHECK(tensor_numel(scale) == state_blocks(n), arg, "%ld scales for the %ld blocks of tensor %d's states", (long)tensor_numel(scale),
                 (long)state_blocks(n), index + 1);
 }
@@ -450,9 +457,9 @@ void adamw(THCState* s, DType dt, int count, const Lists& l, double lr, double b
     if (l.master) check_list(s, l.master[i], p, 4, i, true);
     check_list(s, l.grad[i], p, base, i, false);
     check_list(s, l.mean[i], p, base + 1, i, true);
-    if (eight) check_scales(l.meanScale[i], tensor_numel(p), base + 2, i);
+    if (eight) check_scales(s, l.meanScale[i], tensor_numel(p), base + 2, i);
     check_list(s, l.square[i], p, base + (eight ? 3 : 2), i, true);
-    if (eight) check_scales(l.squareScale[i], tensor_numel(p), base + 4, i);
+    if (eight) check_scales(s, l.squareScale[i], tensor_numel(p), base + 4, i);
   }
   Hyper h;
   h.beta1 = (float)beta1;
@@ -486,12 +493,15 @@ void adamw(THCState* s, DType dt, int count, const Lists& l, double lr, double b
     };
     constexpr int kSize = sizeof(T), kState = E ? 1 : 4;
     const int sizes[7] = {kSize, kSize, kState, kState, E ? 0 : 4, 0, 4};
-    Batch<A, decltype(launch)> batch(h, part_size(E ? kStep8Packs : kStepPacks), sizes, launch);
+    // every copy is made before the first launch: a step that fails has changed nothing
+    std::vector<Operands<P>> all;
+    all.reserve(count);
     for (int i = 0; i < count; ++i) {
       if (!has_elements(l.param[i])) continue;
       note_stream_use(s, {l.param[i], M ? l.master[i] : nullptr, l.grad[i], l.mean[i], l.square[i], E ? l.meanScale[i] : nullptr,
                           E ? l.squareScale[i] : nullptr});
-      void* p[7];
+      Operands<P> o;
+      void** p = o.p;
       p[kParam] = held.add(l.param[i], dt, true);
       p[kGrad] = held.add(l.grad[i], dt, false);
       p[kMean] = held.add(l.mean[i], meanType, true);
@@ -501,8 +511,11 @@ void adamw(THCState* s, DType dt, int count, const Lists& l, double lr, double b
         p[kSquareScale] = held.add(l.squareScale[i], DType::F32, true);
       }
       if constexpr (M) p[P - 1] = held.add(l.master[i], DType::F32, true);
-      batch.add(p, tensor_numel(l.param[i]));
+      o.size = tensor_numel(l.param[i]);
+      all.push_back(o);
     }
+    Batch<A, decltype(launch)> batch(h, part_size(E ? kStep8Packs : kStepPacks), sizes, launch);
+    for (const Operands<P>& o : all) batch.add(o.p, o.size);
     batch.flush();
   };
   using std::false_type;
@@ -533,8 +546,8 @@ void moments(THCState* s, int count, AnyTensor** meanOut, AnyTensor** squareOut,
   for (int i = 0; i < count; ++i) {
     THC_ARG_CHECK(mean[i], 5, "tensor %d is missing", i + 1);
     check_list(s, square[i], mean[i], 7, i, false);
-    check_scales(meanScale[i], tensor_numel(mean[i]), 6, i);
-    check_scales(squareScale[i], tensor_numel(mean[i]), 8, i);
+    check_scales(s, meanScale[i], tensor_numel(mean[i]), 6, i);
+    check_scales(s, squareScale[i], tensor_numel(mean[i]), 8, i);
     THC_ARG_CHECK(meanOut[i], 3, "tensor %d is missing", i + 1);
     THC_ARG_CHECK(squareOut[i], 4, "tensor %d is missing", i + 1);
   }

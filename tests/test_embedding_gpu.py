@@ -276,6 +276,11 @@ def test_refusals(thc):
         w.embedding_grad(t, y, padding=6)
     with pytest.raises(thc.THCError, match="overlap"):
         w.view_as_strided(0, (5, 4), (0, 1)).embedding_grad(t, y)
+    half = thc.Tensor("half").resize((2, 4)).zero()
+    for call in (lambda: thc.Tensor("half").embedding(w, t), lambda: thc.Tensor("float").embedding(w, y), lambda: w.embedding_grad(t, half),
+                 lambda: w.embedding_grad(y, y)):
+        with pytest.raises(ValueError):
+            call()
     # no tokens: an empty output, a gradient of zeros
     assert thc.Tensor("float").embedding(w, thc.Tensor("long")).shape == ()
     w.fill(3).embedding_grad(thc.Tensor("long"), thc.Tensor("float"), accumulate=True)

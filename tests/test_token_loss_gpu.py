@@ -346,3 +346,9 @@ def test_refusals(thc):
     for low, high in ((-0.1, 0.2), (1.5, 0.2), (0.2, -0.2), (float("nan"), 0.2)):
         with pytest.raises(thc.THCError, match="clipped"):
             f().policy_loss(f(), f(), x, tokens, per, per, clip_low=low, clip_high=high)
+    half, longs = thc.Tensor("half"), thc.Tensor("long")
+    for call in (lambda: half.token_log_prob(x, tokens), lambda: f().token_log_prob(x, per), lambda: half.policy_loss(f(), f(), x, tokens, per, per),
+                 lambda: f().policy_loss(f(), half, x, tokens, per, per), lambda: f().policy_loss(longs, f(), x, tokens, per, per),
+                 lambda: f().policy_loss(f(), f(), x, tokens, per, half), lambda: f().policy_loss(f(), f(), x, per, per, per)):
+        with pytest.raises(ValueError):
+            call()
