@@ -141,10 +141,11 @@ struct Grouping {
 constexpr int kGroupThreads = 1024, kGroupWaves = kGroupThreads / 64;
 constexpr int kOwnTokens = 512;      // tokens that one owner takes at most: 32 KiB of counts
 constexpr int kFound = 512;          // positions that a wave remembers between its two sweeps: 64 KiB
-constexpr int kTile = 4096;          // positions that are split together, 4 a lane
-// Splitting costs a launch and saves every owner the sight of the others' positions. us of the whole gradient, swept and split: 1500 x 513
-// 15, 20; 32768 x 1024 47, 51; 49152 x 1024 62, 63; 65536 x 1024 75, 74; 131072 x 1024 167, 124; 300000 x 64 224, 108 (halves, added).
-constexpr int kSplitFrom = 57344;
+constexpr int kTile = 1024;          // positions that are split together, one a lane
+// Splitting costs a launch and saves every owner the sight of the others' positions. us of the whole gradient, swept and split: 8192 x 1024
+// 26.6, 29.6; 32768 x 1024 47.0, 47.1; 65536 x 1024 75, 71; 131072 x 1024 206, 122; 300000 x 64 315, 110 (halves, added). With tiles of
+// 4096 instead of 1024 positions the split ones take 35, 51, 74, 125, 106.
+constexpr int kSplitFrom = 40000;
 constexpr int kMostSplit = 1024;     // owners that they are split between
 constexpr int kAhead = 8;            // loads in flight
 
@@ -152,6 +153,17 @@ __device__ __forceinline__ int wave_sum(int v) {
 #pragma unroll
   for (int m = 32; m >= 1; m >>= 1) v += __shfl_xor(v, m);
   return v;
+}
+
+// The lanes among those with `valid` that hold what this one holds, of `bits` bits: found bit by bit.
+__device__ __forceinline__ uint64_t equal_lanes(uint32_t what, int bits, bool valid) {
+  uint64_t peers = __ballot(valid);
+  for (int b = 0; b < bits; ++b) {
+    const bool one = (what >> b) & 1;
+    const uint64_t set = __ballot(one);
+    peers &= one ? set : ~set;
+  }
+  return peers;
 }
 
 // Calls f(position, token, whether it is one of the table's and not padding) for positions [first, last), 64 side by side and in order.
@@ -174,7 +186,7 @@ __device__ __forceinline__ void each_token(const int64_t* __restrict__ tokens, i
 }
 
 // A tile's positions by owner, in order within each: entries (position, token) and where each owner's begin; padding and tokens outside
-// the table are left out. Equal owners among a wave's lanes are found bit by bit.
+// the table are left out.
 struct Split {
   int2* entry;        // kTile per tile
   int32_t* begin;     // owners + 1 per tile
@@ -198,11 +210,7 @@ __global__ __launch_bounds__(kGroupThreads) void split_kernel(Split to, const in
   for (int u = 0; u < kPer; ++u) {
     const uint32_t token = (uint32_t)k[u] - 1, owner = token & mask;
     valid[u] = (k[u] >> 32) == 0 && token < vocab && token != padding && first + u * 64 < n;
-    uint64_t peers = __ballot(valid[u]);
-    for (int bit = 0; bit < shift; ++bit) {
-      const uint64_t set = __ballot((owner >> bit) & 1);
-      peers &= (owner >> bit) & 1 ? set : ~set;
-    }
+    const uint64_t peers = equal_lanes(owner, shift, valid[u]);
     if (valid[u]) {
       const int at = counts[wave][owner];
       rank[u] = at + __popcll(peers & below);
@@ -265,15 +273,31 @@ __global__ __launch_bounds__(kGroupThreads) void group_kernel(Grouping g, Split 
   // The owner's positions, in order: f(position, token, whether it is the owner's). A wave takes a run of positions, or of tiles.
   auto sweep = [&](const auto& f) {
     if constexpr (SPLIT) {
+      // its shares of a few tiles are asked for together: where they lie, then the first 128 entries of each
+      constexpr int U = kAhead / 2;
       const int tiles = (n + kTile - 1) / kTile, run = (tiles + kGroupWaves - 1) / kGroupWaves;
       const int last = min(tiles, (wave + 1) * run);
-      for (int t = wave * run; t < last; ++t) {
-        const int32_t* begin = split.begin + (int64_t)t * (mask + 2) + me;
-        const int2* entry = split.entry + (int64_t)t * kTile;
-        const int from = begin[0], to = begin[1];
-        for (int j = from; j < to; j += 64) {
-          const int2 e = entry[min(j + lane, to - 1)];
-          f(e.x, (uint32_t)e.y, j + lane < to);
+      for (int t0 = wave * run; t0 < last; t0 += U) {
+        const int32_t* begin = split.begin + (int64_t)min(t0 + (lane >> 1), last - 1) * (mask + 2) + me + (lane & 1);
+        const int bound = lane < 2 * U ? *begin : 0;
+        int from[U], to[U];
+        int2 e[U], more[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          from[u] = __builtin_amdgcn_readlane(bound, 2 * u);
+          to[u] = t0 + u < last ? __builtin_amdgcn_readlane(bound, 2 * u + 1) : from[u];
+          const int2* entry = split.entry + (int64_t)(t0 + u) * kTile + from[u] + lane;
+          if (from[u] + lane < to[u]) e[u] = entry[0];
+          if (from[u] + 64 + lane < to[u]) more[u] = entry[64];
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          if (from[u] < to[u]) f(e[u].x, (uint32_t)e[u].y, from[u] + lane < to[u]);
+          if (from[u] + 64 < to[u]) f(more[u].x, (uint32_t)more[u].y, from[u] + 64 + lane < to[u]);
+          for (int j = from[u] + 128; j < to[u]; j += 64) {
+            const int2 rest = split.entry[(int64_t)(t0 + u) * kTile + min(j + lane, to[u] - 1)];
+            f(rest.x, (uint32_t)rest.y, j + lane < to[u]);
+          }
         }
       }
     } else {
@@ -338,28 +362,22 @@ __global__ __launch_bounds__(kGroupThreads) void group_kernel(Grouping g, Split 
   if (me == mask && threadIdx.x == kGroupThreads - 1) *g.total = slot;
   __syncthreads();
   // up to 64 occurrences, in order: the lanes that hold one token take its next slots
+  const int bits = owned > 1 ? 32 - __clz(owned - 1) : 0;
   auto place = [&](int32_t position, int which, bool own) {
-    uint64_t left = __ballot(own);
-    while (left) {
-      const int leader = __ffsll((unsigned long long)left) - 1;
-      const int token = __shfl(which, leader);
-      const bool same = ((left >> lane) & 1) && which == token;
-      const uint64_t peers = __ballot(same);
-      const int at = counts[wave][token];
-      if (same) {
-        const int to = at + __popcll(peers & below);
-        g.position[to] = position;
-        g.token[to] = (int32_t)(me + ((uint32_t)token << shift));
-      }
+    if (!__ballot(own)) return;
+    const uint64_t peers = equal_lanes(which, bits, own);
+    if (own) {
+      const int at = counts[wave][which], to = at + __popcll(peers & below);
+      g.position[to] = position;
+      g.token[to] = (int32_t)(me + ((uint32_t)which << shift));
       __builtin_amdgcn_wave_barrier();
-      if (lane == leader) counts[wave][token] = at + __popcll(peers);
-      __builtin_amdgcn_wave_barrier();
-      left &= ~peers;
+      if ((peers & below) == 0) counts[wave][which] = at + __popcll(peers);
     }
+    __builtin_amdgcn_wave_barrier();
   };
   if (mine <= kFound) {
     for (int i = lane; i - lane < mine; i += 64) {
-      const int2 f = found[wave][min(i, kFound - 1)];
+      const int2 f = found[wave][min(i, mine - 1)];
       place(f.x, f.y, i < mine);
     }
   } else {      // a common token's owner: its positions again

@@ -151,7 +151,7 @@ def split(thc):
     thc.set_tuning("embedding.split", 0)
     thc.set_tuning("embedding.few", 0)
     yield
-    thc.set_tuning("embedding.split", 57344)
+    thc.set_tuning("embedding.split", 40000)
     thc.set_tuning("embedding.few", 3 << 20)
 
 
