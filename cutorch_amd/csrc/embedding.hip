@@ -18,7 +18,8 @@ namespace {
 // workgroup. Packs lie at element-aligned addresses (rows of any length), a row's last one is moved back into the row and
 // repeats elements of the one before it: the same values are written twice, nothing needs a tail. Stores are streaming ones at every
 // size (us with plain ones and so: 2048 rows of 2048 halves 4.9, 4.8, 8192 x 1024 6.5, 5.5, 65536 x 1024 43.5, 29.0); table rows may
-// come again and are read plainly.
+// come again and are read plainly. Bound by memory: 16392 x 2048 halves out of 32000 rows, as even as words in a text, 16.3 us, 5.5 TB/s of
+// rows written and distinct rows read; 16 rows take 3.3 us, a launch.
 template <typename T, int V, int U>
 __global__ __launch_bounds__(kBlock) void lookup_kernel(T* __restrict__ out, const T* __restrict__ table, const int64_t* __restrict__ tokens,
                                                         int64_t vocab, int64_t tableStride, int32_t dim, uint32_t items,
@@ -130,6 +131,8 @@ void embedding(THCState* s, DType dt, AnyTensor* self, AnyTensor* table, AnyTens
 // Grouping. Token k (0-based) belongs to owner k mod G. An owner sweeps the tokens twice, counts its own and places them; the tokens of
 // the owners before it, which it counts on the way, say where its slots begin: no owner waits for another. A token's slots are side
 // by side and its positions in order; the order of the tokens does not matter to the sums.
+// Bound by latency, sweep by sweep, and by how often the commonest token is counted: 1500 positions 5.6 us, 32768 12.3, 131072 split 23 behind
+// the splitting's 5.
 // Few positions are swept as they are, by every owner. Of many, each owner would look at all: they are first split, tile by tile, into
 // the owners' shares.
 struct Grouping {
@@ -429,7 +432,10 @@ __device__ __forceinline__ void write_partial(float* to, const float (&acc)[V]) 
   }
 }
 
-// V columns a lane; a row's last lane is moved back into the row and leaves the columns that it shares to the lane before it.
+// V columns a lane; a row's last lane is moved back into the row and leaves the columns that it shares to the lane before it. Bound by
+// memory: 32768 x 2048 halves into 50000 rows 63 us, 5.4 TB/s of rows read and written, besides the partial sums, which stay in the caches. (A run
+// that crosses one edge summed to its end by the chunk that it begins in: the fold 6.9 -> 5.4 us, but this 63 -> 72; the few chunks that
+// go on are the launch's end.)
 template <typename T, int V, int U>
 __global__ __launch_bounds__(kBlock) void sum_kernel(GradArgs a, const T* __restrict__ out, T* __restrict__ grad, int64_t vocab,
                                                      int32_t chunkBlocks) {
@@ -493,7 +499,7 @@ __global__ __launch_bounds__(kBlock) void sum_kernel(GradArgs a, const T* __rest
 }
 
 // The token whose run begins in chunk c and goes on behind it: its partial sums. The workgroup's waves take them in turn, four columns
-// a lane, and their sums meet in LDS.
+// a lane, and their sums meet in LDS. 6.9 us for 32768 x 2048, half of it the start of workgroups that find nothing to fold.
 template <typename T>
 __global__ __launch_bounds__(kBlock) void fold_kernel(GradArgs a, T* __restrict__ grad) {
   constexpr int W = kBlock / 64, U = 4;
@@ -550,7 +556,8 @@ __global__ __launch_bounds__(kBlock) void fold_kernel(GradArgs a, T* __restrict_
 }
 
 // Few positions: one launch. A workgroup has one position and 64 lanes of columns; where its token has no earlier position, it lists the later
-// ones and sums their rows, its waves in turn. Every workgroup looks at all tokens, which is what bounds the number of positions.
+// ones and sums their rows, its waves in turn. Every workgroup looks at all tokens, which is what bounds the number of positions: 512 x 2048
+// halves 7.5 us.
 // Workgroups behind the positions zero the rows, kFewRows each, of tokens that do not occur.
 constexpr int kFew = 2048, kFewRows = 64;
 template <typename T, int V>

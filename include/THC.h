@@ -633,17 +633,17 @@ THC_API void THCudaTensor_sumallNoAlloc(THCState *state, THCudaTensor *self, flo
 /* rows with unit stride along the last dim).                                */
 /* ------------------------------------------------------------------------ */
 #define THC_AMD_DECLARE_TOKEN_API(Tensor)                                      \
-  /* self[..., :] = scale * weight[token, :], rounded once. `weight` has two  \
-   * dims; self takes the tokens' sizes and the rows' length. A token outside \
-   * the table reads nothing, its row is NaN. */                               \
+  /* self[..., :] = scale * weight[token, :], a product of floats rounded to  \
+   * the type. `weight` has two dims; self takes the tokens' sizes and the     \
+   * rows' length. A token outside the table reads nothing, its row is NaN. */ \
   THC_API void Tensor##_embedding(THCState *, Tensor *self, Tensor *weight,    \
                                   THCudaLongTensor *tokens, float scale);      \
   /* The gradient of that: gradWeight[v, :] = scale * the sum of gradOutput's  \
-   * rows whose token is v, summed in float in the order of the positions and  \
-   * rounded once; rows of other tokens become 0. With `accumulate` the sums  \
-   * are added to what gradWeight holds and other rows keep it. Positions of   \
-   * `paddingToken` (0: none) and of tokens outside the table are left out.    \
-   * gradWeight keeps its sizes. */                                            \
+   * rows whose token is v, summed in float in an order that the sizes and     \
+   * tokens alone decide; rows of other tokens become 0. With `accumulate` the \
+   * sums are added to what gradWeight holds and other rows keep it (one       \
+   * rounding to the type at the end). Positions of `paddingToken` (0: none)   \
+   * and of tokens outside the table are left out. gradWeight keeps its sizes. */ \
   THC_API void Tensor##_embeddingGrad(THCState *, Tensor *gradWeight,          \
                                       THCudaLongTensor *tokens,                \
                                       Tensor *gradOutput, float scale,         \
