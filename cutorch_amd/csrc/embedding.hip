@@ -662,25 +662,208 @@ __global__ __launch_bounds__(kBlock) void few_kernel(T* __restrict__ grad, int64
   if (wave == 0 && column < dim) finish_row<T, V>(grad + (int64_t)me * gradStride + c0, acc, factor, add, skip);
 }
 
+// Some thousand positions: one launch. A workgroup has an owner's tokens, grouped in LDS as above, and a strip of columns: short runs are summed
+// by a team of lanes each, long ones by all teams, whose sums meet in LDS; rows of tokens that do not occur are zeroed. Bound by latency, step by
+// step, and by the commonest token's workgroups: 1500 x 513 floats 8.1 us.
+constexpr int kOwn = 4096, kOwnWaves = 8, kLongRun = 16, kOwnGrid = 512;
+template <typename T, int V>
+__global__ __launch_bounds__(kOwnWaves * 64) void own_kernel(T* __restrict__ grad, int64_t gradStride, const int64_t* __restrict__ tokens, int32_t n,
+                                                             uint32_t vocab, uint32_t padding, const T* __restrict__ out, int64_t outStride,
+                                                             int32_t dim, int lanes, float factor, bool add, int shift) {
+  using P = Pack<T, V>;
+  constexpr int W = kOwnWaves, kPer = kOwn / (W * 64), U = 8;
+  static_assert(kOwnTokens == W * 64 && V * 64 <= kOwnTokens, "a thread for each token; the sums meet where the counts were");
+  __shared__ int counts[W][kOwnTokens];
+  __shared__ uint32_t found[W][kOwn / W];       // position and token, 16 bits each
+  __shared__ uint16_t list[kOwn], runToken[kOwnTokens], runStart[kOwnTokens + 1], longRun[kOwn / kLongRun];
+  __shared__ uint32_t waveTotal[W];
+  __shared__ uint64_t occurs[W];
+  float(*meet)[V][64] = reinterpret_cast<float(*)[V][64]>(counts);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const uint64_t below = (uint64_t(1) << lane) - 1;
+  const uint32_t mask = (1u << shift) - 1, me = blockIdx.x;
+  const int owned = (int)((vocab - 1 - me) >> shift) + 1;            // me < vocab
+  const int32_t run = (n + W * 64 - 1) / (W * 64) * 64, first = wave * run + lane;
+  uint64_t k[kPer];
+#pragma unroll
+  for (int u = 0; u < kPer; ++u)
+    if (u * 64 < run) k[u] = (uint64_t)tokens[min(first + u * 64, n - 1)];
+  for (int r = lane; r < owned; r += 64) counts[wave][r] = 0;        // (each wave its own)
+  int mine = 0;
+#pragma unroll
+  for (int u = 0; u < kPer; ++u) {
+    if (u * 64 < run) {
+      const int32_t i = first + u * 64;
+      const uint32_t token = (uint32_t)k[u] - 1;
+      const bool own = i < n && (k[u] >> 32) == 0 && token < vocab && token != padding && (token & mask) == me;
+      const uint64_t all = __ballot(own);
+      if (own) {
+        atomicAdd(&counts[wave][token >> shift], 1);      // whole numbers: any order gives the same
+        found[wave][mine + __popcll(all & below)] = (uint32_t)i | (token >> shift) << 16;
+      }
+      mine += __popcll(all);
+    }
+  }
+  __syncthreads();
+  // tokens in order, a thread each; counted side by side: positions (13 bits), tokens that occur (10), long runs
+  const int r = threadIdx.x;
+  int count[W], sum = 0;
+  if (r < owned) {
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+      count[w] = counts[w][r];
+      sum += count[w];
+    }
+  }
+  const uint32_t one = (uint32_t)sum | (sum > 0 ? 1u << 13 : 0) | (sum > kLongRun ? 1u << 23 : 0);
+  uint32_t upto = one;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const uint32_t o = __shfl_up(upto, d);
+    if (lane >= d) upto += o;
+  }
+  if (lane == 63) waveTotal[wave] = upto;
+  const uint64_t some = __ballot(sum > 0);
+  if (lane == 0) occurs[wave] = some;
+  __syncthreads();
+  uint32_t at = upto - one, total = 0;
+#pragma unroll
+  for (int w = 0; w < W; ++w) {
+    if (w < wave) at += waveTotal[w];
+    total += waveTotal[w];
+  }
+  const int runs = (total >> 13) & 1023, longs = total >> 23;
+  if (sum > 0) {
+    int slot = at & 8191;
+    const int u = (at >> 13) & 1023;
+    runToken[u] = (uint16_t)r;
+    runStart[u] = (uint16_t)slot;
+    if (sum > kLongRun) longRun[at >> 23] = (uint16_t)u;
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+      counts[w][r] = slot;
+      slot += count[w];
+    }
+  }
+  if (threadIdx.x == 0) runStart[runs] = (uint16_t)(total & 8191);
+  __syncthreads();
+  const int bits = owned > 1 ? 32 - __clz(owned - 1) : 0;
+  for (int i = lane; i - lane < mine; i += 64) {
+    const bool own = i < mine;
+    const uint32_t f = found[wave][min(i, mine - 1)], which = f >> 16;
+    const uint64_t peers = equal_lanes(which, bits, own);
+    if (own) {
+      const int to = counts[wave][which];
+      list[to + __popcll(peers & below)] = (uint16_t)f;
+      __builtin_amdgcn_wave_barrier();
+      if ((peers & below) == 0) counts[wave][which] = to + __popcll(peers);
+    }
+    __builtin_amdgcn_wave_barrier();
+  }
+  __syncthreads();
+  const int subs = 64 / lanes, sub = lane / lanes, team = wave * subs + sub, teams = W * subs;
+  const int32_t column = ((int32_t)blockIdx.y * lanes + lane % lanes) * V, c0 = min(column, dim - V);
+  const int skip = column - c0;
+  const bool active = column < dim;
+  // positions list[s], list[s + step], ... before `end`
+  auto add_rows = [&](float(&acc)[V], int s, int step, int end) {
+    for (; s < end; s += U * step) {
+      P v[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (s + u * step < end) v[u] = load_pack_unaligned<true, P>(out + (int64_t)list[s + u * step] * outStride + c0);
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (s + u * step < end) {
+#pragma unroll
+          for (int e = 0; e < V; ++e) acc[e] += Cvt<T>::up(v[u].v[e]);
+        }
+      }
+    }
+  };
+  auto row_of = [&](int which) { return grad + (int64_t)(me + ((uint32_t)which << shift)) * gradStride + c0; };
+  for (int j = 0; j < longs; ++j) {
+    const int u = longRun[j];
+    float acc[V];
+#pragma unroll
+    for (int e = 0; e < V; ++e) acc[e] = 0.f;
+    if (active) add_rows(acc, runStart[u] + team, teams, runStart[u + 1]);
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      for (int d = lanes; d < 64; d <<= 1) acc[e] += __shfl_xor(acc[e], d);
+      meet[wave][e][lane] = acc[e];
+    }
+    __syncthreads();
+    if (wave == 0 && sub == 0 && active) {
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+#pragma unroll
+        for (int w = 1; w < W; ++w) acc[e] += meet[w][e][lane];
+      }
+      finish_row<T, V>(row_of(runToken[u]), acc, factor, add, skip);
+    }
+    __syncthreads();
+  }
+  if (!active) return;
+  for (int u = team; u < runs; u += teams) {
+    const int s = runStart[u], end = runStart[u + 1];
+    if (end - s > kLongRun) continue;
+    float acc[V];
+#pragma unroll
+    for (int e = 0; e < V; ++e) acc[e] = 0.f;
+    add_rows(acc, s, 1, end);
+    finish_row<T, V>(row_of(runToken[u]), acc, factor, add, skip);
+  }
+  if (add) return;
+  P zero;
+#pragma unroll
+  for (int e = 0; e < V; ++e) zero.v[e] = Cvt<T>::down(0.f);
+  for (int q = team; q < owned; q += teams)
+    if (!((occurs[q >> 6] >> (q & 63)) & 1)) store_pack_unaligned<false>(row_of(q), zero);
+}
+
 template <typename T>
 void launch_grad(THCState* s, T* grad, int64_t vocab, int64_t gradStride, const int64_t* tokens, int32_t n, const T* out, int64_t outStride,
                  int32_t dim, float factor, int64_t padding, bool add) {
   hipStream_t st = current_stream(s);
   constexpr int kPack = 16 / sizeof(T);
   const int V = dim >= kPack ? kPack : 1;
-  const int32_t fewSlabs = (dim + 64 * V - 1) / (64 * V);
-  // us in three launches and in one (halves, added): 16 positions of 513 9.7, 3.9; 512 x 2048 12.4, 7.5; 1024 x 513 13.6, 9.4; 1500 x 64 12.9,
-  // 10.0; 1024 x 2048 14.5, 14.0; 1500 x 2048 15.3, 20.4; 512 x 8192 15.8, 16.9: the one launch's time goes with the workgroups times what
-  // each looks at.
-  if (n <= kFew && vocab <= int64_t(1) << 28 && (int64_t)n * n * fewSlabs <= tuning("embedding.few", 3 << 20)) {
+  const int32_t packs = (dim + V - 1) / V, fewSlabs = (packs + 63) / 64;
+  const uint32_t left = (uint32_t)(padding - 1);
+  // A launch of owners: strips of columns so narrow, and owners so many, that there are up to 512 workgroups (two a CU; us with 256, 512 and
+  // 1024 of them: 1500 x 513 fp32 7.8, 8.1, 9.6, 2000 x 1000 half 12.3, 11.1, 17.6). The commonest token's sum is a workgroup's for each strip,
+  // which bounds the bytes that are summed; rows are zeroed less evenly than by the three launches, which bounds the table. us in three
+  // launches and in this one, tokens as in text and all the same, added: 2000 x 64 half 15.2, 7.9 and 32.4, 15.0; 1500 x 513 fp32 13.5, 8.1 and
+  // 29, 22; 2000 x 1000 half 15.7, 11.1 and 32, 44; 1500 x 2048 14.9, 11.9 and 27, 58. Tables written whole: 1500 x 513 fp32 into 10007
+  // rows 16.9, 10.7, 2000 x 500 half into 32000 17.8, 19.0.
+  int lanes = 8, shift = 0;
+  while (((vocab - 1) >> shift) + 1 > kOwnTokens) ++shift;
+  while (lanes < 64 && lanes < packs && ((int64_t)(packs + lanes - 1) / lanes << shift) > kOwnGrid) lanes *= 2;
+  while (lanes > 1 && lanes / 2 >= packs) lanes /= 2;
+  const int32_t strips = (packs + lanes - 1) / lanes;
+  while (shift < 8 && (int64_t(2) << shift) <= vocab && ((int64_t)strips << (shift + 1)) <= kOwnGrid) ++shift;
+  const bool own = n <= kOwn && ((int64_t)strips << shift) <= kOwnGrid && (int64_t)n * dim * (int64_t)sizeof(T) <= tuning("embedding.own", 4 << 20) &&
+                   (add || vocab * dim * (int64_t)sizeof(T) <= 24 << 20);
+  // A launch of positions: its time goes with the workgroups times what each looks at. us in that launch, of owners and in three (halves, added):
+  // 16 x 2048 3.7, 5.2, 10.0; 600 x 2048 6.6, 7.7, 13.0; 1024 x 513 8.4, 8.8, 13.8; 1500 x 64 9.6, 7.5, 13.0; 1000 x 2048 13.7, 10.2, 13.7;
+  // 512 x 8192 15.3, 18, 15.1.
+  if (n <= kFew && vocab <= int64_t(1) << 28 && (int64_t)n * n * fewSlabs <= std::min<int64_t>(tuning("embedding.few", 3 << 20), own ? 3 << 19 : 3 << 20)) {
     const dim3 grid((unsigned)(n + (add ? 0 : (vocab + kFewRows - 1) / kFewRows)), fewSlabs);
-    const uint32_t left = (uint32_t)(padding - 1);
-    if (V == 1)
-      hipLaunchKernelGGL((few_kernel<T, 1>), grid, dim3(kBlock), 0, st, grad, gradStride, tokens, n, (uint32_t)vocab, left, out, outStride, dim,
-                         factor, add);
-    else
-      hipLaunchKernelGGL((few_kernel<T, kPack>), grid, dim3(kBlock), 0, st, grad, gradStride, tokens, n, (uint32_t)vocab, left, out, outStride,
-                         dim, factor, add);
+    auto go = [&](auto v) {
+      hipLaunchKernelGGL((few_kernel<T, decltype(v)::value>), grid, dim3(kBlock), 0, st, grad, gradStride, tokens, n, (uint32_t)vocab, left, out,
+                         outStride, dim, factor, add);
+    };
+    if (V == 1) go(std::integral_constant<int, 1>{});
+    else go(std::integral_constant<int, kPack>{});
+    return;
+  }
+  if (own) {
+    auto go = [&](auto v) {
+      hipLaunchKernelGGL((own_kernel<T, decltype(v)::value>), dim3(1u << shift, strips), dim3(kOwnWaves * 64), 0, st, grad, gradStride, tokens, n,
+                         (uint32_t)vocab, left, out, outStride, dim, lanes, factor, add, shift);
+    };
+    if (V == 1) go(std::integral_constant<int, 1>{});
+    else go(std::integral_constant<int, kPack>{});
     return;
   }
   GradArgs a{};
@@ -691,8 +874,7 @@ void launch_grad(THCState* s, T* grad, int64_t vocab, int64_t gradStride, const 
   a.factor = factor;
   a.add = add;
   // a power of two of lanes for a short row, several chunks to a workgroup; whole waves for a long one
-  const int32_t packs = (dim + V - 1) / V;
-  int lanes = 1;
+  lanes = 1;
   while (lanes < 64 && lanes < packs) lanes *= 2;
   const int slabs = (packs + kBlock - 1) / kBlock;
   if (packs > 64) lanes = ((packs + slabs - 1) / slabs + 63) / 64 * 64;
@@ -705,7 +887,7 @@ void launch_grad(THCState* s, T* grad, int64_t vocab, int64_t gradStride, const 
   a.chunk = (int32_t)std::min<int64_t>(64, std::max<int64_t>(std::max(4, std::min(32, n / 4096)), (int64_t)n * lanes * slabs / want));
   a.chunks = (n + a.chunk - 1) / a.chunk;
   // owners: a power of two, none of which has more tokens than it has room to count
-  int shift = 0;
+  shift = 0;
   while ((int64_t(1) << shift) < std::min<int64_t>(vocab, 256) || ((vocab - 1) >> shift) + 1 > kOwnTokens) ++shift;
   while ((int64_t(1) << shift) > vocab) --shift;
   const bool apart = n > tuning("embedding.split", kSplitFrom) && (1 << shift) <= kMostSplit;
@@ -720,7 +902,6 @@ void launch_grad(THCState* s, T* grad, int64_t vocab, int64_t gradStride, const 
   Split split;
   split.entry = reinterpret_cast<int2*>(a.partial + partials);
   split.begin = reinterpret_cast<int32_t*>(split.entry + tiles * kTile);
-  const uint32_t left = (uint32_t)(padding - 1);
   if (apart) {
     hipLaunchKernelGGL(split_kernel, dim3((unsigned)tiles), dim3(kGroupThreads), 0, st, split, tokens, n, (uint32_t)vocab, left, shift);
     hipLaunchKernelGGL(group_kernel<true>, dim3(1u << shift), dim3(kGroupThreads), 0, st, a.g, split, tokens, n, (uint32_t)vocab, left, shift);

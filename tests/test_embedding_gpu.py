@@ -171,6 +171,48 @@ def test_gradient_of_split_positions(thc, split, how, vocab, dim, count):
         _near(grad.numpy(), want, mass, n, "float")
 
 
+WAYS = {"positions": {"embedding.few": 3 << 20, "embedding.own": 0}, "owners": {"embedding.few": 0, "embedding.own": 1 << 40},
+        "three": {"embedding.few": 0, "embedding.own": 0}, "split": {"embedding.few": 0, "embedding.own": 0, "embedding.split": 0}}
+
+
+@pytest.fixture(params=sorted(WAYS))
+def way(thc, request):
+    """A launch of positions, a launch of owners, three launches, and those after a split: where the sizes allow it."""
+    for key, value in WAYS[request.param].items():
+        thc.set_tuning(key, value)
+    yield request.param
+    for key, value in (("embedding.few", 3 << 20), ("embedding.own", 4 << 20), ("embedding.split", 40000)):
+        thc.set_tuning(key, value)
+
+
+@pytest.mark.parametrize("kind", ["float", "half"])
+@pytest.mark.parametrize("how", ["text", "one", "two", "each"])
+@pytest.mark.parametrize("vocab,dim,count", [(1, 1, 2), (2, 3, 4096), (3, 9, 513), (255, 31, 511), (513, 33, 1025), (1000, 7, 4095), (5003, 8, 2049),
+                                             (300, 513, 900), (100000, 16, 3000), (262144, 4, 1500), (40, 1030, 4000), (262145, 4, 100)])
+def test_gradient_in_every_way(thc, way, kind, how, vocab, dim, count):
+    rng = np.random.default_rng(vocab + dim + count)
+    tokens = _tokens(rng, how, vocab, count)
+    tokens[rng.random(count) < 0.02] = vocab + 1
+    padding = 1 if vocab > 2 else 0
+    out = rng.standard_normal((count, dim + 3)).astype(NP[kind])
+    start = _table(rng, vocab, dim + 5, kind)
+    for add in (False, True):
+        # windows of something wider: what is around the gradient stays
+        room = _tensor(thc, start)
+        room.narrow(1, 2, dim).embedding_grad(_tensor(thc, tokens), _tensor(thc, out).narrow(1, 1, dim), 1.25, padding=padding, accumulate=add)
+        got = room.numpy()
+        want, mass, n = _sums((vocab, dim), tokens, np.ascontiguousarray(out[:, 1:dim + 1]), 1.25, padding,
+                              start[:, 2:dim + 2].astype(np.float64) if add else None)
+        _near(got[:, 2:dim + 2], want, mass, n, kind)
+        keeps = np.ascontiguousarray(start) if add else np.where((np.arange(dim + 5) < 2) | (np.arange(dim + 5) >= dim + 2), start, 0).astype(NP[kind])
+        assert_bit_equal(got[n == 0], keeps[n == 0])
+        assert_bit_equal(got[:, :2], start[:, :2])
+        assert_bit_equal(got[:, dim + 2:], start[:, dim + 2:])
+        again = _tensor(thc, start)
+        again.narrow(1, 2, dim).embedding_grad(_tensor(thc, tokens), _tensor(thc, out).narrow(1, 1, dim), 1.25, padding=padding, accumulate=add)
+        assert_bit_equal(again.numpy(), got)
+
+
 @pytest.mark.parametrize("vocab,count", [(262143, 5000), (300001, 4099), (1 << 20, 1000)])
 def test_gradient_of_a_large_table(thc, vocab, count):
     rng = np.random.default_rng(vocab)
