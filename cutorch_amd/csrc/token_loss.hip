@@ -592,27 +592,39 @@ void token_loss(THCState* s, DType dt, const PolicyCall& c) {
     if (c.weight) check_positions(c.weight, rows, 10, "weights");
     THC_ARG_CHECK(c.low >= 0 && c.low <= 1 && c.high >= 0, 11, "the ratio is clipped to 1 - low and 1 + high, low from 0 to 1, high from 0");
   }
-  note_stream_use(s, {c.loss, c.logProb, c.grad, c.logits, c.tokens, c.old, c.advantage, c.reference, c.weight});
+  THC_ARG_CHECK(c.logProb != c.logits && c.logProb != c.grad, policy ? 3 : 2, "the log-probabilities may not be the logits or their gradient");
+  if (policy)
+    THC_ARG_CHECK(c.loss != c.logits && c.loss != c.grad && c.loss != c.logProb, 2, "the losses may not be the logits, their gradient or the log-probabilities");
 
   Rows lr{};
   const bool direct = as_rows(c.logits, &lr);
   TensorRef logits(s, direct ? (tensor_retain(c.logits), c.logits) : tensor_new_contiguous(s, c.logits, dt));
   as_rows(logits.t, &lr);
   Dense tokens(s, c.tokens, DType::I64);
+  TensorRef old(s, nullptr), advantage(s, nullptr), reference(s, nullptr), weight(s, nullptr);
+  if (policy) {
+    auto dense = [&](TensorRef& hold, AnyTensor* t) {
+      if (t) hold.t = tensor_new_contiguous(s, t, DType::F32);
+    };
+    dense(old, c.old);
+    dense(advantage, c.advantage);
+    if (c.kl != 0) dense(reference, c.reference);
+    dense(weight, c.weight);
+  }
+  // outputs may share a storage with each other and with what is read: all are resized before any address is taken
+  tensor_resize_as(s, c.logProb, c.tokens, DType::F32);
+  if (policy) tensor_resize_as(s, c.loss, c.tokens, DType::F32);
+  if (c.grad) tensor_resize_as(s, c.grad, c.logits, dt);
+  note_stream_use(s, {c.loss, c.logProb, c.grad, c.logits, c.tokens, c.old, c.advantage, c.reference, c.weight});
   PolicyArgs a{};
   a.token = tokens.data<int64_t>();
   a.evenWeight = 1.f;
-  TensorRef old(s, nullptr), advantage(s, nullptr), reference(s, nullptr), weight(s, nullptr);
   if (policy) {
-    auto dense = [&](TensorRef& hold, AnyTensor* t) -> const float* {
-      if (!t) return nullptr;
-      hold.t = tensor_new_contiguous(s, t, DType::F32);
-      return (const float*)tensor_data(hold.t, DType::F32);
-    };
-    a.old = dense(old, c.old);
-    a.advantage = dense(advantage, c.advantage);
-    a.reference = c.kl != 0 ? dense(reference, c.reference) : nullptr;
-    a.weight = dense(weight, c.weight);
+    auto data = [&](const TensorRef& t) { return t.t ? (const float*)tensor_data(t.t, DType::F32) : nullptr; };
+    a.old = data(old);
+    a.advantage = data(advantage);
+    a.reference = data(reference);
+    a.weight = data(weight);
     a.evenWeight = (float)(1.0 / (double)rows);
     a.low = (float)(1.0 - c.low);
     a.high = (float)(1.0 + c.high);
@@ -627,17 +639,14 @@ void token_loss(THCState* s, DType dt, const PolicyCall& c) {
     return false;
   };
   TensorRef loss(s, nullptr), logProb(s, nullptr), grad(s, nullptr);
-  tensor_resize_as(s, c.logProb, c.tokens, DType::F32);
   logProb.t = position_output(s, c.logProb, meets(c.logProb, DType::F32, 0));
   a.logProb = (float*)tensor_data(logProb.t, DType::F32);
   if (policy) {
-    tensor_resize_as(s, c.loss, c.tokens, DType::F32);
     loss.t = position_output(s, c.loss, meets(c.loss, DType::F32, 0));
     a.loss = (float*)tensor_data(loss.t, DType::F32);
   }
   Rows gr{};
   if (c.grad) {
-    tensor_resize_as(s, c.grad, c.logits, dt);
     // in the place of the logits, or apart from everything that is read
     bool fits = as_rows(c.grad, &gr) && !overlapping(tensor_layout(c.grad)) && !meets(c.grad, dt, 1);
     if (fits && spans_meet(c.grad, dt, logits.t, dt))

@@ -326,6 +326,28 @@ def test_outputs_on_an_inputs_storage(thc):
     assert_bit_equal(shifted.numpy(), want[2])
 
 
+def test_outputs_that_make_a_shared_storage_grow(thc):
+    """Losses, log-probabilities and gradient are windows behind the inputs, and grow: everything moves with the storage."""
+    rng = np.random.default_rng(13)
+    x, tokens, old, advantage, ref, weight = _case(rng, 30, 50, "float", True, False)
+    want = _run(thc, (x, tokens, old, advantage, ref, weight))
+    t = thc.Tensor.from_numpy
+    end = 1500 + 120
+    room = t(np.concatenate([x.reshape(-1), old, advantage, ref, weight, np.zeros(61, np.float32)]))
+    logits = room.view_as_strided(0, (30, 50), (50, 1))
+    o, a, r, w = (room.narrow(0, 1500 + 30 * i, 30) for i in range(4))
+    lp, loss, g = (room.narrow(0, end + 30 * i, 1) for i in range(3))
+    loss.policy_loss(lp, g, logits, t(tokens), o, a, r, w, 0.2, 0.25, 0.1, 1.0)
+    for got, wanted in ((loss, want[0]), (lp, want[1]), (g, want[2]), (logits, x), (o, old), (a, advantage), (r, ref), (w, weight)):
+        assert_bit_equal(got.numpy(), wanted)
+    with pytest.raises(thc.THCError, match="may not be the logits"):
+        same = t(x)
+        thc.Tensor("float").policy_loss(same, None, same, t(tokens), t(old), t(advantage))
+    with pytest.raises(thc.THCError, match="losses may not be"):
+        lp = thc.Tensor("float")
+        lp.policy_loss(lp, None, t(x), t(tokens), t(old), t(advantage))
+
+
 def test_refusals(thc):
     t = thc.Tensor.from_numpy
     x, tokens, per = t(np.zeros((4, 6), np.float32)), t(np.ones(4, np.int64)), t(np.zeros(4, np.float32))
