@@ -229,8 +229,9 @@ __device__ __forceinline__ void store4_codes(T* to, const T (&from)[4], int n) {
   }
 }
 
-// States in 8 bits: a wave has a block of states per pack, 4 elements a lane. What is behind a tensor's end counts as zeros. Bound by memory in
-// large calls (184 M floats 510 us, 5.8 TB/s), by a wave's one pass from load to store in those that the caches hold (4.5 M floats 19 us).
+// States in 8 bits: a wave has a block of states per pack, 4 elements a lane. What is behind a tensor's end counts as zeros. Bound by
+// arithmetic and memory alike in large calls (184 M floats 510 us, 5.8 TB/s; about 530 instructions for a block of 256), by arithmetic in those
+// that the caches hold (4.5 M floats 19 us).
 // FULL: the tensor does not end in this part.
 template <typename T, bool MASTER, bool NT, bool FULL>
 __device__ __forceinline__ void step8_part(const Hyper& h, void* const* pointers, int64_t base, int left) {
@@ -426,11 +427,12 @@ struct Lists {
 
 int64_t state_blocks(int64_t n) { return (n + kStateBlock - 1) / kStateBlock; }
 
-void check_scales(THCState* s, const AnyTensor* scale, int64_t n, int arg, int index) {
+void check_scales(THCState* s, const AnyTensor* scale, int64_t n, int arg, int index, bool written) {
   THC_ARG_CHECK(scale, arg, "no scales of tensor %d's states", index + 1);
   check_same_gpu(s, 1, &scale);
   THC_ARG_CHECK(tensor_numel(scale) == state_blocks(n), arg, "%ld scales for the %ld blocks of tensor %d's states", (long)tensor_numel(scale),
                 (long)state_blocks(n), index + 1);
+  THC_ARG_CHECK(!written || tensor_is_contiguous(scale) || !overlapping(tensor_layout(scale)), arg, "scales of tensor %d's states overlap", index + 1);
 }
 
 void check_list(THCState* s, const AnyTensor* t, const AnyTensor* like, int arg, int index, bool written) {
@@ -460,9 +462,9 @@ void adamw(THCState* s, DType dt, int count, const Lists& l, double lr, double b
     if (l.master) check_list(s, l.master[i], p, 4, i, true);
     check_list(s, l.grad[i], p, base, i, false);
     check_list(s, l.mean[i], p, base + 1, i, true);
-    if (eight) check_scales(s, l.meanScale[i], tensor_numel(p), base + 2, i);
+    if (eight) check_scales(s, l.meanScale[i], tensor_numel(p), base + 2, i, true);
     check_list(s, l.square[i], p, base + (eight ? 3 : 2), i, true);
-    if (eight) check_scales(s, l.squareScale[i], tensor_numel(p), base + 4, i);
+    if (eight) check_scales(s, l.squareScale[i], tensor_numel(p), base + 4, i, true);
   }
   Hyper h;
   h.beta1 = (float)beta1;
@@ -549,8 +551,8 @@ void moments(THCState* s, int count, AnyTensor** meanOut, AnyTensor** squareOut,
   for (int i = 0; i < count; ++i) {
     THC_ARG_CHECK(mean[i], 5, "tensor %d is missing", i + 1);
     check_list(s, square[i], mean[i], 7, i, false);
-    check_scales(s, meanScale[i], tensor_numel(mean[i]), 6, i);
-    check_scales(s, squareScale[i], tensor_numel(mean[i]), 8, i);
+    check_scales(s, meanScale[i], tensor_numel(mean[i]), 6, i, false);
+    check_scales(s, squareScale[i], tensor_numel(mean[i]), 8, i, false);
     THC_ARG_CHECK(meanOut[i], 3, "tensor %d is missing", i + 1);
     THC_ARG_CHECK(squareOut[i], 4, "tensor %d is missing", i + 1);
   }
@@ -560,9 +562,22 @@ void moments(THCState* s, int count, AnyTensor** meanOut, AnyTensor** squareOut,
   const int sizes[6] = {4, 4, 1, 1, 0, 0};
   Batch<A, decltype(launch)> batch(Hyper{}, part_size(kDecodePacks), sizes, launch);
   Held held(s);
+  // (all are resized before any pointer is taken: they may share a storage)
   for (int i = 0; i < count; ++i) {
     tensor_resize_as(s, meanOut[i], mean[i], DType::F32);
     tensor_resize_as(s, squareOut[i], mean[i], DType::F32);
+  }
+  for (int i = 0; i < count; ++i) {
+    if (!has_elements(mean[i])) continue;
+    const AnyTensor *out[2] = {meanOut[i], squareOut[i]}, *in[2] = {meanScale[i], squareScale[i]};
+    for (int j = 0; j < 2; ++j) {
+      THC_ARG_CHECK(tensor_is_contiguous(out[j]) || !overlapping(tensor_layout(out[j])), 3 + j, "elements of tensor %d overlap", i + 1);
+      for (int k = 0; k < 2; ++k)
+        THC_ARG_CHECK(!spans_meet(out[j], DType::F32, in[k], DType::F32), 3 + j, "tensor %d lies on its scales", i + 1);
+    }
+    THC_ARG_CHECK(!spans_meet(out[0], DType::F32, out[1], DType::F32), 4, "tensor %d's two moments share memory", i + 1);
+  }
+  for (int i = 0; i < count; ++i) {
     if (!has_elements(mean[i])) continue;
     note_stream_use(s, {meanOut[i], squareOut[i], mean[i], meanScale[i], square[i], squareScale[i]});
     void* p[6];

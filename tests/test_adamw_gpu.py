@@ -250,9 +250,28 @@ def test_refusals(thc):
     with pytest.raises(thc.THCError, match="overlap"):
         p = new().view_as_strided(0, (4, 3), (0, 1))
         thc.AdamW([p], [new()]).step()
+    with pytest.raises(thc.THCError, match="scales of tensor 1's states overlap"):
+        thc.AdamW([new(shape=(300,))], [new(shape=(300,))], bits=8, mean_scale=[new(shape=(1,)).view_as_strided(0, (2,), (0,))]).step()
     for bad in (dict(params=[new("half"), new()], grads=[new(), new()]), dict(params=[new()], grads=[]), dict(params=[new()], grads=[new("half")]),
                 dict(params=[new()], grads=[new()], master=[new()]), dict(params=[new()], grads=[new()], bits=16)):
         with pytest.raises(ValueError):
             thc.AdamW(**bad)
     thc.AdamW([], []).step()         # nothing to do
     thc.AdamW([thc.Tensor("float")], [thc.Tensor("float")], bits=8).step()
+
+
+def test_moments_in_windows_of_one_storage(thc):
+    """Outputs that share a storage, which grows for the second one."""
+    rng = np.random.default_rng(8)
+    p, g = _problem(rng, [(300,), (7, 100)], "float")
+    opt = thc.AdamW(_put(thc, p), _put(thc, g), bits=8, **HYPER)
+    opt.step()
+    want = [[t.numpy() for t in l] for l in opt.moments()]
+    room = thc.Tensor("float").resize((350,)).zero()
+    mean, square = opt.moments([room.narrow(0, 0, 300), thc.Tensor("float")], [thc.Tensor("float"), room.narrow(0, 300, 50)])
+    for a, b in zip(mean + square, want[0] + want[1]):
+        assert_bit_equal(a.numpy(), b)
+    with pytest.raises(thc.THCError, match="two moments share memory"):
+        opt.moments([room, thc.Tensor("float")], [room, thc.Tensor("float")])
+    with pytest.raises(thc.THCError, match="lies on its scales"):
+        opt.moments([opt.mean_scale[0], thc.Tensor("float")], [thc.Tensor("float"), thc.Tensor("float")])
