@@ -440,12 +440,11 @@ __device__ __forceinline__ void write_partial(float* to, const float (&acc)[V]) 
 }
 
 // V columns a lane; a row's last lane is moved back into the row and leaves the columns that it shares to the lane before it. Bound by
-// memory: 32768 x 2048 halves into 50000 rows 58 us, 5.8 TB/s of rows read and written, besides the partial sums, which stay in the caches. (A run
+// memory: 32768 x 2048 halves into 50000 rows 60 us, 5.7 TB/s of rows read and written, besides the partial sums, which stay in the caches. (A run
 // that crosses one edge summed to its end by the chunk that it begins in: 1.5 us less to fold, but 9 more here; the few chunks that go on
 // are the launch's end. What sums are added to, asked for together with the rows: the same, for the registers.) Rows are zeroed whole by a
-// workgroup and with plain stores: us of 3000 x 3000 floats into 50000 rows with pieces of 4 KiB and so 166, 150, with streaming stores 159;
-// 5000 x 1000 halves into 200000, whose rows end inside lines, 98, streaming 117.
-template <typename T, int V, int U>
+// workgroup: 3000 x 3000 floats into 50000 rows 166 us with pieces of 4 KiB, 150 so.
+template <typename T, int V, int U, bool NT>
 __global__ __launch_bounds__(kBlock) void sum_kernel(GradArgs a, const T* __restrict__ out, T* __restrict__ grad, int64_t vocab,
                                                      int32_t chunkBlocks) {
   using P = Pack<T, V>;
@@ -463,7 +462,7 @@ __global__ __launch_bounds__(kBlock) void sum_kernel(GradArgs a, const T* __rest
     for (int j = 0; j < 16; ++j) {
       const int64_t row = row0 + (int64_t)j * subs;
       if (j % gridDim.y == blockIdx.y && row < vocab && used[j] == 0) {
-        for (int32_t k = lane * V; k < a.dim; k += a.lanes * V) store_pack_unaligned<false>(grad + row * a.gradStride + min(k, a.dim - V), zero);
+        for (int32_t k = lane * V; k < a.dim; k += a.lanes * V) store_pack_unaligned<NT>(grad + row * a.gradStride + min(k, a.dim - V), zero);
       }
     }
     return;
@@ -995,8 +994,14 @@ void launch_grad(THCState* s, T* grad, int64_t vocab, int64_t gradStride, const 
   const int32_t chunkBlocks = (a.chunks + subs - 1) / subs;
   const int64_t zeroBlocks = add ? 0 : (vocab + subs * 16 - 1) / (subs * 16);
   const dim3 grid((unsigned)(chunkBlocks + zeroBlocks), slabs), block(subs * lanes);
-  if (V == 1) hipLaunchKernelGGL((sum_kernel<T, 1, 8>), grid, block, 0, st, a, out, grad, vocab, chunkBlocks);
-  else hipLaunchKernelGGL((sum_kernel<T, kPack, 8>), grid, block, 0, st, a, out, grad, vocab, chunkBlocks);
+  // Zeros are streaming stores in large tables whose rows are whole lines: us, plain and streaming, of 32768 x 2048 halves into 50000 rows (205 MB)
+  // 84, 78 (68, 77 where the caches still hold the table from the call before), 6000 x 8192 floats into 30000 219, 205; of 8192 x 1024 halves into
+  // 32000 (66 MB) 29.3, 30.8; with lines that rows share, 3000 x 3000 floats into 50000 150, 159, 5000 x 1000 halves into 200000 98, 117.
+  const bool lines = ((uintptr_t)grad | (uintptr_t)(gradStride * sizeof(T)) | (uintptr_t)(dim * sizeof(T))) % 128 == 0;
+  const bool streaming = lines && vocab * dim * (int64_t)sizeof(T) >= int64_t(128) << 20;
+  if (V == 1) hipLaunchKernelGGL((sum_kernel<T, 1, 8, false>), grid, block, 0, st, a, out, grad, vocab, chunkBlocks);
+  else if (!streaming) hipLaunchKernelGGL((sum_kernel<T, kPack, 8, false>), grid, block, 0, st, a, out, grad, vocab, chunkBlocks);
+  else hipLaunchKernelGGL((sum_kernel<T, kPack, 8, true>), grid, block, 0, st, a, out, grad, vocab, chunkBlocks);
   // strips of columns as narrow as leave two workgroups a CU
   const int32_t edges = (a.chunks + 63) / 64, quads = (dim + 3) / 4;
   lanes = 8;

@@ -71,6 +71,20 @@ def test_output_gradient_of_more_than_2_31_elements(thc):
     assert_bit_equal(grad.narrow(0, 20, 400).numpy(), want)
 
 
+@pytest.mark.parametrize("kind,dim", [("half", 1024), ("half", 1032), ("float", 512)])
+def test_gradient_of_a_table_beyond_128_mib(thc, kind, dim):
+    rng = np.random.default_rng(6)
+    rows, count = 70001, 5000
+    dtype = np.float16 if kind == "half" else np.float32
+    tokens = rng.permutation(rows)[:count] + 1
+    out = rng.standard_normal((count, dim)).astype(dtype)
+    grad = thc.Tensor(kind).resize((rows, dim)).fill(7)
+    grad.embedding_grad(thc.Tensor.from_numpy(tokens), thc.Tensor.from_numpy(out), 1.0)
+    want = np.zeros((rows, dim), dtype)
+    want[tokens - 1] = out
+    assert_bit_equal(grad.numpy(), want)
+
+
 @pytest.mark.parametrize("vocab", [262144, 32001])
 def test_losses_of_more_than_2_31_logits(thc, vocab):
     rng = np.random.default_rng(4)
