@@ -131,7 +131,7 @@ void embedding(THCState* s, DType dt, AnyTensor* self, AnyTensor* table, AnyTens
 // Grouping. Token k (0-based) belongs to owner k mod G. An owner sweeps the tokens twice, counts its own and places them; the tokens of
 // the owners before it, which it counts on the way, say where its slots begin: no owner waits for another. A token's slots are side
 // by side and its positions in order; the order of the tokens does not matter to the sums.
-// Bound by latency, sweep by sweep, and by how often the commonest token is counted: 1500 positions 5.6 us, 32768 12.3, 131072 split 23 behind
+// Bound by latency, sweep by sweep, and by how often the commonest token is counted: 1500 positions 5.6 us, 32768 12.3, 131072 split 18 behind
 // the splitting's 5.
 // Few positions are swept as they are, by every owner. Of many, each owner would look at all: they are first split, tile by tile, into
 // the owners' shares.
@@ -143,7 +143,7 @@ struct Grouping {
 };
 constexpr int kGroupThreads = 1024, kGroupWaves = kGroupThreads / 64;
 constexpr int kOwnTokens = 512;      // tokens that one owner takes at most: 32 KiB of counts
-constexpr int kFound = 512;          // positions that a wave remembers between its two sweeps: 64 KiB
+constexpr int kFound = 896;          // positions that a wave remembers between its two sweeps: 112 KiB
 constexpr int kTile = 1024;          // positions that are split together, one a lane
 // Splitting costs a launch and saves every owner the sight of the others' positions. us of the whole gradient, swept and split (rows of 64 halves,
 // added): 8192 positions 18.3, 21.6; 30000 26.4, 26.4; 40000 30.6, 29.3; 65536 36.6, 31.9; 131072 139, 51. Tiles of 4096 positions instead of
@@ -515,7 +515,7 @@ __global__ __launch_bounds__(kBlock) void sum_kernel(GradArgs a, const T* __rest
 // The partial sums of the runs that cross edges, by the first edge that they cross. A workgroup looks at 64 edges, a lane each, and has a strip of
 // columns, four a lane: a run of few partial sums is a team of lanes', of more a wave's, and of many all waves', whose sums meet in LDS.
 // Bound by latency, load by load: 8192 x 1024 halves 5.0 us, 32768 x 2048 6.5 (a workgroup for every edge, most of which have none: 8.7, 6.9; where
-// all tokens are the same, the whole gradient of 32768 x 256 219 us instead of 106).
+// all tokens are the same, the whole gradient of 32768 x 256 219 us instead of 87).
 constexpr int kFoldWaves = 8, kFoldGrid = 512;
 constexpr int kTeamFold = 8, kWaveFold = 32;      // partial sums that a team, and that a wave's teams each, take
 template <typename T>
@@ -541,19 +541,10 @@ __global__ __launch_bounds__(kFoldWaves * 64) void fold_kernel(GradArgs a, T* __
     const uint64_t goesOn = __ballot(crosses && behind == token), over = ~goesOn >> lane;
     int32_t last = (int32_t)edge + 1;
     if (over) last += __ffsll((unsigned long long)over) - 1;
-    if ((goesOn >> 63) != 0 && __ballot(starts && !over) != 0) {
-      // the run that crosses the last of them goes on: to the first edge behind that it does not cross
-      const int32_t it = __builtin_amdgcn_readlane(token, 63);
-      int64_t end = (int64_t)blockIdx.x * 64 + 64;
-      for (;;) {
-        const uint64_t stops = __ballot(token_at((end + lane + 2) * a.chunk) != it);
-        if (stops) {
-          end += __ffsll((unsigned long long)stops) - 1;
-          break;
-        }
-        end += 64;
-      }
-      if (!over) last = (int32_t)end + 1;
+    if (starts && !over) {
+      // the run that crosses the last of them goes on: it begins in this chunk, so its length says where it ends but for one chunk
+      last = (int32_t)edge + (a.g.used[token] - 1) / a.chunk;
+      if (token_at(((int64_t)last + 1) * a.chunk) == token) ++last;
     }
     // those of teams, of waves and of all, one list behind the other
     const int parts = last - (int32_t)edge + 1, kind = parts <= kTeamFold ? 0 : parts <= kWaveFold * subs ? 1 : 2;
