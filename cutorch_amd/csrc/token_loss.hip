@@ -295,6 +295,7 @@ template <typename T, int W, int R, int L, int E, bool REST>
 __global__ __launch_bounds__(W * 64) __attribute__((amdgpu_waves_per_eu(E, E))) void held_row_kernel(PolicyArgs a, const T* logits, RowOffsets lo, T* grad,
                                                                                                RowOffsets go, int32_t vocab, uint32_t rows) {
   constexpr int U = R < 4 ? R : 4, kStep = W * 64, V = 16 / sizeof(T);
+  static_assert(R % U == 0, "registers are taken U packs at a time");
   using P = Pack<T, V>;
   __shared__ Soft lds[W];
   extern __shared__ __attribute__((aligned(16))) char room[];      // L packs a lane
@@ -543,7 +544,7 @@ void launch_rows(THCState* s, const PolicyArgs& a, const T* logits, const Rows& 
   // The least that hold a row, so that a CU has several: one loads while another computes and a third stores. us, halves with gradients:
   // 16384 x 8000 with 4 waves of 4, 8 and 16 packs 82, 84, 100; 8192 x 16000 with 8 waves of 4 and 8, 16 of 8 84, 88, 111; 8192 x 32000
   // with 8 of 8, 16 of 8 and 16 of 16 168, 170, 256; 4096 x 65000 with 16 of 8 and 16 of 16 173, 215; 4096 x 100001 with 8 waves of 16
-  // and 9 more in LDS (two workgroups a CU) and 16 of 16 285, 312; 3000 x 150001 with 16 waves of 16 and 9 347, of 14 and 9 and the end read again 346, 2048 x 262144 439 (with 8 waves 457).
+  // and 9 more in LDS (two workgroups a CU) and 16 of 16 285, 312; 3000 x 150001 with 16 waves of 16 and 9 347, of 12 and 9 and the end read again 347, 2048 x 262144 442 (with 8 waves 457).
   if (packs <= 64) HELD(1, 1, 0, 8, false);
   else if (packs <= 256) HELD(1, 4, 0, 8, false);
   else if (packs <= 1024) HELD(4, 4, 0, 8, false);
@@ -551,7 +552,7 @@ void launch_rows(THCState* s, const PolicyArgs& a, const T* logits, const Rows& 
   else if (packs <= 4096) HELD(8, 8, 0, 6, false);
   else if (packs <= 8192) HELD(16, 8, 0, 8, false);
   else if (packs <= 12800) HELD(8, 16, 9, 4, false);
-  else HELD(16, 14, 9, 4, true);
+  else HELD(16, 12, 9, 4, true);
 #undef HELD
 }
 
