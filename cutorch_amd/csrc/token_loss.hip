@@ -287,7 +287,7 @@ __device__ __forceinline__ void load_to_lds(const void* from, void* to) {
 
 // A workgroup has a row, a lane R packs of it in registers and L in LDS from the first read to the gradient: the row crosses the memory
 // once each way. What is longer than that is read again for the gradient (REST): the first time with plain loads, so that
-// the caches may have it (2048 x 262144 halves 505 us with streaming ones, 440). E: waves a SIMD that the registers leave room for.
+// the caches may have it (2048 x 262144 halves 484 us with streaming ones, 437). E: waves a SIMD that the registers leave room for.
 // Bound by memory, reads and writes in turn: 4096 x 100001 halves, a tenth of them without a weight, 285 us, 5.5 TB/s (a flat copy 6.1); 96 x 1000
 // floats 4.1, a launch. (Workgroups that ask for their next row while this one's gradient is made: 334 to 378 us, 333 to 363 without, for
 // the registers that it takes.)
@@ -544,7 +544,8 @@ void launch_rows(THCState* s, const PolicyArgs& a, const T* logits, const Rows& 
   // The least that hold a row, so that a CU has several: one loads while another computes and a third stores. us, halves with gradients:
   // 16384 x 8000 with 4 waves of 4, 8 and 16 packs 82, 84, 100; 8192 x 16000 with 8 waves of 4 and 8, 16 of 8 84, 88, 111; 8192 x 32000
   // with 8 of 8, 16 of 8 and 16 of 16 168, 170, 256; 4096 x 65000 with 16 of 8 and 16 of 16 173, 215; 4096 x 100001 with 8 waves of 16
-  // and 9 more in LDS (two workgroups a CU) and 16 of 16 285, 312; 3000 x 150001 with 16 waves of 16 and 9 347, of 12 and 9 and the end read again 347, 2048 x 262144 442 (with 8 waves 457).
+  // and 9 more in LDS (two workgroups a CU) and 16 of 16 285, 312; 2048 x 190000 with 16 waves of 16 and 9 282, of 12 and 9 and the end read
+  // again 292, 2048 x 262144 so 437, with 8 waves 457.
   if (packs <= 64) HELD(1, 1, 0, 8, false);
   else if (packs <= 256) HELD(1, 4, 0, 8, false);
   else if (packs <= 1024) HELD(4, 4, 0, 8, false);
@@ -552,6 +553,7 @@ void launch_rows(THCState* s, const PolicyArgs& a, const T* logits, const Rows& 
   else if (packs <= 4096) HELD(8, 8, 0, 6, false);
   else if (packs <= 8192) HELD(16, 8, 0, 8, false);
   else if (packs <= 12800) HELD(8, 16, 9, 4, false);
+  else if (packs <= 25600) HELD(16, 16, 9, 4, false);
   else HELD(16, 12, 9, 4, true);
 #undef HELD
 }
