@@ -396,6 +396,7 @@ struct GradArgs {
   int32_t dim, partialStride, chunk;    // chunk: its slots
   int32_t lanes;         // that share a row
   int32_t chunks;
+  uint32_t zeroShares;   // workgroups for 64 rows; 0: a team for a row
   float factor;
   bool add;
 };
@@ -439,31 +440,73 @@ __device__ __forceinline__ void write_partial(float* to, const float (&acc)[V]) 
   }
 }
 
+// Workgroups that share 64 rows: as many as leave each about 32 KiB. The workgroups above each other along a grid's y take shares, too.
+template <typename T>
+int32_t zero_shares(int64_t dim, int64_t slabs) {
+  return (int32_t)std::max<int64_t>(1, std::min<int64_t>(64, 64 * dim * (int64_t)sizeof(T) >> 15) / slabs);
+}
+__device__ __forceinline__ uint64_t share_of_rows(uint32_t share, uint32_t shares) {
+  const uint32_t i = share * gridDim.y + blockIdx.y, n = shares * gridDim.y, from = 64 * i / n, to = 64 * (i + 1) / n;
+  return from < to ? ~uint64_t(0) >> (64 - (to - from)) << from : 0;
+}
+
+// Zeros to the rows row0 + (the bits of `rows`) by a workgroup: rows side by side are one piece of memory, whose 16-byte packs are
+// counted from a 128-byte line's begin, so that a wave writes whole lines whatever the rows' length. us, pack by pack of each row and so: 1 x 7309 floats into 28416 rows 264, 164,
+// 112 x 5055 into 22959 146, 95, 3000 x 3000 into 50000 157, 147 (at a copy's rate 136, 77, 104).
+template <bool NT, typename T>
+__device__ __forceinline__ void zero_rows(T* grad, int64_t stride, int32_t dim, int64_t row0, uint64_t rows) {
+  constexpr int V = 16 / sizeof(T), kLine = 128 / 16;
+  Pack<T, V> zero;
+#pragma unroll
+  for (int e = 0; e < V; ++e) zero.v[e] = Cvt<T>::down(0.f);
+  while (rows) {
+    const int first = __ffsll((unsigned long long)rows) - 1;
+    const uint64_t from = rows >> first;
+    const int count = stride != dim ? 1 : ~from ? __ffsll((unsigned long long)~from) - 1 : 64;
+    rows &= count == 64 ? 0 : ~(((uint64_t(1) << count) - 1) << first);
+    T* begin = grad + (row0 + first) * stride;
+    const int64_t n = (int64_t)count * dim;
+    const int head = (int)min(n, (int64_t)((16 - ((uintptr_t)begin & 15)) & 15) / (int64_t)sizeof(T));
+    const int64_t packs = (n - head) / V;
+    const int tail = (int)(n - head - packs * V), t = threadIdx.x;
+    if (t < head) begin[t] = zero.v[0];
+    if (t < tail) begin[head + packs * V + t] = zero.v[0];
+    T* body = begin + head;
+    for (int64_t k = t - (int)(((uintptr_t)body >> 4) & (kLine - 1)); k < packs; k += blockDim.x)
+      if (k >= 0) store_pack_unaligned<NT>(body + k * V, zero);
+  }
+}
+
 // V columns a lane; a row's last lane is moved back into the row and leaves the columns that it shares to the lane before it. Bound by
 // memory: 32768 x 2048 halves into 50000 rows 60 us, 5.7 TB/s of rows read and written, besides the partial sums, which stay in the caches. (A run
 // that crosses one edge summed to its end by the chunk that it begins in: 1.5 us less to fold, but 9 more here; the few chunks that go on
-// are the launch's end. What sums are added to, asked for together with the rows: the same, for the registers.) Rows are zeroed whole by a
-// workgroup: 3000 x 3000 floats into 50000 rows 166 us with pieces of 4 KiB, 150 so.
+// are the launch's end. What sums are added to, asked for together with the rows: the same, for the registers.)
 template <typename T, int V, int U, bool NT>
 __global__ __launch_bounds__(kBlock) void sum_kernel(GradArgs a, const T* __restrict__ out, T* __restrict__ grad, int64_t vocab,
                                                      int32_t chunkBlocks) {
   using P = Pack<T, V>;
   const int sub = threadIdx.x / a.lanes, lane = threadIdx.x % a.lanes, subs = blockDim.x / a.lanes;
   const int32_t column = ((int32_t)blockIdx.y * a.lanes + lane) * V;
-  if ((int32_t)blockIdx.x >= chunkBlocks) {     // rows of tokens that do not occur, 16 to a team; whole rows to a workgroup
+  if ((int32_t)blockIdx.x >= chunkBlocks) {
+    const uint32_t block = blockIdx.x - chunkBlocks;
+    if (a.zeroShares > 0) {
+      const int64_t row0 = (int64_t)(block / a.zeroShares) * 64, row = row0 + (threadIdx.x & 63);
+      const uint64_t unused = __ballot(row < vocab && a.g.used[row] == 0);
+      zero_rows<NT>(grad, a.gradStride, a.dim, row0, unused & share_of_rows(block % a.zeroShares, a.zeroShares));
+      return;
+    }
+    // short rows: a team each, 16 one after another, whose tokens' numbers are asked for together
     P zero;
 #pragma unroll
     for (int e = 0; e < V; ++e) zero.v[e] = Cvt<T>::down(0.f);
-    const int64_t row0 = (int64_t)(blockIdx.x - chunkBlocks) * (subs * 16) + sub;
+    const int64_t row0 = (int64_t)block * (subs * 16) + sub;
     int32_t used[16];
 #pragma unroll
     for (int j = 0; j < 16; ++j) used[j] = a.g.used[min(row0 + (int64_t)j * subs, vocab - 1)];
 #pragma unroll
     for (int j = 0; j < 16; ++j) {
       const int64_t row = row0 + (int64_t)j * subs;
-      if (j % gridDim.y == blockIdx.y && row < vocab && used[j] == 0) {
-        for (int32_t k = lane * V; k < a.dim; k += a.lanes * V) store_pack_unaligned<NT>(grad + row * a.gradStride + min(k, a.dim - V), zero);
-      }
+      if (column < a.dim && row < vocab && used[j] == 0) store_pack_unaligned<false>(grad + row * a.gradStride + min(column, a.dim - V), zero);
     }
     return;
   }
@@ -633,7 +676,7 @@ constexpr int kFew = 2048, kFewRows = 64;
 template <typename T, int V>
 __global__ __launch_bounds__(kBlock) void few_kernel(T* __restrict__ grad, int64_t gradStride, const int64_t* __restrict__ tokens, int32_t n,
                                                      uint32_t vocab, uint32_t padding, const T* __restrict__ out, int64_t outStride, int32_t dim,
-                                                     float factor, bool add) {
+                                                     float factor, bool add, uint32_t zeroShares) {
   using P = Pack<T, V>;
   constexpr int W = kBlock / 64, U = 8;
   __shared__ uint64_t same[kFew / 64];
@@ -648,7 +691,7 @@ __global__ __launch_bounds__(kBlock) void few_kernel(T* __restrict__ grad, int64
     return (k >> 32) == 0 && token < vocab && token != padding ? token : ~0u;
   };
   if ((int32_t)blockIdx.x >= n) {
-    const uint32_t row0 = (uint32_t)((int32_t)blockIdx.x - n) * kFewRows;
+    const uint32_t row0 = (blockIdx.x - n) / zeroShares * kFewRows;
     if (threadIdx.x == 0) same[0] = 0;
     __syncthreads();
     for (int32_t i = threadIdx.x; i < n; i += kBlock) {
@@ -656,13 +699,9 @@ __global__ __launch_bounds__(kBlock) void few_kernel(T* __restrict__ grad, int64
       if (token - row0 < (uint32_t)kFewRows) atomicOr((unsigned long long*)&same[0], 1ull << (token - row0));
     }
     __syncthreads();
-    const uint64_t used = same[0];
-    if (column >= dim) return;
-    P zero;
-#pragma unroll
-    for (int e = 0; e < V; ++e) zero.v[e] = Cvt<T>::down(0.f);
-    for (int r = wave; r < kFewRows && row0 + r < vocab; r += W)
-      if (!((used >> r) & 1)) store_pack_unaligned<false>(grad + (int64_t)(row0 + r) * gradStride + c0, zero);
+    uint64_t rows = ~same[0] & share_of_rows((blockIdx.x - n) % zeroShares, zeroShares);
+    if (vocab - row0 < (uint32_t)kFewRows) rows &= (uint64_t(1) << (vocab - row0)) - 1;
+    zero_rows<false>(grad, gradStride, dim, row0, rows);
     return;
   }
   const uint32_t me = token_at(blockIdx.x);
@@ -922,10 +961,11 @@ void launch_grad(THCState* s, T* grad, int64_t vocab, int64_t gradStride, const 
   // 16 x 2048 3.7, 5.2, 10.0; 600 x 2048 6.6, 7.7, 13.0; 1024 x 513 8.4, 8.8, 13.8; 1500 x 64 9.6, 7.5, 13.0; 1000 x 2048 13.7, 10.2, 13.7;
   // 512 x 8192 15.3, 18, 15.1.
   if (n <= kFew && vocab <= int64_t(1) << 28 && (int64_t)n * n * fewSlabs <= std::min<int64_t>(tuning("embedding.few", 3 << 20), own ? 3 << 19 : 3 << 20)) {
-    const dim3 grid((unsigned)(n + (add ? 0 : (vocab + kFewRows - 1) / kFewRows)), fewSlabs);
+    const int32_t shares = zero_shares<T>(dim, fewSlabs);
+    const dim3 grid((unsigned)(n + (add ? 0 : (vocab + kFewRows - 1) / kFewRows * shares)), fewSlabs);
     auto go = [&](auto v) {
       hipLaunchKernelGGL((few_kernel<T, decltype(v)::value>), grid, dim3(kBlock), 0, st, grad, gradStride, tokens, n, (uint32_t)vocab, left, out,
-                         outStride, dim, factor, add);
+                         outStride, dim, factor, add, (uint32_t)shares);
     };
     if (V == 1) go(std::integral_constant<int, 1>{});
     else go(std::integral_constant<int, kPack>{});
@@ -983,7 +1023,9 @@ void launch_grad(THCState* s, T* grad, int64_t vocab, int64_t gradStride, const 
     hipLaunchKernelGGL(group_kernel<false>, dim3(1u << shift), dim3(kGroupThreads), 0, st, a.g, split, tokens, n, (uint32_t)vocab, left, shift);
   }
   const int32_t chunkBlocks = (a.chunks + subs - 1) / subs;
-  const int64_t zeroBlocks = add ? 0 : (vocab + subs * 16 - 1) / (subs * 16);
+  const bool shortRows = dim * (int64_t)sizeof(T) <= 128;
+  a.zeroShares = shortRows ? 0 : zero_shares<T>(dim, slabs);
+  const int64_t zeroBlocks = add ? 0 : shortRows ? (vocab + subs * 16 - 1) / (subs * 16) : (vocab + 63) / 64 * a.zeroShares;
   const dim3 grid((unsigned)(chunkBlocks + zeroBlocks), slabs), block(subs * lanes);
   // Zeros are streaming stores in large tables whose rows are whole lines: us, plain and streaming, of 32768 x 2048 halves into 50000 rows (205 MB)
   // 84, 78 (68, 77 where the caches still hold the table from the call before), 6000 x 8192 floats into 30000 219, 205; of 8192 x 1024 halves into
