@@ -710,16 +710,20 @@ class AdamW(object):
         else:
             lists += [(self.mean, "float"), (self.square, "float")]
         self._arrays = [self._array(l, kind) for l, kind in lists]
-        self._args = [a.buffer_info()[0] if a is not None else 0 for a in self._arrays]
+        self._args = [a[1] for a in self._arrays]
 
     def _array(self, tensors, kind):
+        """(what holds the tensors' addresses side by side, where they begin)"""
         if tensors is None:
-            return None
+            return None, 0
         if len(tensors) != len(self.params):
             raise ValueError("%d tensors for %d parameters" % (len(tensors), len(self.params)))
+        if _fastcall is not None:
+            return _fastcall.addresses(tensors, kind)
         if any([t.kind != kind for t in tensors]):
             raise ValueError("a tensor of another type than %s" % kind)
-        return array.array("Q", [t.a for t in tensors])
+        addresses = array.array("Q", [t.a for t in tensors])
+        return addresses, addresses.buffer_info()[0]
 
     def step(self, grad_scale=1.0):
         """One step from what the gradients hold, times grad_scale."""
@@ -734,7 +738,7 @@ class AdamW(object):
         mean = [Tensor("float") for _ in self.params] if mean is None else mean
         square = [Tensor("float") for _ in self.params] if square is None else square
         arrays = [self._array(mean, "float"), self._array(square, "float")]
-        _CALLS["float"]["adamW8Moments"](len(self.params), *[a.buffer_info()[0] for a in arrays], *self._args[-4:])
+        _CALLS["float"]["adamW8Moments"](len(self.params), arrays[0][1], arrays[1][1], *self._args[-4:])
         return mean, square
 
 

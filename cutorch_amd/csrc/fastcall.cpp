@@ -278,9 +278,46 @@ PyObject* py_half_bits(PyObject*, PyObject* o) {
   return PyLong_FromLong(h.bits);
 }
 
+// addresses(tensors, kind): their addresses side by side, for an entry point that takes a list of tensors, and where they begin. (The
+// same in Python, 294 tensors: 42 us; so 14.)
+PyObject *kAddress, *kKind;
+PyObject* addresses(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  if (n != 2) {
+    PyErr_SetString(PyExc_TypeError, "addresses(tensors, kind)");
+    return nullptr;
+  }
+  PyObject* all = PySequence_Fast(args[0], "a list of tensors");
+  if (!all) return nullptr;
+  const Py_ssize_t count = PySequence_Fast_GET_SIZE(all);
+  PyObject* bytes = PyBytes_FromStringAndSize(nullptr, count * (Py_ssize_t)sizeof(unsigned long long));
+  unsigned long long* to = bytes ? reinterpret_cast<unsigned long long*>(PyBytes_AS_STRING(bytes)) : nullptr;
+  bool good = bytes != nullptr;
+  for (Py_ssize_t i = 0; good && i < count; ++i) {
+    PyObject* t = PySequence_Fast_GET_ITEM(all, i);
+    Py_INCREF(t);
+    PyObject *kind = PyObject_GetAttr(t, kKind), *address = kind ? PyObject_GetAttr(t, kAddress) : nullptr;
+    const int same = address ? PyObject_RichCompareBool(kind, args[1], Py_EQ) : -1;
+    if (same == 0) PyErr_Format(PyExc_ValueError, "a tensor of another type than %S", args[1]);
+    good = same == 1;
+    if (good) {
+      const unsigned long long a = PyLong_AsUnsignedLongLong(address);
+      good = !(a == (unsigned long long)-1 && PyErr_Occurred());
+      std::memcpy(to + i, &a, sizeof(a));
+    }
+    Py_XDECREF(address);
+    Py_XDECREF(kind);
+    Py_DECREF(t);
+  }
+  Py_DECREF(all);
+  PyObject* result = good ? Py_BuildValue("(OK)", bytes, (unsigned long long)(uintptr_t)to) : nullptr;
+  Py_XDECREF(bytes);
+  return result;
+}
+
 PyMethodDef kMethods[] = {{"setup", setup, METH_VARARGS, nullptr},
                           {"bind", bind, METH_VARARGS, nullptr},
                           {"half_bits", py_half_bits, METH_O, nullptr},
+                          {"addresses", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(addresses)), METH_FASTCALL, nullptr},
                           {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_fastcall", "Calls of libTHC.so's entry points.", -1, kMethods};
 
@@ -294,5 +331,8 @@ PyMODINIT_FUNC PyInit__fastcall() {
   FunctionType.tp_vectorcall_offset = offsetof(Function, call);
   FunctionType.tp_call = PyVectorcall_Call;
   if (PyType_Ready(&FunctionType) < 0) return nullptr;
+  kAddress = PyUnicode_InternFromString("a");
+  kKind = PyUnicode_InternFromString("kind");
+  if (!kAddress || !kKind) return nullptr;
   return PyModule_Create(&kModule);
 }
