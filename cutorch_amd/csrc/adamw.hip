@@ -10,7 +10,8 @@
 //   v = top (c / 255)^4             c = round(255 (v / top)^(1/4)), at least 1 where v > 0
 //
 // A code step is 1.6 % of the value near the top and a value of a hundredth of it still has a tenth of the codes. No v that is
-// not zero is held as zero: the next step would divide by the root of its own gradient's share alone. What scales all of a block
+// not zero is held as zero: the next step would divide by the root of its own gradient's share alone. So that code 1 stands for a number even
+// where a block's largest v is tiny, a top that is not zero is 2^-116 at least; means below 2^-120 are held as zeros. What scales all of a block
 // (the growth of the moments in the first steps) is in the float and is not rounded to codes.
 #include <algorithm>
 #include <cmath>
@@ -23,7 +24,8 @@ namespace thc {
 namespace {
 
 constexpr int kStateBlock = 256;        // elements that share a scale: 4 a lane of one wave
-constexpr float kSmallestTop = 0x1p-120f;   // below it a block of states is held as zeros: the reciprocal stays finite
+constexpr float kSmallestMean = 0x1p-120f;     // below it a block of means is held as zeros: the reciprocal stays finite
+constexpr float kSmallestSquare = 0x1p-116f;   // a block of squares has this for its top at least, unless all are zero: (1 / 255)^4 of it is 2^-148
 
 struct Hyper {
   float beta1, oneMinusBeta1, beta2, oneMinusBeta2, rootScale, eps, keep, rate, gradScale;
@@ -40,7 +42,7 @@ __device__ __forceinline__ float share_root(float x) {
 }
 // The nearest floats to the roots of second moments, which may be infinite, or so small that a step without eps divides by very little.
 // A wave takes the short root where all it has are zeros or in that one's range, and sqrtf else. As bits a NaN and what is negative are above
-// infinity, and zero less one above all. us of 8-bit steps of 4.5 M floats, 4.4 M halves and 184 M floats: 15.2, 14.5, 468 so, 16.4, 15.8, 493 with
+// infinity, and zero less one above all. us of 8-bit steps of 4.5 M floats, 4.4 M halves and 184 M floats: 14.7, 14.5, 463 so, 16.4, 15.8, 493 with
 // sqrtf alone.
 __device__ __forceinline__ void moment_roots(float (&root)[4], const float (&v)[4]) {
   uint32_t low = ~0u, high = 0;
@@ -221,10 +223,8 @@ __device__ __forceinline__ float wave_top(uint32_t bits) {
   step(integral_constant<int, 0x143>{}, integral_constant<int, 0xc>{});   // lane 31 to the last two rows
   return __uint_as_float((uint32_t)__builtin_amdgcn_readlane(v, 63));
 }
-__device__ __forceinline__ float inverse_top(float& top) {
-  if (top < kSmallestTop) top = 0.f;
-  return top > 0.f ? 1.f / top : 0.f;
-}
+// 1 / top; 0 where a block has nothing to code (zeros, or a top that is not finite, which makes NaN of all of it).
+__device__ __forceinline__ float inverse_of(float top) { return top > 0.f ? 1.f / top : 0.f; }
 template <typename T>
 __device__ __forceinline__ void load4_codes(T (&to)[4], const T* from, int n) {
   using P = Pack<T, 4>;
@@ -307,14 +307,16 @@ __device__ __forceinline__ void step8_part(const Hyper& h, void* const* pointers
       if constexpr (MASTER) store4<NT>(master + i, p[u], n);
       store4<NT>(param + i, p[u], n);
       float newMean = wave_top(maxMean), newSquare = wave_top(maxSquare);
-      const float inverseMean = inverse_top(newMean), inverseSquare = inverse_top(newSquare);
+      if (newMean < kSmallestMean) newMean = 0.f;
+      if (newSquare > 0.f) newSquare = fmaxf(newSquare, kSmallestSquare);
+      const float inverseMean = inverse_of(newMean), inverseSquare = inverse_of(newSquare);
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const float c = rintf(share_root(fabsf(m[e]) * inverseMean) * 127.f);
         codeMean[u][e] = (int8_t)(int)(m[e] < 0.f ? -c : c);
-        const float share = v[e] * inverseSquare;
-        const float d = rintf(share_root(share_root(share)) * 255.f);
-        codeSquare[u][e] = (uint8_t)(int)(share > 0.f ? fmaxf(d, 1.f) : d);
+        // (an infinite top has no inverse, and its codes are 0; the share of a v that is not zero may be, below a large top)
+        const float d = rintf(share_root(share_root(v[e] * inverseSquare)) * 255.f);
+        codeSquare[u][e] = (uint8_t)(int)(v[e] > 0.f && inverseSquare > 0.f ? fmaxf(d, 1.f) : d);
       }
       store4_codes<NT>(mean + i, codeMean[u], n);
       store4_codes<NT>(square + i, codeSquare[u], n);

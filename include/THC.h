@@ -687,8 +687,10 @@ THC_AMD_DECLARE_TOKEN_API(THCudaHalfTensor)
  * float (the largest magnitude) for each 256 elements of a tensor in its
  * logical order, ceil(n / 256) of them:
  *   m = meanScale (c / 127) |c / 127|,  v = squareScale (c / 255)^4
- * with the nearest codes, v's at least 1 where v > 0. Zeros begin a run. A
- * moment that is not finite makes its 256 elements' moments NaN.
+ * with the nearest codes, v's at least 1 where v > 0. squareScale is 2^-116 at
+ * least where a v of its 256 is not zero, so that none of those is held as
+ * zero; means whose largest is below 2^-120 are held as zeros. Zeros begin a
+ * run. A moment that is not finite makes its 256 elements' moments NaN.
  * adamW8Moments writes the moments that such states hold as floats. */
 THC_API void THCudaTensor_adamW(THCState *state, int count, THCudaTensor **param,
                                 THCudaTensor **grad, THCudaTensor **mean,
