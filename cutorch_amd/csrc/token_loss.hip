@@ -563,7 +563,7 @@ void check_positions(const AnyTensor* t, int64_t rows, int arg, const char* what
   THC_ARG_CHECK(tensor_numel(t) == rows, arg, "%ld %s for %ld rows of logits", (long)tensor_numel(t), what, (long)rows);
 }
 
-// Outputs take the tokens' sizes and are written densely; `meets`: one lies on what the call reads.
+// Outputs take the tokens' sizes and are written densely; `meets`: one lies on what the call reads or within the gradient.
 AnyTensor* position_output(THCState* s, AnyTensor* out, bool meets) {
   if (tensor_is_contiguous(out) && !meets) {
     tensor_retain(out);
@@ -618,6 +618,18 @@ void token_loss(THCState* s, DType dt, const PolicyCall& c) {
   tensor_resize_as(s, c.logProb, c.tokens, DType::F32);
   if (policy) tensor_resize_as(s, c.loss, c.tokens, DType::F32);
   if (c.grad) tensor_resize_as(s, c.grad, c.logits, dt);
+  // Outputs on one another would be written over by each other's workgroups: dense ones are refused. Those with gaps may lie in each other's:
+  // losses and log-probabilities that do are copied there behind the launches.
+  auto apart = [&](const AnyTensor* x, DType xt, const AnyTensor* y, DType yt, int arg, const char* what) {
+    THC_ARG_CHECK(!spans_meet(x, xt, y, yt) || !tensor_is_contiguous(x) || !tensor_is_contiguous(y), arg, "%s share memory", what);
+  };
+  if (policy) {
+    apart(c.loss, DType::F32, c.logProb, DType::F32, 2, "the losses and the log-probabilities");
+    if (c.grad) {
+      apart(c.loss, DType::F32, c.grad, dt, 2, "the losses and the gradient");
+      apart(c.logProb, DType::F32, c.grad, dt, 3, "the log-probabilities and the gradient");
+    }
+  }
   note_stream_use(s, {c.loss, c.logProb, c.grad, c.logits, c.tokens, c.old, c.advantage, c.reference, c.weight});
   PolicyArgs a{};
   a.token = tokens.data<int64_t>();
@@ -642,10 +654,10 @@ void token_loss(THCState* s, DType dt, const PolicyCall& c) {
     return false;
   };
   TensorRef loss(s, nullptr), logProb(s, nullptr), grad(s, nullptr);
-  logProb.t = position_output(s, c.logProb, meets(c.logProb, DType::F32, 0));
+  logProb.t = position_output(s, c.logProb, meets(c.logProb, DType::F32, 0) || spans_meet(c.logProb, DType::F32, c.grad, dt));
   a.logProb = (float*)tensor_data(logProb.t, DType::F32);
   if (policy) {
-    loss.t = position_output(s, c.loss, meets(c.loss, DType::F32, 0));
+    loss.t = position_output(s, c.loss, meets(c.loss, DType::F32, 0) || spans_meet(c.loss, DType::F32, c.grad, dt));
     a.loss = (float*)tensor_data(loss.t, DType::F32);
   }
   Rows gr{};

@@ -663,6 +663,7 @@ THC_API void THCudaTensor_sumallNoAlloc(THCState *state, THCudaTensor *self, flo
    * be the logits themselves; null: losses alone). weight null: 1 / rows.     \
    * A row of weight 0 is not read: its loss, log-probability and gradient     \
    * are 0 whatever it holds. refLogProb null, or klCoef 0: no KL term.        \
+   * The three outputs may not lie on one another, on inputs they may.         \
    * The loss of the batch is the sum of `loss`. */                            \
   THC_API void Tensor##_policyLoss(                                            \
       THCState *, THCudaTensor *loss, THCudaTensor *logProb,                   \
