@@ -15,6 +15,7 @@
 // (the growth of the moments in the first steps) is in the float and is not rounded to codes.
 #include <algorithm>
 #include <cmath>
+#include <functional>
 #include <type_traits>
 #include <vector>
 
@@ -571,6 +572,40 @@ void adamw(THCState* s, DType dt, int count, const Lists& l, double lr, double b
   held.write_back();
 }
 
+// All tensors are decoded side by side: an output on another tensor's scales or output would be written before or after those are read or
+// written. Looked for among the dense operands, which are used where they are, in the order of their addresses.
+void refuse_meeting(int count, AnyTensor** meanOut, AnyTensor** squareOut, AnyTensor** mean, AnyTensor** meanScale, AnyTensor** squareScale) {
+  struct Span {
+    const void* storage;
+    int64_t first, last;      // elements
+    int arg, index;           // arg: of an output, 0 for scales
+  };
+  std::vector<Span> spans;
+  spans.reserve(4 * (size_t)count);
+  for (int i = 0; i < count; ++i) {
+    if (!has_elements(mean[i])) continue;
+    const AnyTensor* t[4] = {meanOut[i], squareOut[i], meanScale[i], squareScale[i]};
+    const int args[4] = {3, 4, 0, 0};
+    for (int k = 0; k < 4; ++k)
+      if (tensor_is_contiguous(t[k])) spans.push_back(Span{t[k]->storage, t[k]->storageOffset, t[k]->storageOffset + tensor_numel(t[k]), args[k], i});
+  }
+  std::sort(spans.begin(), spans.end(), [](const Span& a, const Span& b) {
+    if (a.storage != b.storage) return std::less<const void*>()(a.storage, b.storage);
+    return a.first < b.first;
+  });
+  // those before it that reach farthest: of the outputs, and of the scales
+  const Span *out = nullptr, *scale = nullptr;
+  for (const Span& x : spans) {
+    for (const Span* y : {out, scale}) {
+      if (!y || y->storage != x.storage || y->last <= x.first || (!x.arg && !y->arg)) continue;
+      const Span &one = x.arg ? x : *y, &other = x.arg ? *y : x;
+      THC_ARG_CHECK(false, one.arg, "tensor %d lies on tensor %d's %s", one.index + 1, other.index + 1, other.arg ? "moments" : "scales");
+    }
+    const Span*& farthest = x.arg ? out : scale;
+    if (!farthest || farthest->storage != x.storage || farthest->last < x.last) farthest = &x;
+  }
+}
+
 // Floats of 8-bit states.
 void moments(THCState* s, int count, AnyTensor** meanOut, AnyTensor** squareOut, AnyTensor** mean, AnyTensor** meanScale, AnyTensor** square,
              AnyTensor** squareScale) {
@@ -605,18 +640,24 @@ void moments(THCState* s, int count, AnyTensor** meanOut, AnyTensor** squareOut,
     }
     THC_ARG_CHECK(!spans_meet(out[0], DType::F32, out[1], DType::F32), 4, "tensor %d's two moments share memory", i + 1);
   }
+  refuse_meeting(count, meanOut, squareOut, mean, meanScale, squareScale);
+  // every copy is made before the first launch: outputs may lie in the gaps of scales that are read through one
+  std::vector<Operands<6>> all;
+  all.reserve(count);
   for (int i = 0; i < count; ++i) {
     if (!has_elements(mean[i])) continue;
     note_stream_use(s, {meanOut[i], squareOut[i], mean[i], meanScale[i], square[i], squareScale[i]});
-    void* p[6];
-    p[kParam] = held.add(meanOut[i], DType::F32, true);
-    p[kGrad] = held.add(squareOut[i], DType::F32, true);
-    p[kMean] = held.add(mean[i], DType::I8, false);
-    p[kSquare] = held.add(square[i], DType::U8, false);
-    p[kMeanScale] = held.add(meanScale[i], DType::F32, false);
-    p[kSquareScale] = held.add(squareScale[i], DType::F32, false);
-    batch.add(p, tensor_numel(mean[i]));
+    Operands<6> o;
+    o.p[kParam] = held.add(meanOut[i], DType::F32, true);
+    o.p[kGrad] = held.add(squareOut[i], DType::F32, true);
+    o.p[kMean] = held.add(mean[i], DType::I8, false);
+    o.p[kSquare] = held.add(square[i], DType::U8, false);
+    o.p[kMeanScale] = held.add(meanScale[i], DType::F32, false);
+    o.p[kSquareScale] = held.add(squareScale[i], DType::F32, false);
+    o.size = tensor_numel(mean[i]);
+    all.push_back(o);
   }
+  for (const Operands<6>& o : all) batch.add(o.p, o.size);
   batch.flush();
   THC_CHECK(hipGetLastError());
   note_kernel("adamw8-moments");

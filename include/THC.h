@@ -692,7 +692,8 @@ THC_AMD_DECLARE_TOKEN_API(THCudaHalfTensor)
  * least where a v of its 256 is not zero, so that none of those is held as
  * zero; means whose largest is below 2^-120 are held as zeros. Zeros begin a
  * run. A moment that is not finite makes its 256 elements' moments NaN.
- * adamW8Moments writes the moments that such states hold as floats. */
+ * adamW8Moments writes the moments that such states hold as floats; its
+ * outputs may not lie on one another or on any tensor's scales. */
 THC_API void THCudaTensor_adamW(THCState *state, int count, THCudaTensor **param,
                                 THCudaTensor **grad, THCudaTensor **mean,
                                 THCudaTensor **square, double lr, double beta1,
