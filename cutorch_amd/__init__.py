@@ -671,11 +671,22 @@ class Tensor(object):
         return self._real_out(self._calls["maxall"](self.a))
 
 
+def _operands(name):
+    """One of the optimizer's lists: read as a tuple, replaced as a whole."""
+    return property(lambda self: self._lists.get(name), lambda self, tensors: self._hold(name, tensors))
+
+
 class AdamW(object):
     """AdamW on a list of parameters, one call a step for all of them. `grads` are the tensors that the gradients are in at each
     step. The moments are kept in floats, or with bits=8 in codes with a float for each 256 elements. Half parameters may
     have float copies (`master`) that the steps go from. mean, square (and mean_scale, square_scale with 8 bits): the states
-    of an earlier run, as `step` is the number of steps it had made; zeros otherwise."""
+    of an earlier run, as `step` is the number of steps it had made; zeros otherwise.
+
+    The lists are tuples of the optimizer's own, which keep their tensors alive; another list is assigned to go on with it
+    (opt.grads = [...]; opt.master = None leaves the copies)."""
+
+    params, grads, master = _operands("params"), _operands("grads"), _operands("master")
+    mean, square, mean_scale, square_scale = (_operands(name) for name in ("mean", "square", "mean_scale", "square_scale"))
 
     def __init__(self, params, grads, master=None, lr=1e-3, beta1=0.9, beta2=0.999, eps=1e-8, weight_decay=0.01, bits=32, mean=None,
                  square=None, mean_scale=None, square_scale=None, step=0):
@@ -690,34 +701,48 @@ class AdamW(object):
         if master is not None and self.kind != "half":
             raise ValueError("float copies are of half parameters")
         self.lr, self.beta1, self.beta2, self.eps, self.weight_decay, self.steps, self.bits = lr, beta1, beta2, eps, weight_decay, step, bits
-        self.params, self.grads, self.master = list(params), list(grads), list(master) if master is not None else None
+        # the lists as the entry points take them: name -> type
+        self._kinds = {"params": self.kind}
+        if self.kind == "half":
+            self._kinds["master"] = "float"
+        self._kinds["grads"] = self.kind
+        self._kinds.update([("mean", "char"), ("mean_scale", "float"), ("square", "byte"), ("square_scale", "float")] if bits == 8 else
+                           [("mean", "float"), ("square", "float")])
+        self._lists, self._arrays, self._args = {}, {}, []
+        self._count = len(params)
 
         def zeros(kind, shape):
             return Tensor(kind).resize(shape).zero() if shape else Tensor(kind)
 
-        def state(given, kind, blocks=False):
-            if given is not None:
-                return list(given)
-            return [zeros(kind, (-(-p.numel() // 256),) if blocks and p.numel() else () if blocks else p.shape) for p in self.params]
+        def state(name, given):
+            if given is None and name in self._kinds:
+                blocks = name.endswith("_scale")
+                given = [zeros(self._kinds[name], (-(-p.numel() // 256),) if blocks and p.numel() else () if blocks else p.shape)
+                         for p in params]
+            self._hold(name, given)
 
-        self.mean = state(mean, "char" if bits == 8 else "float")
-        self.square = state(square, "byte" if bits == 8 else "float")
-        self.mean_scale = state(mean_scale, "float", True) if bits == 8 else None
-        self.square_scale = state(square_scale, "float", True) if bits == 8 else None
-        lists = [(self.params, self.kind)] + ([(self.master, "float")] if self.kind == "half" else []) + [(self.grads, self.kind)]
-        if bits == 8:
-            lists += [(self.mean, "char"), (self.mean_scale, "float"), (self.square, "byte"), (self.square_scale, "float")]
+        self._hold("params", params)
+        self._hold("grads", grads)
+        self._hold("master", master)
+        for name, given in (("mean", mean), ("square", square), ("mean_scale", mean_scale), ("square_scale", square_scale)):
+            state(name, given)
+
+    def _hold(self, name, tensors):
+        """Takes a list: its tensors, which live as long as their addresses are here."""
+        if tensors is None and (name == "master" or name not in self._kinds):
+            held = None, 0
+        elif name not in self._kinds:
+            raise ValueError("%s parameters with %d-bit states have no %s" % (self.kind, self.bits, name))
         else:
-            lists += [(self.mean, "float"), (self.square, "float")]
-        self._arrays = [self._array(l, kind) for l, kind in lists]
-        self._args = [a[1] for a in self._arrays]
+            tensors = tuple(tensors)
+            held = self._array(tensors, self._kinds[name])
+        self._lists[name], self._arrays[name] = tensors, held
+        self._args = [self._arrays.get(n, (None, 0))[1] for n in self._kinds]
 
     def _array(self, tensors, kind):
         """(what holds the tensors' addresses side by side, where they begin)"""
-        if tensors is None:
-            return None, 0
-        if len(tensors) != len(self.params):
-            raise ValueError("%d tensors for %d parameters" % (len(tensors), len(self.params)))
+        if len(tensors) != self._count:
+            raise ValueError("%d tensors for %d parameters" % (len(tensors), self._count))
         if _fastcall is not None:
             return _fastcall.addresses(tensors, kind)
         if any([t.kind != kind for t in tensors]):
@@ -728,7 +753,7 @@ class AdamW(object):
     def step(self, grad_scale=1.0):
         """One step from what the gradients hold, times grad_scale."""
         _CALLS[self.kind]["adamW8" if self.bits == 8 else "adamW"](
-            len(self.params), *self._args, self.lr, self.beta1, self.beta2, self.eps, self.weight_decay, self.steps + 1, grad_scale)
+            self._count, *self._args, self.lr, self.beta1, self.beta2, self.eps, self.weight_decay, self.steps + 1, grad_scale)
         self.steps += 1
 
     def moments(self, mean=None, square=None):
@@ -738,7 +763,7 @@ class AdamW(object):
         mean = [Tensor("float") for _ in self.params] if mean is None else mean
         square = [Tensor("float") for _ in self.params] if square is None else square
         arrays = [self._array(mean, "float"), self._array(square, "float")]
-        _CALLS["float"]["adamW8Moments"](len(self.params), arrays[0][1], arrays[1][1], *self._args[-4:])
+        _CALLS["float"]["adamW8Moments"](self._count, arrays[0][1], arrays[1][1], *self._args[-4:])
         return mean, square
 
 
