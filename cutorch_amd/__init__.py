@@ -694,6 +694,7 @@ class AdamW(object):
             bits = 8
         if bits not in (8, 32):
             raise ValueError("states have 8 or 32 bits")
+        params = tuple(params)
         kinds = {p.kind for p in params}
         if kinds - {"float", "half"} or len(kinds) > 1:
             raise ValueError("parameters are all float or all half")

@@ -101,3 +101,10 @@ def test_a_list_that_does_not_fit_changes_nothing(made):
         opt.grads = None
     opt.step()
     assert opt.grads is held and made[-1] == ("adamW", [[t.a for t in l] for l in (opt.params, opt.grads, opt.mean, opt.square)])
+
+
+def test_parameters_may_come_from_a_generator(made):
+    opt = thc.AdamW((p for p in [_Stub("half"), _Stub("half")]), (g for g in [_Stub("half"), _Stub("half")]))
+    assert len(opt.params) == 2 and opt.kind == "half"
+    opt.step()
+    assert len(made[-1][1][0]) == 2
