@@ -680,7 +680,7 @@ class AdamW(object):
     """AdamW on a list of parameters, one call a step for all of them. `grads` are the tensors that the gradients are in at each
     step. The moments are kept in floats, or with bits=8 in codes with a float for each 256 elements. Half parameters may
     have float copies (`master`) that the steps go from. mean, square (and mean_scale, square_scale with 8 bits): the states
-    of an earlier run, as `step` is the number of steps it had made; zeros otherwise.
+    of an earlier run, as `step` is the number of steps it had made, all of them together; zeros before the first step.
 
     The lists are tuples of the optimizer's own, which keep their tensors alive; another list is assigned to go on with it
     (opt.grads = [...]; opt.master = None leaves the copies)."""
@@ -702,6 +702,8 @@ class AdamW(object):
         if master is not None and self.kind != "half":
             raise ValueError("float copies are of half parameters")
         self.lr, self.beta1, self.beta2, self.eps, self.weight_decay, self.steps, self.bits = lr, beta1, beta2, eps, weight_decay, step, bits
+        if step > 0 and (mean is None or square is None or (bits == 8 and (mean_scale is None or square_scale is None))):
+            raise ValueError("a run that has made %d steps goes on without all of its states" % step)
         # the lists as the entry points take them: name -> type
         self._kinds = {"params": self.kind}
         if self.kind == "half":

@@ -108,3 +108,18 @@ def test_parameters_may_come_from_a_generator(made):
     assert len(opt.params) == 2 and opt.kind == "half"
     opt.step()
     assert len(made[-1][1][0]) == 2
+
+
+@pytest.mark.parametrize("bits,names", [(32, ("mean", "square")), (8, ("mean", "mean_scale", "square", "square_scale"))])
+def test_an_earlier_run_is_resumed_with_all_its_states(made, bits, names):
+    kinds = {"mean": "char" if bits == 8 else "float", "square": "byte" if bits == 8 else "float", "mean_scale": "float", "square_scale": "float"}
+    for some in range(2 ** len(names)):
+        states = {n: [_Stub(kinds[n])] for i, n in enumerate(names) if some >> i & 1}
+        if len(states) == len(names):
+            opt = thc.AdamW([_Stub()], [_Stub()], bits=bits, step=3, **states)
+            assert opt.steps == 3 and all(getattr(opt, n) == tuple(states[n]) for n in names)
+        else:
+            with pytest.raises(ValueError, match="without all of"):
+                thc.AdamW([_Stub()], [_Stub()], bits=bits, step=3, **states)
+        # before the first step all of them are zeros, whoever makes them
+        assert thc.AdamW([_Stub()], [_Stub()], bits=bits, **states).steps == 0
