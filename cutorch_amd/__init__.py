@@ -759,10 +759,22 @@ class AdamW(object):
             self._count, *self._args, self.lr, self.beta1, self.beta2, self.eps, self.weight_decay, self.steps + 1, grad_scale)
         self.steps += 1
 
+    def _copied(self, given, states):
+        if given is None:
+            return list(states)
+        self._array(given, "float")      # (as many as there are, and floats)
+        for t, state in zip(given, states):
+            if t.shape != state.shape:
+                t.resize(state.shape)
+            if t.a != state.a and state.numel():
+                t.copy(state)
+        return given
+
     def moments(self, mean=None, square=None):
-        """(mean, square): lists of float tensors with the moments, those given or new ones; of 32-bit states the states themselves."""
+        """(mean, square): lists of float tensors with the moments, those given or new ones; the states themselves where 32-bit
+        ones are asked for without tensors to copy them to."""
         if self.bits == 32:
-            return self.mean, self.square
+            return self._copied(mean, self.mean), self._copied(square, self.square)
         mean = [Tensor("float") for _ in self.params] if mean is None else mean
         square = [Tensor("float") for _ in self.params] if square is None else square
         arrays = [self._array(mean, "float"), self._array(square, "float")]

@@ -86,3 +86,33 @@ def test_outputs_side_by_side_and_in_gaps(thc):
     mean, square = opt.moments(outs[:4], outs[4:])
     for a, b in zip(mean + square, want[0] + want[1]):
         assert_bit_equal(a.numpy(), b)
+
+
+def test_32_bit_moments_in_the_tensors_given(thc):
+    rng = np.random.default_rng(10)
+    shapes = SIZES + [()]
+    p, g = _problem(rng, SIZES, "float")
+    opt = thc.AdamW(_put(thc, p) + [thc.Tensor("float")], _put(thc, g) + [thc.Tensor("float")], **HYPER)
+    opt.step()
+    states = [[x.numpy() for x in l[:4]] for l in (opt.mean, opt.square)]      # (the last one has no elements)
+    # new ones, one of another size, and every second column of something wider
+    wide = thc.Tensor("float").resize((7, 200)).fill(7)
+    mean, square = ([thc.Tensor("float") for _ in shapes] for _ in range(2))
+    mean[0].resize((9, 9))
+    mean[1] = wide.view_as_strided(0, (7, 100), (200, 2))
+    got = opt.moments(mean, square)
+    assert got[0] is mean and got[1] is square
+    for given, held in zip(got, states):
+        assert given[4].numel() == 0
+        for a, b in zip(given, held):
+            assert_bit_equal(a.numpy(), b)
+    assert np.all(wide.numpy()[:, 1::2] == 7)
+    opt.step()
+    assert_bit_equal(mean[0].numpy(), states[0][0])         # the run has gone on, the copies have not
+    # those not given are the states themselves, and the states may be given
+    mean, square = opt.moments(square=square)
+    assert [x.a for x in mean] == [x.a for x in opt.mean] and not np.array_equal(square[0].numpy(), states[1][0])
+    assert_bit_equal(opt.moments(opt.mean)[0][0].numpy(), mean[0].numpy())
+    for bad in ([thc.Tensor("float")], [thc.Tensor("half") for _ in shapes]):
+        with pytest.raises(ValueError):
+            opt.moments(bad)
