@@ -286,15 +286,14 @@ PyObject* addresses(PyObject*, PyObject* const* args, Py_ssize_t n) {
     PyErr_SetString(PyExc_TypeError, "addresses(tensors, kind)");
     return nullptr;
   }
-  PyObject* all = PySequence_Fast(args[0], "a list of tensors");
+  PyObject* all = PySequence_Tuple(args[0]);      // (an attribute may be a call, which may change a list)
   if (!all) return nullptr;
-  const Py_ssize_t count = PySequence_Fast_GET_SIZE(all);
+  const Py_ssize_t count = PyTuple_GET_SIZE(all);
   PyObject* bytes = PyBytes_FromStringAndSize(nullptr, count * (Py_ssize_t)sizeof(unsigned long long));
   unsigned long long* to = bytes ? reinterpret_cast<unsigned long long*>(PyBytes_AS_STRING(bytes)) : nullptr;
   bool good = bytes != nullptr;
   for (Py_ssize_t i = 0; good && i < count; ++i) {
-    PyObject* t = PySequence_Fast_GET_ITEM(all, i);
-    Py_INCREF(t);
+    PyObject* t = PyTuple_GET_ITEM(all, i);
     PyObject *kind = PyObject_GetAttr(t, kKind), *address = kind ? PyObject_GetAttr(t, kAddress) : nullptr;
     const int same = address ? PyObject_RichCompareBool(kind, args[1], Py_EQ) : -1;
     if (same == 0) PyErr_Format(PyExc_ValueError, "a tensor of another type than %S", args[1]);
@@ -306,7 +305,6 @@ PyObject* addresses(PyObject*, PyObject* const* args, Py_ssize_t n) {
     }
     Py_XDECREF(address);
     Py_XDECREF(kind);
-    Py_DECREF(t);
   }
   Py_DECREF(all);
   PyObject* result = good ? Py_BuildValue("(OK)", bytes, (unsigned long long)(uintptr_t)to) : nullptr;
