@@ -627,10 +627,12 @@ THC_API void THCudaTensor_sumallNoAlloc(THCState *state, THCudaTensor *self, flo
 /* The two ends of a language model and its training step, for float and     */
 /* half tensors. No counterpart in the reference. Tokens are 1-based, as all */
 /* indices here. Every call is asynchronous on the current stream and gives  */
-/* the same bits for the same inputs; temporaries come from the state's      */
-/* allocator. Operands may be strided; those that a kernel does not take     */
-/* where they are go through dense copies (all but windows and batches of    */
-/* rows with unit stride along the last dim).                                */
+/* the same bits for the same inputs (log-probabilities and losses: of rows  */
+/* at the same addresses modulo 128 bytes, which decide what a lane sums);   */
+/* temporaries come from the state's allocator. Operands may be strided;     */
+/* those that a kernel does not take where they are go through dense copies  */
+/* (all but windows and batches of rows with unit stride along the last      */
+/* dim).                                                                     */
 /* ------------------------------------------------------------------------ */
 #define THC_AMD_DECLARE_TOKEN_API(Tensor)                                      \
   /* self[..., :] = scale * weight[token, :], a product of floats rounded to  \
@@ -682,7 +684,7 @@ THC_AMD_DECLARE_TOKEN_API(THCudaHalfTensor)
  * in float, `step` counted from 1. The lists hold one tensor per parameter, of
  * the parameter's sizes. Half parameters may have float copies (`master`, null
  * for none): the step then goes from those and the parameters are their
- * rounded values. No tensor may appear twice.
+ * rounded values. No tensor that is written may appear twice.
  *
  * adamW8 keeps the moments in 8 bits: codes of the parameter's sizes and one
  * float (the largest magnitude) for each 256 elements of a tensor in its
