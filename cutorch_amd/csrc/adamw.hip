@@ -81,7 +81,8 @@ __device__ __forceinline__ void adamw_step(const Hyper& h, float (&p)[4], const 
 // The tensors of one launch travel as kernel arguments, so that no table has to reach the device first: the parameter, the gradient, the
 // moments, with 8-bit states their scales, and the float copies if there are any. A launch costs the host more the more arguments
 // it has (2.4 us for few, about 4 for 4 KiB), so there is a form for few tensors and one for as many as 4 KiB hold (147 tensors of a few
-// thousand floats in two launches 11.0 us, in three of 64 15.2; 291 tensors, 24 M halves with float copies, 122, 56 a launch 127).
+// thousand floats in two launches 11.0 us, in three of 64 15.2). Large ones take 56 a launch: their workgroups find theirs with one load
+// (202 M halves with float copies 962 us, with up to 77 a launch 975).
 enum { kParam, kGrad, kMean, kSquare, kMeanScale, kSquareScale };
 template <int POINTERS, int N>
 struct Args {
@@ -94,7 +95,7 @@ struct Args {
     int64_t size;
   } item[N];
 };
-constexpr int kFewItems = 32;
+constexpr int kFewItems = 32, kLargeItems = 56;
 template <int POINTERS>
 constexpr int kManyItems = (4096 - 48) / (8 * POINTERS + 12);
 
@@ -555,12 +556,9 @@ void adamw(THCState* s, DType dt, int count, const Lists& l, double lr, double b
   using std::true_type;
   auto typed = [&](auto type, auto master, auto bits) {
     using std::integral_constant;
-    auto stored = [&](auto items) {
-      if (nt) run(type, master, bits, true_type{}, items);
-      else run(type, master, bits, false_type{}, items);
-    };
-    if (count <= kFewItems) stored(integral_constant<int, kFewItems>{});
-    else stored(integral_constant<int, 0>{});      // as many as fit
+    if (nt) run(type, master, bits, true_type{}, integral_constant<int, kLargeItems>{});
+    else if (count <= kFewItems) run(type, master, bits, false_type{}, integral_constant<int, kFewItems>{});
+    else run(type, master, bits, false_type{}, integral_constant<int, 0>{});      // as many as fit
   };
   auto states = [&](auto bits) {
     if (!half) typed(float{}, false_type{}, bits);
