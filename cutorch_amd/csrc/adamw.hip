@@ -44,7 +44,7 @@ __device__ __forceinline__ float share_root(float x) {
 // The nearest floats to the roots of second moments, which may be infinite, or so small that a step without eps divides by very little.
 // A wave takes the short root where all it has are zeros or in that one's range, and sqrtf else. As bits a NaN and what is negative are above
 // infinity, and zero less one above all. us of 8-bit steps of 4.5 M floats, 4.4 M halves and 184 M floats: 14.7, 14.5, 463 so, 16.4, 15.8, 493 with
-// sqrtf alone.
+// sqrtf alone. Steps with 32-bit states wait for memory and take sqrtf (202 M halves with float copies 956, 960 with this).
 __device__ __forceinline__ void moment_roots(float (&root)[4], const float (&v)[4]) {
   uint32_t low = ~0u, high = 0;
 #pragma unroll
@@ -61,28 +61,21 @@ __device__ __forceinline__ void moment_roots(float (&root)[4], const float (&v)[
   }
 }
 
-// Four neighbours' step.
-__device__ __forceinline__ void adamw_step(const Hyper& h, float (&p)[4], const float (&grad)[4], float (&m)[4], float (&v)[4]) {
-  float root[4];
-#pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    const float g = grad[e] * h.gradScale;
-    m[e] = m[e] * h.beta1 + g * h.oneMinusBeta1;
-    v[e] = v[e] * h.beta2 + (g * g) * h.oneMinusBeta2;
-  }
-  moment_roots(root, v);
-#pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    const float divisor = root[e] * h.rootScale + h.eps;
-    p[e] = p[e] * h.keep - (m[e] / divisor) * h.rate;
-  }
+__device__ __forceinline__ void take_gradient(const Hyper& h, float g, float& m, float& v) {
+  g = g * h.gradScale;
+  m = m * h.beta1 + g * h.oneMinusBeta1;
+  v = v * h.beta2 + (g * g) * h.oneMinusBeta2;
+}
+__device__ __forceinline__ float stepped(const Hyper& h, float p, float m, float root) {
+  return p * h.keep - (m / (root * h.rootScale + h.eps)) * h.rate;
 }
 
 // The tensors of one launch travel as kernel arguments, so that no table has to reach the device first: the parameter, the gradient, the
 // moments, with 8-bit states their scales, and the float copies if there are any. A launch costs the host more the more arguments
 // it has (2.4 us for few, about 4 for 4 KiB), so there is a form for few tensors and one for as many as 4 KiB hold (147 tensors of a few
-// thousand floats in two launches 11.0 us, in three of 64 15.2). Large ones take 56 a launch: their workgroups find theirs with one load
-// (202 M halves with float copies 962 us, with up to 77 a launch 975).
+// thousand floats in two launches 11.0 us, in three of 64 15.2). Large ones take 56 a launch, where one
+// load finds a workgroup's tensor as among any up to 64: of 202 M halves with float copies, 147 tensors, two sets in turn take 961 us, with up to 77 a launch 978
+// (one set again and again 934 and 938; 291 small tensors, 24 M halves, 127 and 122).
 enum { kParam, kGrad, kMean, kSquare, kMeanScale, kSquareScale };
 template <int POINTERS, int N>
 struct Args {
@@ -183,7 +176,11 @@ __device__ __forceinline__ void step_part(const Hyper& h, void* const* pointers,
     const int i = (u * kBlock + threadIdx.x) * 4;
     if (FULL || i < left) {
       const int n = FULL ? 4 : left - i;
-      adamw_step(h, p[u], g[u], m[u], v[u]);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        take_gradient(h, g[u][e], m[u][e], v[u][e]);
+        p[u][e] = stepped(h, p[u][e], m[u][e], sqrtf(v[u][e]));
+      }
       store4<NT>(mean + i, m[u], n);
       store4<NT>(square + i, v[u], n);
       if constexpr (MASTER) store4<NT>(master + i, p[u], n);
@@ -290,16 +287,18 @@ __device__ __forceinline__ void step8_part(const Hyper& h, void* const* pointers
     const int block = u * (kBlock / 64) + wave, i = block * kStateBlock + lane * 4;
     if (FULL || block * kStateBlock < left) {
       const int n = FULL ? 4 : left - i;
-      float m[4], v[4];
+      float m[4], v[4], root[4];
       uint32_t maxMean = 0, maxSquare = 0;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         m[e] = decode_mean(codeMean[u][e], topMean[u]);
         v[e] = decode_square(codeSquare[u][e], topSquare[u]);
+        take_gradient(h, g[u][e], m[e], v[e]);
       }
-      adamw_step(h, p[u], g[u], m, v);
+      moment_roots(root, v);
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
+        p[u][e] = stepped(h, p[u][e], m[e], root[e]);
         if (FULL || e < n) {          // (zeros behind the end may meet a factor that is not finite)
           maxMean = max(maxMean, __float_as_uint(fabsf(m[e])));
           maxSquare = max(maxSquare, __float_as_uint(v[e]));
