@@ -149,7 +149,7 @@ __device__ __forceinline__ void store4(T* to, const float (&from)[4], int n) {
   }
 }
 
-// States in 32 bits, in place. FULL: the tensor does not end in this part. Bound by memory: 202 M halves with float copies 950 us, 6.0 TB/s;
+// States in 32 bits, in place. FULL: the tensor does not end in this part. Bound by memory: 202 M halves with float copies 955 us, 5.9 TB/s;
 // a model of 27 tensors and 120 thousand floats 4.4 us, the launch and the host's work for it.
 template <typename T, bool MASTER, bool NT, bool FULL>
 __device__ __forceinline__ void step_part(const Hyper& h, void* const* pointers, int64_t base, int left) {
@@ -251,8 +251,8 @@ __device__ __forceinline__ void store4_codes(T* to, const T (&from)[4], int n) {
 }
 
 // States in 8 bits: a wave has a block of states per pack, 4 elements a lane. What is behind a tensor's end counts as zeros. Bound by
-// arithmetic and memory alike in large calls (184 M floats 510 us, 5.8 TB/s; about 530 instructions for a block of 256), by arithmetic in those
-// that the caches hold (4.5 M floats 19 us).
+// arithmetic and memory alike in large calls (184 M floats 501 us, 5.9 TB/s, halves alone 489, 3.8; about 530 instructions for a block of 256), by
+// arithmetic in those that the caches hold (4.5 M floats 17.4 us, halves 18.4).
 // FULL: the tensor does not end in this part.
 template <typename T, bool MASTER, bool NT, bool FULL>
 __device__ __forceinline__ void step8_part(const Hyper& h, void* const* pointers, int64_t base, int left) {
