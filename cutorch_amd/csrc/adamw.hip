@@ -624,6 +624,10 @@ void moments(THCState* s, int count, AnyTensor** meanOut, AnyTensor** squareOut,
   const int sizes[6] = {4, 4, 1, 1, 0, 0};
   Batch<A, decltype(launch)> batch(Hyper{}, part_size(kDecodePacks), sizes, launch);
   Held held(s);
+  // Dense operands are used where they are; those with gaps are read and written by copies around the launches, and may lie in each other's.
+  auto dense_meet = [](const AnyTensor* a, const AnyTensor* b) {
+    return spans_meet(a, DType::F32, b, DType::F32) && tensor_is_contiguous(a) && tensor_is_contiguous(b);
+  };
   // (all are resized before any pointer is taken: they may share a storage)
   for (int i = 0; i < count; ++i) {
     tensor_resize_as(s, meanOut[i], mean[i], DType::F32);
@@ -634,10 +638,9 @@ void moments(THCState* s, int count, AnyTensor** meanOut, AnyTensor** squareOut,
     const AnyTensor *out[2] = {meanOut[i], squareOut[i]}, *in[2] = {meanScale[i], squareScale[i]};
     for (int j = 0; j < 2; ++j) {
       THC_ARG_CHECK(tensor_is_contiguous(out[j]) || !overlapping(tensor_layout(out[j])), 3 + j, "elements of tensor %d overlap", i + 1);
-      for (int k = 0; k < 2; ++k)
-        THC_ARG_CHECK(!spans_meet(out[j], DType::F32, in[k], DType::F32), 3 + j, "tensor %d lies on its scales", i + 1);
+      for (int k = 0; k < 2; ++k) THC_ARG_CHECK(!dense_meet(out[j], in[k]), 3 + j, "tensor %d lies on its scales", i + 1);
     }
-    THC_ARG_CHECK(!spans_meet(out[0], DType::F32, out[1], DType::F32), 4, "tensor %d's two moments share memory", i + 1);
+    THC_ARG_CHECK(!dense_meet(out[0], out[1]), 4, "tensor %d's two moments share memory", i + 1);
   }
   refuse_meeting(count, meanOut, squareOut, mean, meanScale, squareScale);
   // every copy is made before the first launch: outputs may lie in the gaps of scales that are read through one

@@ -81,7 +81,7 @@ def test_outputs_side_by_side_and_in_gaps(thc):
     for s in SIZES + SIZES:
         outs.append(room.view_as_strided(2 * at, s, (2,) if len(s) == 1 else (2 * s[1], 2)))
         at += int(np.prod(s))
-    outs[0], outs[4] = thc.Tensor("float"), thc.Tensor("float")      # (a tensor's own scales may not even share its span)
+    outs[0], outs[4] = thc.Tensor("float"), thc.Tensor("float")
     outs[1], outs[5], outs[3], outs[7] = (thc.Tensor("float") for _ in range(4))
     mean, square = opt.moments(outs[:4], outs[4:])
     for a, b in zip(mean + square, want[0] + want[1]):
@@ -116,3 +116,25 @@ def test_32_bit_moments_in_the_tensors_given(thc):
     for bad in ([thc.Tensor("float")], [thc.Tensor("half") for _ in shapes]):
         with pytest.raises(ValueError):
             opt.moments(bad)
+
+
+def test_a_tensors_two_moments_as_columns(thc):
+    """Mean and square side by side for each element, and in the gaps of the tensor's own scales: spans that meet, elements that do not."""
+    plain = _stepped(thc)
+    want = [[x.numpy() for x in l] for l in plain.moments()]
+    room = thc.Tensor("float").resize((300, 4)).fill(7)
+
+    def beside(blocks):
+        return ([room.view_as_strided(2, (blocks[0],), (4,))] + [thc.Tensor("float").resize((n,)).zero() for n in blocks[1:]],
+                [room.view_as_strided(3, (blocks[0],), (4,))] + [thc.Tensor("float").resize((n,)).zero() for n in blocks[1:]])
+
+    opt = _stepped(thc, lambda blocks: [[t.zero() for t in l] for l in beside(blocks)])
+    mean, square = _new(thc), _new(thc)
+    mean[0], square[0] = room.select(1, 0), room.select(1, 1)
+    opt.moments(mean, square)
+    for a, b in zip(mean + square, want[0] + want[1]):
+        assert_bit_equal(a.numpy(), b)
+    held = room.numpy()[:, 2:]
+    assert_bit_equal(held[:2, 0].copy(), plain.mean_scale[0].numpy())
+    assert_bit_equal(held[:2, 1].copy(), plain.square_scale[0].numpy())
+    assert np.all(held[2:] == 7)
