@@ -261,12 +261,18 @@ def _declare(l):
         opt(T + "_embeddingGrad", None, P, TP, TP, TP, C.c_float, C.c_long, C.c_int)
         opt(T + "_tokenLogProb", None, P, TP, TP, TP)
         opt(T + "_policyLoss", None, P, *([TP] * 9 + [C.c_double] * 4))
+        opt(T + "_layerNorm", None, P, TP, TP, TP, TP, C.c_double)
+        opt(T + "_layerNormGrad", None, P, *([TP] * 6 + [C.c_double, C.c_int]))
+        opt(T + "_rotary", None, P, TP, TP, TP, TP, C.c_double, C.c_int, C.c_int)
+        opt(T + "_rotaryFrequencies", None, P, TP, C.c_long, *([C.c_double] * 5))
+        opt(T + "_orthogonalize", None, P, TP, TP, C.c_int, C.c_double)
         # lists of tensors (arrays of their addresses) and the step's numbers
         masters = 1 if kind == "half" else 0
         step = [C.c_double] * 5 + [C.c_long, C.c_double]
         opt(T + "_adamW", None, P, C.c_int, *([P] * (4 + masters) + step))
         opt(T + "_adamW8", None, P, C.c_int, *([P] * (6 + masters) + step))
         opt(T + "_adamW8Moments", None, P, C.c_int, *([P] * 6))
+        opt(T + "_muon", None, P, C.c_int, *([P] * (3 + masters) + [C.c_double] * 3 + [C.c_int] * 2 + [C.c_double] * 3))
     l.THCudaByteTensor_logicalall.argtypes = [P, TP]
     l.THCudaByteTensor_logicalany.argtypes = [P, TP]
     l.THCudaHalfTensor_copyCuda.argtypes = [P, TP, TP]
@@ -630,6 +636,46 @@ class Tensor(object):
                                     clip_low, clip_high, kl, grad_scale)
         return self
 
+    def layer_norm(self, src, weight=None, bias=None, eps=1e-5):
+        """self = src's rows less their mean, over their deviation, times weight plus bias (a number for each column)."""
+        for t in (src, weight, bias):
+            if t is not None and t.kind != self.kind:
+                raise ValueError("a norm's operands are of one type")
+        self._calls["layerNorm"](self.a, src.a, weight.a if weight is not None else 0, bias.a if bias is not None else 0, eps)
+        return self
+
+    def layer_norm_grad(self, grad_weight, grad_bias, src, grad_output, weight=None, eps=1e-5, accumulate=False):
+        """self = the gradient of layer_norm's src; grad_weight and grad_bias (None: not wanted) those of its weight and bias,
+        added to with `accumulate`."""
+        for t in (grad_weight, grad_bias, src, grad_output, weight):
+            if t is not None and t.kind != self.kind:
+                raise ValueError("a norm's operands are of one type")
+        self._calls["layerNormGrad"](self.a, *[t.a if t is not None else 0 for t in (grad_weight, grad_bias, src, grad_output, weight)], eps,
+                                     accumulate)
+        return self
+
+    def rotary(self, src, positions, frequencies, scale=1.0, interleaved=False, inverse=False):
+        """self = src, (..., tokens, heads, elements), with each head's first 2 * len(frequencies) elements turned in pairs by its
+        token's position (None: the place among the tokens) times the frequencies; `inverse` turns back, which is the gradient."""
+        if src.kind != self.kind or (positions is not None and positions.kind != "long") or frequencies.kind != "double":
+            raise ValueError("heads of one type, long positions, double frequencies")
+        self._calls["rotary"](self.a, src.a, positions.a if positions is not None else 0, frequencies.a, scale, interleaved, inverse)
+        return self
+
+    def rotary_frequencies(self, dim, base=10000.0, factor=1.0, length=0.0, slow=0.0, fast=0.0):
+        """self (double) = the dim / 2 frequencies of `dim` turned elements, for contexts `factor` times as long as `length`."""
+        if self.kind != "double":
+            raise ValueError("frequencies are double")
+        self._calls["rotaryFrequencies"](self.a, dim, base, factor, length, slow, fast)
+        return self
+
+    def orthogonalize(self, src, steps=5, eps=1e-7):
+        """self = src's matrices (of the last two dims) after that many Newton-Schulz steps, their singular values near 1."""
+        if src.kind != self.kind:
+            raise ValueError("the result has its matrices' type")
+        self._calls["orthogonalize"](self.a, src.a, steps, eps)
+        return self
+
     def sumall(self):
         return self._calls["sumall"](self.a)
 
@@ -676,24 +722,17 @@ def _operands(name):
     return property(lambda self: self._lists.get(name), lambda self, tensors: self._hold(name, tensors))
 
 
-class AdamW(object):
-    """AdamW on a list of parameters, one call a step for all of them. `grads` are the tensors that the gradients are in at each
-    step. The moments are kept in floats, or with bits=8 in codes with a float for each 256 elements. Half parameters may
-    have float copies (`master`) that the steps go from. mean, square (and mean_scale, square_scale with 8 bits): the states
-    of an earlier run, as `step` is the number of steps it had made, all of them together; zeros before the first step.
+def _zeros(kind, shape):
+    return Tensor(kind).resize(shape).zero() if shape else Tensor(kind)
 
-    The lists are tuples of the optimizer's own, which keep their tensors alive; another list is assigned to go on with it
-    (opt.grads = [...]; opt.master = None leaves the copies)."""
+
+class _Optimizer(object):
+    """The lists of an optimizer. A subclass says which there are and of what types (_kinds, in the order of its entry point's
+    arguments) and how many tensors each has (_count)."""
 
     params, grads, master = _operands("params"), _operands("grads"), _operands("master")
-    mean, square, mean_scale, square_scale = (_operands(name) for name in ("mean", "square", "mean_scale", "square_scale"))
 
-    def __init__(self, params, grads, master=None, lr=1e-3, beta1=0.9, beta2=0.999, eps=1e-8, weight_decay=0.01, bits=32, mean=None,
-                 square=None, mean_scale=None, square_scale=None, step=0):
-        if mean_scale is not None or square_scale is not None:
-            bits = 8
-        if bits not in (8, 32):
-            raise ValueError("states have 8 or 32 bits")
+    def _begin(self, params, master):
         params = tuple(params)
         kinds = {p.kind for p in params}
         if kinds - {"float", "half"} or len(kinds) > 1:
@@ -701,41 +740,20 @@ class AdamW(object):
         self.kind = kinds.pop() if kinds else "float"
         if master is not None and self.kind != "half":
             raise ValueError("float copies are of half parameters")
-        self.lr, self.beta1, self.beta2, self.eps, self.weight_decay, self.steps, self.bits = lr, beta1, beta2, eps, weight_decay, step, bits
-        if step > 0 and (mean is None or square is None or (bits == 8 and (mean_scale is None or square_scale is None))):
-            raise ValueError("a run that has made %d steps goes on without all of its states" % step)
-        # the lists as the entry points take them: name -> type
         self._kinds = {"params": self.kind}
         if self.kind == "half":
             self._kinds["master"] = "float"
         self._kinds["grads"] = self.kind
-        self._kinds.update([("mean", "char"), ("mean_scale", "float"), ("square", "byte"), ("square_scale", "float")] if bits == 8 else
-                           [("mean", "float"), ("square", "float")])
         self._lists, self._arrays, self._args = {}, {}, []
         self._count = len(params)
-
-        def zeros(kind, shape):
-            return Tensor(kind).resize(shape).zero() if shape else Tensor(kind)
-
-        def state(name, given):
-            if given is None and name in self._kinds:
-                blocks = name.endswith("_scale")
-                given = [zeros(self._kinds[name], (-(-p.numel() // 256),) if blocks and p.numel() else () if blocks else p.shape)
-                         for p in params]
-            self._hold(name, given)
-
-        self._hold("params", params)
-        self._hold("grads", grads)
-        self._hold("master", master)
-        for name, given in (("mean", mean), ("square", square), ("mean_scale", mean_scale), ("square_scale", square_scale)):
-            state(name, given)
+        return params
 
     def _hold(self, name, tensors):
         """Takes a list: its tensors, which live as long as their addresses are here."""
         if tensors is None and (name == "master" or name not in self._kinds):
             held = None, 0
         elif name not in self._kinds:
-            raise ValueError("%s parameters with %d-bit states have no %s" % (self.kind, self.bits, name))
+            raise ValueError("%s parameters%s have no %s" % (self.kind, self._states, name))
         else:
             tensors = tuple(tensors)
             held = self._array(tensors, self._kinds[name])
@@ -752,6 +770,46 @@ class AdamW(object):
             raise ValueError("a tensor of another type than %s" % kind)
         addresses = array.array("Q", [t.a for t in tensors])
         return addresses, addresses.buffer_info()[0]
+
+
+class AdamW(_Optimizer):
+    """AdamW on a list of parameters, one call a step for all of them. `grads` are the tensors that the gradients are in at each
+    step. The moments are kept in floats, or with bits=8 in codes with a float for each 256 elements. Half parameters may
+    have float copies (`master`) that the steps go from. mean, square (and mean_scale, square_scale with 8 bits): the states
+    of an earlier run, as `step` is the number of steps it had made, all of them together; zeros before the first step.
+
+    The lists are tuples of the optimizer's own, which keep their tensors alive; another list is assigned to go on with it
+    (opt.grads = [...]; opt.master = None leaves the copies)."""
+
+    mean, square, mean_scale, square_scale = (_operands(name) for name in ("mean", "square", "mean_scale", "square_scale"))
+
+    def __init__(self, params, grads, master=None, lr=1e-3, beta1=0.9, beta2=0.999, eps=1e-8, weight_decay=0.01, bits=32, mean=None,
+                 square=None, mean_scale=None, square_scale=None, step=0):
+        if mean_scale is not None or square_scale is not None:
+            bits = 8
+        if bits not in (8, 32):
+            raise ValueError("states have 8 or 32 bits")
+        params = self._begin(params, master)
+        self.lr, self.beta1, self.beta2, self.eps, self.weight_decay, self.steps, self.bits = lr, beta1, beta2, eps, weight_decay, step, bits
+        if step > 0 and (mean is None or square is None or (bits == 8 and (mean_scale is None or square_scale is None))):
+            raise ValueError("a run that has made %d steps goes on without all of its states" % step)
+        self._states = " with %d-bit states" % bits
+        # the lists as the entry points take them: name -> type
+        self._kinds.update([("mean", "char"), ("mean_scale", "float"), ("square", "byte"), ("square_scale", "float")] if bits == 8 else
+                           [("mean", "float"), ("square", "float")])
+
+        def state(name, given):
+            if given is None and name in self._kinds:
+                blocks = name.endswith("_scale")
+                given = [_zeros(self._kinds[name], (-(-p.numel() // 256),) if blocks and p.numel() else () if blocks else p.shape)
+                         for p in params]
+            self._hold(name, given)
+
+        self._hold("params", params)
+        self._hold("grads", grads)
+        self._hold("master", master)
+        for name, given in (("mean", mean), ("square", square), ("mean_scale", mean_scale), ("square_scale", square_scale)):
+            state(name, given)
 
     def step(self, grad_scale=1.0):
         """One step from what the gradients hold, times grad_scale."""
@@ -780,6 +838,33 @@ class AdamW(object):
         arrays = [self._array(mean, "float"), self._array(square, "float")]
         _CALLS["float"]["adamW8Moments"](self._count, arrays[0][1], arrays[1][1], *self._args[-4:])
         return mean, square
+
+
+class Muon(_Optimizer):
+    """The optimizer of matrices: momentum, whose matrices are brought near orthogonal by Newton-Schulz steps, and decay, one call a
+    step for all parameters. The last two dims of a parameter are a matrix; vectors and tables are AdamW's. `grads` are the
+    tensors that the gradients are in at each step. Half parameters may have float copies (`master`) that the steps go from.
+    momentum: that of an earlier run; zeros at first. match_rms: steps of the size of AdamW's, whose elements are that on average.
+    The lists are as AdamW's."""
+
+    momentum = _operands("momentum")
+
+    def __init__(self, params, grads, master=None, lr=0.02, beta=0.95, weight_decay=0.0, nesterov=True, steps=5, eps=1e-7, match_rms=0.0,
+                 momentum=None):
+        params = self._begin(params, master)
+        self.lr, self.beta, self.weight_decay, self.nesterov, self.steps, self.eps, self.match_rms = (
+            lr, beta, weight_decay, nesterov, steps, eps, match_rms)
+        self._states = ""
+        self._kinds["momentum"] = "float"
+        self._hold("params", params)
+        self._hold("grads", grads)
+        self._hold("master", master)
+        self._hold("momentum", [_zeros("float", p.shape) for p in params] if momentum is None else momentum)
+
+    def step(self, grad_scale=1.0):
+        """One step from what the gradients hold, times grad_scale."""
+        _CALLS[self.kind]["muon"](self._count, *self._args, self.lr, self.beta, self.weight_decay, self.nesterov, self.steps, self.eps,
+                                  self.match_rms, grad_scale)
 
 
 def cached_memory():

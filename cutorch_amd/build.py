@@ -25,7 +25,7 @@ SOURCES = ["general.cpp", "tensor.cpp", "math.cpp", "math_wide.cpp", "caching_al
            "apply_rawmath_u32u64.hip", "apply_rawmath_f64.hip", "apply_w_i8.hip", "apply_w_i16.hip", "apply_w_i32.hip", "apply_w_i64.hip", "apply_w_f64.hip",
            "apply_cvt_u8.hip", "apply_cvt_i8.hip", "apply_cvt_i16.hip", "apply_cvt_i32.hip", "apply_cvt_i64.hip",
            "apply_cvt_f16.hip", "apply_cvt_f32.hip", "apply_cvt_f64.hip", "apply_policy.hip",
-           "embedding.hip", "token_loss.hip", "adamw.hip"]
+           "embedding.hip", "token_loss.hip", "adamw.hip", "layer_norm.hip", "rotary.hip", "muon.hip"]
 HEADERS = ["common.hpp", "layout.hpp", "device_util.hpp", os.path.join("..", "..", "include", "THC.h")]   # every source
 APPLY_HEADERS = ["apply_plan.hpp", "apply_impl.hpp", "apply_ldstile.hpp", "apply_wide.hpp"]   # apply*.hip, convert.hip
 REDUCE_HEADERS = ["reduce_plan.hpp", "reduce_impl.hpp"]                                       # reduce*.hip, scan.hip, no_alloc.hip
@@ -60,7 +60,7 @@ EXTRA_DEPS = {"caching_allocator.cpp": ["caching_pool.hpp", "stream_guard.hpp"],
               "scan.hip": ["stream_guard.hpp", "scan_ticket.hpp"], "no_alloc.hip": ["stream_guard.hpp"], "convert.hip": ["stream_guard.hpp"]}
 EXTRA_DEPS.update({"apply_cvt_%s.hip" % t: ["apply_convert_impl.hpp", "apply_skinny.hpp"]
                    for t in ("u8", "i8", "i16", "i32", "i64", "f16", "f32", "f64")})
-EXTRA_DEPS.update({src: ["training.hpp", "stream_guard.hpp"] for src in ("embedding.hip", "token_loss.hip", "adamw.hip")})
+EXTRA_DEPS.update({src: ["training.hpp", "stream_guard.hpp"] for src in ("embedding.hip", "token_loss.hip", "adamw.hip", "layer_norm.hip", "rotary.hip", "muon.hip")})
 EXTRA_DEPS["apply_raw.hip"] = ["apply_skinny.hpp"]
 
 

@@ -384,35 +384,6 @@ __global__ __launch_bounds__(kBlock) void decode_kernel(A a) {
 }
 
 // ------------------------------------------------------------------------- host --
-// Operands that are used where they are if they are dense, else through a copy.
-struct Held {
-  THCState* s;
-  struct One {
-    AnyTensor* tensor;     // the caller's
-    AnyTensor* dense;
-    DType dt;
-    bool written;
-  };
-  std::vector<One> all;
-  explicit Held(THCState* s_) : s(s_) {}
-  Held(const Held&) = delete;
-  Held& operator=(const Held&) = delete;
-  ~Held() {
-    for (One& o : all) tensor_free(s, o.dense);
-  }
-  void* add(AnyTensor* t, DType dt, bool written) {
-    if (tensor_is_contiguous(t)) return tensor_data(t, dt);
-    if (all.size() == all.capacity()) all.reserve(2 * all.size() + 8);
-    AnyTensor* dense = tensor_new_contiguous(s, t, dt);
-    all.push_back(One{t, dense, dt, written});
-    return tensor_data(dense, dt);
-  }
-  void write_back() {
-    for (One& o : all)
-      if (o.written) copy_tensor(s, o.dt, o.tensor, o.dense, false);
-  }
-};
-
 template <int POINTERS>
 struct Operands {
   void* p[POINTERS];
@@ -461,14 +432,6 @@ void check_scales(THCState* s, const AnyTensor* scale, int64_t n, int arg, int i
   THC_ARG_CHECK(tensor_numel(scale) == state_blocks(n), arg, "%ld scales for the %ld blocks of tensor %d's states", (long)tensor_numel(scale),
                 (long)state_blocks(n), index + 1);
   THC_ARG_CHECK(!written || tensor_is_contiguous(scale) || !overlapping(tensor_layout(scale)), arg, "scales of tensor %d's states overlap", index + 1);
-}
-
-void check_list(THCState* s, const AnyTensor* t, const AnyTensor* like, int arg, int index, bool written) {
-  THC_ARG_CHECK(t, arg, "tensor %d is missing", index + 1);
-  check_same_gpu(s, 1, &t);
-  THC_ARG_CHECK(t->nDimension <= kMaxDims, arg, "%s", kDimWarning);
-  THC_ARG_CHECK(same_sizes(t, like), arg, "tensor %d has other sizes than its parameter", index + 1);
-  THC_ARG_CHECK(!written || tensor_is_contiguous(t) || !overlapping(tensor_layout(t)), arg, "elements of tensor %d overlap", index + 1);
 }
 
 void adamw(THCState* s, DType dt, int count, const Lists& l, double lr, double beta1, double beta2, double eps, double weightDecay, long step,

@@ -108,16 +108,6 @@ struct RowParts {
 constexpr int kRowsAcross = 21;
 __device__ __forceinline__ uint32_t grid_row() { return blockIdx.x + (blockIdx.y << kRowsAcross); }
 
-struct RowOffsets {
-  int64_t stride, outerStride;
-  Divisor<uint32_t> inner;
-  __device__ __forceinline__ int64_t at(uint32_t row) const {
-    uint32_t q, r;
-    inner.divmod(row, q, r);
-    return (int64_t)q * outerStride + (int64_t)r * stride;
-  }
-};
-
 // What a position brings along and what it gets, besides its row.
 struct PolicyArgs {
   const int64_t* token;
@@ -479,14 +469,6 @@ __global__ __launch_bounds__(W * 64) void join_kernel(PolicyArgs a, const T* log
         if (k + u * kStep < end && x.has(k + u * kStep)) store_gradient<T>(out, x.head + (k + u * kStep) * V, v[u], r);
     }
   }
-}
-
-RowOffsets offsets_of(const Rows& r) {
-  RowOffsets o;
-  o.stride = r.stride;
-  o.outerStride = r.outerStride;
-  o.inner.set((uint64_t)r.inner);
-  return o;
 }
 
 template <typename T>

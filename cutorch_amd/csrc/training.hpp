@@ -1,7 +1,8 @@
-// What the operators of a language model's training step share on the host: rows of tensors of any rank, dense operands,
-// workspaces, and the guard of their entry points.
+// What the operators of a language model's training step share on the host: rows of tensors of any rank, dense operands, lists of
+// tensors, workspaces, and the guard of their entry points.
 #pragma once
 #include <new>
+#include <vector>
 
 #include "common.hpp"
 #include "device_util.hpp"
@@ -54,6 +55,24 @@ inline bool as_rows(const AnyTensor* t, Rows* r) {
   return true;
 }
 
+// The same in a kernel, for fewer than 2^31 rows.
+struct RowOffsets {
+  int64_t stride, outerStride;
+  Divisor<uint32_t> inner;
+  __device__ __forceinline__ int64_t at(uint32_t row) const {
+    uint32_t q, r;
+    inner.divmod(row, q, r);
+    return (int64_t)q * outerStride + (int64_t)r * stride;
+  }
+};
+inline RowOffsets offsets_of(const Rows& r) {
+  RowOffsets o;
+  o.stride = r.stride;
+  o.outerStride = r.outerStride;
+  o.inner.set((uint64_t)r.inner);
+  return o;
+}
+
 // A tensor as an operand that kernels read: itself if it is contiguous, else a dense copy that lives as long as this.
 struct Dense {
   TensorRef ref;
@@ -99,5 +118,43 @@ inline bool spans_meet(const AnyTensor* a, DType da, const AnyTensor* b, DType d
 }
 
 inline bool has_elements(const AnyTensor* t) { return t->nDimension > 0 && tensor_numel(t) > 0; }
+
+// Operands that are used where they are if they are dense, else through a copy.
+struct Held {
+  THCState* s;
+  struct One {
+    AnyTensor* tensor;     // the caller's
+    AnyTensor* dense;
+    DType dt;
+    bool written;
+  };
+  std::vector<One> all;
+  explicit Held(THCState* s_) : s(s_) {}
+  Held(const Held&) = delete;
+  Held& operator=(const Held&) = delete;
+  ~Held() {
+    for (One& o : all) tensor_free(s, o.dense);
+  }
+  void* add(AnyTensor* t, DType dt, bool written) {
+    if (tensor_is_contiguous(t)) return tensor_data(t, dt);
+    if (all.size() == all.capacity()) all.reserve(2 * all.size() + 8);
+    AnyTensor* dense = tensor_new_contiguous(s, t, dt);
+    all.push_back(One{t, dense, dt, written});
+    return tensor_data(dense, dt);
+  }
+  void write_back() {
+    for (One& o : all)
+      if (o.written) copy_tensor(s, o.dt, o.tensor, o.dense, false);
+  }
+};
+
+// A tensor of an optimizer's list.
+inline void check_list(THCState* s, const AnyTensor* t, const AnyTensor* like, int arg, int index, bool written) {
+  THC_ARG_CHECK(t, arg, "tensor %d is missing", index + 1);
+  check_same_gpu(s, 1, &t);
+  THC_ARG_CHECK(t->nDimension <= kMaxDims, arg, "%s", kDimWarning);
+  THC_ARG_CHECK(same_sizes(t, like), arg, "tensor %d has other sizes than its parameter", index + 1);
+  THC_ARG_CHECK(!written || tensor_is_contiguous(t) || !overlapping(tensor_layout(t)), arg, "elements of tensor %d overlap", index + 1);
+}
 
 }  // namespace thc

@@ -676,6 +676,58 @@ THC_API void THCudaTensor_sumallNoAlloc(THCState *state, THCudaTensor *self, flo
 THC_AMD_DECLARE_TOKEN_API(THCudaTensor)
 THC_AMD_DECLARE_TOKEN_API(THCudaHalfTensor)
 
+/* What a decoder needs between those two ends, under the same conditions.     */
+#define THC_AMD_DECLARE_DECODER_API(Tensor)                                    \
+  /* self = (x - m) / sqrt(v + eps) * weight + bias along the last dim, m and  \
+   * v each row's mean and (biased) variance, in float with one rounding at    \
+   * the end. weight and bias: a number for each column, null for ones and     \
+   * zeros. self takes the input's sizes and may be the input. */              \
+  THC_API void Tensor##_layerNorm(THCState *, Tensor *self, Tensor *input,     \
+                                  Tensor *weight, Tensor *bias, double eps);   \
+  /* The gradients of that; the statistics are taken from the input again.     \
+   * gradWeight and gradBias (null: not wanted) are written, or added to with  \
+   * `accumulate`, in an order of sums that the sizes alone decide. gradInput  \
+   * takes the input's sizes and may be the input or gradOutput; the three     \
+   * outputs may not lie on one another. weight null: ones. */                 \
+  THC_API void Tensor##_layerNormGrad(                                         \
+      THCState *, Tensor *gradInput, Tensor *gradWeight, Tensor *gradBias,     \
+      Tensor *input, Tensor *gradOutput, Tensor *weight, double eps,           \
+      int accumulate);                                                         \
+  /* Heads turned by their token's position. The input's last dims are heads   \
+   * and their elements, those before them tokens; a position (from 0, any     \
+   * whole number) for each token, or for each of dim -3, which the sequences  \
+   * of a batch then share; null: the place along that dim. The first          \
+   * 2 n elements of a head are turned in pairs by position * frequency, n the \
+   * number of frequencies: element j with j + n, or 2 j with 2 j + 1 if       \
+   * `interleaved`; the others stay as they are. The turned pairs are          \
+   * multiplied by `scale`. `inverse` turns back: the gradient's way, with the \
+   * same scale. Angles are products of 64 bits. self takes the input's sizes  \
+   * and may be the input. */                                                  \
+  THC_API void Tensor##_rotary(THCState *, Tensor *self, Tensor *input,        \
+                               THCudaLongTensor *positions,                    \
+                               THCudaDoubleTensor *frequencies, double scale,  \
+                               int interleaved, int inverse);                  \
+  /* Newton-Schulz steps on each matrix of the last two dims:                  \
+   *   X = G / (|G| + eps);  X = a X + b (X X') X + c (X X')^2 X, `steps` times \
+   * with |G| the root of the sum of squares and a, b, c = 3.4445, -4.7750,    \
+   * 2.0315, which brings singular values to 0.7 ... 1.2. Products are as      \
+   * exact as float ones, the result rounds once to the type. self takes the   \
+   * input's sizes and may be the input. */                                    \
+  THC_API void Tensor##_orthogonalize(THCState *, Tensor *self, Tensor *input, \
+                                      int steps, double eps);
+THC_AMD_DECLARE_DECODER_API(THCudaTensor)
+THC_AMD_DECLARE_DECODER_API(THCudaHalfTensor)
+/* Frequencies for the rotary positions of `dim` turned elements, dim / 2 of
+ * them: base^(-2 j / dim) radians a position. For contexts longer than the
+ * `length` that a model was made for, frequencies that turn `slow` times or
+ * less within it are divided by `factor`, those that turn `fast` times or more
+ * are not, and those between in part; slow = fast: all are divided. */
+THC_API void THCudaDoubleTensor_rotaryFrequencies(THCState *state,
+                                                  THCudaDoubleTensor *self,
+                                                  long dim, double base,
+                                                  double factor, double length,
+                                                  double slow, double fast);
+
 /* One AdamW step of `count` tensors, in place:
  *   g = gradScale grad;  m = beta1 m + (1 - beta1) g;
  *   v = beta2 v + (1 - beta2) g^2
@@ -728,5 +780,27 @@ THC_API void THCudaTensor_adamW8Moments(THCState *state, int count,
                                         THCudaTensor **meanScale,
                                         THCudaByteTensor **squareCode,
                                         THCudaTensor **squareScale);
+
+/* One step of the optimizer of `count` matrices, in place:
+ *   g = gradScale grad;  m = beta m + g;  u = g + beta m if nesterov, else m
+ *   p = p (1 - lr weightDecay) - rate orthogonalize(u, steps, eps)
+ * with rate = lr sqrt(max(1, rows / columns)), or, with matchRms > 0,
+ * lr matchRms sqrt(max(rows, columns)): the size of an AdamW step whose
+ * elements are matchRms on average. The last two dims of a parameter are a
+ * matrix, those before them a batch of matrices of their own; vectors and
+ * tables are AdamW's. Lists as there: one tensor per parameter, of its sizes,
+ * the momentum in float (zeros begin a run), float copies of half parameters
+ * (`master`) or null. No tensor that is written may appear twice. */
+THC_API void THCudaTensor_muon(THCState *state, int count, THCudaTensor **param,
+                               THCudaTensor **grad, THCudaTensor **momentum,
+                               double lr, double beta, double weightDecay,
+                               int nesterov, int steps, double eps,
+                               double matchRms, double gradScale);
+THC_API void THCudaHalfTensor_muon(THCState *state, int count,
+                                   THCudaHalfTensor **param, THCudaTensor **master,
+                                   THCudaHalfTensor **grad, THCudaTensor **momentum,
+                                   double lr, double beta, double weightDecay,
+                                   int nesterov, int steps, double eps,
+                                   double matchRms, double gradScale);
 
 #endif /* THC_AMD_THC_H */
