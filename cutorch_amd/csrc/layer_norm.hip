@@ -134,15 +134,17 @@ __global__ __launch_bounds__(L * TEAMS) void norm_kernel(NormArgs<T> a) {
   float w[P][V], b[P][V];
   load_columns<T, V, P, L>(a.weight, packs, w, 1.f);
   load_columns<T, V, P, L>(a.bias, packs, b, 0.f);
+  Pack<T, V> raw[P] = {};
+  load_row<T, V, P, L>(a.x + a.xo.at(min(blockIdx.x * TEAMS + team, a.rows - 1)), packs, raw);
   for (uint32_t first = blockIdx.x * TEAMS; first < a.rows; first += gridDim.x * TEAMS) {
     const uint32_t row = min(first + team, a.rows - 1);
-    Pack<T, V> raw[P] = {};
-    load_row<T, V, P, L>(a.x + a.xo.at(row), packs, raw);
     float x[P][V];
 #pragma unroll
     for (int p = 0; p < P; ++p)
 #pragma unroll
       for (int e = 0; e < V; ++e) x[p][e] = Cvt<T>::up(raw[p].v[e]);
+    // the next row is asked for before this one is computed
+    if (first + gridDim.x * TEAMS < a.rows) load_row<T, V, P, L>(a.x + a.xo.at(min(first + gridDim.x * TEAMS + team, a.rows - 1)), packs, raw);
     clear_skipped<V, L, P>(packs, x);
     float one[1] = {0.f};
 #pragma unroll
@@ -209,16 +211,28 @@ __global__ __launch_bounds__(L * TEAMS) void norm_grad_kernel(GradArgs<T> a) {
   for (int p = 0; p < P; ++p)
 #pragma unroll
     for (int e = 0; e < V; ++e) dw[p][e] = db[p][e] = 0.f;
+  Pack<T, V> raw[P] = {}, next[P] = {};
+  {
+    const uint32_t row = min(blockIdx.x * TEAMS + team, a.rows - 1);
+    load_row<T, V, P, L>(a.x + a.xo.at(row), packs, raw);
+    load_row<T, V, P, L>(a.g + a.go.at(row), packs, next);
+  }
   for (uint32_t first = blockIdx.x * TEAMS; first < a.rows; first += gridDim.x * TEAMS) {
     const uint32_t row = min(first + team, a.rows - 1);
-    Pack<T, V> raw[P] = {}, graw[P] = {};
-    load_row<T, V, P, L>(a.x + a.xo.at(row), packs, raw);
-    load_row<T, V, P, L>(a.g + a.go.at(row), packs, graw);
     float d[P][V];
+    Pack<T, V> graw[P];
 #pragma unroll
-    for (int p = 0; p < P; ++p)
+    for (int p = 0; p < P; ++p) {
+      graw[p] = next[p];
 #pragma unroll
       for (int e = 0; e < V; ++e) d[p][e] = Cvt<T>::up(raw[p].v[e]);
+    }
+    // the next row is asked for before this one is computed
+    if (first + gridDim.x * TEAMS < a.rows) {
+      const uint32_t then = min(first + gridDim.x * TEAMS + team, a.rows - 1);
+      load_row<T, V, P, L>(a.x + a.xo.at(then), packs, raw);
+      load_row<T, V, P, L>(a.g + a.go.at(then), packs, next);
+    }
     clear_skipped<V, L, P>(packs, d);
     float one[1] = {0.f};
 #pragma unroll
@@ -484,10 +498,17 @@ void launch_norm(THCState* s, const NormArgs<T>& a) {
   const int64_t cus = num_compute_units(s), packs = (a.dim + V - 1) / V;
   auto go = [&](auto vec, auto lanes, auto teams, auto each) {
     constexpr int VV = decltype(vec)::value, L = decltype(lanes)::value, TEAMS = decltype(teams)::value, P = decltype(each)::value;
-    const int64_t groups = ((int64_t)a.rows + TEAMS - 1) / TEAMS, most = cus * std::max(1, 2048 / (L * TEAMS));
+    const int64_t groups = ((int64_t)a.rows + TEAMS - 1) / TEAMS, most = cus * std::max(1, (int)tuning("norm.threads", 2048) / (L * TEAMS));
     hipLaunchKernelGGL((norm_kernel<T, VV, L, TEAMS, P>), dim3((unsigned)std::min(groups, most)), dim3(L * TEAMS), 0, st, a);
   };
 #define GO(VV, L, TEAMS, P) go(integral_constant<int, VV>{}, integral_constant<int, L>{}, integral_constant<int, TEAMS>{}, integral_constant<int, P>{})
+  const long way = tuning("norm.way", 0);
+  if (way == 1 && packs <= 256) { GO(V, 64, 4, 4); return; }
+  if (way == 2 && packs <= 256) { GO(V, 128, 2, 2); return; }
+  if (way == 5 && packs <= 512) { GO(V, 128, 2, 4); return; }
+  if (way == 6 && packs <= 512) { GO(V, 512, 1, 1); return; }
+  if (way == 3 && packs <= 256) { GO(V, 128, 1, 2); return; }
+  if (way == 4 && packs <= 256) { GO(V, 256, 2, 1); return; }
   if (a.dim < V) GO(1, 8, 32, 1);
   else if (packs <= 8) GO(V, 8, 32, 1);
   else if (packs <= 16) GO(V, 16, 16, 1);
@@ -532,20 +553,26 @@ void launch_grad(THCState* s, GradArgs<T>& a, const WeightGrads<T>& to) {
       return;
     }
     // a workgroup's sums cross memory twice: each has some rows at least
-    const int64_t count = std::max<int64_t>(1, std::min(groups / 4, cus * std::max(1, 512 / (L * TEAMS))));
+    const int64_t count = std::max<int64_t>(1, std::min(groups / (int64_t)tuning("norm.each", 4), cus * std::max(1, (int)tuning("norm.gthreads", 512) / (L * TEAMS))));
     Workspace w(s, bytes(count));
     parts(count, w);
     hipLaunchKernelGGL((norm_grad_kernel<T, VV, L, TEAMS, P, true>), dim3((unsigned)count), dim3(L * TEAMS), 0, st, a);
     join(count);
   };
 #define GO(VV, L, TEAMS, P) go(integral_constant<int, VV>{}, integral_constant<int, L>{}, integral_constant<int, TEAMS>{}, integral_constant<int, P>{})
+  const long way = tuning("norm.gway", 0);
   if (a.dim < V) GO(1, 8, 32, 1);
   else if (packs <= 8) GO(V, 8, 32, 1);
   else if (packs <= 16) GO(V, 16, 16, 1);
   else if (packs <= 32) GO(V, 32, 8, 1);
   else if (packs <= 64) GO(V, 64, 4, 1);
   else if (packs <= 128) GO(V, 64, 4, 2);
+  else if (packs <= 256 && way == 1) GO(V, 128, 2, 2);
+  else if (packs <= 256 && way == 2) GO(V, 256, 1, 1);
   else if (packs <= 256) GO(V, 64, 4, 4);
+  else if (packs <= 512 && way == 1) GO(V, 128, 2, 4);
+  else if (packs <= 512 && way == 2) GO(V, 512, 1, 1);
+  else if (packs <= 512 && way == 3) GO(V, 256, 2, 2);
   else if (packs <= 512) GO(V, 256, 1, 2);
   else if (packs <= 1024) GO(V, 256, 1, 4);
   else if (packs <= 2048) GO(V, 512, 1, 4);

@@ -25,17 +25,16 @@ constexpr float kA = 3.4445f, kB = -4.7750f, kC = 2.0315f;
 constexpr float kScaleA = 16384.f, kScaleB = 8192.f;
 
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
-typedef _Float16 half4 __attribute__((ext_vector_type(4)));
 typedef float acc16 __attribute__((ext_vector_type(16)));
 typedef unsigned uint4v __attribute__((ext_vector_type(4)));
 
 // A matrix of R rows and K columns as the products read it: rows of blocks of 32 columns, each block the 32 upper halves and the 32 lower ones,
 // 128 bytes. Columns up to the next multiple of 32 hold zeros.
-constexpr int kBlockK = 32;
+constexpr int kBlockK = 32, kBlockBytes = 128, kLower = 64;
 __host__ __device__ constexpr int64_t blocks_of(int64_t k) { return (k + kBlockK - 1) / kBlockK; }
-__host__ __device__ constexpr int64_t row_bytes(int64_t k) { return blocks_of(k) * 128; }
+__host__ __device__ constexpr int64_t row_bytes(int64_t k) { return blocks_of(k) * kBlockBytes; }
 __device__ __forceinline__ int64_t split_at(int64_t row, int32_t column, int64_t rowBytes) {
-  return row * rowBytes + (column >> 5) * 128 + (column & 31) * 2;      // of the upper half; the lower one 64 bytes on
+  return row * rowBytes + (column >> 5) * kBlockBytes + (column & 31) * 2;      // of the upper half; the lower one kLower bytes on
 }
 
 // `batch` matrices of m x n, m <= n, X short side first; `tall`: their tensors have n rows and m columns.
@@ -63,14 +62,24 @@ struct Place {
   Matrix a;
   uint32_t index;      // of the workgroup within one matrix
   int32_t batch;
-  uint32_t begin;      // of the descriptor's workgroups
 };
+// Workgroups go to the eight dies in turn: of every 512 (what the chip has at a time), and of what is left, those of one die get neighbouring numbers, so
+// that what they read in common comes from its own cache. (All of a launch in eight runs would leave dies idle whose matrices have shorter sums.)
+constexpr uint32_t kDies = 8, kRound = 512;
+__device__ __forceinline__ uint32_t by_die(uint32_t block, uint32_t blocks) {
+  const uint32_t first = block / kRound * kRound, count = min(kRound, blocks - first), at = block - first;
+  const uint32_t each = count / kDies, more = count % kDies, die = at % kDies;
+  return first + die * each + min(die, more) + at / kDies;
+}
 // The matrix of this workgroup, `each` workgroups (by the matrix) for one of a batch.
 template <typename F>
 __device__ __forceinline__ Place place_of(const Group& g, uint32_t block, F each) {
-  int k = 0;
-  while (k + 1 < g.count && block >= g.first[k + 1]) ++k;
-  Place p{g.matrix[k], block - g.first[k], 0, g.first[k]};
+  // (a lane looks at a matrix: one after another they would wait for the arguments a time each)
+  static_assert(kMatrices <= 64, "a lane each");
+  const int lane = threadIdx.x & 63;
+  const uint32_t next = g.first[min(lane, kMatrices - 1) + 1];
+  const int k = __popcll(__ballot(lane + 1 < g.count && block >= next));
+  Place p{g.matrix[k], block - g.first[k], 0};
   const uint32_t n = each(p.a);
   p.batch = (int32_t)(p.index / n);
   p.index -= p.batch * n;
@@ -86,6 +95,33 @@ struct Update {
   int32_t nesterov;
 };
 
+// Eight neighbouring elements of a tensor, or as many as there are and zeros.
+template <typename T>
+__device__ __forceinline__ void load_values(const T* at, int64_t count, float (&v)[8]) {
+  if (count >= 8) {
+    constexpr int N = 16 / sizeof(T);
+#pragma unroll
+    for (int k = 0; k < 8 / N; ++k) {
+      const Pack<T, N> t = load_pack_unaligned<false, Pack<T, N>>(at + k * N);
+#pragma unroll
+      for (int e = 0; e < N; ++e) v[k * N + e] = Cvt<T>::up(t.v[e]);
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = e < count ? Cvt<T>::up(at[e]) : 0.f;
+  }
+}
+__device__ __forceinline__ void store_values(float* at, int64_t count, const float (&v)[8]) {
+  if (count >= 8) {
+#pragma unroll
+    for (int k = 0; k < 2; ++k) store_pack_unaligned<false>(at + k * 4, Pack<float, 4>{v[k * 4], v[k * 4 + 1], v[k * 4 + 2], v[k * 4 + 3]});
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (e < count) at[e] = v[e];
+  }
+}
+
 // The sum of squares of a part of a matrix, in 64 bits; the optimizer's momentum on the way.
 template <typename T, bool MUON>
 __global__ __launch_bounds__(kBlock) void norm_kernel(Group g, Update h, double* parts) {
@@ -95,15 +131,31 @@ __global__ __launch_bounds__(kBlock) void norm_kernel(Group g, Update h, double*
   const T* in = static_cast<const T*>(p.a.in) + p.batch * size;
   float* momentum = MUON ? p.a.momentum + p.batch * size : nullptr;
   double sum = 0;
-  for (int64_t i = from + threadIdx.x; i < to; i += kBlock) {
-    float u = Cvt<T>::up(in[i]);
-    if constexpr (MUON) {
-      u *= h.gradScale;
-      const float m = __builtin_fmaf(momentum[i], h.beta, u);
-      momentum[i] = m;
-      u = h.nesterov ? __builtin_fmaf(m, h.beta, u) : m;
+  constexpr int U = 2;
+  for (int64_t i = from + threadIdx.x * 8; i < to; i += U * kBlock * 8) {
+    float u[U][8], m[U][8];
+#pragma unroll
+    for (int k = 0; k < U; ++k) {
+      const int64_t at = i + k * kBlock * 8;
+      if (at < to) load_values(in + at, to - at, u[k]);
+      if (MUON && at < to) load_values(momentum + at, to - at, m[k]);
     }
-    sum += (double)u * u;
+#pragma unroll
+    for (int k = 0; k < U; ++k) {
+      const int64_t at = i + k * kBlock * 8;
+      if (at >= to) continue;
+      if constexpr (MUON) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float grad = u[k][e] * h.gradScale;
+          m[k][e] = __builtin_fmaf(m[k][e], h.beta, grad);
+          u[k][e] = h.nesterov ? __builtin_fmaf(m[k][e], h.beta, grad) : m[k][e];
+        }
+        store_values(momentum + at, to - at, m[k]);
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) sum += (double)u[k][e] * u[k][e];      // (zeros behind the end)
+    }
   }
   for (int d = 32; d >= 1; d >>= 1) sum += __shfl_xor(sum, d);
   if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = sum;
@@ -123,13 +175,21 @@ __device__ __forceinline__ Split split(float x) {
   s.l = (_Float16)(x - (float)s.h);
   return s;
 }
-__device__ __forceinline__ void store_split(char* plane, int64_t at, float x) {
-  const Split s = split(x);
-  *reinterpret_cast<_Float16*>(plane + at) = s.h;
-  *reinterpret_cast<_Float16*>(plane + at + 64) = s.l;
-}
-__device__ __forceinline__ float load_split(const char* plane, int64_t at) {
-  return (float)*reinterpret_cast<const _Float16*>(plane + at) + (float)*reinterpret_cast<const _Float16*>(plane + at + 64);
+// Eight neighbouring elements of a plane.
+struct Eight {
+  half8 h, l;
+};
+__device__ __forceinline__ Eight load_eight(const char* at) { return Eight{*reinterpret_cast<const half8*>(at), *reinterpret_cast<const half8*>(at + kLower)}; }
+__device__ __forceinline__ void store_eight(char* at, const float (&v)[8]) {
+  half8 h, l;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const Split s = split(v[e]);
+    h[e] = s.h;
+    l[e] = s.l;
+  }
+  *reinterpret_cast<half8*>(at) = h;
+  *reinterpret_cast<half8*>(at + kLower) = l;
 }
 
 // A tile of 64 x 64 elements of the tensor into both planes, over the norm.
@@ -156,33 +216,50 @@ __global__ __launch_bounds__(kBlock) void split_kernel(Group g, Update h, const 
   const int32_t r0 = (int32_t)(p.index / across) * 64, c0 = (int32_t)(p.index % across) * 64;
   const T* in = static_cast<const T*>(a.in) + p.batch * size;
   const float* momentum = MUON ? a.momentum + p.batch * size : nullptr;
-  for (int i = threadIdx.x; i < 64 * 64; i += kBlock) {
-    const int32_t r = r0 + i / 64, c = c0 + i % 64;
-    float u = 0.f;
-    if (r < rows && c < cols) {
-      const int64_t at = (int64_t)r * cols + c;
-      u = Cvt<T>::up(in[at]);
-      if constexpr (MUON) u = h.nesterov ? __builtin_fmaf(momentum[at], h.beta, u * h.gradScale) : momentum[at];
-      u *= factor;
-    }
-    tile[i / 64][i % 64] = u;
-  }
-  __syncthreads();
   char *work = a.work + p.batch * work_bytes(a), *byRow = a.tall ? work + plane_x(a) : work, *byColumn = a.tall ? work : work + plane_x(a);
   const int64_t rowBytes = row_bytes(cols), columnBytes = row_bytes(rows);
   const int32_t colEnd = (int32_t)blocks_of(cols) * kBlockK, rowEnd = (int32_t)blocks_of(rows) * kBlockK;
-  for (int i = threadIdx.x; i < 64 * 64; i += kBlock) {
-    const int32_t x = i / 64, y = i % 64;
-    if (r0 + x < rows && c0 + y < colEnd) store_split(byRow, split_at(r0 + x, c0 + y, rowBytes), tile[x][y]);
-    if (c0 + x < cols && r0 + y < rowEnd) store_split(byColumn, split_at(c0 + x, r0 + y, columnBytes), tile[y][x]);
+  // thread t has eight columns of rows t / 8 and t / 8 + 32, then eight rows of such columns
+  const int32_t eighth = (threadIdx.x & 7) * 8, line = threadIdx.x >> 3;
+#pragma unroll
+  for (int k = 0; k < 64; k += 32) {
+    const int32_t r = r0 + line + k, c = c0 + eighth;
+    float u[8] = {};
+    if (r < rows && c < cols) {
+      const int64_t at = (int64_t)r * cols + c;
+      load_values(in + at, cols - c, u);
+      if constexpr (MUON) {
+        float m[8];
+        load_values(momentum + at, cols - c, m);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) u[e] = h.nesterov ? __builtin_fmaf(m[e], h.beta, u[e] * h.gradScale) : m[e];
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      u[e] *= factor;
+      if (c + e >= cols) u[e] = 0.f;
+      tile[line + k][eighth + e] = u[e];
+    }
+    if (r < rows && c < colEnd) store_eight(byRow + split_at(r, c, rowBytes), u);
+  }
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < 64; k += 32) {
+    const int32_t c = c0 + line + k, r = r0 + eighth;
+    float u[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) u[e] = r + e < rows ? tile[eighth + e][line + k] : 0.f;
+    if (c < cols && r < rowEnd) store_eight(byColumn + split_at(c, r, columnBytes), u);
   }
 }
 
 // ----------------------------------------------------------------- products --
 // C = P Q', P and Q in the split layout: a workgroup has a tile of 128 x 128, each of its four waves 64 x 64 of that as 2 x 2 products of
 // 32 x 32. A block of 32 columns of both operands, upper and lower halves, is 32 KiB of LDS; the next one is on its way there while one is
-// multiplied. A row's eight 16-byte pieces lie in the order of their number xor the row's, so that lanes that read the same piece of
-// neighbouring rows meet all banks.
+// multiplied, and there is room for two workgroups a CU. A row's eight 16-byte pieces lie in the order of their number xor half the row's, so that
+// sixteen lanes that read the same piece of neighbouring rows meet all banks. (Blocks of 16 columns, four of which are on their way: 5 % slower, as
+// waves meet at twice as many barriers.)
 constexpr int kTile = 128;
 __host__ __device__ inline int32_t tiles_of(int32_t n) { return (n + kTile - 1) / kTile; }
 
@@ -206,7 +283,19 @@ struct Operand {
   int64_t rowBytes;
   int32_t count;         // rows from there on
 };
-__device__ __forceinline__ void product(const Operand& P, const Operand& Q, int32_t blocks, char* lds, acc16 (&acc)[2][2]) {
+// The sum over blocks of 32 columns is one of up to eight sums of equal parts, added up in their order: parts that several workgroups make come to the
+// same bits as those that one makes, so that a matrix's result does not depend on what else a call has. As many as give each CU two workgroups
+// where a matrix has few tiles.
+__host__ __device__ inline int32_t sum_parts(int32_t blocks, uint32_t tiles) {
+  const int32_t most = tiles <= 256 ? 512 / (int32_t)tiles : 8;
+  return max(1, min(blocks / 16, min(most, 8)));
+}
+__host__ __device__ inline int32_t part_begin(int32_t blocks, int32_t parts, int32_t k) { return (int32_t)((int64_t)blocks * k / parts); }
+
+constexpr int kStages = 2, kStageBytes = 2 * kTile * kBlockBytes, kOperandBytes = kTile * kBlockBytes;
+// Adds the parts first ... last - 1 of `parts` to `total`.
+__device__ __forceinline__ void product(const Operand& P, const Operand& Q, int32_t blocks, int32_t parts, int32_t first, int32_t last, char* lds,
+                                        acc16 (&total)[2][2]) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const uint32_t base = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)lds;
   const uint4v fromP = resource(P.rows, (uint32_t)min(P.count, kTile) * (uint32_t)P.rowBytes), fromQ = resource(Q.rows, (uint32_t)min(Q.count, kTile) * (uint32_t)Q.rowBytes);
@@ -214,34 +303,46 @@ __device__ __forceinline__ void product(const Operand& P, const Operand& Q, int3
   uint32_t offP[4], offQ[4];
 #pragma unroll
   for (int q = 0; q < 4; ++q) {
-    const int32_t row = (q * 4 + wave) * 8 + (lane >> 3), piece = (lane & 7) ^ (lane >> 3);
+    const int32_t row = (q * 4 + wave) * 8 + (lane >> 3), piece = (lane & 7) ^ ((row >> 1) & 7);
     offP[q] = (uint32_t)min(row, P.count - 1) * (uint32_t)P.rowBytes + piece * 16;
     offQ[q] = (uint32_t)min(row, Q.count - 1) * (uint32_t)Q.rowBytes + piece * 16;
   }
   auto load = [&](int32_t k, uint32_t stage) {
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
-      const uint32_t to = __builtin_amdgcn_readfirstlane(base + stage * 32768 + (q * 4 + wave) * 1024);
-      load_to_lds(fromP, offP[q], k * 128, to);
-      load_to_lds(fromQ, offQ[q], k * 128, to + 16384);
+      const uint32_t to = __builtin_amdgcn_readfirstlane(base + stage * kStageBytes + (q * 4 + wave) * 1024);
+      load_to_lds(fromP, offP[q], k * kBlockBytes, to);
+      load_to_lds(fromQ, offQ[q], k * kBlockBytes, to + kOperandBytes);
     }
   };
-  const int rowP = (wave >> 1) * 64 + (lane & 31), rowQ = (wave & 1) * 64 + (lane & 31);
-  load(0, 0);
-  for (int32_t k = 0; k < blocks; ++k) {
+  const int rowP = ((wave >> 1) * 64 + (lane & 31)) * kBlockBytes, rowQ = ((wave & 1) * 64 + (lane & 31)) * kBlockBytes + kOperandBytes;
+  acc16 acc[2][2] = {};
+  int32_t part = first, until = part_begin(blocks, parts, first + 1);
+  const int32_t begin = part_begin(blocks, parts, first), end = part_begin(blocks, parts, last);
+  load(begin, 0);
+  for (int32_t k = begin; k < end; ++k) {
+    if (k == until) {
+      until = part_begin(blocks, parts, ++part + 1);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        total[q >> 1][q & 1] += acc[q >> 1][q & 1];
+        acc[q >> 1][q & 1] = acc16{};
+      }
+    }
+    const uint32_t stage = (uint32_t)(k - begin) & 1;
     wait_loads_and_barrier();
-    if (k + 1 < blocks) load(k + 1, (k + 1) & 1);
-    const char *fp = lds + (k & 1) * 32768 + rowP * 128, *fq = lds + (k & 1) * 32768 + 16384 + rowQ * 128;
+    if (k + 1 < end) load(k + 1, stage ^ 1);      // (whose room was read last before the barrier)
+    const char *fp = lds + stage * kStageBytes + rowP, *fq = lds + stage * kStageBytes + rowQ;
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
-      const int high = ((2 * s + (lane >> 5)) ^ (lane & 7)) * 16, low = ((4 + 2 * s + (lane >> 5)) ^ (lane & 7)) * 16;
+      const int swizzle = (lane >> 1) & 7, high = ((2 * s + (lane >> 5)) ^ swizzle) * 16, low = ((4 + 2 * s + (lane >> 5)) ^ swizzle) * 16;
       half8 ph[2], pl[2], qh[2], ql[2];
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        ph[i] = *reinterpret_cast<const half8*>(fp + i * 4096 + high);
-        pl[i] = *reinterpret_cast<const half8*>(fp + i * 4096 + low);
-        qh[i] = *reinterpret_cast<const half8*>(fq + i * 4096 + high);
-        ql[i] = *reinterpret_cast<const half8*>(fq + i * 4096 + low);
+        ph[i] = *reinterpret_cast<const half8*>(fp + i * 32 * kBlockBytes + high);
+        pl[i] = *reinterpret_cast<const half8*>(fp + i * 32 * kBlockBytes + low);
+        qh[i] = *reinterpret_cast<const half8*>(fq + i * 32 * kBlockBytes + high);
+        ql[i] = *reinterpret_cast<const half8*>(fq + i * 32 * kBlockBytes + low);
       }
 #pragma unroll
       for (int i = 0; i < 2; ++i)
@@ -253,6 +354,8 @@ __device__ __forceinline__ void product(const Operand& P, const Operand& Q, int3
         }
     }
   }
+#pragma unroll
+  for (int q = 0; q < 4; ++q) total[q >> 1][q & 1] += acc[q >> 1][q & 1];
 }
 
 enum Op { kGram, kPolynomial, kStep, kLast };
@@ -262,36 +365,88 @@ __host__ __device__ inline uint32_t product_tiles(const Matrix& a, bool symmetri
   return symmetric ? symmetric_tiles(tiles_of(a.m)) : (uint32_t)(tiles_of(a.m) * (int64_t)tiles_of(a.n));
 }
 
+// Tiles in an order in which neighbours share operands: bands of eight rows of them, column by column.
+constexpr int kBand = 8;
+__device__ __forceinline__ void tile_at(uint32_t index, int32_t down, int32_t across, int32_t& ti, int32_t& tj) {
+  const uint32_t band = index / (uint32_t)(kBand * across), rest = index - band * (kBand * across), rows = min(kBand, down - (int32_t)band * kBand);
+  ti = (int32_t)(band * kBand + rest % rows);
+  tj = (int32_t)(rest / rows);
+}
+// The same for tiles on and above the diagonal: a band begins with its triangle.
+__device__ __forceinline__ void symmetric_tile_at(uint32_t index, int32_t tiles, int32_t& ti, int32_t& tj) {
+  int32_t first = 0;
+  for (;; first += kBand) {
+    const int32_t rows = min(kBand, tiles - first);
+    const uint32_t triangle = symmetric_tiles(rows), count = triangle + (uint32_t)rows * (uint32_t)(tiles - first - rows);
+    if (index < count) {
+      if (index < triangle) {
+        int32_t column = 0;
+        while (index > (uint32_t)column) index -= ++column;
+        ti = first + (int32_t)index;
+        tj = first + column;
+      } else {
+        index -= triangle;
+        ti = first + (int32_t)(index % rows);
+        tj = first + rows + (int32_t)(index / rows);
+      }
+      return;
+    }
+    index -= count;
+  }
+}
+
+template <typename T, typename F>
+__device__ __forceinline__ void eight_of(T* at, int32_t count, F f) {
+  if (count >= 8) {
+    constexpr int N = 16 / sizeof(T);
+    Pack<T, N> v[8 / N];
+#pragma unroll
+    for (int k = 0; k < 8 / N; ++k) v[k] = load_pack_unaligned<false, Pack<T, N>>(at + k * N);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f(e, v[e / N].v[e % N]);
+#pragma unroll
+    for (int k = 0; k < 8 / N; ++k) store_pack_unaligned<false>(at + k * N, v[k]);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (e < count) f(e, at[e]);
+  }
+}
+
 // One of a step's three products and what is made of it. The first two are symmetric: tiles above the diagonal go to both places. `turn`: which of the
-// two pairs of planes X is in. The last step's result goes to the tensor, or into the parameter.
-template <int OP, typename T, bool MUON>
-__global__ __launch_bounds__(256) void product_kernel(Group g, Update h, int turn) {
-  __shared__ __attribute__((aligned(128))) char lds[65536];
+// two pairs of planes X is in. The last step's result goes to the tensor, or into the parameter. The sums pass through LDS, so that memory sees whole
+// packs of neighbouring elements in both directions.
+constexpr int kProductLds = kTile * (kTile + 4) * 4;
+static_assert(kStages * kStageBytes <= kProductLds, "blocks and sums take turns");
+// The last tiles, which would leave much of the chip idle, are cut into the parts of their sums: a workgroup for each leaves its sums in memory, and a
+// launch behind this one (JOIN) adds them up and goes on from there.
+struct Tail {
+  uint32_t whole;      // tiles before them
+  int32_t parts;       // 1: none are cut
+  acc16* sums;         // of each part: 4 products of each of 256 lanes
+};
+template <int OP, typename T, bool MUON, bool JOIN>
+__global__ __launch_bounds__(256, 2) void product_kernel(Group g, Update h, int turn, Tail tail) {
+  __shared__ __attribute__((aligned(128))) char lds[kProductLds];
   constexpr bool kSymmetric = OP == kGram || OP == kPolynomial;
-  const Place p = place_of(g, blockIdx.x, [](const Matrix& a) { return product_tiles(a, kSymmetric); });
+  const uint32_t unit = JOIN ? blockIdx.x >> 2 : by_die(blockIdx.x, gridDim.x);
+  const bool cut = !JOIN && unit >= tail.whole;
+  const uint32_t tile = JOIN ? tail.whole + unit : cut ? tail.whole + (unit - tail.whole) / (uint32_t)tail.parts : unit;
+  const Place p = place_of(g, tile, [](const Matrix& a) { return product_tiles(a, kSymmetric); });
   const Matrix& a = p.a;
   char* work = a.work + p.batch * work_bytes(a);
   const int64_t px = plane_x(a), pt = plane_t(a);
   char *x = work + turn * (px + pt), *t = x + px, *xn = work + (turn ^ 1) * (px + pt), *tn = xn + px, *am = work + 2 * (px + pt), *bm = am + plane_a(a);
   const int64_t bytesM = row_bytes(a.m), bytesN = row_bytes(a.n);
   const bool flipped = OP == kLast && a.tall;      // the tensor's rows are the longer side: its tile is the product's transpose
+  const int32_t rows = flipped ? a.n : a.m, cols = kSymmetric || flipped ? a.m : a.n;
   int32_t ti, tj;
-  if constexpr (kSymmetric) {
-    // row by row of the upper triangle
-    const int32_t n = tiles_of(a.m);
-    ti = 0;
-    uint32_t rest = p.index;
-    while (rest >= (uint32_t)(n - ti)) {
-      rest -= n - ti;
-      ++ti;
-    }
-    tj = ti + (int32_t)rest;
-  } else {
-    const int32_t n = tiles_of(flipped ? a.m : a.n);
-    ti = (int32_t)(p.index / n);
-    tj = (int32_t)(p.index % n);
-  }
-  const int32_t rows = flipped ? a.n : a.m, cols = kSymmetric || flipped ? a.m : a.n, i0 = ti * kTile, j0 = tj * kTile;
+  if constexpr (kSymmetric) symmetric_tile_at(p.index, tiles_of(a.m), ti, tj);
+  else tile_at(p.index, tiles_of(rows), tiles_of(cols), ti, tj);
+  // (the joining launch has a workgroup for each wave's quarter of a tile: one CU alone would wait long for what all parts left)
+  constexpr int kSpan = JOIN ? kTile / 2 : kTile, kStride = kSpan + 4;      // floats: columns of sums, four rows at once, meet all banks
+  const int32_t i0 = ti * kTile + (JOIN ? (int32_t)(blockIdx.x >> 1 & 1) * kSpan : 0), j0 = tj * kTile + (JOIN ? (int32_t)(blockIdx.x & 1) * kSpan : 0);
+  if (JOIN && (i0 >= rows || j0 >= cols)) return;
   const char *from, *with;
   int64_t bytesK;
   if constexpr (OP == kGram) {
@@ -303,72 +458,100 @@ __global__ __launch_bounds__(256) void product_kernel(Group g, Update h, int tur
     with = OP == kPolynomial ? am : flipped ? bm : t;
   }
   const Operand P{from + i0 * bytesK, bytesK, rows - i0}, Q{with + j0 * bytesK, bytesK, cols - j0};
-  acc16 acc[2][2] = {};
-  product(P, Q, (int32_t)(bytesK / 128), lds, acc);
+  // The sums as columns: a lane has column `lane % 32` of each 32 x 32 product, four rows in a row of each eight.
+  float* sums = reinterpret_cast<float*>(lds);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int64_t size = (int64_t)a.m * a.n;
-  // a lane has column `lane % 32` of each 32 x 32 product, four rows in a row of each eight
+  auto keep = [&](int quarter, int q, const acc16& acc) {
 #pragma unroll
-  for (int bi = 0; bi < 2; ++bi) {
+    for (int r = 0; r < 4; ++r) {
+      const int i = (quarter >> 1) * 64 + (q >> 1) * 32 + r * 8 + (lane >> 5) * 4, j = (quarter & 1) * 64 + (q & 1) * 32 + (lane & 31);
+      *reinterpret_cast<Pack<float, 4>*>(sums + j * kStride + i) = Pack<float, 4>{acc[r * 4], acc[r * 4 + 1], acc[r * 4 + 2], acc[r * 4 + 3]};
+    }
+  };
+  if constexpr (JOIN) {
+    // (a wave for each of the four products)
+    const acc16* from16 = tail.sums + (int64_t)unit * tail.parts * 1024 + wave * 256 + (blockIdx.x & 3) * 64 + lane;
+    acc16 acc = {};
+#pragma unroll 8
+    for (int k = 0; k < tail.parts; ++k) acc += from16[k * 1024];
+    keep(0, wave, acc);
+  } else {
+    const int32_t blocks = (int32_t)(bytesK / kBlockBytes), parts = sum_parts(blocks, product_tiles(a, kSymmetric)), part = cut ? (int32_t)((unit - tail.whole) % (uint32_t)tail.parts) : 0;
+    acc16 acc[2][2] = {};
+    product(P, Q, blocks, parts, part, cut ? part + 1 : parts, lds, acc);
+    if (cut) {
+      acc16* to16 = tail.sums + (int64_t)(unit - tail.whole) * 1024 + threadIdx.x;
 #pragma unroll
-    for (int bj = 0; bj < 2; ++bj) {
-      const int32_t j = j0 + (wave & 1) * 64 + bj * 32 + (lane & 31);
+      for (int q = 0; q < 4; ++q) to16[q * 256] = acc[q >> 1][q & 1];
+      return;
+    }
+    __syncthreads();
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const int32_t i = i0 + (wave >> 1) * 64 + bi * 32 + q * 8 + (lane >> 5) * 4;
-        float v[4];
+    for (int q = 0; q < 4; ++q) keep(wave, q, acc[q >> 1][q & 1]);
+  }
+  __syncthreads();
+  // Rows: a thread has eight columns of every kRows-th row. (Few of these steps at a time: each of their instructions runs but a few times, and has
+  // to come from memory first.)
+  constexpr int kAcross = kSpan / 8, kRows = 256 / kAcross;
+  const int32_t jt = (threadIdx.x % kAcross) * 8, it = threadIdx.x / kAcross, j = j0 + jt;
+  const int32_t colEnd = (int32_t)blocks_of(cols) * kBlockK;
+  const char* base = OP == kPolynomial ? am : flipped ? t : x;
+  const int64_t baseBytes = OP == kPolynomial || flipped ? bytesM : bytesN;
+#pragma unroll 2
+  for (int u = 0; u < kSpan; u += kRows) {
+    const int32_t i = i0 + it + u;
+    Eight one{};
+    if (OP != kGram && i < rows && j < colEnd) one = load_eight(base + split_at(i, j, baseBytes));
+    float v[8];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const bool inside = i + e < rows && j < cols;
-          const float sum = acc[bi][bj][q * 4 + e];
-          if constexpr (OP == kGram) {
-            v[e] = sum * (kScaleA / (a.scale * a.scale));
-          } else if constexpr (OP == kPolynomial) {
-            const float one = inside ? load_split(am, split_at(i + e, j, bytesM)) : 0.f;
-            v[e] = __builtin_fmaf(one, kB * (kScaleB / kScaleA), sum * (kC * kScaleB / (kScaleA * kScaleA)));
-          } else {
-            const float one = inside ? (flipped ? load_split(t, split_at(i + e, j, bytesM)) : load_split(x, split_at(i + e, j, bytesN))) : 0.f;
-            v[e] = __builtin_fmaf(one, kA, sum * (1.f / kScaleB));
-          }
-          if (!inside) v[e] = 0.f;
-        }
-        if constexpr (OP == kLast) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            if (i + e >= rows || j >= cols) continue;
-            const int64_t at = p.batch * size + (int64_t)(i + e) * cols + j;
-            const float o = v[e] / a.scale;
-            T* out = static_cast<T*>(a.out);
-            if constexpr (MUON) {
-              const float was = a.master ? a.master[at] : Cvt<T>::up(out[at]), is = __builtin_fmaf(o, -a.rate, was * h.keep);
-              if (a.master) a.master[at] = is;
-              out[at] = rounded<T>(is);
-            } else {
-              out[at] = rounded<T>(o);
-            }
-          }
-        } else {
-          char* direct = OP == kGram ? am : OP == kPolynomial ? bm : xn;
-          char* mirrored = OP == kStep ? tn : direct;
-          const int64_t bytesDirect = OP == kStep ? bytesN : bytesM;
-          const int32_t colEnd = (int32_t)blocks_of(cols) * kBlockK, rowEnd = (int32_t)blocks_of(rows) * kBlockK;
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (i + e < rows && j < colEnd) store_split(direct, split_at(i + e, j, bytesDirect), v[e]);
-          if ((OP == kStep || ti != tj) && j < cols && i < rowEnd) {
-            half4 hi, lo;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const Split s = split(v[e]);
-              hi[e] = s.h;
-              lo[e] = s.l;
-            }
-            char* to = mirrored + split_at(j, i, bytesM);
-            *reinterpret_cast<half4*>(to) = hi;
-            *reinterpret_cast<half4*>(to + 64) = lo;
-          }
-        }
+    for (int e = 0; e < 8; ++e) {
+      const float sum = sums[(jt + e) * kStride + it + u];
+      if constexpr (OP == kGram) {
+        v[e] = sum * (kScaleA / (a.scale * a.scale));
+      } else {
+        const float o = (float)one.h[e] + (float)one.l[e];
+        if constexpr (OP == kPolynomial) v[e] = __builtin_fmaf(o, kB * (kScaleB / kScaleA), sum * (kC * kScaleB / (kScaleA * kScaleA)));
+        else v[e] = __builtin_fmaf(o, kA, sum * (1.f / kScaleB));
       }
+      if (i >= rows || j + e >= cols) v[e] = 0.f;
+    }
+    if constexpr (OP == kLast) {
+      if (i >= rows || j >= cols) continue;
+      const int64_t at = p.batch * ((int64_t)a.m * a.n) + (int64_t)i * cols + j;
+      const float down = 1.f / a.scale;      // (a power of two)
+      T* out = static_cast<T*>(a.out) + at;
+      if constexpr (MUON) {
+        if (a.master) {
+          eight_of(a.master + at, cols - j, [&](int e, float& was) { v[e] = was = __builtin_fmaf(v[e] * down, -a.rate, was * h.keep); });
+          eight_of(out, cols - j, [&](int e, T& o) { o = rounded<T>(v[e]); });
+        } else {
+          eight_of(out, cols - j, [&](int e, T& o) { o = rounded<T>(__builtin_fmaf(v[e] * down, -a.rate, Cvt<T>::up(o) * h.keep)); });
+        }
+      } else {
+        eight_of(out, cols - j, [&](int e, T& o) { o = rounded<T>(v[e] * down); });
+      }
+    } else {
+      if (i < rows && j < colEnd) store_eight((OP == kGram ? am : OP == kPolynomial ? bm : xn) + split_at(i, j, OP == kStep ? bytesN : bytesM), v);
+      if (OP == kStep || ti != tj) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sums[(jt + e) * kStride + it + u] = v[e];
+      }
+    }
+  }
+  if constexpr (OP != kLast) {
+    if (OP != kStep && ti == tj) return;
+    __syncthreads();
+    // and columns, in the same way
+    char* mirrored = OP == kGram ? am : OP == kPolynomial ? bm : tn;
+    const int32_t rowEnd = (int32_t)blocks_of(rows) * kBlockK, i = i0 + jt;
+#pragma unroll 2
+    for (int u = 0; u < kSpan; u += kRows) {
+      const int32_t c = it + u;
+      if (j0 + c >= cols || i >= rowEnd) continue;
+      const Pack<float, 4>* from4 = reinterpret_cast<const Pack<float, 4>*>(sums + c * kStride + jt);
+      const Pack<float, 4> low = from4[0], high = from4[1];
+      const float v[8] = {low.v[0], low.v[1], low.v[2], low.v[3], high.v[0], high.v[1], high.v[2], high.v[3]};
+      store_eight(mirrored + split_at(j0 + c, i, bytesM), v);
     }
   }
 }
@@ -391,16 +574,64 @@ float scale_of(int64_t m, int64_t n) {
   return (float)(1 << e);
 }
 
-// Workspace that the matrices of one pass share: enough of them to fill the chip many times over.
-constexpr int64_t kPassBytes = int64_t(1) << 30;
+// Workspace that the matrices of one pass share: enough of them to fill the chip many times over (72 matrices of 150 M halves in passes of 0.25, 0.5, 1, 2,
+// 4 GiB: 14.7, 12.4, 11.5, 11.2, 11.2 ms).
+constexpr int64_t kPassBytes = int64_t(2) << 30;
 
 struct Bytes {
   int64_t work, norms;
 };
 Bytes bytes_of(const Matrix& a) { return Bytes{work_bytes(a) * a.batch, (int64_t)norm_parts(a) * a.batch * 8}; }
 
+// The tiles of the last round of workgroups, two to a CU, if cutting them saves more than the joining launch costs: by what a block takes a workgroup
+// that has its CU to itself (0.45 us) or shares it (0.7), by that launch and by the sums' way through memory (0.026 us a part of a tile).
+Tail tail_of(const Group& g, int op, int64_t cus) {
+  const uint32_t tiles = g.first[g.count];
+  uint32_t rest = tiles % (uint32_t)(2 * cus);
+  auto blocks = [&](int k) { return (int32_t)blocks_of(op == kGram ? g.matrix[k].n : g.matrix[k].m); };
+  auto parts_of = [&](int k) { return sum_parts(blocks(k), product_tiles(g.matrix[k], op == kGram || op == kPolynomial)); };
+  Tail t{tiles, 1, nullptr};
+  const int32_t most = blocks(g.count - 1), parts = parts_of(g.count - 1);
+  int k = g.count - 1;
+  while (k > 0 && parts_of(k - 1) == parts) --k;
+  rest = std::min(rest, tiles - g.first[k]);
+  if (rest == 0 || parts == 1) return t;
+  auto cost = [&](int64_t units, double length) {
+    return (units <= cus ? 0.45 : 0.7 * (double)((units + 2 * cus - 1) / (2 * cus))) * length;
+  };
+  const int64_t units = (int64_t)rest * parts;
+  if (cost(units, (double)most / parts) + 6 + 0.026 * (double)units < cost(rest, most)) {
+    t.whole = tiles - rest;
+    t.parts = parts;
+  }
+  return t;
+}
+int64_t tail_bytes(const Group& g, const Tail& t) { return t.parts > 1 ? (int64_t)(g.first[g.count] - t.whole) * t.parts * kTile * kTile * 4 : 0; }
+
+template <int OP, typename T, bool MUON>
+void launch_product(THCState* s, const Group& g, const Update& h, int turn, const Tail& tail) {
+  hipStream_t st = current_stream(s);
+  const uint32_t rest = g.first[g.count] - tail.whole;
+  hipLaunchKernelGGL((product_kernel<OP, T, MUON, false>), dim3(tail.whole + rest * tail.parts), dim3(256), 0, st, g, h, turn, tail);
+  if (rest) hipLaunchKernelGGL((product_kernel<OP, T, MUON, true>), dim3(rest * 4), dim3(256), 0, st, g, h, turn, tail);
+}
+
+// The products' numbers of workgroups and tails.
+struct Plan {
+  Group symmetric, full;
+  Tail gram, polynomial, step;
+  Plan(const Group& g, int64_t cus) : symmetric(g), full(g) {
+    number(symmetric, [](const Matrix& a) { return product_tiles(a, true); });
+    number(full, [](const Matrix& a) { return product_tiles(a, false); });
+    gram = tail_of(symmetric, kGram, cus);
+    polynomial = tail_of(symmetric, kPolynomial, cus);
+    step = tail_of(full, kStep, cus);
+  }
+  int64_t bytes() const { return std::max({tail_bytes(symmetric, gram), tail_bytes(symmetric, polynomial), tail_bytes(full, step)}); }
+};
+
 template <typename T, bool MUON>
-void run_group(THCState* s, Group& g, const Update& h, int steps, char* work, double* norms) {
+void run_group(THCState* s, Group& g, const Update& h, int steps, char* work, double* norms, acc16* sums) {
   hipStream_t st = current_stream(s);
   for (int k = 0; k < g.count; ++k) {
     g.matrix[k].work = work;
@@ -411,15 +642,14 @@ void run_group(THCState* s, Group& g, const Update& h, int steps, char* work, do
   hipLaunchKernelGGL((norm_kernel<T, MUON>), dim3(parts), dim3(kBlock), 0, st, g, h, norms);
   const uint32_t tiles = number(g, tiles64);
   hipLaunchKernelGGL((split_kernel<T, MUON>), dim3(tiles), dim3(kBlock), 0, st, g, h, norms);
-  Group symmetric = g;
-  const uint32_t half = number(symmetric, [](const Matrix& a) { return product_tiles(a, true); });
-  const uint32_t whole = number(g, [](const Matrix& a) { return product_tiles(a, false); });
+  Plan plan(g, num_compute_units(s));
+  plan.gram.sums = plan.polynomial.sums = plan.step.sums = sums;
   for (int k = 0; k < steps; ++k) {
     const int turn = k & 1;
-    hipLaunchKernelGGL((product_kernel<kGram, T, MUON>), dim3(half), dim3(256), 0, st, symmetric, h, turn);
-    hipLaunchKernelGGL((product_kernel<kPolynomial, T, MUON>), dim3(half), dim3(256), 0, st, symmetric, h, turn);
-    if (k + 1 < steps) hipLaunchKernelGGL((product_kernel<kStep, T, MUON>), dim3(whole), dim3(256), 0, st, g, h, turn);
-    else hipLaunchKernelGGL((product_kernel<kLast, T, MUON>), dim3(whole), dim3(256), 0, st, g, h, turn);
+    launch_product<kGram, float, false>(s, plan.symmetric, h, turn, plan.gram);
+    launch_product<kPolynomial, float, false>(s, plan.symmetric, h, turn, plan.polynomial);
+    if (k + 1 < steps) launch_product<kStep, float, false>(s, plan.full, h, turn, plan.step);
+    else launch_product<kLast, T, MUON>(s, plan.full, h, turn, plan.step);
   }
 }
 
@@ -455,8 +685,12 @@ void run(THCState* s, const std::vector<Matrix>& all, const Update& h, int steps
       add(piece);
     }
   }
-  Workspace work(s, most.work), norms(s, most.norms);
-  for (Group& g : groups) run_group<T, MUON>(s, g, h, steps, work.data(), reinterpret_cast<double*>(norms.data()));
+  if (groups.empty()) return;
+  int64_t tails = 8;
+  for (const Group& g : groups) tails = std::max(tails, Plan(g, num_compute_units(s)).bytes());
+  Workspace work(s, most.work), norms(s, most.norms), sums(s, tails);
+  for (Group& g : groups)
+    run_group<T, MUON>(s, g, h, steps, work.data(), reinterpret_cast<double*>(norms.data()), reinterpret_cast<acc16*>(sums.data()));
 }
 
 void check_matrices(const AnyTensor* t, int arg) {
