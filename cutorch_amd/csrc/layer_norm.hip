@@ -123,7 +123,8 @@ __device__ __forceinline__ void load_columns(const T* from, const Packs<V, L, P>
   }
 }
 
-// A team of L lanes has a row in registers from its read to its write; teams go on to other rows with the weights that they hold.
+// A team of L lanes has a row in registers from its read to its write; teams go on to other rows with the weights that they hold, the next of which is
+// asked for before the one at hand is computed. Bound by memory: 16392 rows of 2048 halves 25.3 us, 5.3 TB/s.
 template <typename T, int V, int L, int TEAMS, int P>
 __global__ __launch_bounds__(L * TEAMS) void norm_kernel(NormArgs<T> a) {
   __shared__ float lds[L > 64 ? 3 * TEAMS * (L / 64) : 1];
@@ -193,9 +194,9 @@ struct GradArgs {
 };
 
 // The same with the sums over rows of what a lane's columns add to the weights' gradients, which stay in its registers; the workgroup's teams join
-// theirs at the end.
-template <typename T, int V, int L, int TEAMS, int P, bool WEIGHTS>
-__global__ __launch_bounds__(L * TEAMS) void norm_grad_kernel(GradArgs<T> a) {
+// theirs at the end. Bound by memory and, in halves, by arithmetic nearly as much: 16392 rows of 4096 halves 88 us with the joining launch, 4.6 TB/s.
+template <typename T, int V, int L, int TEAMS, int P, bool WEIGHTS, bool AHEAD>
+__global__ __launch_bounds__(L * TEAMS, 2) void norm_grad_kernel(GradArgs<T> a) {
   __shared__ float lds[L > 64 ? 5 * TEAMS * (L / 64) : 1];
   constexpr int kCols = L * P * V;                                       // (teams that share a wave join by lanes first)
   constexpr int kJoin = L < 64 ? L * TEAMS / 64 : TEAMS;
@@ -212,13 +213,14 @@ __global__ __launch_bounds__(L * TEAMS) void norm_grad_kernel(GradArgs<T> a) {
 #pragma unroll
     for (int e = 0; e < V; ++e) dw[p][e] = db[p][e] = 0.f;
   Pack<T, V> raw[P] = {}, next[P] = {};
-  {
-    const uint32_t row = min(blockIdx.x * TEAMS + team, a.rows - 1);
+  auto load = [&](uint32_t first) {
+    const uint32_t row = min(first + team, a.rows - 1);
     load_row<T, V, P, L>(a.x + a.xo.at(row), packs, raw);
     load_row<T, V, P, L>(a.g + a.go.at(row), packs, next);
-  }
+  };
+  if (AHEAD) load(blockIdx.x * TEAMS);
   for (uint32_t first = blockIdx.x * TEAMS; first < a.rows; first += gridDim.x * TEAMS) {
-    const uint32_t row = min(first + team, a.rows - 1);
+    if (!AHEAD) load(first);
     float d[P][V];
     Pack<T, V> graw[P];
 #pragma unroll
@@ -228,11 +230,7 @@ __global__ __launch_bounds__(L * TEAMS) void norm_grad_kernel(GradArgs<T> a) {
       for (int e = 0; e < V; ++e) d[p][e] = Cvt<T>::up(raw[p].v[e]);
     }
     // the next row is asked for before this one is computed
-    if (first + gridDim.x * TEAMS < a.rows) {
-      const uint32_t then = min(first + gridDim.x * TEAMS + team, a.rows - 1);
-      load_row<T, V, P, L>(a.x + a.xo.at(then), packs, raw);
-      load_row<T, V, P, L>(a.g + a.go.at(then), packs, next);
-    }
+    if (AHEAD && first + gridDim.x * TEAMS < a.rows) load(first + gridDim.x * TEAMS);
     clear_skipped<V, L, P>(packs, d);
     float one[1] = {0.f};
 #pragma unroll
@@ -261,8 +259,8 @@ __global__ __launch_bounds__(L * TEAMS) void norm_grad_kernel(GradArgs<T> a) {
     const float c = four[0] / n, r = 1.f / sqrtf(four[1] / n - c * c + a.eps);
     // mean(g w h) and mean(g w), times r
     const float meanH = (four[3] - c * four[2]) * r / n * r, meanG = four[2] / n * r;
-    const bool valid = first + team < a.rows;
-    T* out = a.dx + a.dxo.at(row);
+    if (TEAMS > 1 && first + team >= a.rows) continue;      // (all of a wave's lanes that still sum are back together at its next row)
+    T* out = a.dx + a.dxo.at(first + team);
 #pragma unroll
     for (int p = 0; p < P; ++p) {
       Pack<T, V> v;
@@ -271,11 +269,11 @@ __global__ __launch_bounds__(L * TEAMS) void norm_grad_kernel(GradArgs<T> a) {
         const float h = (d[p][e] - c) * r, g = Cvt<T>::up(graw[p].v[e]);
         v.v[e] = rounded<T>(__builtin_fmaf(-h, meanH, __builtin_fmaf(g * w[p][e], r, -meanG)));
         if constexpr (WEIGHTS) {
-          dw[p][e] = valid ? __builtin_fmaf(g, h, dw[p][e]) : dw[p][e];
-          db[p][e] = valid ? db[p][e] + g : db[p][e];
+          dw[p][e] = __builtin_fmaf(g, h, dw[p][e]);
+          db[p][e] += g;
         }
       }
-      if (valid) store_row(out, packs, p, v);
+      store_row(out, packs, p, v);
     }
   }
   if constexpr (WEIGHTS) {
@@ -498,28 +496,23 @@ void launch_norm(THCState* s, const NormArgs<T>& a) {
   const int64_t cus = num_compute_units(s), packs = (a.dim + V - 1) / V;
   auto go = [&](auto vec, auto lanes, auto teams, auto each) {
     constexpr int VV = decltype(vec)::value, L = decltype(lanes)::value, TEAMS = decltype(teams)::value, P = decltype(each)::value;
-    const int64_t groups = ((int64_t)a.rows + TEAMS - 1) / TEAMS, most = cus * std::max(1, (int)tuning("norm.threads", 2048) / (L * TEAMS));
+    const int64_t groups = ((int64_t)a.rows + TEAMS - 1) / TEAMS, most = cus * std::max(1, (P == 1 ? 2048 : 1024) / (L * TEAMS));
     hipLaunchKernelGGL((norm_kernel<T, VV, L, TEAMS, P>), dim3((unsigned)std::min(groups, most)), dim3(L * TEAMS), 0, st, a);
   };
 #define GO(VV, L, TEAMS, P) go(integral_constant<int, VV>{}, integral_constant<int, L>{}, integral_constant<int, TEAMS>{}, integral_constant<int, P>{})
-  const long way = tuning("norm.way", 0);
-  if (way == 1 && packs <= 256) { GO(V, 64, 4, 4); return; }
-  if (way == 2 && packs <= 256) { GO(V, 128, 2, 2); return; }
-  if (way == 5 && packs <= 512) { GO(V, 128, 2, 4); return; }
-  if (way == 6 && packs <= 512) { GO(V, 512, 1, 1); return; }
-  if (way == 3 && packs <= 256) { GO(V, 128, 1, 2); return; }
-  if (way == 4 && packs <= 256) { GO(V, 256, 2, 1); return; }
+  // Two packs a lane where rows have them: half of the lanes that meet at a sum. us for 16392 rows of 2048 halves with 64 lanes of 4 packs, 128 of 2 and 256 of
+  // 1: 26.5, 25.3, 31.2; 65536 of 500 with 32 of 2 and 64 of 1 32.2, 34.4.
   if (a.dim < V) GO(1, 8, 32, 1);
   else if (packs <= 8) GO(V, 8, 32, 1);
   else if (packs <= 16) GO(V, 16, 16, 1);
   else if (packs <= 32) GO(V, 32, 8, 1);
-  else if (packs <= 64) GO(V, 64, 4, 1);
+  else if (packs <= 64) GO(V, 32, 8, 2);
   else if (packs <= 128) GO(V, 64, 4, 2);
-  else if (packs <= 256) GO(V, 256, 1, 1);
+  else if (packs <= 256) GO(V, 128, 2, 2);
   else if (packs <= 512) GO(V, 256, 1, 2);
   else if (packs <= 1024) GO(V, 256, 1, 4);
   else if (packs <= 2048) GO(V, 512, 1, 4);
-  else if (packs <= 4096 && V == 4) GO(4, 1024, 1, 4);
+  else if (V == 4 && packs <= 4096) GO(V, (V == 4 ? 1024 : 512), 1, 4);      // (a length that halves have already)
   else hipLaunchKernelGGL((long_norm_kernel<T>), dim3((unsigned)std::min<int64_t>(a.rows, cus * 2)), dim3(kLong), 0, st, a);
 #undef GO
 }
@@ -544,39 +537,37 @@ void launch_grad(THCState* s, GradArgs<T>& a, const WeightGrads<T>& to) {
   auto join = [&](int64_t count) {
     hipLaunchKernelGGL((join_kernel<T>), dim3((a.dim + 31) / 32, 2), dim3(1024), 0, st, a.weightPart, a.biasPart, to.weight, to.bias, (int32_t)count, a.dim, (int)to.accumulate);
   };
-  auto go = [&](auto vec, auto lanes, auto teams, auto each) {
+  auto go = [&](auto vec, auto lanes, auto teams, auto each, auto ahead, int64_t threads) {
     constexpr int VV = decltype(vec)::value, L = decltype(lanes)::value, TEAMS = decltype(teams)::value, P = decltype(each)::value;
-    const int64_t groups = ((int64_t)a.rows + TEAMS - 1) / TEAMS;
+    constexpr bool A = decltype(ahead)::value;
+    const int64_t groups = ((int64_t)a.rows + TEAMS - 1) / TEAMS, most = cus * std::max<int64_t>(1, threads / (L * TEAMS));
     if (!sums) {
-      const int64_t most = cus * std::max(1, 2048 / (L * TEAMS));
-      hipLaunchKernelGGL((norm_grad_kernel<T, VV, L, TEAMS, P, false>), dim3((unsigned)std::min(groups, most)), dim3(L * TEAMS), 0, st, a);
+      hipLaunchKernelGGL((norm_grad_kernel<T, VV, L, TEAMS, P, false, A>), dim3((unsigned)std::min(groups, 2 * most)), dim3(L * TEAMS), 0, st, a);
       return;
     }
-    // a workgroup's sums cross memory twice: each has some rows at least
-    const int64_t count = std::max<int64_t>(1, std::min(groups / (int64_t)tuning("norm.each", 4), cus * std::max(1, (int)tuning("norm.gthreads", 512) / (L * TEAMS))));
+    // a workgroup's sums cross memory twice: each has two rows at least
+    const int64_t count = std::max<int64_t>(1, std::min(groups / 2, most));
     Workspace w(s, bytes(count));
     parts(count, w);
-    hipLaunchKernelGGL((norm_grad_kernel<T, VV, L, TEAMS, P, true>), dim3((unsigned)count), dim3(L * TEAMS), 0, st, a);
+    hipLaunchKernelGGL((norm_grad_kernel<T, VV, L, TEAMS, P, true, A>), dim3((unsigned)count), dim3(L * TEAMS), 0, st, a);
     join(count);
   };
-#define GO(VV, L, TEAMS, P) go(integral_constant<int, VV>{}, integral_constant<int, L>{}, integral_constant<int, TEAMS>{}, integral_constant<int, P>{})
-  const long way = tuning("norm.gway", 0);
-  if (a.dim < V) GO(1, 8, 32, 1);
-  else if (packs <= 8) GO(V, 8, 32, 1);
-  else if (packs <= 16) GO(V, 16, 16, 1);
-  else if (packs <= 32) GO(V, 32, 8, 1);
-  else if (packs <= 64) GO(V, 64, 4, 1);
-  else if (packs <= 128) GO(V, 64, 4, 2);
-  else if (packs <= 256 && way == 1) GO(V, 128, 2, 2);
-  else if (packs <= 256 && way == 2) GO(V, 256, 1, 1);
-  else if (packs <= 256) GO(V, 64, 4, 4);
-  else if (packs <= 512 && way == 1) GO(V, 128, 2, 4);
-  else if (packs <= 512 && way == 2) GO(V, 512, 1, 1);
-  else if (packs <= 512 && way == 3) GO(V, 256, 2, 2);
-  else if (packs <= 512) GO(V, 256, 1, 2);
-  else if (packs <= 1024) GO(V, 256, 1, 4);
-  else if (packs <= 2048) GO(V, 512, 1, 4);
-  else if (packs <= 4096 && V == 4) GO(4, 1024, 1, 4);
+#define GO(VV, L, TEAMS, P, A, THREADS) \
+  go(integral_constant<int, VV>{}, integral_constant<int, L>{}, integral_constant<int, TEAMS>{}, integral_constant<int, P>{}, integral_constant<bool, A>{}, THREADS)
+  // The last number: threads a CU. More hide the two sums of a row better, and make more rows of sums that cross memory. us with 512, 768 and 1024 of
+  // them: 16384 rows of 4096 halves 90, 88, 106, of 2048 48, 50, 59, 16384 of 2000 floats 76, 80, 84; 65536 of 500 halves 63, 56, 55. The next row is
+  // asked for early where registers allow it (4096 halves 148 without, 88 with).
+  if (a.dim < V) GO(1, 8, 32, 1, true, 1024);
+  else if (packs <= 8) GO(V, 8, 32, 1, true, 1024);
+  else if (packs <= 16) GO(V, 16, 16, 1, true, 1024);
+  else if (packs <= 32) GO(V, 32, 8, 1, true, 1024);
+  else if (packs <= 64) GO(V, 64, 4, 1, true, 1024);
+  else if (packs <= 128) GO(V, 64, 4, 2, true, 512);
+  else if (packs <= 256) GO(V, 128, 2, 2, true, 512);
+  else if (packs <= 512) GO(V, 256, 1, 2, true, V == 8 ? 768 : 512);
+  else if (packs <= 1024) GO(V, 256, 1, 4, true, 512);
+  else if (packs <= 2048) GO(V, 512, 1, 4, true, 512);
+  else if (V == 4 && packs <= 4096) GO(V, (V == 4 ? 1024 : 512), 1, 4, (V == 8), 1024);
   else {
     const dim3 grid((unsigned)std::min<int64_t>(a.rows, cus * 2));
     Workspace stats(s, (int64_t)a.rows * sizeof(RowStats));

@@ -25,6 +25,7 @@ constexpr float kA = 3.4445f, kB = -4.7750f, kC = 2.0315f;
 constexpr float kScaleA = 16384.f, kScaleB = 8192.f;
 
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
+typedef _Float16 half4 __attribute__((ext_vector_type(4)));
 typedef float acc16 __attribute__((ext_vector_type(16)));
 typedef unsigned uint4v __attribute__((ext_vector_type(4)));
 
@@ -88,7 +89,10 @@ __device__ __forceinline__ Place place_of(const Group& g, uint32_t block, F each
 
 // ------------------------------------------------------------ norms, planes --
 constexpr int kNormPart = 16384;      // elements a workgroup
-__host__ __device__ inline uint32_t norm_parts(const Matrix& a) { return (uint32_t)(((int64_t)a.m * a.n + kNormPart - 1) / kNormPart); }
+// (none of those whose one workgroup makes its norm by itself)
+constexpr int kShort = 128, kStrip = 128;
+__host__ __device__ inline bool is_alone(const Matrix& a) { return a.m <= kShort && a.n <= kStrip; }
+__host__ __device__ inline uint32_t norm_parts(const Matrix& a) { return is_alone(a) ? 0 : (uint32_t)(((int64_t)a.m * a.n + kNormPart - 1) / kNormPart); }
 
 struct Update {
   float beta, gradScale, keep, eps;
@@ -169,7 +173,10 @@ __global__ __launch_bounds__(kBlock) void norm_kernel(Group g, Update h, double*
 struct Split {
   _Float16 h, l;
 };
+// (The operation before it must not become one with the rounding to half: it would round once there and twice for the lower half, which now and then then
+// goes with another upper one.)
 __device__ __forceinline__ Split split(float x) {
+  asm("" : "+v"(x));
   Split s;
   s.h = (_Float16)x;
   s.l = (_Float16)(x - (float)s.h);
@@ -556,6 +563,316 @@ __global__ __launch_bounds__(256, 2) void product_kernel(Group g, Update h, int 
   }
 }
 
+// ---------------------------------------------------------- short matrices --
+// Up to 128 rows: A and B are one tile each, and what bounds a step is how long its launches wait for memory one after another (12 matrices of 65 x 513: 17
+// launches of 9 to 17 us each). A workgroup has a strip of 128 columns of X. It adds up the strips' shares of A, makes B of it by itself,
+// takes its strip through the step and leaves the strip's share of the next A: one launch a step, and one for all steps where X is a single strip.
+// LDS: one plane for A, then B, then the new X, a second one for the strip's transpose, both split, rows of 16-byte pieces in the order of their
+// number xor what brings sixteen rows to different banks.
+constexpr int kShortThreads = 1024, kFewStrips = 8;
+__host__ __device__ inline bool is_short(const Matrix& a) { return a.m <= kShort; }
+__host__ __device__ inline int32_t strips_of(const Matrix& a) { return (a.n + kStrip - 1) / kStrip; }
+__host__ __device__ inline int32_t bands_of(const Matrix& a) { return (a.m + 31) / 32; }
+__host__ __device__ inline int64_t gram_bytes(const Matrix& a) { return (int64_t)bands_of(a) * bands_of(a) * 4096; }
+// X', the strips' shares of A for this step and the next, their sum.
+__host__ __device__ inline int64_t short_bytes(const Matrix& a) { return plane_t(a) + (2 * (int64_t)strips_of(a) + 1) * gram_bytes(a); }
+__host__ __device__ inline int short_lds(int bands) { return bands * 32 * 512 + kStrip * bands * 128; }
+
+struct Plane {
+  char* at;
+  int rowBytes;      // a multiple of 128
+  __device__ __forceinline__ int piece(int row, int k) const {
+    return row * rowBytes + ((k ^ ((rowBytes & 128) ? row >> 1 & 7 : row & 15)) << 4);
+  }
+  // of the upper half of an element; the lower one is 4 pieces on
+  __device__ __forceinline__ char* upper(int row, int column) const { return at + piece(row, (column >> 5) * 8 + (column >> 3 & 3)) + (column & 7) * 2; }
+  __device__ __forceinline__ char* lower(int row, int column) const { return at + piece(row, (column >> 5) * 8 + 4 + (column >> 3 & 3)) + (column & 7) * 2; }
+  __device__ __forceinline__ void store4(int row, int column, const float (&x)[4]) const {
+    half4 h, l;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const Split s = split(x[e]);
+      h[e] = s.h;
+      l[e] = s.l;
+    }
+    *reinterpret_cast<half4*>(upper(row, column)) = h;
+    *reinterpret_cast<half4*>(lower(row, column)) = l;
+  }
+};
+// 32 x 32 of P Q' over `blocks` blocks of 32 columns. Three sums side by side: one would wait for itself.
+__device__ __forceinline__ acc16 small_product(const Plane& P, int i0, const Plane& Q, int j0, int blocks) {
+  const int lane = threadIdx.x & 63, rowP = i0 + (lane & 31), rowQ = j0 + (lane & 31), k0 = lane >> 5;
+  acc16 high = {}, right = {}, left = {};
+#pragma unroll 2
+  for (int k = 0; k < 2 * blocks; ++k) {
+    const int at = (k >> 1) * 8 + (k & 1) * 2 + k0;
+    const half8 ph = *reinterpret_cast<const half8*>(P.at + P.piece(rowP, at)), pl = *reinterpret_cast<const half8*>(P.at + P.piece(rowP, at + 4));
+    const half8 qh = *reinterpret_cast<const half8*>(Q.at + Q.piece(rowQ, at)), ql = *reinterpret_cast<const half8*>(Q.at + Q.piece(rowQ, at + 4));
+    high = __builtin_amdgcn_mfma_f32_32x32x16_f16(ph, qh, high, 0, 0, 0);
+    right = __builtin_amdgcn_mfma_f32_32x32x16_f16(ph, ql, right, 0, 0, 0);
+    left = __builtin_amdgcn_mfma_f32_32x32x16_f16(pl, qh, left, 0, 0, 0);
+  }
+  return high + (right + left);
+}
+// Four lanes side by side that have a column of 4 x 4 each get a row each.
+template <int CONTROL>
+__device__ __forceinline__ float from_neighbour(float x) {
+  return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), CONTROL, 0xf, 0xf, true));
+}
+__device__ __forceinline__ void transpose4(float (&v)[4]) {
+  const bool odd = threadIdx.x & 1, second = threadIdx.x & 2;
+#pragma unroll
+  for (int k = 0; k < 4; k += 2) {      // 2 x 2 blocks within themselves
+    const float mine = odd ? v[k] : v[k + 1], theirs = from_neighbour<0xb1>(mine);
+    (odd ? v[k] : v[k + 1]) = theirs;
+  }
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {         // and the two off the diagonal against each other
+    const float mine = second ? v[k] : v[k + 2], theirs = from_neighbour<0x4e>(mine);
+    (second ? v[k] : v[k + 2]) = theirs;
+  }
+}
+
+// A workgroup's strip. Its sixteen waves have one of the 32 x 32 products each, of which there are 4 x 4 at most.
+struct Strip {
+  const Matrix& a;
+  int bands, blocks, j0, lane, wave;      // blocks: of 32 columns in the strip
+  Plane square, fresh, across;            // A or B; the new X in the same place; the strip's transpose
+  __device__ __forceinline__ Strip(const Matrix& m, int strip, char* lds) : a(m) {
+    bands = bands_of(m);
+    j0 = strip * kStrip;
+    blocks = (min(kStrip, m.n - j0) + 31) / 32;
+    lane = threadIdx.x & 63;
+    wave = threadIdx.x >> 6;
+    square = Plane{lds, bands * 128};
+    fresh = Plane{lds, 512};
+    across = Plane{lds + bands * 32 * 512, bands * 128};
+  }
+  // f(its place) for this wave's product, of `down` x `over`
+  template <typename F>
+  __device__ __forceinline__ void each(int down, int over, F f) const {
+    if (wave < down * over) f(wave / over, wave % over);
+  }
+  // f(e0, row, column) for the first of each four rows that a lane has of a product
+  template <typename F>
+  __device__ __forceinline__ void fours(int ti, int tj, F f) const {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) f(q * 4, ti * 32 + q * 8 + (lane >> 5) * 4, tj * 32 + (lane & 31));
+  }
+  // From A (its sums, as the products leave them) to B in the square.
+  __device__ __forceinline__ void polynomial(acc16& sums) const {
+    const float scale = kScaleA / (a.scale * a.scale);
+    each(bands, bands, [&](int ti, int tj) {
+      sums *= scale;
+      fours(ti, tj, [&](int e, int i, int j) { square.store4(j, i, {sums[e], sums[e + 1], sums[e + 2], sums[e + 3]}); });
+    });
+    __syncthreads();
+    each(bands, bands, [&](int ti, int tj) {
+      const acc16 twice = small_product(square, ti * 32, square, tj * 32, bands);
+#pragma unroll
+      for (int e = 0; e < 16; ++e) sums[e] = __builtin_fmaf(sums[e], kB * (kScaleB / kScaleA), twice[e] * (kC * kScaleB / (kScaleA * kScaleA)));
+    });
+    __syncthreads();
+    each(bands, bands, [&](int ti, int tj) {
+      fours(ti, tj, [&](int e, int i, int j) { square.store4(j, i, {sums[e], sums[e + 1], sums[e + 2], sums[e + 3]}); });
+    });
+    __syncthreads();
+  }
+  // The next X, times its scale.
+  __device__ __forceinline__ void step(acc16& x) const {
+    each(bands, blocks, [&](int ti, int tj) {
+      x = small_product(square, ti * 32, across, tj * 32, bands);
+      fours(ti, tj, [&](int e, int i, int j) {
+        const half4 h = *reinterpret_cast<const half4*>(across.upper(j, i)), l = *reinterpret_cast<const half4*>(across.lower(j, i));
+#pragma unroll
+        for (int k = 0; k < 4; ++k) x[e + k] = __builtin_fmaf((float)h[k] + (float)l[k], kA, x[e + k] * (1.f / kScaleB));
+      });
+    });
+    __syncthreads();
+  }
+  // X into both planes, then the strip's share of A.
+  __device__ __forceinline__ void gram(const acc16& x, acc16& sums) const {
+    each(bands, blocks, [&](int ti, int tj) {
+      fours(ti, tj, [&](int e, int i, int j) {
+        const float v[4] = {x[e], x[e + 1], x[e + 2], x[e + 3]};
+        across.store4(j, i, v);
+        float row[4] = {v[0], v[1], v[2], v[3]};
+        transpose4(row);
+        fresh.store4(i + (lane & 3), j & ~3, row);
+      });
+    });
+    __syncthreads();
+    each(bands, bands, [&](int ti, int tj) { sums = small_product(fresh, ti * 32, fresh, tj * 32, blocks); });
+    __syncthreads();
+  }
+  // Element (row, column of the strip) of a matrix that begins at element `at` of its tensor; -1: there is none.
+  __device__ __forceinline__ int64_t place(int64_t at, int i, int j) const {
+    const int32_t column = j0 + j;
+    if (i >= a.m || column >= a.n) return -1;
+    return at + (a.tall ? (int64_t)column * a.m + i : (int64_t)i * a.n + column);
+  }
+  // The result to the tensor or into the parameter; `at`: of this matrix.
+  template <typename T, bool MUON>
+  __device__ __forceinline__ void emit(const acc16& x, const Update& h, int64_t at) const {
+    const float down = 1.f / a.scale;
+    each(bands, blocks, [&](int ti, int tj) {
+      fours(ti, tj, [&](int e, int i, int j) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int64_t to = place(at, i + k, j);
+          if (to < 0) continue;
+          T* out = static_cast<T*>(a.out) + to;
+          const float o = x[e + k] * down;
+          if constexpr (MUON) {
+            const float was = a.master ? a.master[to] : Cvt<T>::up(*out), is = __builtin_fmaf(o, -a.rate, was * h.keep);
+            if (a.master) a.master[to] = is;
+            *out = rounded<T>(is);
+          } else {
+            *out = rounded<T>(o);
+          }
+        }
+      });
+    });
+  }
+};
+
+// The strip's transpose and its share of A into memory.
+__device__ __forceinline__ void leave(const Strip& strip, const acc16& sums, char* work, uint32_t index, int turn) {
+  const Matrix& a = strip.a;
+  const int pieces = strip.bands * 8, rows = min(kStrip, a.n - strip.j0);
+  uint4v* to = reinterpret_cast<uint4v*>(work + (int64_t)strip.j0 * strip.bands * 128);
+  for (int k = threadIdx.x; k < rows * pieces; k += kShortThreads)
+    to[k] = *reinterpret_cast<const uint4v*>(strip.across.at + strip.across.piece(k / pieces, k % pieces));
+  acc16* share = reinterpret_cast<acc16*>(work + plane_t(a) + ((int64_t)turn * strips_of(a) + index) * gram_bytes(a));
+  strip.each(strip.bands, strip.bands, [&](int ti, int tj) { share[(ti * strip.bands + tj) * 64 + strip.lane] = sums; });
+}
+
+// The strip's elements into both planes, over the norm, which a strip that is the whole matrix makes by itself (and the momentum with it). WHOLE: all
+// of the launch's are, and go through all steps in it.
+template <typename T, bool MUON, bool WHOLE>
+__global__ __launch_bounds__(kShortThreads) void short_begin_kernel(Group g, Update h, const double* parts, int steps) {
+  extern __shared__ __attribute__((aligned(256))) char lds[];
+  __shared__ double norms[kShortThreads / 64];
+  const Place p = place_of(g, blockIdx.x, [](const Matrix& a) { return (uint32_t)strips_of(a); });
+  const Matrix& a = p.a;
+  const int64_t at = p.batch * ((int64_t)a.m * a.n);
+  const Strip strip(a, (int)p.index, lds);
+  const bool alone = WHOLE || is_alone(a);
+  const T* in = static_cast<const T*>(a.in);
+  acc16 x = {}, was = {}, sums = {};
+  strip.each(strip.bands, strip.blocks, [&](int ti, int tj) {
+    strip.fours(ti, tj, [&](int e, int i, int j) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int64_t from = strip.place(at, i + k, j);
+        if (from < 0) continue;
+        x[e + k] = Cvt<T>::up(in[from]);
+        if constexpr (MUON) was[e + k] = a.momentum[from];
+      }
+    });
+  });
+  double sum = 0;
+  strip.each(strip.bands, strip.blocks, [&](int ti, int tj) {
+    strip.fours(ti, tj, [&](int e, int i, int j) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        float u = x[e + k];
+        if constexpr (MUON) {
+          const float grad = u * h.gradScale, m = alone ? __builtin_fmaf(was[e + k], h.beta, grad) : was[e + k];
+          if (alone) {
+            const int64_t to = strip.place(at, i + k, j);
+            if (to >= 0) a.momentum[to] = m;
+          }
+          u = h.nesterov ? __builtin_fmaf(m, h.beta, grad) : m;
+        }
+        x[e + k] = u;
+        if (alone) sum += (double)u * u;
+      }
+    });
+  });
+  if (!alone) {
+    const uint32_t n = norm_parts(a);
+    const double* mine = parts + a.norms + (int64_t)p.batch * n;
+    for (uint32_t i = threadIdx.x; i < n; i += kShortThreads) sum += mine[i];
+  }
+  for (int d = 32; d >= 1; d >>= 1) sum += __shfl_xor(sum, d);
+  if (strip.lane == 0) norms[strip.wave] = sum;
+  __syncthreads();
+  sum = 0;
+  for (int w = 0; w < kShortThreads / 64; ++w) sum += norms[w];
+  const float factor = (float)((double)a.scale / (sqrt(sum) + (double)h.eps));
+  x *= factor;
+  strip.gram(x, sums);
+  if constexpr (WHOLE) {
+    for (int k = 0; k < steps; ++k) {
+      strip.polynomial(sums);
+      strip.step(x);
+      if (k + 1 < steps) strip.gram(x, sums);
+    }
+    strip.emit<T, MUON>(x, h, at);
+  } else {
+    char* work = a.work + p.batch * short_bytes(a);
+    leave(strip, sums, work, p.index, 0);
+  }
+}
+
+// The sum of many strips' shares of A, before the step that takes it.
+constexpr int kShareThreads = 64;
+__host__ __device__ inline uint32_t share_parts(const Matrix& a) { return (uint32_t)(gram_bytes(a) / 16 / kShareThreads); }
+__global__ __launch_bounds__(kShareThreads) void shares_kernel(Group g, int turn) {
+  const Place p = place_of(g, blockIdx.x, [](const Matrix& a) { return share_parts(a); });
+  const Matrix& a = p.a;
+  const int strips = strips_of(a);
+  const int64_t bytes = gram_bytes(a), step = bytes / 16;
+  char* shares = a.work + p.batch * short_bytes(a) + plane_t(a);
+  typedef float float4v __attribute__((ext_vector_type(4)));
+  const int64_t k = (int64_t)p.index * kShareThreads + threadIdx.x;
+  const float4v* from = reinterpret_cast<const float4v*>(shares + turn * strips * bytes) + k;
+  float4v sum = {};
+#pragma unroll 8
+  for (int s = 0; s < strips; ++s) sum += from[s * step];
+  reinterpret_cast<float4v*>(shares + 2 * strips * bytes)[k] = sum;
+}
+
+template <typename T, bool MUON, bool LAST>
+__global__ __launch_bounds__(kShortThreads) void short_step_kernel(Group g, Update h, int turn) {
+  extern __shared__ __attribute__((aligned(256))) char lds[];
+  const Place p = place_of(g, blockIdx.x, [](const Matrix& a) { return (uint32_t)strips_of(a); });
+  const Matrix& a = p.a;
+  const Strip strip(a, (int)p.index, lds);
+  char* work = a.work + p.batch * short_bytes(a);
+  // the strip's transpose is on its way while A is made
+  const int pieces = strip.bands * 8, rows = min(kStrip, a.n - strip.j0), all = kStrip * pieces;
+  const uint4v* from = reinterpret_cast<const uint4v*>(work + (int64_t)strip.j0 * strip.bands * 128);
+  uint4v held[4];
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    const int k = threadIdx.x + q * kShortThreads;
+    held[q] = k < rows * pieces ? from[k] : uint4v{0, 0, 0, 0};
+  }
+  const int strips = strips_of(a);
+  const int64_t bytes = gram_bytes(a);
+  const char* shares = work + plane_t(a) + (strips > kFewStrips ? 2 * strips : turn * strips) * bytes;
+  acc16 sums = {}, x = {};
+  strip.each(strip.bands, strip.bands, [&](int ti, int tj) {
+    const acc16* mine = reinterpret_cast<const acc16*>(shares) + (ti * strip.bands + tj) * 64 + strip.lane;
+    for (int k = 0; k < (strips > kFewStrips ? 1 : strips); ++k) sums += mine[k * (bytes / 64)];
+  });
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    const int k = threadIdx.x + q * kShortThreads;
+    if (k < all) *reinterpret_cast<uint4v*>(strip.across.at + strip.across.piece(k / pieces, k % pieces)) = held[q];
+  }
+  strip.polynomial(sums);
+  strip.step(x);
+  if constexpr (LAST) {
+    strip.emit<T, MUON>(x, h, p.batch * ((int64_t)a.m * a.n));
+  } else {
+    strip.gram(x, sums);
+    leave(strip, sums, work, p.index, turn ^ 1);
+  }
+}
+
 // ----------------------------------------------------------------- launches --
 template <typename Count>
 uint32_t number(Group& g, Count count) {
@@ -581,7 +898,8 @@ constexpr int64_t kPassBytes = int64_t(2) << 30;
 struct Bytes {
   int64_t work, norms;
 };
-Bytes bytes_of(const Matrix& a) { return Bytes{work_bytes(a) * a.batch, (int64_t)norm_parts(a) * a.batch * 8}; }
+int64_t each_bytes(const Matrix& a) { return is_short(a) ? short_bytes(a) : work_bytes(a); }
+Bytes bytes_of(const Matrix& a) { return Bytes{each_bytes(a) * a.batch, (int64_t)norm_parts(a) * a.batch * 8}; }
 
 // The tiles of the last round of workgroups, two to a CU, if cutting them saves more than the joining launch costs: by what a block takes a workgroup
 // that has its CU to itself (0.45 us) or shares it (0.7), by that launch and by the sums' way through memory (0.026 us a part of a tile).
@@ -631,6 +949,37 @@ struct Plan {
 };
 
 template <typename T, bool MUON>
+void run_short(THCState* s, Group& g, const Update& h, int steps, const double* norms) {
+  hipStream_t st = current_stream(s);
+  int bands = 0;
+  bool many = false, whole = true;
+  for (int k = 0; k < g.count; ++k) {
+    whole = whole && is_alone(g.matrix[k]);
+    bands = std::max(bands, bands_of(g.matrix[k]));
+    many = many || strips_of(g.matrix[k]) > kFewStrips;
+  }
+  const int lds = short_lds(bands);
+  const dim3 threads(kShortThreads);
+  Group shares = g;
+  const uint32_t parts = many ? number(shares, share_parts) : 0;
+  const dim3 strips(number(g, [](const Matrix& a) { return (uint32_t)strips_of(a); }));
+  auto roomy = [&](auto kernel) {
+    if (lds > 65536) THC_CHECK(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, lds));
+    return kernel;
+  };
+  if (whole) {
+    hipLaunchKernelGGL(roomy(short_begin_kernel<T, MUON, true>), strips, threads, lds, st, g, h, norms, steps);
+    return;
+  }
+  hipLaunchKernelGGL(roomy(short_begin_kernel<T, MUON, false>), strips, threads, lds, st, g, h, norms, steps);
+  for (int k = 0; k < steps; ++k) {
+    if (many) hipLaunchKernelGGL(shares_kernel, dim3(parts), dim3(kShareThreads), 0, st, shares, k & 1);
+    if (k + 1 < steps) hipLaunchKernelGGL(roomy(short_step_kernel<float, false, false>), strips, threads, lds, st, g, h, k & 1);
+    else hipLaunchKernelGGL(roomy(short_step_kernel<T, MUON, true>), strips, threads, lds, st, g, h, k & 1);
+  }
+}
+
+template <typename T, bool MUON>
 void run_group(THCState* s, Group& g, const Update& h, int steps, char* work, double* norms, acc16* sums) {
   hipStream_t st = current_stream(s);
   for (int k = 0; k < g.count; ++k) {
@@ -639,7 +988,11 @@ void run_group(THCState* s, Group& g, const Update& h, int steps, char* work, do
   }
   const uint32_t parts = number(g, norm_parts);
   for (int k = 0; k < g.count; ++k) g.matrix[k].norms = g.first[k];
-  hipLaunchKernelGGL((norm_kernel<T, MUON>), dim3(parts), dim3(kBlock), 0, st, g, h, norms);
+  if (parts) hipLaunchKernelGGL((norm_kernel<T, MUON>), dim3(parts), dim3(kBlock), 0, st, g, h, norms);
+  if (is_short(g.matrix[0])) {
+    run_short<T, MUON>(s, g, h, steps, norms);
+    return;
+  }
   const uint32_t tiles = number(g, tiles64);
   hipLaunchKernelGGL((split_kernel<T, MUON>), dim3(tiles), dim3(kBlock), 0, st, g, h, norms);
   Plan plan(g, num_compute_units(s));
@@ -653,42 +1006,49 @@ void run_group(THCState* s, Group& g, const Update& h, int steps, char* work, do
   }
 }
 
-// Matrices by as many as a launch's arguments hold and a pass's workspace has room for; that is taken before the first launch.
+// Matrices, short and others, by as many as a launch's arguments hold and a pass's workspace has room for; that is taken before the first launch.
 template <typename T, bool MUON>
 void run(THCState* s, const std::vector<Matrix>& all, const Update& h, int steps) {
   std::vector<Group> groups;
-  Bytes most{0, 0}, sum{0, 0};
-  auto add = [&](const Matrix& a) {
-    const Bytes b = bytes_of(a);
-    if (groups.empty() || groups.back().count == kMatrices || sum.work + b.work > kPassBytes) {
-      groups.emplace_back();
-      groups.back().count = 0;
-      sum = Bytes{0, 0};
-    }
-    Group& g = groups.back();
-    g.matrix[g.count++] = a;
-    sum.work += b.work;
-    sum.norms += b.norms;
-    most.work = std::max(most.work, sum.work);
-    most.norms = std::max(most.norms, sum.norms);
-  };
-  for (const Matrix& a : all) {
-    // a batch in pieces
-    const int64_t each = std::max<int64_t>(1, kPassBytes / work_bytes(a)), size = (int64_t)a.m * a.n;
-    for (int64_t first = 0; first < a.batch; first += each) {
-      Matrix piece = a;
-      piece.batch = (int32_t)std::min<int64_t>(each, a.batch - first);
-      piece.in = static_cast<const T*>(a.in) + first * size;
-      piece.out = static_cast<T*>(a.out) + first * size;
-      if (a.momentum) piece.momentum = a.momentum + first * size;
-      if (a.master) piece.master = a.master + first * size;
-      add(piece);
+  Bytes most{0, 0};
+  for (bool few : {true, false}) {
+    Bytes sum{0, 0};
+    bool open = false;
+    auto add = [&](const Matrix& a) {
+      const Bytes b = bytes_of(a);
+      if (!open || groups.back().count == kMatrices || sum.work + b.work > kPassBytes) {
+        groups.emplace_back();
+        groups.back().count = 0;
+        sum = Bytes{0, 0};
+        open = true;
+      }
+      Group& g = groups.back();
+      g.matrix[g.count++] = a;
+      sum.work += b.work;
+      sum.norms += b.norms;
+      most.work = std::max(most.work, sum.work);
+      most.norms = std::max(most.norms, sum.norms);
+    };
+    for (const Matrix& a : all) {
+      if (is_short(a) != few) continue;
+      // a batch in pieces: by the workspace, and by what the workgroups of a launch are counted in
+      const int64_t size = (int64_t)a.m * a.n;
+      const int64_t each = std::max<int64_t>(1, std::min<int64_t>(kPassBytes / each_bytes(a), 1 << 20));
+      for (int64_t first = 0; first < a.batch; first += each) {
+        Matrix piece = a;
+        piece.batch = (int32_t)std::min<int64_t>(each, a.batch - first);
+        piece.in = static_cast<const T*>(a.in) + first * size;
+        piece.out = static_cast<T*>(a.out) + first * size;
+        if (a.momentum) piece.momentum = a.momentum + first * size;
+        if (a.master) piece.master = a.master + first * size;
+        add(piece);
+      }
     }
   }
-  if (groups.empty()) return;
   int64_t tails = 8;
-  for (const Group& g : groups) tails = std::max(tails, Plan(g, num_compute_units(s)).bytes());
-  Workspace work(s, most.work), norms(s, most.norms), sums(s, tails);
+  for (const Group& g : groups)
+    if (!is_short(g.matrix[0])) tails = std::max(tails, Plan(g, num_compute_units(s)).bytes());
+  Workspace work(s, std::max<int64_t>(8, most.work)), norms(s, std::max<int64_t>(8, most.norms)), sums(s, tails);
   for (Group& g : groups)
     run_group<T, MUON>(s, g, h, steps, work.data(), reinterpret_cast<double*>(norms.data()), reinterpret_cast<acc16*>(sums.data()));
 }
