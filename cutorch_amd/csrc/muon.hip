@@ -267,8 +267,10 @@ __global__ __launch_bounds__(kBlock) void split_kernel(Group g, Update h, const 
 // multiplied, and there is room for two workgroups a CU. A row's eight 16-byte pieces lie in the order of their number xor half the row's, so that
 // sixteen lanes that read the same piece of neighbouring rows meet all banks. (Blocks of 16 columns, four of which are on their way: 5 % slower, as
 // waves meet at twice as many barriers.)
-constexpr int kTile = 128;
-__host__ __device__ inline int32_t tiles_of(int32_t n) { return (n + kTile - 1) / kTile; }
+// Few matrices of some hundred rows would leave most CUs idle with that: they take tiles of 64 x 64, a wave's part 32 x 32, three blocks on their way. The
+// sums of an element are the same ones.
+constexpr int kTile = 128, kSmallTile = 64;
+__host__ __device__ inline int32_t tiles_of(int32_t n, int32_t tile) { return (n + tile - 1) / tile; }
 
 __device__ __forceinline__ uint4v resource(const void* p, uint32_t bytes) {
   const uint64_t a = reinterpret_cast<uint64_t>(p);
@@ -283,7 +285,11 @@ __device__ __forceinline__ uint4v resource(const void* p, uint32_t bytes) {
 __device__ __forceinline__ void load_to_lds(uint4v from, uint32_t laneOffset, uint32_t offset, uint32_t lds) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(lds), "v"(laneOffset), "s"(from), "s"(offset) : "memory");
 }
-__device__ __forceinline__ void wait_loads_and_barrier() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+// Until at most N of this wave's loads are on their way, then until all waves are there.
+template <int N>
+__device__ __forceinline__ void wait_loads_and_barrier() {
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
+}
 
 struct Operand {
   const char* rows;      // of the tile's first row
@@ -299,54 +305,66 @@ __host__ __device__ inline int32_t sum_parts(int32_t blocks, uint32_t tiles) {
 }
 __host__ __device__ inline int32_t part_begin(int32_t blocks, int32_t parts, int32_t k) { return (int32_t)((int64_t)blocks * k / parts); }
 
-constexpr int kStages = 2, kStageBytes = 2 * kTile * kBlockBytes, kOperandBytes = kTile * kBlockBytes;
-// Adds the parts first ... last - 1 of `parts` to `total`.
+template <int TILE>
+struct Stages {
+  static constexpr int kCount = TILE == kTile ? 2 : 4, kOperand = TILE * kBlockBytes, kBytes = 2 * kOperand;
+};
+// Adds the parts first ... last - 1 of `parts` to `total`, products of 32 x 32 of which a wave has W x W.
+template <int TILE, int W = TILE / 64>
 __device__ __forceinline__ void product(const Operand& P, const Operand& Q, int32_t blocks, int32_t parts, int32_t first, int32_t last, char* lds,
-                                        acc16 (&total)[2][2]) {
+                                        acc16 (&total)[W][W]) {
+  constexpr int kStages = Stages<TILE>::kCount, kStageBytes = Stages<TILE>::kBytes, kOperandBytes = Stages<TILE>::kOperand;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const uint32_t base = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)lds;
-  const uint4v fromP = resource(P.rows, (uint32_t)min(P.count, kTile) * (uint32_t)P.rowBytes), fromQ = resource(Q.rows, (uint32_t)min(Q.count, kTile) * (uint32_t)Q.rowBytes);
-  // 16 KiB of an operand are 16 loads of a wave, 8 rows each; wave w has those with numbers w, w + 4, ...
-  uint32_t offP[4], offQ[4];
+  const uint4v fromP = resource(P.rows, (uint32_t)min(P.count, TILE) * (uint32_t)P.rowBytes), fromQ = resource(Q.rows, (uint32_t)min(Q.count, TILE) * (uint32_t)Q.rowBytes);
+  // an operand's block is loads of a wave of 8 rows each; wave w has those with numbers w, w + 4, ...
+  constexpr int U = TILE / 32;
+  uint32_t offP[U], offQ[U];
 #pragma unroll
-  for (int q = 0; q < 4; ++q) {
+  for (int q = 0; q < U; ++q) {
     const int32_t row = (q * 4 + wave) * 8 + (lane >> 3), piece = (lane & 7) ^ ((row >> 1) & 7);
     offP[q] = (uint32_t)min(row, P.count - 1) * (uint32_t)P.rowBytes + piece * 16;
     offQ[q] = (uint32_t)min(row, Q.count - 1) * (uint32_t)Q.rowBytes + piece * 16;
   }
   auto load = [&](int32_t k, uint32_t stage) {
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
+    for (int q = 0; q < U; ++q) {
       const uint32_t to = __builtin_amdgcn_readfirstlane(base + stage * kStageBytes + (q * 4 + wave) * 1024);
       load_to_lds(fromP, offP[q], k * kBlockBytes, to);
       load_to_lds(fromQ, offQ[q], k * kBlockBytes, to + kOperandBytes);
     }
   };
-  const int rowP = ((wave >> 1) * 64 + (lane & 31)) * kBlockBytes, rowQ = ((wave & 1) * 64 + (lane & 31)) * kBlockBytes + kOperandBytes;
-  acc16 acc[2][2] = {};
+  const int rowP = ((wave >> 1) * (TILE / 2) + (lane & 31)) * kBlockBytes, rowQ = ((wave & 1) * (TILE / 2) + (lane & 31)) * kBlockBytes + kOperandBytes;
+  acc16 acc[W][W] = {};
   int32_t part = first, until = part_begin(blocks, parts, first + 1);
   const int32_t begin = part_begin(blocks, parts, first), end = part_begin(blocks, parts, last);
-  load(begin, 0);
+#pragma unroll
+  for (int k = 0; k < kStages - 1; ++k)
+    if (begin + k < end) load(begin + k, k);
+  uint32_t stage = 0;
   for (int32_t k = begin; k < end; ++k) {
     if (k == until) {
       until = part_begin(blocks, parts, ++part + 1);
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        total[q >> 1][q & 1] += acc[q >> 1][q & 1];
-        acc[q >> 1][q & 1] = acc16{};
+      for (int q = 0; q < W * W; ++q) {
+        total[q / W][q % W] += acc[q / W][q % W];
+        acc[q / W][q % W] = acc16{};
       }
     }
-    const uint32_t stage = (uint32_t)(k - begin) & 1;
-    wait_loads_and_barrier();
-    if (k + 1 < end) load(k + 1, stage ^ 1);      // (whose room was read last before the barrier)
+    // this block is there when only the later ones' loads are on their way; the one that is asked for now takes the room that was read last before
+    // the barrier
+    if (kStages > 2 && k + kStages - 2 < end) wait_loads_and_barrier<2 * U * (kStages - 2)>();
+    else wait_loads_and_barrier<0>();
+    if (k + kStages - 1 < end) load(k + kStages - 1, stage == 0 ? kStages - 1 : stage - 1);
     const char *fp = lds + stage * kStageBytes + rowP, *fq = lds + stage * kStageBytes + rowQ;
+    stage = stage == kStages - 1 ? 0 : stage + 1;
     // all of the block's operands are asked for before the first product (2 % quicker than by halves)
-    half8 ph[2][2], pl[2][2], qh[2][2], ql[2][2];
+    half8 ph[2][W], pl[2][W], qh[2][W], ql[2][W];
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
       const int swizzle = (lane >> 1) & 7, high = ((2 * s + (lane >> 5)) ^ swizzle) * 16, low = ((4 + 2 * s + (lane >> 5)) ^ swizzle) * 16;
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
+      for (int i = 0; i < W; ++i) {
         ph[s][i] = *reinterpret_cast<const half8*>(fp + i * 32 * kBlockBytes + high);
         qh[s][i] = *reinterpret_cast<const half8*>(fq + i * 32 * kBlockBytes + high);
         ql[s][i] = *reinterpret_cast<const half8*>(fq + i * 32 * kBlockBytes + low);
@@ -354,12 +372,12 @@ __device__ __forceinline__ void product(const Operand& P, const Operand& Q, int3
       }
     }
     __builtin_amdgcn_sched_barrier(0);
-    // products into the same sums lie four apart
-    auto products = [&](const half8 (&p)[2], const half8 (&q)[2]) {
+    // products into the same sums lie W x W apart
+    auto products = [&](const half8 (&p)[W], const half8 (&q)[W]) {
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
+      for (int i = 0; i < W; ++i)
 #pragma unroll
-        for (int j = 0; j < 2; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(p[i], q[j], acc[i][j], 0, 0, 0);
+        for (int j = 0; j < W; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(p[i], q[j], acc[i][j], 0, 0, 0);
     };
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
@@ -369,14 +387,14 @@ __device__ __forceinline__ void product(const Operand& P, const Operand& Q, int3
     }
   }
 #pragma unroll
-  for (int q = 0; q < 4; ++q) total[q >> 1][q & 1] += acc[q >> 1][q & 1];
+  for (int q = 0; q < W * W; ++q) total[q / W][q % W] += acc[q / W][q % W];
 }
 
 enum Op { kGram, kPolynomial, kStep, kLast };
 
 __host__ __device__ inline uint32_t symmetric_tiles(int32_t t) { return (uint32_t)(t * (int64_t)(t + 1) / 2); }
-__host__ __device__ inline uint32_t product_tiles(const Matrix& a, bool symmetric) {
-  return symmetric ? symmetric_tiles(tiles_of(a.m)) : (uint32_t)(tiles_of(a.m) * (int64_t)tiles_of(a.n));
+__host__ __device__ inline uint32_t product_tiles(const Matrix& a, bool symmetric, int32_t tile = kTile) {
+  return symmetric ? symmetric_tiles(tiles_of(a.m, tile)) : (uint32_t)(tiles_of(a.m, tile) * (int64_t)tiles_of(a.n, tile));
 }
 
 // Tiles in an order in which neighbours share operands: bands of eight rows of them, column by column.
@@ -430,23 +448,25 @@ __device__ __forceinline__ void eight_of(T* at, int32_t count, F f) {
 // One of a step's three products and what is made of it. The first two are symmetric: tiles above the diagonal go to both places. `turn`: which of the
 // two pairs of planes X is in. The last step's result goes to the tensor, or into the parameter. The sums pass through LDS, so that memory sees whole
 // packs of neighbouring elements in both directions.
-constexpr int kProductLds = kTile * (kTile + 4) * 4;
-static_assert(kStages * kStageBytes <= kProductLds, "blocks and sums take turns");
 // The last tiles, which would leave much of the chip idle, are cut into the parts of their sums: a workgroup for each leaves its sums in memory, and a
 // launch behind this one (JOIN) adds them up and goes on from there.
 struct Tail {
   uint32_t whole;      // tiles before them
   int32_t parts;       // 1: none are cut
-  acc16* sums;         // of each part: 4 products of each of 256 lanes
+  acc16* sums;         // of each part: the products of each of 256 lanes
 };
-template <int OP, typename T, bool MUON, bool JOIN>
+template <int OP, typename T, bool MUON, bool JOIN, int TILE>
 __global__ __launch_bounds__(256, 2) void product_kernel(Group g, Update h, int turn, Tail tail) {
-  __shared__ __attribute__((aligned(128))) char lds[kProductLds];
+  // (the joining launch has a workgroup for each wave's quarter of a large tile: one CU alone would wait long for what all parts left)
+  constexpr int W = TILE / 64, kQuarters = JOIN ? W * W : 1, kSpan = JOIN ? 64 : TILE;
+  constexpr int kStride = kSpan + 4;      // floats: columns of sums, four rows at once, meet all banks
+  constexpr int kSums = kSpan * kStride * 4, kBlocks = JOIN ? 0 : Stages<TILE>::kCount * Stages<TILE>::kBytes;
+  __shared__ __attribute__((aligned(128))) char lds[kSums > kBlocks ? kSums : kBlocks];
   constexpr bool kSymmetric = OP == kGram || OP == kPolynomial;
-  const uint32_t unit = JOIN ? blockIdx.x >> 2 : by_die(blockIdx.x, gridDim.x);
+  const uint32_t unit = JOIN ? blockIdx.x / kQuarters : by_die(blockIdx.x, gridDim.x), quarter = blockIdx.x % kQuarters;
   const bool cut = !JOIN && unit >= tail.whole;
   const uint32_t tile = JOIN ? tail.whole + unit : cut ? tail.whole + (unit - tail.whole) / (uint32_t)tail.parts : unit;
-  const Place p = place_of(g, tile, [](const Matrix& a) { return product_tiles(a, kSymmetric); });
+  const Place p = place_of(g, tile, [](const Matrix& a) { return product_tiles(a, kSymmetric, TILE); });
   const Matrix& a = p.a;
   char* work = a.work + p.batch * work_bytes(a);
   const int64_t px = plane_x(a), pt = plane_t(a);
@@ -455,12 +475,12 @@ __global__ __launch_bounds__(256, 2) void product_kernel(Group g, Update h, int 
   const bool flipped = OP == kLast && a.tall;      // the tensor's rows are the longer side: its tile is the product's transpose
   const int32_t rows = flipped ? a.n : a.m, cols = kSymmetric || flipped ? a.m : a.n;
   int32_t ti, tj;
-  if constexpr (kSymmetric) symmetric_tile_at(p.index, tiles_of(a.m), ti, tj);
-  else tile_at(p.index, tiles_of(rows), tiles_of(cols), ti, tj);
-  // (the joining launch has a workgroup for each wave's quarter of a tile: one CU alone would wait long for what all parts left)
-  constexpr int kSpan = JOIN ? kTile / 2 : kTile, kStride = kSpan + 4;      // floats: columns of sums, four rows at once, meet all banks
-  const int32_t i0 = ti * kTile + (JOIN ? (int32_t)(blockIdx.x >> 1 & 1) * kSpan : 0), j0 = tj * kTile + (JOIN ? (int32_t)(blockIdx.x & 1) * kSpan : 0);
-  if (JOIN && (i0 >= rows || j0 >= cols)) return;
+  if constexpr (kSymmetric) symmetric_tile_at(p.index, tiles_of(a.m, TILE), ti, tj);
+  else tile_at(p.index, tiles_of(rows, TILE), tiles_of(cols, TILE), ti, tj);
+  const int32_t i0 = ti * TILE + (int32_t)(quarter >> 1) * kSpan, j0 = tj * TILE + (int32_t)(quarter & 1) * kSpan;
+  if (JOIN && (i0 >= rows || j0 >= cols || (kSymmetric && i0 > j0))) return;
+  // Symmetric products hold each of their elements once: above the diagonal. (Element (j, i) sums its lower halves' products the other way round.)
+  const bool diagonal = kSymmetric && i0 == j0;
   const char *from, *with;
   int64_t bytesK;
   if constexpr (OP == kGram) {
@@ -475,33 +495,34 @@ __global__ __launch_bounds__(256, 2) void product_kernel(Group g, Update h, int 
   // The sums as columns: a lane has column `lane % 32` of each 32 x 32 product, four rows in a row of each eight.
   float* sums = reinterpret_cast<float*>(lds);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  auto keep = [&](int quarter, int q, const acc16& acc) {
+  auto keep = [&](int down, int over, const acc16& acc) {      // 32 x 32 at these times 32
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      const int i = (quarter >> 1) * 64 + (q >> 1) * 32 + r * 8 + (lane >> 5) * 4, j = (quarter & 1) * 64 + (q & 1) * 32 + (lane & 31);
+      const int i = down * 32 + r * 8 + (lane >> 5) * 4, j = over * 32 + (lane & 31);
       *reinterpret_cast<Pack<float, 4>*>(sums + j * kStride + i) = Pack<float, 4>{acc[r * 4], acc[r * 4 + 1], acc[r * 4 + 2], acc[r * 4 + 3]};
     }
   };
   if constexpr (JOIN) {
-    // (a wave for each of the four products)
-    const acc16* from16 = tail.sums + (int64_t)unit * tail.parts * 1024 + wave * 256 + (blockIdx.x & 3) * 64 + lane;
+    // each of the four waves has one of the 2 x 2 products of 64 x 64
+    constexpr int kEach = W * W * 256;
+    const acc16* from16 = tail.sums + (int64_t)unit * tail.parts * kEach + (W == 2 ? wave * 256 + quarter * 64 : wave * 64) + lane;
     acc16 acc = {};
 #pragma unroll 8
-    for (int k = 0; k < tail.parts; ++k) acc += from16[k * 1024];
-    keep(0, wave, acc);
+    for (int k = 0; k < tail.parts; ++k) acc += from16[k * kEach];
+    keep(wave >> 1, wave & 1, acc);
   } else {
     const int32_t blocks = (int32_t)(bytesK / kBlockBytes), parts = sum_parts(blocks, product_tiles(a, kSymmetric)), part = cut ? (int32_t)((unit - tail.whole) % (uint32_t)tail.parts) : 0;
-    acc16 acc[2][2] = {};
-    product(P, Q, blocks, parts, part, cut ? part + 1 : parts, lds, acc);
+    acc16 acc[W][W] = {};
+    product<TILE>(P, Q, blocks, parts, part, cut ? part + 1 : parts, lds, acc);
     if (cut) {
-      acc16* to16 = tail.sums + (int64_t)(unit - tail.whole) * 1024 + threadIdx.x;
+      acc16* to16 = tail.sums + (int64_t)(unit - tail.whole) * (W * W * 256) + threadIdx.x;
 #pragma unroll
-      for (int q = 0; q < 4; ++q) to16[q * 256] = acc[q >> 1][q & 1];
+      for (int q = 0; q < W * W; ++q) to16[q * 256] = acc[q / W][q % W];
       return;
     }
     __syncthreads();
 #pragma unroll
-    for (int q = 0; q < 4; ++q) keep(wave, q, acc[q >> 1][q & 1]);
+    for (int q = 0; q < W * W; ++q) keep((wave >> 1) * W + q / W, (wave & 1) * W + q % W, acc[q / W][q % W]);
   }
   __syncthreads();
   // Rows: a thread has eight columns of every kRows-th row. (Few of these steps at a time: each of their instructions runs but a few times, and has
@@ -519,7 +540,8 @@ __global__ __launch_bounds__(256, 2) void product_kernel(Group g, Update h, int 
     float v[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const float sum = sums[(jt + e) * kStride + it + u];
+      const int column = jt + e, row = it + u;
+      const float sum = diagonal && row > column ? sums[row * kStride + column] : sums[column * kStride + row];
       if constexpr (OP == kGram) {
         v[e] = sum * (kScaleA / (a.scale * a.scale));
       } else {
@@ -546,14 +568,14 @@ __global__ __launch_bounds__(256, 2) void product_kernel(Group g, Update h, int 
       }
     } else {
       if (i < rows && j < colEnd) store_eight((OP == kGram ? am : OP == kPolynomial ? bm : xn) + split_at(i, j, OP == kStep ? bytesN : bytesM), v);
-      if (OP == kStep || ti != tj) {
+      if (!diagonal) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) sums[(jt + e) * kStride + it + u] = v[e];
       }
     }
   }
   if constexpr (OP != kLast) {
-    if (OP != kStep && ti == tj) return;
+    if (diagonal) return;
     __syncthreads();
     // and columns, in the same way
     char* mirrored = OP == kGram ? am : OP == kPolynomial ? bm : tn;
@@ -576,7 +598,7 @@ __global__ __launch_bounds__(256, 2) void product_kernel(Group g, Update h, int 
 // takes its strip through the step and leaves the strip's share of the next A: one launch a step, and one for all steps where X is a single strip.
 // LDS: one plane for A, then B, then the new X, a second one for the strip's transpose, both split, rows of 16-byte pieces in the order of their
 // number xor what brings sixteen rows to different banks.
-constexpr int kShortThreads = 1024, kFewStrips = 8;
+constexpr int kShortThreads = 1024;
 __host__ __device__ inline bool is_short(const Matrix& a) { return a.m <= kShort; }
 __host__ __device__ inline int32_t strips_of(const Matrix& a) { return (a.n + kStrip - 1) / kStrip; }
 __host__ __device__ inline int32_t bands_of(const Matrix& a) { return (a.m + 31) / 32; }
@@ -823,7 +845,7 @@ __global__ __launch_bounds__(kShortThreads) void short_begin_kernel(Group g, Upd
   }
 }
 
-// The sum of many strips' shares of A, before the step that takes it.
+// The sum of the strips' shares of A, before the step that takes it: where each strip's workgroup would read many of them. (The order is the same.)
 constexpr int kShareThreads = 64;
 __host__ __device__ inline uint32_t share_parts(const Matrix& a) { return (uint32_t)(gram_bytes(a) / 16 / kShareThreads); }
 __global__ __launch_bounds__(kShareThreads) void shares_kernel(Group g, int turn) {
@@ -842,7 +864,7 @@ __global__ __launch_bounds__(kShareThreads) void shares_kernel(Group g, int turn
 }
 
 template <typename T, bool MUON, bool LAST>
-__global__ __launch_bounds__(kShortThreads) void short_step_kernel(Group g, Update h, int turn) {
+__global__ __launch_bounds__(kShortThreads) void short_step_kernel(Group g, Update h, int turn, bool summed) {
   extern __shared__ __attribute__((aligned(256))) char lds[];
   const Place p = place_of(g, blockIdx.x, [](const Matrix& a) { return (uint32_t)strips_of(a); });
   const Matrix& a = p.a;
@@ -859,11 +881,11 @@ __global__ __launch_bounds__(kShortThreads) void short_step_kernel(Group g, Upda
   }
   const int strips = strips_of(a);
   const int64_t bytes = gram_bytes(a);
-  const char* shares = work + plane_t(a) + (strips > kFewStrips ? 2 * strips : turn * strips) * bytes;
+  const char* shares = work + plane_t(a) + (summed ? 2 * strips : turn * strips) * bytes;
   acc16 sums = {}, x = {};
   strip.each(strip.bands, strip.bands, [&](int ti, int tj) {
     const acc16* mine = reinterpret_cast<const acc16*>(shares) + (ti * strip.bands + tj) * 64 + strip.lane;
-    for (int k = 0; k < (strips > kFewStrips ? 1 : strips); ++k) sums += mine[k * (bytes / 64)];
+    for (int k = 0; k < (summed ? 1 : strips); ++k) sums += mine[k * (bytes / 64)];
   });
 #pragma unroll
   for (int q = 0; q < 4; ++q) {
@@ -908,63 +930,75 @@ struct Bytes {
 int64_t each_bytes(const Matrix& a) { return is_short(a) ? short_bytes(a) : work_bytes(a); }
 Bytes bytes_of(const Matrix& a) { return Bytes{each_bytes(a) * a.batch, (int64_t)norm_parts(a) * a.batch * 8}; }
 
-// The tiles of the last round of workgroups, two to a CU, if cutting them saves more than the joining launch costs: by what a block takes a workgroup
-// that has its CU to itself (0.45 us) or shares it (0.7), by that launch and by the sums' way through memory (0.026 us a part of a tile).
-Tail tail_of(const Group& g, int op, int64_t cus) {
-  const uint32_t tiles = g.first[g.count];
-  uint32_t rest = tiles % (uint32_t)(2 * cus);
-  auto blocks = [&](int k) { return (int32_t)blocks_of(op == kGram ? g.matrix[k].n : g.matrix[k].m); };
-  auto parts_of = [&](int k) { return sum_parts(blocks(k), product_tiles(g.matrix[k], op == kGram || op == kPolynomial)); };
-  Tail t{tiles, 1, nullptr};
-  const int32_t most = blocks(g.count - 1), parts = parts_of(g.count - 1);
-  int k = g.count - 1;
-  while (k > 0 && parts_of(k - 1) == parts) --k;
-  rest = std::min(rest, tiles - g.first[k]);
-  if (rest == 0 || parts == 1) return t;
-  auto cost = [&](int64_t units, double length) {
-    return (units <= cus ? 0.45 : 0.7 * (double)((units + 2 * cus - 1) / (2 * cus))) * length;
-  };
-  const int64_t units = (int64_t)rest * parts;
-  if (cost(units, (double)most / parts) + 6 + 0.026 * (double)units < cost(rest, most)) {
-    t.whole = tiles - rest;
-    t.parts = parts;
+// One of a step's products over a group: its tiles, numbered, and which of them are cut.
+struct Launch {
+  Group g;
+  int32_t tile;
+  Tail tail;
+  // Small tiles where large ones would be fewer than three for four CUs. us with large and with small ones: one matrix of 256 x 256 268, 124, of 512 x 512 362,
+  // 173, of 1024 x 1024 529, 260, of 1024 x 4096 (whose step has 256 large ones) 524, 535; eight of 512 x 512 380, 218.
+  // Cut are the tiles of the last round of workgroups, two to a CU, if that saves more than the joining launch costs: by what a block takes a
+  // workgroup that has its CU to itself (0.45 us, small tiles 0.2) or shares it (0.7, 0.25), by that launch and by the sums' way through memory (0.026 us,
+  // 0.007, a part of a tile).
+  Launch(const Group& from, int op, int64_t cus) : g(from) {
+    const bool symmetric = op == kGram || op == kPolynomial;
+    const uint32_t large = number(g, [&](const Matrix& a) { return product_tiles(a, symmetric); });
+    tile = (int64_t)large * 4 <= 3 * cus ? kSmallTile : kTile;
+    const uint32_t tiles = tile == kTile ? large : number(g, [&](const Matrix& a) { return product_tiles(a, symmetric, kSmallTile); });
+    auto blocks = [&](int k) { return (int32_t)blocks_of(op == kGram ? g.matrix[k].n : g.matrix[k].m); };
+    auto parts_of = [&](int k) { return sum_parts(blocks(k), product_tiles(g.matrix[k], symmetric)); };
+    tail = Tail{tiles, 1, nullptr};
+    const int32_t most = blocks(g.count - 1), parts = parts_of(g.count - 1);
+    int k = g.count - 1;
+    while (k > 0 && parts_of(k - 1) == parts) --k;
+    const uint32_t rest = std::min(tiles % (uint32_t)(2 * cus), tiles - g.first[k]);
+    if (rest == 0 || parts == 1) return;
+    const bool small = tile == kSmallTile;
+    auto cost = [&](int64_t units, double length) {
+      return (units <= cus ? (small ? 0.2 : 0.45) : (small ? 0.25 : 0.7) * (double)((units + 2 * cus - 1) / (2 * cus))) * length;
+    };
+    const int64_t units = (int64_t)rest * parts;
+    if (cost(units, (double)most / parts) + 6 + (small ? 0.007 : 0.026) * (double)units < cost(rest, most)) {
+      tail.whole = tiles - rest;
+      tail.parts = parts;
+    }
   }
-  return t;
-}
-int64_t tail_bytes(const Group& g, const Tail& t) { return t.parts > 1 ? (int64_t)(g.first[g.count] - t.whole) * t.parts * kTile * kTile * 4 : 0; }
-
-template <int OP, typename T, bool MUON>
-void launch_product(THCState* s, const Group& g, const Update& h, int turn, const Tail& tail) {
-  hipStream_t st = current_stream(s);
-  const uint32_t rest = g.first[g.count] - tail.whole;
-  hipLaunchKernelGGL((product_kernel<OP, T, MUON, false>), dim3(tail.whole + rest * tail.parts), dim3(256), 0, st, g, h, turn, tail);
-  if (rest) hipLaunchKernelGGL((product_kernel<OP, T, MUON, true>), dim3(rest * 4), dim3(256), 0, st, g, h, turn, tail);
-}
-
-// The products' numbers of workgroups and tails.
+  uint32_t rest() const { return g.first[g.count] - tail.whole; }
+  int64_t bytes() const { return (int64_t)rest() * tail.parts * tile * tile * 4; }
+  template <int OP, typename T, bool MUON>
+  void go(THCState* s, const Update& h, int turn) const {
+    if (tile == kTile) go_tiles<OP, T, MUON, kTile>(s, h, turn);
+    else go_tiles<OP, T, MUON, kSmallTile>(s, h, turn);
+  }
+  template <int OP, typename T, bool MUON, int TILE>
+  void go_tiles(THCState* s, const Update& h, int turn) const {
+    hipStream_t st = current_stream(s);
+    const dim3 grid(tail.whole + rest() * tail.parts), joins(rest() * (TILE / 64) * (TILE / 64));
+    hipLaunchKernelGGL((product_kernel<OP, T, MUON, false, TILE>), grid, dim3(256), 0, st, g, h, turn, tail);
+    if (rest()) hipLaunchKernelGGL((product_kernel<OP, T, MUON, true, TILE>), joins, dim3(256), 0, st, g, h, turn, tail);
+  }
+};
 struct Plan {
-  Group symmetric, full;
-  Tail gram, polynomial, step;
-  Plan(const Group& g, int64_t cus) : symmetric(g), full(g) {
-    number(symmetric, [](const Matrix& a) { return product_tiles(a, true); });
-    number(full, [](const Matrix& a) { return product_tiles(a, false); });
-    gram = tail_of(symmetric, kGram, cus);
-    polynomial = tail_of(symmetric, kPolynomial, cus);
-    step = tail_of(full, kStep, cus);
-  }
-  int64_t bytes() const { return std::max({tail_bytes(symmetric, gram), tail_bytes(symmetric, polynomial), tail_bytes(full, step)}); }
+  Launch gram, polynomial, step;
+  Plan(const Group& g, int64_t cus) : gram(g, kGram, cus), polynomial(g, kPolynomial, cus), step(g, kStep, cus) {}
+  int64_t bytes() const { return std::max({gram.bytes(), polynomial.bytes(), step.bytes()}); }
 };
 
 template <typename T, bool MUON>
 void run_short(THCState* s, Group& g, const Update& h, int steps, const double* norms) {
   hipStream_t st = current_stream(s);
-  int bands = 0;
-  bool many = false, whole = true;
+  int bands = 0, most = 0;
+  bool whole = true;
+  int64_t read = 0;
   for (int k = 0; k < g.count; ++k) {
-    whole = whole && is_alone(g.matrix[k]);
-    bands = std::max(bands, bands_of(g.matrix[k]));
-    many = many || strips_of(g.matrix[k]) > kFewStrips;
+    const Matrix& a = g.matrix[k];
+    whole = whole && is_alone(a);
+    bands = std::max(bands, bands_of(a));
+    most = std::max(most, strips_of(a));
+    read += (int64_t)a.batch * strips_of(a) * strips_of(a) * gram_bytes(a);
   }
+  // (12 matrices of 65 x 513, 5 strips and 11 MB of shares: 97 us without the sums' launches, XX with; 40 of 100 x 1000, 8 strips and 168 MB: 329, YY)
+  const bool many = most > 8 || read > (int64_t(24) << 20);
   const int lds = short_lds(bands);
   const dim3 threads(kShortThreads);
   Group shares = g;
@@ -981,8 +1015,8 @@ void run_short(THCState* s, Group& g, const Update& h, int steps, const double* 
   hipLaunchKernelGGL(roomy(short_begin_kernel<T, MUON, false>), strips, threads, lds, st, g, h, norms, steps);
   for (int k = 0; k < steps; ++k) {
     if (many) hipLaunchKernelGGL(shares_kernel, dim3(parts), dim3(kShareThreads), 0, st, shares, k & 1);
-    if (k + 1 < steps) hipLaunchKernelGGL(roomy(short_step_kernel<float, false, false>), strips, threads, lds, st, g, h, k & 1);
-    else hipLaunchKernelGGL(roomy(short_step_kernel<T, MUON, true>), strips, threads, lds, st, g, h, k & 1);
+    if (k + 1 < steps) hipLaunchKernelGGL(roomy(short_step_kernel<float, false, false>), strips, threads, lds, st, g, h, k & 1, many);
+    else hipLaunchKernelGGL(roomy(short_step_kernel<T, MUON, true>), strips, threads, lds, st, g, h, k & 1, many);
   }
 }
 
@@ -1003,13 +1037,13 @@ void run_group(THCState* s, Group& g, const Update& h, int steps, char* work, do
   const uint32_t tiles = number(g, tiles64);
   hipLaunchKernelGGL((split_kernel<T, MUON>), dim3(tiles), dim3(kBlock), 0, st, g, h, norms);
   Plan plan(g, num_compute_units(s));
-  plan.gram.sums = plan.polynomial.sums = plan.step.sums = sums;
+  plan.gram.tail.sums = plan.polynomial.tail.sums = plan.step.tail.sums = sums;
   for (int k = 0; k < steps; ++k) {
     const int turn = k & 1;
-    launch_product<kGram, float, false>(s, plan.symmetric, h, turn, plan.gram);
-    launch_product<kPolynomial, float, false>(s, plan.symmetric, h, turn, plan.polynomial);
-    if (k + 1 < steps) launch_product<kStep, float, false>(s, plan.full, h, turn, plan.step);
-    else launch_product<kLast, T, MUON>(s, plan.full, h, turn, plan.step);
+    plan.gram.go<kGram, float, false>(s, h, turn);
+    plan.polynomial.go<kPolynomial, float, false>(s, h, turn);
+    if (k + 1 < steps) plan.step.go<kStep, float, false>(s, h, turn);
+    else plan.step.go<kLast, T, MUON>(s, h, turn);
   }
 }
 
