@@ -540,8 +540,8 @@ __global__ __launch_bounds__(256, 2) void product_kernel(Group g, Update h, int 
     float v[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const int column = jt + e, row = it + u;
-      const float sum = diagonal && row > column ? sums[row * kStride + column] : sums[column * kStride + row];
+      float sum = sums[(jt + e) * kStride + it + u];
+      if (kSymmetric && diagonal && it + u > jt + e) sum = sums[(it + u) * kStride + jt + e];
       if constexpr (OP == kGram) {
         v[e] = sum * (kScaleA / (a.scale * a.scale));
       } else {
@@ -930,38 +930,49 @@ struct Bytes {
 int64_t each_bytes(const Matrix& a) { return is_short(a) ? short_bytes(a) : work_bytes(a); }
 Bytes bytes_of(const Matrix& a) { return Bytes{each_bytes(a) * a.batch, (int64_t)norm_parts(a) * a.batch * 8}; }
 
-// One of a step's products over a group: its tiles, numbered, and which of them are cut.
+// What workgroups that each multiply `blocks` blocks take, us, as measured with one matrix of 256 to 4096 rows: up to one to a CU, or rounds of two to each.
+double product_time(int32_t tile, double blocks, int64_t units, int64_t cus, bool cut) {
+  const double fixed = tile == kTile ? (cut ? 5 : 11) : (cut ? 3 : 6);      // (parts have no results to write)
+  if (units <= cus) return (tile == kTile ? 0.74 : 0.325) * blocks + fixed;
+  return (double)((units + 2 * cus - 1) / (2 * cus)) * ((tile == kTile ? 1.08 : 0.43) * blocks + fixed);
+}
+
+// One of a step's products over a group: its tiles, numbered, and which of them are cut: those of the last round of workgroups, if that saves more than
+// the joining launch costs. Large or small tiles by what they take. us with large, large and cut, small, small and cut ones: A of 256 x 256
+// 17, -, 8, -; of 512 x 2048 55, 23, 26, 17; of 1024 x 1024 33, 24, 16, 20; of 2048 x 8192 198, 111, 181, 133; of 4096 x 4096 235, 161, 243, 215.
 struct Launch {
   Group g;
   int32_t tile;
   Tail tail;
-  // Small tiles where large ones would be fewer than three for four CUs. us with large and with small ones: one matrix of 256 x 256 268, 124, of 512 x 512 362,
-  // 173, of 1024 x 1024 529, 260, of 1024 x 4096 (whose step has 256 large ones) 524, 535; eight of 512 x 512 380, 218.
-  // Cut are the tiles of the last round of workgroups, two to a CU, if that saves more than the joining launch costs: by what a block takes a
-  // workgroup that has its CU to itself (0.45 us, small tiles 0.2) or shares it (0.7, 0.25), by that launch and by the sums' way through memory (0.026 us,
-  // 0.007, a part of a tile).
   Launch(const Group& from, int op, int64_t cus) : g(from) {
     const bool symmetric = op == kGram || op == kPolynomial;
-    const uint32_t large = number(g, [&](const Matrix& a) { return product_tiles(a, symmetric); });
-    tile = (int64_t)large * 4 <= 3 * cus ? kSmallTile : kTile;
-    const uint32_t tiles = tile == kTile ? large : number(g, [&](const Matrix& a) { return product_tiles(a, symmetric, kSmallTile); });
     auto blocks = [&](int k) { return (int32_t)blocks_of(op == kGram ? g.matrix[k].n : g.matrix[k].m); };
     auto parts_of = [&](int k) { return sum_parts(blocks(k), product_tiles(g.matrix[k], symmetric)); };
-    tail = Tail{tiles, 1, nullptr};
-    const int32_t most = blocks(g.count - 1), parts = parts_of(g.count - 1);
-    int k = g.count - 1;
-    while (k > 0 && parts_of(k - 1) == parts) --k;
-    const uint32_t rest = std::min(tiles % (uint32_t)(2 * cus), tiles - g.first[k]);
-    if (rest == 0 || parts == 1) return;
-    const bool small = tile == kSmallTile;
-    auto cost = [&](int64_t units, double length) {
-      return (units <= cus ? (small ? 0.2 : 0.45) : (small ? 0.25 : 0.7) * (double)((units + 2 * cus - 1) / (2 * cus))) * length;
+    const int32_t parts = parts_of(g.count - 1);
+    int same = g.count - 1;      // the first of the matrices at the end whose sums have as many parts
+    while (same > 0 && parts_of(same - 1) == parts) --same;
+    auto plan = [&](int32_t t, Tail& to) {
+      const uint32_t tiles = number(g, [&](const Matrix& a) { return product_tiles(a, symmetric, t); });
+      double length = 0;
+      for (int k = 0; k < g.count; ++k) length += (double)blocks(k) * (g.first[k + 1] - g.first[k]) / tiles;
+      const uint32_t last = tiles % (uint32_t)(2 * cus), rest = std::min(last, tiles - g.first[same]);
+      const double rounds = product_time(t, length, tiles - last, cus, false);
+      to = Tail{tiles, 1, nullptr};
+      if (last == 0) return rounds;
+      const double tail = (double)blocks(g.count - 1), whole = product_time(t, tail, last, cus, false);
+      const int64_t units = (int64_t)rest * parts;
+      const double cut = product_time(t, tail / parts, units, cus, true) + 7 + (t == kTile ? 0.014 : 0.002) * (double)units;
+      const bool cuts = parts > 1 && rest == last && cut < whole;
+      if (cuts) {
+        to.whole = tiles - rest;
+        to.parts = parts;
+      }
+      return (tiles > last ? rounds : 0) + (cuts ? cut : whole);
     };
-    const int64_t units = (int64_t)rest * parts;
-    if (cost(units, (double)most / parts) + 6 + (small ? 0.007 : 0.026) * (double)units < cost(rest, most)) {
-      tail.whole = tiles - rest;
-      tail.parts = parts;
-    }
+    Tail large, small;
+    tile = plan(kTile, large) <= plan(kSmallTile, small) ? kTile : kSmallTile;
+    if (tile == kTile) plan(kTile, large);      // (which numbers them)
+    tail = tile == kTile ? large : small;
   }
   uint32_t rest() const { return g.first[g.count] - tail.whole; }
   int64_t bytes() const { return (int64_t)rest() * tail.parts * tile * tile * 4; }
