@@ -209,6 +209,13 @@ void fill_registry() {
   add<void, int, T, T, T, T, T, T, double, double, double, double, double, long, double>("vittttttdddddld");
   add<void, int, T, T, T, T, T, T, T, double, double, double, double, double, long, double>("vitttttttdddddld");
   add<void, int, T, T, T, T, T, T>("vitttttt");
+  add<void, T, T, T, T, double>("vttttd");
+  add<void, T, T, T, T, T, T, double, int>("vttttttdi");
+  add<void, T, T, T, T, double, int, int>("vttttdii");
+  add<void, T, long, double, double, double, double, double>("vtlddddd");
+  add<void, T, T, int, double>("vttid");
+  add<void, int, T, T, T, double, double, double, int, int, double, double, double>("vitttdddiiddd");
+  add<void, int, T, T, T, T, double, double, double, int, int, double, double, double>("vittttdddiiddd");
   add<float, T, float>("ftf");
   add<float, T, Half>("fte");
   add<double, T, double>("dtd");

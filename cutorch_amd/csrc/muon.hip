@@ -1060,7 +1060,9 @@ void run_group(THCState* s, Group& g, const Update& h, int steps, char* work, do
 
 // Matrices, short and others, by as many as a launch's arguments hold and a pass's workspace has room for; that is taken before the first launch.
 template <typename T, bool MUON>
-void run(THCState* s, const std::vector<Matrix>& all, const Update& h, int steps) {
+void run(THCState* s, std::vector<Matrix>& all, const Update& h, int steps) {
+  // (equal ones side by side, long sums first: what is left of a launch at its end is short)
+  std::stable_sort(all.begin(), all.end(), [](const Matrix& a, const Matrix& b) { return a.n != b.n ? a.n > b.n : a.m > b.m; });
   std::vector<Group> groups;
   Bytes most{0, 0};
   for (bool few : {true, false}) {
@@ -1147,8 +1149,9 @@ void orthogonalize(THCState* s, DType dt, AnyTensor* self, AnyTensor* input, int
   Matrix a = matrix_of(input);
   a.in = tensor_data(in.ref.t, dt);
   a.out = tensor_data(out.t, dt);
-  if (dt == DType::F32) run<float, false>(s, {a}, h, steps);
-  else run<__half, false>(s, {a}, h, steps);
+  std::vector<Matrix> all{a};
+  if (dt == DType::F32) run<float, false>(s, all, h, steps);
+  else run<__half, false>(s, all, h, steps);
   THC_CHECK(hipGetLastError());
   note_kernel("orthogonalize");
   if (out.t != self) copy_tensor(s, dt, self, out.t, false);
