@@ -528,6 +528,7 @@ void launch_grad(THCState* s, GradArgs<T>& a, const WeightGrads<T>& to) {
   hipStream_t st = current_stream(s);
   const int64_t cus = num_compute_units(s), packs = (a.dim + V - 1) / V;
   const bool sums = to.weight || to.bias;
+  if (sums || packs > (V == 4 ? 4096 : 2048)) refuse_capture(s, "the gradient of a norm's weights, or of long rows,");
   auto parts = [&](int64_t count, Workspace& w) {
     float* p = reinterpret_cast<float*>(w.data());
     a.weightPart = to.weight ? p : nullptr;
@@ -606,6 +607,7 @@ struct RowInput {
       tensor_retain(t);
       ref.t = t;
     } else {
+      refuse_capture(s, "a norm of rows that lie apart");
       ref.t = tensor_new_contiguous(s, t, dt);
       as_rows(ref.t, &rows);
     }
@@ -631,6 +633,7 @@ struct RowOutput {
       tensor_retain(t);
       ref.t = t;
     } else {
+      refuse_capture(s, "a norm whose output lies apart or on what it reads");
       ref.t = tensor_new_with_size(s, t->nDimension, t->size, d);
       as_rows(ref.t, &rows);
     }
@@ -640,6 +643,12 @@ struct RowOutput {
   }
 };
 
+// A row of numbers for the columns, dense.
+AnyTensor* columns(THCState* s, AnyTensor* t, DType dt) {
+  if (t && !tensor_is_contiguous(t)) refuse_capture(s, "a norm with strided weights");
+  return t ? tensor_new_contiguous(s, t, dt) : nullptr;
+}
+
 template <typename T>
 const T* data_of(const TensorRef& r, DType dt) {
   return r.t ? static_cast<const T*>(tensor_data(r.t, dt)) : nullptr;
@@ -648,7 +657,7 @@ const T* data_of(const TensorRef& r, DType dt) {
 template <typename T>
 void run_norm(THCState* s, DType dt, AnyTensor* self, AnyTensor* input, AnyTensor* weight, AnyTensor* bias, float eps) {
   RowInput x(s, input, dt);
-  TensorRef w(s, weight ? tensor_new_contiguous(s, weight, dt) : nullptr), b(s, bias ? tensor_new_contiguous(s, bias, dt) : nullptr);
+  TensorRef w(s, columns(s, weight, dt)), b(s, columns(s, bias, dt));
   RowOutput y(s, self, dt, {&x}, {w.t, b.t});
   NormArgs<T> a;
   a.x = data_of<T>(x.ref, dt);
@@ -711,7 +720,7 @@ template <typename T>
 void run_grad(THCState* s, DType dt, AnyTensor* gradInput, AnyTensor* gradWeight, AnyTensor* gradBias, AnyTensor* input, AnyTensor* gradOutput,
               AnyTensor* weight, float eps, bool accumulate) {
   RowInput x(s, input, dt), g(s, gradOutput, dt);
-  TensorRef w(s, weight ? tensor_new_contiguous(s, weight, dt) : nullptr);
+  TensorRef w(s, columns(s, weight, dt));
   ColumnOutput dw(s, gradWeight, dt, accumulate, {x.ref.t, g.ref.t, w.t}), db(s, gradBias, dt, accumulate, {x.ref.t, g.ref.t, w.t});
   RowOutput dx(s, gradInput, dt, {&x, &g}, {w.t, gradWeight, gradBias});
   GradArgs<T> a{};

@@ -59,6 +59,7 @@ struct Group {
   uint32_t first[kMatrices + 1];      // the first workgroup of each
   int32_t count;
 };
+static_assert(sizeof(Group) + 64 <= 4096, "kernel arguments");
 struct Place {
   Matrix a;
   uint32_t index;      // of the workgroup within one matrix
@@ -170,6 +171,18 @@ __global__ __launch_bounds__(kBlock) void norm_kernel(Group g, Update h, double*
   }
 }
 
+// What elements are multiplied by: their scale over the norm, which may lie beyond the floats where elements are near their ends. (Powers of two round
+// nothing.)
+struct Factor {
+  float first, second;
+  __device__ __forceinline__ Factor(float scale, double sum, float eps) {
+    const double f = (double)scale / (sqrt(sum) + (double)eps);
+    first = f > 0x1p100 ? 0x1p64f : f < 0x1p-100 ? 0x1p-64f : 1.f;
+    second = (float)(f / (double)first);
+  }
+  __device__ __forceinline__ float operator()(float x) const { return x * first * second; }
+};
+
 struct Split {
   _Float16 h, l;
 };
@@ -218,7 +231,7 @@ __global__ __launch_bounds__(kBlock) void split_kernel(Group g, Update h, const 
   __syncthreads();
   sum = 0;
   for (int w = 0; w < kBlock / 64; ++w) sum += lds[w];
-  const float factor = (float)((double)a.scale / (sqrt(sum) + (double)h.eps));
+  const Factor factor(a.scale, sum, h.eps);
   const int32_t rows = a.tall ? a.n : a.m, cols = a.tall ? a.m : a.n, across = (cols + 63) / 64;
   const int32_t r0 = (int32_t)(p.index / across) * 64, c0 = (int32_t)(p.index % across) * 64;
   const T* in = static_cast<const T*>(a.in) + p.batch * size;
@@ -244,7 +257,7 @@ __global__ __launch_bounds__(kBlock) void split_kernel(Group g, Update h, const 
     }
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      u[e] *= factor;
+      u[e] = factor(u[e]);
       if (c + e >= cols) u[e] = 0.f;
       tile[line + k][eighth + e] = u[e];
     }
@@ -829,8 +842,9 @@ __global__ __launch_bounds__(kShortThreads) void short_begin_kernel(Group g, Upd
   __syncthreads();
   sum = 0;
   for (int w = 0; w < kShortThreads / 64; ++w) sum += norms[w];
-  const float factor = (float)((double)a.scale / (sqrt(sum) + (double)h.eps));
-  x *= factor;
+  const Factor factor(a.scale, sum, h.eps);
+#pragma unroll
+  for (int e = 0; e < 16; ++e) x[e] = factor(x[e]);
   strip.gram(x, sums);
   if constexpr (WHOLE) {
     for (int k = 0; k < steps; ++k) {
@@ -1008,7 +1022,7 @@ void run_short(THCState* s, Group& g, const Update& h, int steps, const double* 
     most = std::max(most, strips_of(a));
     read += (int64_t)a.batch * strips_of(a) * strips_of(a) * gram_bytes(a);
   }
-  // (12 matrices of 65 x 513, 5 strips and 11 MB of shares: 97 us without the sums' launches, XX with; 40 of 100 x 1000, 8 strips and 168 MB: 329, YY)
+  // (40 matrices of 100 x 1000, 8 strips and 168 MB of shares: 329 us without the sums' launches, 255 with; a launch that few bytes would not pay takes 5)
   const bool many = most > 8 || read > (int64_t(24) << 20);
   const int lds = short_lds(bands);
   const dim3 threads(kShortThreads);
@@ -1137,6 +1151,7 @@ void orthogonalize(THCState* s, DType dt, AnyTensor* self, AnyTensor* input, int
     return;
   }
   check_matrices(input, 3);
+  refuse_capture(s, "orthogonalising");
   tensor_resize_as(s, self, input, dt);
   note_stream_use(s, {self, input});
   Dense in(s, input, dt);
@@ -1178,6 +1193,7 @@ void muon(THCState* s, DType dt, int count, const Lists& l, double lr, double be
     check_list(s, l.momentum[i], p, base + 1, i, true);
     if (has_elements(p)) check_matrices(p, 3);
   }
+  refuse_capture(s, "a step of the optimizer of matrices");
   Update h;
   h.beta = (float)beta;
   h.gradScale = (float)gradScale;

@@ -195,9 +195,11 @@ void run_rotary(THCState* s, DType dt, AnyTensor* self, AnyTensor* input, AnyTen
     tensor_retain(input);
     x.t = input;
   } else {
+    refuse_capture(s, "a turn of heads that lie apart");
     x.t = tensor_new_contiguous(s, input, dt);
     as_tokens(x.t, &xt, &a.xHead);
   }
+  if ((positions && !tensor_is_contiguous(positions)) || !tensor_is_contiguous(frequencies)) refuse_capture(s, "a turn by strided positions or frequencies");
   TensorRef at(s, positions ? tensor_new_contiguous(s, positions, DType::I64) : nullptr);
   Dense f(s, frequencies, DType::F64);
   bool direct = as_tokens(self, &yt, &a.yHead) && !overlapping(tensor_layout(self)), inPlace = false;
@@ -211,6 +213,7 @@ void run_rotary(THCState* s, DType dt, AnyTensor* self, AnyTensor* input, AnyTen
     tensor_retain(self);
     y.t = self;
   } else {
+    refuse_capture(s, "a turn whose output lies apart or on what it reads");
     inPlace = false;
     y.t = tensor_new_with_size(s, self->nDimension, self->size, dt);
     as_tokens(y.t, &yt, &a.yHead);

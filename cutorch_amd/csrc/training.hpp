@@ -94,6 +94,14 @@ struct Workspace {
   char* data() const { return static_cast<char*>(tensor_data(ref.t, DType::I64)); }
 };
 
+// For calls that take temporary memory: a captured graph would go on using it after it has gone back to the allocator.
+inline void refuse_capture(THCState* s, const char* why) {
+  hipStream_t st = current_stream(s);
+  hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+  if (st && hipStreamIsCapturing(st, &status) == hipSuccess && status != hipStreamCaptureStatusNone)
+    raise_error("%s takes temporary memory and cannot be captured", why);
+}
+
 inline bool same_sizes(const AnyTensor* a, const AnyTensor* b) {
   if (a->nDimension != b->nDimension) return false;
   for (int d = 0; d < a->nDimension; ++d)
