@@ -4,8 +4,8 @@
 //   muon            m = beta m + g;  u = g + beta m (or m);  p = p (1 - lr decay) - rate orthogonalize(u)
 //
 // The products run on the matrix cores in half precision, every factor as a sum of two halves (x = h + l, 22 bits): h h' + h l' + l h' is as exact
-// as a product of floats (measured against 64 bits after five steps: 2e-6 of the result's norm, as float products have), at a third of the
-// halves' rate, where float products have a sixteenth of it. One half alone would leave 1e-3 to 5e-3. Sums are in float throughout, the norm's in 64 bits.
+// as a product of floats (4096 x 4096 against 64 bits after five steps: 5e-7 of the result's norm, float products 3e-6), at a third of the
+// halves' rate, where float products have a ninth of it (1190 and 126 TFLOP/s in products of that size). One half alone would leave 1e-3 to 5e-3. Sums are in float throughout, the norm's in 64 bits.
 // Singular values of X stay below 1.21 once they are at most 1 (a s + b s^3 + c s^5 on 0 ... 1.21), so no element of X, A and B leaves
 // +-1.21, +-1.46, +-2.81, and each is held times a power of two that brings its usual size to where halves are exact, and its
 // largest below their largest: S for X, 2^14 for A, 2^13 for B.
@@ -277,7 +277,8 @@ __global__ __launch_bounds__(kBlock) void split_kernel(Group g, Update h, const 
 // ----------------------------------------------------------------- products --
 // C = P Q', P and Q in the split layout: a workgroup has a tile of 128 x 128, each of its four waves 64 x 64 of that as 2 x 2 products of
 // 32 x 32. A block of 32 columns of both operands, upper and lower halves, is 32 KiB of LDS; the next one is on its way there while one is
-// multiplied, and there is room for two workgroups a CU. A row's eight 16-byte pieces lie in the order of their number xor half the row's, so that
+// multiplied, and there is room for two workgroups a CU. Bound by the matrix cores' power: 1024 tiles of 4096 columns 350 us, 1180 TFLOP/s of halves,
+// with the cores busy in 60 % of the cycles at 1.9 GHz; a library's product of halves of that size reaches 1190. A row's eight 16-byte pieces lie in the order of their number xor half the row's, so that
 // sixteen lanes that read the same piece of neighbouring rows meet all banks. (Blocks of 16 columns, four of which are on their way: 5 % slower, as
 // waves meet at twice as many barriers.)
 // Few matrices of some hundred rows would leave most CUs idle with that: they take tiles of 64 x 64, a wave's part 32 x 32, three blocks on their way. The

@@ -676,7 +676,10 @@ THC_API void THCudaTensor_sumallNoAlloc(THCState *state, THCudaTensor *self, flo
 THC_AMD_DECLARE_TOKEN_API(THCudaTensor)
 THC_AMD_DECLARE_TOKEN_API(THCudaHalfTensor)
 
-/* What a decoder needs between those two ends, under the same conditions.     */
+/* What a decoder needs between those two ends, under the same conditions. On */
+/* dense operands layerNorm, rotary and layerNormGrad of the input alone (rows */
+/* of up to 16384 elements) take no temporary memory and may be captured into */
+/* a graph; the others, and the optimizer of matrices, refuse to be.           */
 #define THC_AMD_DECLARE_DECODER_API(Tensor)                                    \
   /* self = (x - m) / sqrt(v + eps) * weight + bias along the last dim, m and  \
    * v each row's mean and (biased) variance, in float with one rounding at    \

@@ -84,3 +84,24 @@ def test_many_matrices(thc, rows, cols):
     one = thc.Tensor("half").orthogonalize(thc.Tensor("half").resize((rows, cols)).fill(1)).numpy()
     for i in (0, 1, count // 2, count - 6):
         assert_bit_equal(x.select(0, i).numpy(), one)
+
+
+def test_one_matrix(thc):
+    """One element a row, at the far end: the result has them there, by the polynomial of numbers."""
+    rows, cols = 2100, 1 << 20
+    rng = np.random.default_rng(4)
+    at = cols - 1 - rng.permutation(5000)[:rows]
+    values = (rng.choice([-1, 1], rows) * np.exp(rng.uniform(-2, 0, rows))).astype(np.float16)
+    x = thc.Tensor("half").resize((rows, cols)).zero()
+    ends = np.zeros((rows, 5000), np.float16)
+    ends[np.arange(rows), at - (cols - 5000)] = values
+    x.narrow(1, cols - 5000, 5000).copy(thc.Tensor.from_numpy(ends))
+    x.orthogonalize(x, 2)
+    s = values.astype(np.float64) / (np.linalg.norm(values.astype(np.float64)) + 1e-7)
+    for _ in range(2):
+        s = 3.4445 * s - 4.7750 * s ** 3 + 2.0315 * s ** 5
+    got = x.narrow(1, cols - 5000, 5000).numpy().astype(np.float64)
+    mine = got[np.arange(rows), at - (cols - 5000)]
+    assert np.all(np.abs(mine - s) <= 1.5 * 2.0 ** -11 * np.abs(s))      # (the rounding to half, and 2^-22 a few times)
+    got[np.arange(rows), at - (cols - 5000)] = 0
+    assert np.all(got == 0) and np.all(x.narrow(1, 0, 3000).numpy() == 0)

@@ -234,6 +234,38 @@ def test_passes_and_pieces(thc):
     assert all(np.array_equal(got[0], x) for x in got)
 
 
+@pytest.mark.parametrize("kind", ["float", "half"])
+def test_a_matrix_does_not_depend_on_the_others(thc, kind):
+    """Sizes of every way through the kernels, whose tiles and launches are chosen by all of a call's matrices: the bits of calls of their own."""
+    rng = np.random.default_rng(6)
+    shapes = [(600, 600), (65, 513), (128, 128), (30, 2000), (300, 1500), (40, 40), (1300, 260), (129, 129), (513, 65), (7, 3), (1024, 1100), (200, 3000)] * 2
+    t = thc.Tensor.from_numpy
+    params = [rng.standard_normal(s).astype(NP[kind]) for s in shapes]
+    grads = [_matrix(rng, s[0], s[1], kind) for s in shapes]
+    together = [t(p) for p in params]
+    opt = thc.Muon(together, [t(g) for g in grads])
+    opt.step(0.5)
+    opt.step(0.5)
+    for i, (p, g) in enumerate(zip(params, grads)):
+        alone = t(p)
+        one = thc.Muon([alone], [t(g)])
+        one.step(0.5)
+        one.step(0.5)
+        assert_bit_equal(together[i].numpy(), alone.numpy(), "matrix %d" % i)
+        assert_bit_equal(opt.momentum[i].numpy(), one.momentum[0].numpy())
+
+
+def test_ends_of_the_floats(thc):
+    """Elements so small or large that one float does not hold what they are multiplied by."""
+    t = thc.Tensor.from_numpy
+    for rows, cols in ((20, 30), (40, 300), (150, 140)):
+        g = np.round(_matrix(np.random.default_rng(rows), rows, cols, "float") * 64).astype(np.float32)
+        want = thc.Tensor("float").orthogonalize(t(g), 5, 0.0).numpy()
+        for e in (-148, -130, 110, 118):      # (times a power of two: nothing rounds)
+            got = thc.Tensor("float").orthogonalize(t(np.ldexp(g, e)), 5, 0.0).numpy()
+            assert_bit_equal(got, want, "2^%d" % e)
+
+
 def test_list_of_views_keeps_what_is_around(thc):
     rng = np.random.default_rng(3)
     t = thc.Tensor.from_numpy
