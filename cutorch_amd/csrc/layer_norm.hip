@@ -59,12 +59,18 @@ __device__ __forceinline__ void team_sum(float (&v)[N], float* lds) {
   }
 }
 
+// 1 / sqrt(v), a unit in the last place off at most: the instruction, which takes numbers below the normal ones for zero.
+__device__ __forceinline__ float inverse_root(float v) {
+  return v < 0x1p-96f ? __builtin_amdgcn_rsqf(v * 0x1p96f) * 0x1p48f : __builtin_amdgcn_rsqf(v);
+}
+
 // The packs of a row that a lane of a team of L has: pack p begins at element at[p], the first skip[p] of its V elements belong to the pack before
-// it (a row's last pack is moved back into the row, so that reads need no tail; V where there is no pack at all).
+// it (a row's last pack is moved back into the row, so that reads need no tail; V where there is no pack at all). `whole`: none is moved.
 template <int V, int L, int P>
 struct Packs {
   int32_t at[P], skip[P];
-  __device__ __forceinline__ Packs(int32_t lane, int32_t dim) {
+  bool whole;
+  __device__ __forceinline__ Packs(int32_t lane, int32_t dim) : whole(dim == V * L * P) {
 #pragma unroll
     for (int p = 0; p < P; ++p) {
       const int32_t first = (lane + p * L) * V;
@@ -77,6 +83,7 @@ struct Packs {
 // Elements that count elsewhere become 0.
 template <int V, int L, int P>
 __device__ __forceinline__ void clear_skipped(const Packs<V, L, P>& packs, float (&x)[P][V]) {
+  if (packs.whole) return;
 #pragma unroll
   for (int p = 0; p < P; ++p) {
     if (packs.skip[p]) {
@@ -98,7 +105,7 @@ struct NormArgs {
 
 template <typename T, int V, int P, int L>
 __device__ __forceinline__ void store_row(T* row, const Packs<V, L, P>& packs, int p, const Pack<T, V>& v) {
-  if (packs.skip[p] == 0) {
+  if (packs.whole || packs.skip[p] == 0) {
     store_pack_unaligned<true>(row + packs.at[p], v);
   } else if (packs.has(p)) {
 #pragma unroll
@@ -109,15 +116,21 @@ __device__ __forceinline__ void store_row(T* row, const Packs<V, L, P>& packs, i
 template <typename T, int V, int P, int L>
 __device__ __forceinline__ void load_row(const T* row, const Packs<V, L, P>& packs, Pack<T, V> (&v)[P]) {
 #pragma unroll
+  for (int p = 0; p < P; ++p) v[p] = load_pack_unaligned<true, Pack<T, V>>(row + packs.at[p]);
+}
+template <typename T, int V, int P>
+__device__ __forceinline__ void to_floats(const Pack<T, V> (&v)[P], float (&x)[P][V]) {
+#pragma unroll
   for (int p = 0; p < P; ++p)
-    if (packs.has(p)) v[p] = load_pack_unaligned<true, Pack<T, V>>(row + packs.at[p]);
+#pragma unroll
+    for (int e = 0; e < V; ++e) x[p][e] = Cvt<T>::up(v[p].v[e]);
 }
 template <typename T, int V, int P, int L>
 __device__ __forceinline__ void load_columns(const T* from, const Packs<V, L, P>& packs, float (&v)[P][V], float otherwise) {
 #pragma unroll
   for (int p = 0; p < P; ++p) {
     Pack<T, V> t{};
-    if (from && packs.has(p)) t = load_pack_unaligned<false, Pack<T, V>>(from + packs.at[p]);
+    if (from) t = load_pack_unaligned<false, Pack<T, V>>(from + packs.at[p]);
 #pragma unroll
     for (int e = 0; e < V; ++e) v[p][e] = from ? Cvt<T>::up(t.v[e]) : otherwise;
   }
@@ -131,19 +144,16 @@ __global__ __launch_bounds__(L * TEAMS) void norm_kernel(NormArgs<T> a) {
   const int32_t lane = threadIdx.x % L;
   const uint32_t team = threadIdx.x / L;
   const Packs<V, L, P> packs(lane, a.dim);
-  const float n = (float)a.dim;
+  const float n = (float)a.dim, share = 1.f / n;
   float w[P][V], b[P][V];
   load_columns<T, V, P, L>(a.weight, packs, w, 1.f);
   load_columns<T, V, P, L>(a.bias, packs, b, 0.f);
-  Pack<T, V> raw[P] = {};
+  Pack<T, V> raw[P];
   load_row<T, V, P, L>(a.x + a.xo.at(min(blockIdx.x * TEAMS + team, a.rows - 1)), packs, raw);
   for (uint32_t first = blockIdx.x * TEAMS; first < a.rows; first += gridDim.x * TEAMS) {
     const uint32_t row = min(first + team, a.rows - 1);
     float x[P][V];
-#pragma unroll
-    for (int p = 0; p < P; ++p)
-#pragma unroll
-      for (int e = 0; e < V; ++e) x[p][e] = Cvt<T>::up(raw[p].v[e]);
+    to_floats(raw, x);
     // the next row is asked for before this one is computed
     if (first + gridDim.x * TEAMS < a.rows) load_row<T, V, P, L>(a.x + a.xo.at(min(first + gridDim.x * TEAMS + team, a.rows - 1)), packs, raw);
     clear_skipped<V, L, P>(packs, x);
@@ -168,14 +178,14 @@ __global__ __launch_bounds__(L * TEAMS) void norm_kernel(NormArgs<T> a) {
         two[1] = __builtin_fmaf(x[p][e], x[p][e], two[1]);
       }
     team_sum<2, L, TEAMS>(two, lds + TEAMS * (L / 64));
-    const float c = two[0] / n, r = 1.f / sqrtf(two[1] / n - c * c + a.eps);
+    const float c = two[0] * share, r = inverse_root(two[1] * share - c * c + a.eps), cr = -c * r;
     if (first + team < a.rows) {
       T* out = a.y + a.yo.at(row);
 #pragma unroll
       for (int p = 0; p < P; ++p) {
         Pack<T, V> v;
 #pragma unroll
-        for (int e = 0; e < V; ++e) v.v[e] = rounded<T>(__builtin_fmaf((x[p][e] - c) * r, w[p][e], b[p][e]));
+        for (int e = 0; e < V; ++e) v.v[e] = rounded<T>(__builtin_fmaf(__builtin_fmaf(x[p][e], r, cr), w[p][e], b[p][e]));
         store_row(out, packs, p, v);
       }
     }
@@ -204,7 +214,7 @@ __global__ __launch_bounds__(L * TEAMS, 2) void norm_grad_kernel(GradArgs<T> a) 
   const int32_t lane = threadIdx.x % L;
   const uint32_t team = threadIdx.x / L;
   const Packs<V, L, P> packs(lane, a.dim);
-  const float n = (float)a.dim;
+  const float n = (float)a.dim, share = 1.f / n;
   float w[P][V], dw[P][V], db[P][V];
   load_columns<T, V, P, L>(a.weight, packs, w, 1.f);
   clear_skipped<V, L, P>(packs, w);
@@ -212,23 +222,18 @@ __global__ __launch_bounds__(L * TEAMS, 2) void norm_grad_kernel(GradArgs<T> a) 
   for (int p = 0; p < P; ++p)
 #pragma unroll
     for (int e = 0; e < V; ++e) dw[p][e] = db[p][e] = 0.f;
-  Pack<T, V> raw[P] = {}, next[P] = {};
+  Pack<T, V> raw[P], graw[P];
   auto load = [&](uint32_t first) {
     const uint32_t row = min(first + team, a.rows - 1);
     load_row<T, V, P, L>(a.x + a.xo.at(row), packs, raw);
-    load_row<T, V, P, L>(a.g + a.go.at(row), packs, next);
+    load_row<T, V, P, L>(a.g + a.go.at(row), packs, graw);
   };
   if (AHEAD) load(blockIdx.x * TEAMS);
   for (uint32_t first = blockIdx.x * TEAMS; first < a.rows; first += gridDim.x * TEAMS) {
     if (!AHEAD) load(first);
-    float d[P][V];
-    Pack<T, V> graw[P];
-#pragma unroll
-    for (int p = 0; p < P; ++p) {
-      graw[p] = next[p];
-#pragma unroll
-      for (int e = 0; e < V; ++e) d[p][e] = Cvt<T>::up(raw[p].v[e]);
-    }
+    float d[P][V], g[P][V];
+    to_floats(raw, d);
+    to_floats(graw, g);
     // the next row is asked for before this one is computed
     if (AHEAD && first + gridDim.x * TEAMS < a.rows) load(first + gridDim.x * TEAMS);
     clear_skipped<V, L, P>(packs, d);
@@ -249,16 +254,16 @@ __global__ __launch_bounds__(L * TEAMS, 2) void norm_grad_kernel(GradArgs<T> a) 
     for (int p = 0; p < P; ++p)
 #pragma unroll
       for (int e = 0; e < V; ++e) {
-        const float gw = Cvt<T>::up(graw[p].v[e]) * w[p][e];             // (w is 0 where d is)
+        const float gw = g[p][e] * w[p][e];             // (w is 0 where d is)
         four[0] += d[p][e];
         four[1] = __builtin_fmaf(d[p][e], d[p][e], four[1]);
         four[2] += gw;
         four[3] = __builtin_fmaf(gw, d[p][e], four[3]);
       }
     team_sum<4, L, TEAMS>(four, lds + TEAMS * (L / 64));
-    const float c = four[0] / n, r = 1.f / sqrtf(four[1] / n - c * c + a.eps);
+    const float c = four[0] * share, r = inverse_root(four[1] * share - c * c + a.eps), cr = -c * r;
     // mean(g w h) and mean(g w), times r
-    const float meanH = (four[3] - c * four[2]) * r / n * r, meanG = four[2] / n * r;
+    const float meanH = (four[3] - c * four[2]) * r * share * r, meanG = four[2] * share * r;
     if (TEAMS > 1 && first + team >= a.rows) continue;      // (all of a wave's lanes that still sum are back together at its next row)
     T* out = a.dx + a.dxo.at(first + team);
 #pragma unroll
@@ -266,11 +271,11 @@ __global__ __launch_bounds__(L * TEAMS, 2) void norm_grad_kernel(GradArgs<T> a) 
       Pack<T, V> v;
 #pragma unroll
       for (int e = 0; e < V; ++e) {
-        const float h = (d[p][e] - c) * r, g = Cvt<T>::up(graw[p].v[e]);
-        v.v[e] = rounded<T>(__builtin_fmaf(-h, meanH, __builtin_fmaf(g * w[p][e], r, -meanG)));
+        const float h = __builtin_fmaf(d[p][e], r, cr);
+        v.v[e] = rounded<T>(__builtin_fmaf(-h, meanH, __builtin_fmaf(g[p][e] * w[p][e], r, -meanG)));
         if constexpr (WEIGHTS) {
-          dw[p][e] = __builtin_fmaf(g, h, dw[p][e]);
-          db[p][e] += g;
+          dw[p][e] = __builtin_fmaf(g[p][e], h, dw[p][e]);
+          db[p][e] += g[p][e];
         }
       }
       store_row(out, packs, p, v);
