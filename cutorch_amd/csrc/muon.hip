@@ -7,8 +7,8 @@
 // as a product of floats (4096 x 4096 against 64 bits after five steps: 5e-7 of the result's norm, float products 3e-6), at a third of the
 // halves' rate, where float products have a ninth of it (1190 and 126 TFLOP/s in products of that size). One half alone would leave 1e-3 to 5e-3. Sums are in float throughout, the norm's in 64 bits.
 // Singular values of X stay below 1.21 once they are at most 1 (a s + b s^3 + c s^5 on 0 ... 1.21), so no element of X, A and B leaves
-// +-1.21, +-1.46, +-2.81, and each is held times a power of two that brings its usual size to where halves are exact, and its
-// largest below their largest: S for X, 2^14 for A, 2^13 for B.
+// +-1.21, +-1.46, +-2.81, nor P = a + B, P P' and P P' P'' +-a, +-a^2 and +-a^3, and each is held times a power of two that brings its usual size to
+// where halves are exact, and its largest below their largest: S for X, 2^14 for A and P A, 2^13 for B and P, 2^12 and 2^10 for P P' and P P' P''.
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
@@ -40,7 +40,7 @@ __device__ __forceinline__ int64_t split_at(int64_t row, int32_t column, int64_t
 
 // `batch` matrices of m x n, m <= n, X short side first; `tall`: their tensors have n rows and m columns.
 struct Matrix {
-  char* work;                  // X, X', the next X, the next X', A, B of each one
+  char* work;                  // X, X', the next X, the next X', and two planes of m x m, or four, of each one
   const void* in;              // what is orthogonalised, or the gradient
   void* out;                   // what the result goes to, or the parameter
   float *momentum, *master;    // of the optimizer
@@ -51,7 +51,13 @@ struct Matrix {
 __host__ __device__ inline int64_t plane_x(const Matrix& a) { return a.m * row_bytes(a.n); }
 __host__ __device__ inline int64_t plane_t(const Matrix& a) { return a.n * row_bytes(a.m); }
 __host__ __device__ inline int64_t plane_a(const Matrix& a) { return a.m * row_bytes(a.m); }
-__host__ __device__ inline int64_t work_bytes(const Matrix& a) { return 2 * (plane_x(a) + plane_t(a) + plane_a(a)); }
+// Where n = r m is long, several steps read X once: P = a + B takes A on to the next step's, P A P, as well as X, and what X is multiplied by is those
+// steps' P P' P''. In units of m^3, five steps cost 7.5 r + 2.5 one by one, 4.5 r + 5.5 as 2 + 2 + 1 and 3 r + 7 as 3 + 2. us, one by one and in these
+// two ways: 8192 x 2048 2023, 1612, 1407; 1024 x 4096 489, 431, 407; eight of these 2455, 1923, 1680; 2048 x 4096 1187, 1119, 1085; 1024 x 2048 343, 345, 348 (more
+// launches); 256 x 512 141, 145, 152; 1024 x 1536 298, 314, 325; 4096 x 4096 4046, 4124, 4160.
+// (A rule on each matrix alone: its bits do not depend on what else a call has.)
+__host__ __device__ inline bool is_long(const Matrix& a) { return a.n / 2 >= a.m; }
+__host__ __device__ inline int64_t work_bytes(const Matrix& a) { return 2 * (plane_x(a) + plane_t(a)) + (is_long(a) ? 4 : 2) * plane_a(a); }
 
 constexpr int kMatrices = 48;
 struct Group {
@@ -404,7 +410,17 @@ __device__ __forceinline__ void product(const Operand& P, const Operand& Q, int3
   for (int q = 0; q < W * W; ++q) total[q / W][q % W] += acc[q / W][q % W];
 }
 
-enum Op { kGram, kPolynomial, kStep, kLast };
+// What becomes of the products' sums, with the planes of m x m by number:
+//   kGram         to = X X'
+//   kPolynomial   to = b from + c from from + own (on the diagonal)
+//   kProduct      to = from with
+//   kStep, kLast  the next X = own X + from X
+enum Op { kGram, kPolynomial, kProduct, kStep, kLast };
+struct Way {
+  int turn;               // which of the two pairs of planes X is in
+  int from, with, to;
+  float own, factor;      // factor: of the sums, from the factors' scales to the result's (kProduct, kStep, kLast)
+};
 
 __host__ __device__ inline uint32_t symmetric_tiles(int32_t t) { return (uint32_t)(t * (int64_t)(t + 1) / 2); }
 __host__ __device__ inline uint32_t product_tiles(const Matrix& a, bool symmetric, int32_t tile = kTile) {
@@ -459,9 +475,9 @@ __device__ __forceinline__ void eight_of(T* at, int32_t count, F f) {
   }
 }
 
-// One of a step's three products and what is made of it. The first two are symmetric: tiles above the diagonal go to both places. `turn`: which of the
-// two pairs of planes X is in. The last step's result goes to the tensor, or into the parameter. The sums pass through LDS, so that memory sees whole
-// packs of neighbouring elements in both directions.
+// One of a step's products and what is made of it. Those of m x m are symmetric (their factors are polynomials of one A): tiles above the diagonal go to
+// both places. The last step's result goes to the tensor, or into the parameter. The sums pass through LDS, so that memory sees whole packs of
+// neighbouring elements in both directions.
 // The last tiles, which would leave much of the chip idle, are cut into the parts of their sums: a workgroup for each leaves its sums in memory, and a
 // launch behind this one (JOIN) adds them up and goes on from there.
 struct Tail {
@@ -470,13 +486,13 @@ struct Tail {
   acc16* sums;         // of each part: the products of each of 256 lanes
 };
 template <int OP, typename T, bool MUON, bool JOIN, int TILE>
-__global__ __launch_bounds__(256, 2) void product_kernel(Group g, Update h, int turn, Tail tail) {
+__global__ __launch_bounds__(256, 2) void product_kernel(Group g, Update h, Way way, Tail tail) {
   // (the joining launch has a workgroup for each wave's quarter of a large tile: one CU alone would wait long for what all parts left)
   constexpr int W = TILE / 64, kQuarters = JOIN ? W * W : 1, kSpan = JOIN ? 64 : TILE;
   constexpr int kStride = kSpan + 4;      // floats: columns of sums, four rows at once, meet all banks
   constexpr int kSums = kSpan * kStride * 4, kBlocks = JOIN ? 0 : Stages<TILE>::kCount * Stages<TILE>::kBytes;
   __shared__ __attribute__((aligned(128))) char lds[kSums > kBlocks ? kSums : kBlocks];
-  constexpr bool kSymmetric = OP == kGram || OP == kPolynomial;
+  constexpr bool kSymmetric = OP != kStep && OP != kLast;
   const uint32_t unit = JOIN ? blockIdx.x / kQuarters : by_die(blockIdx.x, gridDim.x), quarter = blockIdx.x % kQuarters;
   const bool cut = !JOIN && unit >= tail.whole;
   const uint32_t tile = JOIN ? tail.whole + unit : cut ? tail.whole + (unit - tail.whole) / (uint32_t)tail.parts : unit;
@@ -484,7 +500,9 @@ __global__ __launch_bounds__(256, 2) void product_kernel(Group g, Update h, int 
   const Matrix& a = p.a;
   char* work = a.work + p.batch * work_bytes(a);
   const int64_t px = plane_x(a), pt = plane_t(a);
-  char *x = work + turn * (px + pt), *t = x + px, *xn = work + (turn ^ 1) * (px + pt), *tn = xn + px, *am = work + 2 * (px + pt), *bm = am + plane_a(a);
+  char *x = work + way.turn * (px + pt), *t = x + px, *xn = work + (way.turn ^ 1) * (px + pt), *tn = xn + px, *square = work + 2 * (px + pt);
+  const char *left = square + way.from * plane_a(a), *right = square + way.with * plane_a(a);
+  char* to = square + way.to * plane_a(a);
   const int64_t bytesM = row_bytes(a.m), bytesN = row_bytes(a.n);
   const bool flipped = OP == kLast && a.tall;      // the tensor's rows are the longer side: its tile is the product's transpose
   const int32_t rows = flipped ? a.n : a.m, cols = kSymmetric || flipped ? a.m : a.n;
@@ -502,8 +520,8 @@ __global__ __launch_bounds__(256, 2) void product_kernel(Group g, Update h, int 
     bytesK = bytesN;
   } else {
     bytesK = bytesM;
-    from = OP == kPolynomial ? am : flipped ? t : bm;
-    with = OP == kPolynomial ? am : flipped ? bm : t;
+    from = flipped ? t : left;
+    with = kSymmetric ? right : flipped ? left : t;
   }
   const Operand P{from + i0 * bytesK, bytesK, rows - i0}, Q{with + j0 * bytesK, bytesK, cols - j0};
   // The sums as columns: a lane has column `lane % 32` of each 32 x 32 product, four rows in a row of each eight.
@@ -544,13 +562,13 @@ __global__ __launch_bounds__(256, 2) void product_kernel(Group g, Update h, int 
   constexpr int kAcross = kSpan / 8, kRows = 256 / kAcross;
   const int32_t jt = (threadIdx.x % kAcross) * 8, it = threadIdx.x / kAcross, j = j0 + jt;
   const int32_t colEnd = (int32_t)blocks_of(cols) * kBlockK;
-  const char* base = OP == kPolynomial ? am : flipped ? t : x;
-  const int64_t baseBytes = OP == kPolynomial || flipped ? bytesM : bytesN;
+  const char* base = kSymmetric ? right : flipped ? t : x;
+  const int64_t baseBytes = kSymmetric || flipped ? bytesM : bytesN;
 #pragma unroll 2
   for (int u = 0; u < kSpan; u += kRows) {
     const int32_t i = i0 + it + u;
     Eight one{};
-    if (OP != kGram && i < rows && j < colEnd) one = load_eight(base + split_at(i, j, baseBytes));
+    if (OP != kGram && OP != kProduct && (OP == kPolynomial || way.own != 0) && i < rows && j < colEnd) one = load_eight(base + split_at(i, j, baseBytes));
     float v[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
@@ -558,10 +576,12 @@ __global__ __launch_bounds__(256, 2) void product_kernel(Group g, Update h, int 
       if (kSymmetric && diagonal && it + u > jt + e) sum = sums[(it + u) * kStride + jt + e];
       if constexpr (OP == kGram) {
         v[e] = sum * (kScaleA / (a.scale * a.scale));
+      } else if constexpr (OP == kProduct) {
+        v[e] = sum * way.factor;
       } else {
         const float o = (float)one.h[e] + (float)one.l[e];
-        if constexpr (OP == kPolynomial) v[e] = __builtin_fmaf(o, kB * (kScaleB / kScaleA), sum * (kC * kScaleB / (kScaleA * kScaleA)));
-        else v[e] = __builtin_fmaf(o, kA, sum * (1.f / kScaleB));
+        if constexpr (OP == kPolynomial) v[e] = __builtin_fmaf(o, kB * (kScaleB / kScaleA), sum * (kC * kScaleB / (kScaleA * kScaleA))) + (i == j + e ? way.own * kScaleB : 0.f);
+        else v[e] = __builtin_fmaf(o, way.own, sum * way.factor);
       }
       if (i >= rows || j + e >= cols) v[e] = 0.f;
     }
@@ -581,7 +601,7 @@ __global__ __launch_bounds__(256, 2) void product_kernel(Group g, Update h, int 
         eight_of(out, cols - j, [&](int e, T& o) { o = rounded<T>(v[e] * down); });
       }
     } else {
-      if (i < rows && j < colEnd) store_eight((OP == kGram ? am : OP == kPolynomial ? bm : xn) + split_at(i, j, OP == kStep ? bytesN : bytesM), v);
+      if (i < rows && j < colEnd) store_eight((OP == kStep ? xn : to) + split_at(i, j, OP == kStep ? bytesN : bytesM), v);
       if (!diagonal) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) sums[(jt + e) * kStride + it + u] = v[e];
@@ -592,7 +612,7 @@ __global__ __launch_bounds__(256, 2) void product_kernel(Group g, Update h, int 
     if (diagonal) return;
     __syncthreads();
     // and columns, in the same way
-    char* mirrored = OP == kGram ? am : OP == kPolynomial ? bm : tn;
+    char* mirrored = OP == kStep ? tn : to;
     const int32_t rowEnd = (int32_t)blocks_of(rows) * kBlockK, i = i0 + jt;
 #pragma unroll 2
     for (int u = 0; u < kSpan; u += kRows) {
@@ -609,7 +629,9 @@ __global__ __launch_bounds__(256, 2) void product_kernel(Group g, Update h, int 
 // ---------------------------------------------------------- short matrices --
 // Up to 128 rows: A and B are one tile each, and what bounds a step is how long its launches wait for memory one after another (12 matrices of 65 x 513: 17
 // launches of 9 to 17 us each). A workgroup has a strip of 128 columns of X. It adds up the strips' shares of A, makes B of it by itself,
-// takes its strip through the step and leaves the strip's share of the next A: one launch a step, and one for all steps where X is a single strip.
+// takes its strip through the step and leaves the strip's share of the next A. Two steps a launch (three of halves) where it takes A along, P A P: a launch
+// costs some 8 us, a step in it 8 (12 of 65 x 513 floats 98 us with a launch for each, 82 so; of 128 x 512 121 and 106), most of them in its products'
+// reads of LDS and in splitting what they leave. One launch for all steps where X is a single strip, which makes each A from X.
 // LDS: one plane for A, then B, then the new X, a second one for the strip's transpose, both split, rows of 16-byte pieces in the order of their
 // number xor what brings sixteen rows to different banks.
 constexpr int kShortThreads = 1024;
@@ -642,20 +664,22 @@ struct Plane {
     *reinterpret_cast<half4*>(lower(row, column)) = l;
   }
 };
-// 32 x 32 of P Q' over `blocks` blocks of 32 columns. Three sums side by side: one would wait for itself.
+// 32 x 32 of P Q' over `blocks` blocks of 32 columns. Two sums side by side, and none in two products in a row (three: 3 % slower).
 __device__ __forceinline__ acc16 small_product(const Plane& P, int i0, const Plane& Q, int j0, int blocks) {
-  const int lane = threadIdx.x & 63, rowP = i0 + (lane & 31), rowQ = j0 + (lane & 31), k0 = lane >> 5;
-  acc16 high = {}, right = {}, left = {};
+  int lane = threadIdx.x & 63;
+  asm volatile("" : "+v"(lane));      // (addresses are made where they are used: kept through the steps they would be registers' spills)
+  const int rowP = i0 + (lane & 31), rowQ = j0 + (lane & 31), k0 = lane >> 5;
+  acc16 high = {}, rest = {};
 #pragma unroll 2
   for (int k = 0; k < 2 * blocks; ++k) {
     const int at = (k >> 1) * 8 + (k & 1) * 2 + k0;
     const half8 ph = *reinterpret_cast<const half8*>(P.at + P.piece(rowP, at)), pl = *reinterpret_cast<const half8*>(P.at + P.piece(rowP, at + 4));
     const half8 qh = *reinterpret_cast<const half8*>(Q.at + Q.piece(rowQ, at)), ql = *reinterpret_cast<const half8*>(Q.at + Q.piece(rowQ, at + 4));
+    rest = __builtin_amdgcn_mfma_f32_32x32x16_f16(ph, ql, rest, 0, 0, 0);
     high = __builtin_amdgcn_mfma_f32_32x32x16_f16(ph, qh, high, 0, 0, 0);
-    right = __builtin_amdgcn_mfma_f32_32x32x16_f16(ph, ql, right, 0, 0, 0);
-    left = __builtin_amdgcn_mfma_f32_32x32x16_f16(pl, qh, left, 0, 0, 0);
+    rest = __builtin_amdgcn_mfma_f32_32x32x16_f16(pl, qh, rest, 0, 0, 0);
   }
-  return high + (right + left);
+  return high + rest;
 }
 // Four lanes side by side that have a column of 4 x 4 each get a row each.
 template <int CONTROL>
@@ -699,14 +723,16 @@ struct Strip {
   // f(e0, row, column) for the first of each four rows that a lane has of a product
   template <typename F>
   __device__ __forceinline__ void fours(int ti, int tj, F f) const {
+    int lane = this->lane;
+    asm volatile("" : "+v"(lane));
 #pragma unroll
     for (int q = 0; q < 4; ++q) f(q * 4, ti * 32 + q * 8 + (lane >> 5) * 4, tj * 32 + (lane & 31));
   }
-  // From A (its sums, as the products leave them) to B in the square.
-  __device__ __forceinline__ void polynomial(acc16& sums) const {
-    const float scale = kScaleA / (a.scale * a.scale);
+  // Sums as the products leave them to A.
+  __device__ __forceinline__ void scaled(acc16& sums) const { sums *= kScaleA / (a.scale * a.scale); }
+  // From A to B in the square.
+  __device__ __forceinline__ void polynomial(acc16 sums) const {
     each(bands, bands, [&](int ti, int tj) {
-      sums *= scale;
       fours(ti, tj, [&](int e, int i, int j) { square.store4(j, i, {sums[e], sums[e + 1], sums[e + 2], sums[e + 3]}); });
     });
     __syncthreads();
@@ -732,6 +758,26 @@ struct Strip {
       });
     });
     __syncthreads();
+  }
+  // After a step, from its A and B to the next A, (a + B) A (a + B), and X to its place. (A and P A pass through the transpose's room.)
+  __device__ __forceinline__ void turn(const acc16& x, acc16& sums) const {
+    const Plane other{across.at, bands * 128};
+#pragma unroll 1
+    for (int k = 0; k < 2; ++k) {
+      each(bands, bands, [&](int ti, int tj) {
+        fours(ti, tj, [&](int e, int i, int j) { other.store4(j, i, {sums[e], sums[e + 1], sums[e + 2], sums[e + 3]}); });
+      });
+      __syncthreads();
+      each(bands, bands, [&](int ti, int tj) {
+        const acc16 rest = small_product(square, ti * 32, other, tj * 32, bands);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) sums[e] = __builtin_fmaf(sums[e], kA, rest[e] * (1.f / kScaleB));
+      });
+      __syncthreads();
+    }
+    each(bands, blocks, [&](int ti, int tj) {
+      fours(ti, tj, [&](int e, int i, int j) { across.store4(j, i, {x[e], x[e + 1], x[e + 2], x[e + 3]}); });
+    });
   }
   // X into both planes, then the strip's share of A.
   __device__ __forceinline__ void gram(const acc16& x, acc16& sums) const {
@@ -849,6 +895,7 @@ __global__ __launch_bounds__(kShortThreads) void short_begin_kernel(Group g, Upd
   strip.gram(x, sums);
   if constexpr (WHOLE) {
     for (int k = 0; k < steps; ++k) {
+      strip.scaled(sums);
       strip.polynomial(sums);
       strip.step(x);
       if (k + 1 < steps) strip.gram(x, sums);
@@ -879,7 +926,7 @@ __global__ __launch_bounds__(kShareThreads) void shares_kernel(Group g, int turn
 }
 
 template <typename T, bool MUON, bool LAST>
-__global__ __launch_bounds__(kShortThreads) void short_step_kernel(Group g, Update h, int turn, bool summed) {
+__global__ __launch_bounds__(kShortThreads) void short_step_kernel(Group g, Update h, int turn, bool summed, int steps) {
   extern __shared__ __attribute__((aligned(256))) char lds[];
   const Place p = place_of(g, blockIdx.x, [](const Matrix& a) { return (uint32_t)strips_of(a); });
   const Matrix& a = p.a;
@@ -907,8 +954,19 @@ __global__ __launch_bounds__(kShortThreads) void short_step_kernel(Group g, Upda
     const int k = threadIdx.x + q * kShortThreads;
     if (k < all) *reinterpret_cast<uint4v*>(strip.across.at + strip.across.piece(k / pieces, k % pieces)) = held[q];
   }
-  strip.polynomial(sums);
-  strip.step(x);
+  strip.scaled(sums);
+#pragma unroll 1
+  for (int k = 0;;) {
+    strip.polynomial(sums);
+    strip.step(x);
+    if (++k == steps) break;
+    if (is_alone(a)) {
+      strip.gram(x, sums);
+      strip.scaled(sums);
+    } else {
+      strip.turn(x, sums);
+    }
+  }
   if constexpr (LAST) {
     strip.emit<T, MUON>(x, h, p.batch * ((int64_t)a.m * a.n));
   } else {
@@ -942,6 +1000,8 @@ constexpr int64_t kPassBytes = int64_t(2) << 30;
 struct Bytes {
   int64_t work, norms;
 };
+enum Kind { kShortOnes, kLongOnes, kOthers };      // whose launches are others
+int kind_of(const Matrix& a) { return is_short(a) ? kShortOnes : is_long(a) ? kLongOnes : kOthers; }
 int64_t each_bytes(const Matrix& a) { return is_short(a) ? short_bytes(a) : work_bytes(a); }
 Bytes bytes_of(const Matrix& a) { return Bytes{each_bytes(a) * a.batch, (int64_t)norm_parts(a) * a.batch * 8}; }
 
@@ -960,7 +1020,7 @@ struct Launch {
   int32_t tile;
   Tail tail;
   Launch(const Group& from, int op, int64_t cus) : g(from) {
-    const bool symmetric = op == kGram || op == kPolynomial;
+    const bool symmetric = op != kStep;
     auto blocks = [&](int k) { return (int32_t)blocks_of(op == kGram ? g.matrix[k].n : g.matrix[k].m); };
     auto parts_of = [&](int k) { return sum_parts(blocks(k), product_tiles(g.matrix[k], symmetric)); };
     const int32_t parts = parts_of(g.count - 1);
@@ -992,16 +1052,16 @@ struct Launch {
   uint32_t rest() const { return g.first[g.count] - tail.whole; }
   int64_t bytes() const { return (int64_t)rest() * tail.parts * tile * tile * 4; }
   template <int OP, typename T, bool MUON>
-  void go(THCState* s, const Update& h, int turn) const {
-    if (tile == kTile) go_tiles<OP, T, MUON, kTile>(s, h, turn);
-    else go_tiles<OP, T, MUON, kSmallTile>(s, h, turn);
+  void go(THCState* s, const Update& h, const Way& way) const {
+    if (tile == kTile) go_tiles<OP, T, MUON, kTile>(s, h, way);
+    else go_tiles<OP, T, MUON, kSmallTile>(s, h, way);
   }
   template <int OP, typename T, bool MUON, int TILE>
-  void go_tiles(THCState* s, const Update& h, int turn) const {
+  void go_tiles(THCState* s, const Update& h, const Way& way) const {
     hipStream_t st = current_stream(s);
     const dim3 grid(tail.whole + rest() * tail.parts), joins(rest() * (TILE / 64) * (TILE / 64));
-    hipLaunchKernelGGL((product_kernel<OP, T, MUON, false, TILE>), grid, dim3(256), 0, st, g, h, turn, tail);
-    if (rest()) hipLaunchKernelGGL((product_kernel<OP, T, MUON, true, TILE>), joins, dim3(256), 0, st, g, h, turn, tail);
+    hipLaunchKernelGGL((product_kernel<OP, T, MUON, false, TILE>), grid, dim3(256), 0, st, g, h, way, tail);
+    if (rest()) hipLaunchKernelGGL((product_kernel<OP, T, MUON, true, TILE>), joins, dim3(256), 0, st, g, h, way, tail);
   }
 };
 struct Plan {
@@ -1010,6 +1070,11 @@ struct Plan {
   int64_t bytes() const { return std::max({gram.bytes(), polynomial.bytes(), step.bytes()}); }
 };
 
+// How many steps go with one A from X. An error of A grows with what it belongs to, up to 12 times a step where singular values are small. Two steps
+// leave what single ones do: against 64 bits after five steps, of the result's norm, singly, as 2 + 2 + 1 and by products of floats: 12 of 65 x 513 1.1e-6,
+// 1.2e-6, 1.3e-6, 2 of 256 x 1024 1.5e-6, 2.3e-6, 1.7e-6, 1024 x 4096 1.8e-6, 1.9e-6, 3.3e-6. 3 + 2 is as good where many directions share the norm (2.1e-6
+// of 1024 x 4096), not where few do (3.2e-6 of 65 x 513, 6.7e-6 of 33 x 500; 4 + 1 2e-5 to 6e-5): for halves, which come with 2e-4 of their own.
+int chain_of(int done, int steps, bool halves) { return halves && done == 0 && steps % 2 && steps >= 3 ? 3 : std::min(2, steps - done); }
 template <typename T, bool MUON>
 void run_short(THCState* s, Group& g, const Update& h, int steps, const double* norms) {
   hipStream_t st = current_stream(s);
@@ -1039,10 +1104,12 @@ void run_short(THCState* s, Group& g, const Update& h, int steps, const double* 
     return;
   }
   hipLaunchKernelGGL(roomy(short_begin_kernel<T, MUON, false>), strips, threads, lds, st, g, h, norms, steps);
-  for (int k = 0; k < steps; ++k) {
-    if (many) hipLaunchKernelGGL(shares_kernel, dim3(parts), dim3(kShareThreads), 0, st, shares, k & 1);
-    if (k + 1 < steps) hipLaunchKernelGGL(roomy(short_step_kernel<float, false, false>), strips, threads, lds, st, g, h, k & 1, many);
-    else hipLaunchKernelGGL(roomy(short_step_kernel<T, MUON, true>), strips, threads, lds, st, g, h, k & 1, many);
+  for (int done = 0, turn = 0; done < steps; turn ^= 1) {
+    const int chain = chain_of(done, steps, std::is_same_v<T, __half>);
+    done += chain;
+    if (many) hipLaunchKernelGGL(shares_kernel, dim3(parts), dim3(kShareThreads), 0, st, shares, turn);
+    if (done < steps) hipLaunchKernelGGL(roomy(short_step_kernel<float, false, false>), strips, threads, lds, st, g, h, turn, many, chain);
+    else hipLaunchKernelGGL(roomy(short_step_kernel<T, MUON, true>), strips, threads, lds, st, g, h, turn, many, chain);
   }
 }
 
@@ -1064,12 +1131,33 @@ void run_group(THCState* s, Group& g, const Update& h, int steps, char* work, do
   hipLaunchKernelGGL((split_kernel<T, MUON>), dim3(tiles), dim3(kBlock), 0, st, g, h, norms);
   Plan plan(g, num_compute_units(s));
   plan.gram.tail.sums = plan.polynomial.tail.sums = plan.step.tail.sums = sums;
-  for (int k = 0; k < steps; ++k) {
-    const int turn = k & 1;
-    plan.gram.go<kGram, float, false>(s, h, turn);
-    plan.polynomial.go<kPolynomial, float, false>(s, h, turn);
-    if (k + 1 < steps) plan.step.go<kStep, float, false>(s, h, turn);
-    else plan.step.go<kLast, T, MUON>(s, h, turn);
+  const bool chained = is_long(g.matrix[0]);
+  for (int done = 0, turn = 0; done < steps; turn ^= 1) {
+    plan.gram.go<kGram, float, false>(s, h, Way{turn, 0, 0, 0, 0, 0});
+    Way way{turn, 1, 0, 0, kA, 1 / kScaleB};
+    if (chained) {
+      const int last = done + chain_of(done, steps, std::is_same_v<T, __half>);
+      int a = 0, p = 1, c = 2, q = 1;
+      float scale = kScaleB;      // of Q
+      plan.polynomial.go<kPolynomial, float, false>(s, h, Way{turn, a, a, p, kA, 0});
+      while (++done < last) {
+        plan.polynomial.go<kProduct, float, false>(s, h, Way{turn, p, a, c, 0, 1 / kScaleB});
+        plan.polynomial.go<kProduct, float, false>(s, h, Way{turn, c, p, a, 0, 1 / kScaleB});
+        plan.polynomial.go<kPolynomial, float, false>(s, h, Way{turn, a, a, c, kA, 0});
+        const int free = q == p ? 3 : p, next = scale == kScaleB ? 2 : 4;      // (Q's elements stay below a^2, a^3)
+        plan.polynomial.go<kProduct, float, false>(s, h, Way{turn, c, q, free, 0, 1 / (kScaleB * next)});
+        scale /= next;
+        p = c;
+        c = q;
+        q = free;
+      }
+      way = Way{turn, q, 0, 0, 0, 1 / scale};
+    } else {
+      plan.polynomial.go<kPolynomial, float, false>(s, h, Way{turn, 0, 0, 1, 0, 0});
+      ++done;
+    }
+    if (done < steps) plan.step.go<kStep, float, false>(s, h, way);
+    else plan.step.go<kLast, T, MUON>(s, h, way);
   }
 }
 
@@ -1080,7 +1168,7 @@ void run(THCState* s, std::vector<Matrix>& all, const Update& h, int steps) {
   std::stable_sort(all.begin(), all.end(), [](const Matrix& a, const Matrix& b) { return a.n != b.n ? a.n > b.n : a.m > b.m; });
   std::vector<Group> groups;
   Bytes most{0, 0};
-  for (bool few : {true, false}) {
+  for (int kind : {kShortOnes, kLongOnes, kOthers}) {
     Bytes sum{0, 0};
     bool open = false;
     auto add = [&](const Matrix& a) {
@@ -1099,7 +1187,7 @@ void run(THCState* s, std::vector<Matrix>& all, const Update& h, int steps) {
       most.norms = std::max(most.norms, sum.norms);
     };
     for (const Matrix& a : all) {
-      if (is_short(a) != few) continue;
+      if (kind_of(a) != kind) continue;
       // a batch in pieces: by the workspace, and by what the workgroups of a launch are counted in
       const int64_t size = (int64_t)a.m * a.n;
       const int64_t each = std::max<int64_t>(1, std::min<int64_t>(kPassBytes / each_bytes(a), 1 << 20));

@@ -322,3 +322,69 @@ def test_refusals(thc):
         thc.Muon([x], [x])._hold("mean", [x])
     assert np.all(x.numpy() == 1)
     assert F("float").orthogonalize(F("float")).shape == ()
+
+
+def _chained(x, lengths, noise=None, eps=1e-7):
+    """The definition in float64 with one X X' for several steps: A' = P A P, X'' = P' P X. `noise` as in `_steps`."""
+    x = x.astype(np.float64)
+    x = x / (np.linalg.norm(x) + eps)
+
+    def off(m):
+        if noise is None:
+            return m
+        size = np.abs(m) + np.sqrt((m ** 2).mean())
+        return (m + size * 2.0 ** -22 * noise.uniform(-1, 1, m.shape)).astype(np.float32)
+
+    tall = x.shape[0] > x.shape[1]
+    if tall:
+        x = x.T
+    one = np.eye(len(x))
+    for length in lengths:
+        x = off(x)
+        a, q = off(x @ x.T), None
+        for k in range(length):
+            p = off(A * one + np.float64(B) * a + np.float64(C) * (a @ a))
+            q = p if q is None else off(p @ q)
+            if k + 1 < length:
+                a = off(off(p @ a) @ p)
+        x = q @ x
+    return np.asarray(x.T if tall else x, np.float64)
+
+
+@pytest.mark.parametrize("kind", ["float", "half"])
+@pytest.mark.parametrize("rows,cols,steps", [(129, 258, 5), (257, 129, 5), (258, 129, 4), (140, 1201, 1), (1201, 140, 2), (140, 1201, 3), (200, 3001, 5),
+                                             (513, 1030, 6), (130, 600, 7), (20, 500, 1), (500, 20, 2), (100, 300, 3), (129, 70, 4), (70, 129, 7)])
+def test_steps_that_share_a_product(thc, kind, rows, cols, steps):
+    """Matrices at least twice as long as high, and those of up to 128 rows: several steps with one X X'. With singular values from 1 to 1e-4 too."""
+    odd = steps % 2
+    lengths = [2] * (steps // 2) + [1] * odd if kind == "float" or steps == 1 else [3] * odd + [2] * ((steps - 3 * odd) // 2)
+    rng = np.random.default_rng(rows + cols + steps)
+    m = min(rows, cols)
+    u, v = np.linalg.qr(rng.standard_normal((rows, m)))[0], np.linalg.qr(rng.standard_normal((cols, m)))[0]
+    for g in (_matrix(rng, rows, cols, kind), ((u * np.logspace(0, -4, m)) @ v.T * 0.5).astype(NP[kind])):
+        want = _steps(g, steps)
+        assert np.linalg.norm(_chained(g, lengths) - want) <= 2.0 ** -40 * np.linalg.norm(want)
+        got = thc.Tensor(kind).orthogonalize(thc.Tensor.from_numpy(g), steps).numpy().astype(np.float64)
+        # eight times what rounding did in these steps, in either order, and the rounding to the type
+        room = 8 * max(np.linalg.norm(f(g, *how, noise=np.random.default_rng(1)) - want) for f, how in ((_chained, (lengths,)), (_steps, (steps,))))
+        beyond = np.maximum(np.abs(got - want) - UNIT[kind] * np.abs(want) * 1.01 - TINY[kind], 0)
+        assert np.linalg.norm(beyond) <= room + 2.0 ** -24 * np.linalg.norm(want), np.linalg.norm(beyond) / room
+
+
+@pytest.mark.parametrize("kind", ["float", "half"])
+@pytest.mark.parametrize("rows,cols", [(70, 300), (300, 70), (140, 700), (700, 140), (260, 2000)])
+def test_one_element_a_row_of_long_matrices(thc, kind, rows, cols):
+    rng = np.random.default_rng(rows + cols)
+    m = min(rows, cols)
+    g = np.zeros((rows, cols), NP[kind])
+    at = rng.permutation(rows)[:m], rng.permutation(cols)[:m]
+    values = (rng.choice([-1, 1], m) * np.exp(rng.uniform(-3, 0, m))).astype(NP[kind])
+    g[at] = values
+    got = thc.Tensor(kind).orthogonalize(thc.Tensor.from_numpy(g)).numpy().astype(np.float64)
+    want = _scalar_steps(values.astype(np.float64) / (np.linalg.norm(g.astype(np.float64)) + 1e-7))
+    where = np.ones_like(got, bool)
+    where[at] = False
+    assert np.all(got[where] == 0)
+    # 10 roundings a step relative to the value, as where steps go one by one, and those of the shared products: five of an operand for each of three
+    # steps more, which a following step makes at most 2.8 of (a^2 of A's relative error against the slope of its square root's)
+    assert np.all(np.abs(got[at] - want) <= ((5 * 10 + 3 * 5 * 2.8) * 2.0 ** -22 + UNIT[kind] * 1.01) * np.abs(want) * 1.5), np.max(np.abs(got[at] / want - 1))
