@@ -495,7 +495,9 @@ __global__ __launch_bounds__(256, 2) void product_kernel(Group g, Update h, Way 
   constexpr bool kSymmetric = OP != kStep && OP != kLast;
   const uint32_t unit = JOIN ? blockIdx.x / kQuarters : by_die(blockIdx.x, gridDim.x), quarter = blockIdx.x % kQuarters;
   const bool cut = !JOIN && unit >= tail.whole;
-  const uint32_t tile = JOIN ? tail.whole + unit : cut ? tail.whole + (unit - tail.whole) / (uint32_t)tail.parts : unit;
+  // (of the tiles that are cut, the first parts of all, then the second ones, ...: a die's workgroups read less that way, 1024 x 4096 halves 395 -> 386 us)
+  const uint32_t rest = (gridDim.x - tail.whole) / (uint32_t)tail.parts;
+  const uint32_t tile = JOIN ? tail.whole + unit : cut ? tail.whole + (unit - tail.whole) % rest : unit;
   const Place p = place_of(g, tile, [](const Matrix& a) { return product_tiles(a, kSymmetric, TILE); });
   const Matrix& a = p.a;
   char* work = a.work + p.batch * work_bytes(a);
@@ -543,11 +545,11 @@ __global__ __launch_bounds__(256, 2) void product_kernel(Group g, Update h, Way 
     for (int k = 0; k < tail.parts; ++k) acc += from16[k * kEach];
     keep(wave >> 1, wave & 1, acc);
   } else {
-    const int32_t blocks = (int32_t)(bytesK / kBlockBytes), parts = sum_parts(blocks, product_tiles(a, kSymmetric)), part = cut ? (int32_t)((unit - tail.whole) % (uint32_t)tail.parts) : 0;
+    const int32_t blocks = (int32_t)(bytesK / kBlockBytes), parts = sum_parts(blocks, product_tiles(a, kSymmetric)), part = cut ? (int32_t)((unit - tail.whole) / rest) : 0;
     acc16 acc[W][W] = {};
     product<TILE>(P, Q, blocks, parts, part, cut ? part + 1 : parts, lds, acc);
     if (cut) {
-      acc16* to16 = tail.sums + (int64_t)(unit - tail.whole) * (W * W * 256) + threadIdx.x;
+      acc16* to16 = tail.sums + ((int64_t)(tile - tail.whole) * tail.parts + part) * (W * W * 256) + threadIdx.x;
 #pragma unroll
       for (int q = 0; q < W * W; ++q) to16[q * 256] = acc[q / W][q % W];
       return;
