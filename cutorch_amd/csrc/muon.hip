@@ -96,10 +96,7 @@ __device__ __forceinline__ Place place_of(const Group& g, uint32_t block, F each
 
 // ------------------------------------------------------------ norms, planes --
 constexpr int kNormPart = 16384;      // elements a workgroup
-// (none of those whose one workgroup makes its norm by itself)
-constexpr int kShort = 128, kStrip = 128;
-__host__ __device__ inline bool is_alone(const Matrix& a) { return a.m <= kShort && a.n <= kStrip; }
-__host__ __device__ inline uint32_t norm_parts(const Matrix& a) { return is_alone(a) ? 0 : (uint32_t)(((int64_t)a.m * a.n + kNormPart - 1) / kNormPart); }
+__host__ __device__ inline uint32_t norm_parts(const Matrix& a) { return (uint32_t)(((int64_t)a.m * a.n + kNormPart - 1) / kNormPart); }
 
 struct Update {
   float beta, gradScale, keep, eps;
@@ -181,8 +178,8 @@ __global__ __launch_bounds__(kBlock) void norm_kernel(Group g, Update h, double*
 // nothing.)
 struct Factor {
   float first, second;
-  __device__ __forceinline__ Factor(float scale, double sum, float eps) {
-    const double f = (double)scale / (sqrt(sum) + (double)eps);
+  __device__ __forceinline__ Factor(float scale, double sum, float eps) : Factor((double)scale / (sqrt(sum) + (double)eps)) {}
+  __device__ __forceinline__ explicit Factor(double f) {
     first = f > 0x1p100 ? 0x1p64f : f < 0x1p-100 ? 0x1p-64f : 1.f;
     second = (float)(f / (double)first);
   }
@@ -636,13 +633,16 @@ __global__ __launch_bounds__(256, 2) void product_kernel(Group g, Update h, Way 
 // reads of LDS and in splitting what they leave. One launch for all steps where X is a single strip, which makes each A from X.
 // LDS: one plane for A, then B, then the new X, a second one for the strip's transpose, both split, rows of 16-byte pieces in the order of their
 // number xor what brings sixteen rows to different banks.
-constexpr int kShortThreads = 1024;
+// No launch makes the norm first: a strip begins over its own norm, by a power of two, and the step that adds up the shares knows all strips' norms.
+constexpr int kShortThreads = 1024, kShort = 128, kStrip = 128;
 __host__ __device__ inline bool is_short(const Matrix& a) { return a.m <= kShort; }
+__host__ __device__ inline bool is_alone(const Matrix& a) { return is_short(a) && a.n <= kStrip; }
 __host__ __device__ inline int32_t strips_of(const Matrix& a) { return (a.n + kStrip - 1) / kStrip; }
 __host__ __device__ inline int32_t bands_of(const Matrix& a) { return (a.m + 31) / 32; }
 __host__ __device__ inline int64_t gram_bytes(const Matrix& a) { return (int64_t)bands_of(a) * bands_of(a) * 4096; }
-// X', the strips' shares of A for this step and the next, their sum.
-__host__ __device__ inline int64_t short_bytes(const Matrix& a) { return plane_t(a) + (2 * (int64_t)strips_of(a) + 1) * gram_bytes(a); }
+// X', the strips' shares of A for this step and the next, their sum; the strips' sums of squares and the sum of those.
+__host__ __device__ inline int64_t shares_end(const Matrix& a) { return plane_t(a) + (2 * (int64_t)strips_of(a) + 1) * gram_bytes(a); }
+__host__ __device__ inline int64_t short_bytes(const Matrix& a) { return shares_end(a) + ((int64_t)strips_of(a) + 1 + 31) / 32 * 256; }
 __host__ __device__ inline int short_lds(int bands) { return bands * 32 * 512 + kStrip * bands * 128; }
 
 struct Plane {
@@ -749,14 +749,14 @@ struct Strip {
     });
     __syncthreads();
   }
-  // The next X, times its scale.
-  __device__ __forceinline__ void step(acc16& x) const {
+  // The next X, times its scale and `factor`.
+  __device__ __forceinline__ void step(acc16& x, float factor) const {
     each(bands, blocks, [&](int ti, int tj) {
       x = small_product(square, ti * 32, across, tj * 32, bands);
       fours(ti, tj, [&](int e, int i, int j) {
         const half4 h = *reinterpret_cast<const half4*>(across.upper(j, i)), l = *reinterpret_cast<const half4*>(across.lower(j, i));
 #pragma unroll
-        for (int k = 0; k < 4; ++k) x[e + k] = __builtin_fmaf((float)h[k] + (float)l[k], kA, x[e + k] * (1.f / kScaleB));
+        for (int k = 0; k < 4; ++k) x[e + k] = __builtin_fmaf((float)h[k] + (float)l[k], kA, x[e + k] * (1.f / kScaleB)) * factor;
       });
     });
     __syncthreads();
@@ -838,17 +838,26 @@ __device__ __forceinline__ void leave(const Strip& strip, const acc16& sums, cha
   strip.each(strip.bands, strip.bands, [&](int ti, int tj) { share[(ti * strip.bands + tj) * 64 + strip.lane] = sums; });
 }
 
-// The strip's elements into both planes, over the norm, which a strip that is the whole matrix makes by itself (and the momentum with it). WHOLE: all
-// of the launch's are, and go through all steps in it.
+// A strip's elements are at first multiplied by 2^this: S over their norm, or up to twice as much.
+__device__ __forceinline__ int strip_exponent(double squares, float scale) {
+  const int e = (int)(__double_as_longlong(squares) >> 52) - 1023;      // of the greatest power of two up to it
+  return ilogbf(scale) - (squares > 0 ? e >> 1 : -150);
+}
+// What a strip's X then lacks to be over the whole norm, at most 1.
+__device__ __forceinline__ float strip_factor(double norm, double squares, const Matrix& a) {
+  return (float)ldexp((double)a.scale / norm, -strip_exponent(squares, a.scale));
+}
+constexpr int kFewStrips = 8;
+
+// The strip's elements into both planes (and the momentum). WHOLE: all of the launch's strips are whole matrices, and go through all steps in it.
 template <typename T, bool MUON, bool WHOLE>
-__global__ __launch_bounds__(kShortThreads) void short_begin_kernel(Group g, Update h, const double* parts, int steps) {
+__global__ __launch_bounds__(kShortThreads) void short_begin_kernel(Group g, Update h, int steps) {
   extern __shared__ __attribute__((aligned(256))) char lds[];
   __shared__ double norms[kShortThreads / 64];
   const Place p = place_of(g, blockIdx.x, [](const Matrix& a) { return (uint32_t)strips_of(a); });
   const Matrix& a = p.a;
   const int64_t at = p.batch * ((int64_t)a.m * a.n);
   const Strip strip(a, (int)p.index, lds);
-  const bool alone = WHOLE || is_alone(a);
   const T* in = static_cast<const T*>(a.in);
   acc16 x = {}, was = {}, sums = {};
   strip.each(strip.bands, strip.blocks, [&](int ti, int tj) {
@@ -869,29 +878,23 @@ __global__ __launch_bounds__(kShortThreads) void short_begin_kernel(Group g, Upd
       for (int k = 0; k < 4; ++k) {
         float u = x[e + k];
         if constexpr (MUON) {
-          const float grad = u * h.gradScale, m = alone ? __builtin_fmaf(was[e + k], h.beta, grad) : was[e + k];
-          if (alone) {
-            const int64_t to = strip.place(at, i + k, j);
-            if (to >= 0) a.momentum[to] = m;
-          }
+          const float grad = u * h.gradScale, m = __builtin_fmaf(was[e + k], h.beta, grad);
+          const int64_t to = strip.place(at, i + k, j);
+          if (to >= 0) a.momentum[to] = m;
           u = h.nesterov ? __builtin_fmaf(m, h.beta, grad) : m;
         }
         x[e + k] = u;
-        if (alone) sum += (double)u * u;
+        sum += (double)u * u;
       }
     });
   });
-  if (!alone) {
-    const uint32_t n = norm_parts(a);
-    const double* mine = parts + a.norms + (int64_t)p.batch * n;
-    for (uint32_t i = threadIdx.x; i < n; i += kShortThreads) sum += mine[i];
-  }
   for (int d = 32; d >= 1; d >>= 1) sum += __shfl_xor(sum, d);
   if (strip.lane == 0) norms[strip.wave] = sum;
   __syncthreads();
   sum = 0;
   for (int w = 0; w < kShortThreads / 64; ++w) sum += norms[w];
-  const Factor factor(a.scale, sum, h.eps);
+  const bool alone = WHOLE || is_alone(a);
+  const Factor factor = alone ? Factor(a.scale, sum, h.eps) : Factor(ldexp(1.0, strip_exponent(sum, a.scale)));
 #pragma unroll
   for (int e = 0; e < 16; ++e) x[e] = factor(x[e]);
   strip.gram(x, sums);
@@ -899,20 +902,21 @@ __global__ __launch_bounds__(kShortThreads) void short_begin_kernel(Group g, Upd
     for (int k = 0; k < steps; ++k) {
       strip.scaled(sums);
       strip.polynomial(sums);
-      strip.step(x);
+      strip.step(x, 1.f);
       if (k + 1 < steps) strip.gram(x, sums);
     }
     strip.emit<T, MUON>(x, h, at);
   } else {
     char* work = a.work + p.batch * short_bytes(a);
     leave(strip, sums, work, p.index, 0);
+    if (threadIdx.x == 0) reinterpret_cast<double*>(work + shares_end(a))[p.index] = sum;
   }
 }
 
 // The sum of the strips' shares of A, before the step that takes it: where each strip's workgroup would read many of them. (The order is the same.)
 constexpr int kShareThreads = 64;
 __host__ __device__ inline uint32_t share_parts(const Matrix& a) { return (uint32_t)(gram_bytes(a) / 16 / kShareThreads); }
-__global__ __launch_bounds__(kShareThreads) void shares_kernel(Group g, int turn) {
+__global__ __launch_bounds__(kShareThreads) void shares_kernel(Group g, Update h, int turn, bool first) {
   const Place p = place_of(g, blockIdx.x, [](const Matrix& a) { return share_parts(a); });
   const Matrix& a = p.a;
   const int strips = strips_of(a);
@@ -922,13 +926,31 @@ __global__ __launch_bounds__(kShareThreads) void shares_kernel(Group g, int turn
   const int64_t k = (int64_t)p.index * kShareThreads + threadIdx.x;
   const float4v* from = reinterpret_cast<const float4v*>(shares + turn * strips * bytes) + k;
   float4v sum = {};
+  if (first && !is_alone(a)) {
+    double* norms = reinterpret_cast<double*>(a.work + p.batch * short_bytes(a) + shares_end(a));
+    double squares = 0;
+    if (strips <= kFewStrips) {
+      for (int s = 0; s < strips; ++s) squares += norms[s];
+    } else {
+      for (int s = threadIdx.x; s < strips; s += kShareThreads) squares += norms[s];
+      for (int d = 32; d >= 1; d >>= 1) squares += __shfl_xor(squares, d);
+    }
+    if (p.index == 0 && threadIdx.x == 0) norms[strips] = squares;
+    const double norm = sqrt(squares) + (double)h.eps;
+#pragma unroll 4
+    for (int s = 0; s < strips; ++s) {
+      const float f = strip_factor(norm, norms[s], a);
+      sum += from[s * step] * (f * f);
+    }
+  } else {
 #pragma unroll 8
-  for (int s = 0; s < strips; ++s) sum += from[s * step];
+    for (int s = 0; s < strips; ++s) sum += from[s * step];
+  }
   reinterpret_cast<float4v*>(shares + 2 * strips * bytes)[k] = sum;
 }
 
 template <typename T, bool MUON, bool LAST>
-__global__ __launch_bounds__(kShortThreads) void short_step_kernel(Group g, Update h, int turn, bool summed, int steps) {
+__global__ __launch_bounds__(kShortThreads) void short_step_kernel(Group g, Update h, int turn, bool summed, bool first, int steps) {
   extern __shared__ __attribute__((aligned(256))) char lds[];
   const Place p = place_of(g, blockIdx.x, [](const Matrix& a) { return (uint32_t)strips_of(a); });
   const Matrix& a = p.a;
@@ -947,9 +969,21 @@ __global__ __launch_bounds__(kShortThreads) void short_step_kernel(Group g, Upda
   const int64_t bytes = gram_bytes(a);
   const char* shares = work + plane_t(a) + (summed ? 2 * strips : turn * strips) * bytes;
   acc16 sums = {}, x = {};
+  const bool weighed = first && !is_alone(a);
+  const double* norms = reinterpret_cast<const double*>(work + shares_end(a));
+  double norm = 0;
+  if (weighed) {
+    if (summed) norm = norms[strips];
+    else for (int k = 0; k < strips; ++k) norm += norms[k];
+    norm = sqrt(norm) + (double)h.eps;
+  }
+  float factor = weighed ? strip_factor(norm, norms[p.index], a) : 1.f;
   strip.each(strip.bands, strip.bands, [&](int ti, int tj) {
     const acc16* mine = reinterpret_cast<const acc16*>(shares) + (ti * strip.bands + tj) * 64 + strip.lane;
-    for (int k = 0; k < (summed ? 1 : strips); ++k) sums += mine[k * (bytes / 64)];
+    for (int k = 0; k < (summed ? 1 : strips); ++k) {
+      const float f = weighed && !summed ? strip_factor(norm, norms[k], a) : 1.f;
+      sums += mine[k * (bytes / 64)] * (f * f);
+    }
   });
 #pragma unroll
   for (int q = 0; q < 4; ++q) {
@@ -960,8 +994,9 @@ __global__ __launch_bounds__(kShortThreads) void short_step_kernel(Group g, Upda
 #pragma unroll 1
   for (int k = 0;;) {
     strip.polynomial(sums);
-    strip.step(x);
+    strip.step(x, factor);
     if (++k == steps) break;
+    factor = 1.f;
     if (is_alone(a)) {
       strip.gram(x, sums);
       strip.scaled(sums);
@@ -1005,7 +1040,7 @@ struct Bytes {
 enum Kind { kShortOnes, kLongOnes, kOthers };      // whose launches are others
 int kind_of(const Matrix& a) { return is_short(a) ? kShortOnes : is_long(a) ? kLongOnes : kOthers; }
 int64_t each_bytes(const Matrix& a) { return is_short(a) ? short_bytes(a) : work_bytes(a); }
-Bytes bytes_of(const Matrix& a) { return Bytes{each_bytes(a) * a.batch, (int64_t)norm_parts(a) * a.batch * 8}; }
+Bytes bytes_of(const Matrix& a) { return Bytes{each_bytes(a) * a.batch, is_short(a) ? 0 : (int64_t)norm_parts(a) * a.batch * 8}; }
 
 // What workgroups that each multiply `blocks` blocks take, us, as measured with one matrix of 256 to 4096 rows: up to one to a CU, or rounds of two to each.
 double product_time(int32_t tile, double blocks, int64_t units, int64_t cus, bool cut) {
@@ -1078,7 +1113,7 @@ struct Plan {
 // of 1024 x 4096), not where few do (3.2e-6 of 65 x 513, 6.7e-6 of 33 x 500; 4 + 1 2e-5 to 6e-5): for halves, which come with 2e-4 of their own.
 int chain_of(int done, int steps, bool halves) { return halves && done == 0 && steps % 2 && steps >= 3 ? 3 : std::min(2, steps - done); }
 template <typename T, bool MUON>
-void run_short(THCState* s, Group& g, const Update& h, int steps, const double* norms) {
+void run_short(THCState* s, Group& g, const Update& h, int steps) {
   hipStream_t st = current_stream(s);
   int bands = 0, most = 0;
   bool whole = true;
@@ -1091,7 +1126,7 @@ void run_short(THCState* s, Group& g, const Update& h, int steps, const double* 
     read += (int64_t)a.batch * strips_of(a) * strips_of(a) * gram_bytes(a);
   }
   // (40 matrices of 100 x 1000, 8 strips and 168 MB of shares: 329 us without the sums' launches, 255 with; a launch that few bytes would not pay takes 5)
-  const bool many = most > 8 || read > (int64_t(24) << 20);
+  const bool many = most > kFewStrips || read > (int64_t(24) << 20);
   const int lds = short_lds(bands);
   const dim3 threads(kShortThreads);
   Group shares = g;
@@ -1102,16 +1137,17 @@ void run_short(THCState* s, Group& g, const Update& h, int steps, const double* 
     return kernel;
   };
   if (whole) {
-    hipLaunchKernelGGL(roomy(short_begin_kernel<T, MUON, true>), strips, threads, lds, st, g, h, norms, steps);
+    hipLaunchKernelGGL(roomy(short_begin_kernel<T, MUON, true>), strips, threads, lds, st, g, h, steps);
     return;
   }
-  hipLaunchKernelGGL(roomy(short_begin_kernel<T, MUON, false>), strips, threads, lds, st, g, h, norms, steps);
+  hipLaunchKernelGGL(roomy(short_begin_kernel<T, MUON, false>), strips, threads, lds, st, g, h, steps);
   for (int done = 0, turn = 0; done < steps; turn ^= 1) {
     const int chain = chain_of(done, steps, std::is_same_v<T, __half>);
+    const bool first = done == 0;
     done += chain;
-    if (many) hipLaunchKernelGGL(shares_kernel, dim3(parts), dim3(kShareThreads), 0, st, shares, turn);
-    if (done < steps) hipLaunchKernelGGL(roomy(short_step_kernel<float, false, false>), strips, threads, lds, st, g, h, turn, many, chain);
-    else hipLaunchKernelGGL(roomy(short_step_kernel<T, MUON, true>), strips, threads, lds, st, g, h, turn, many, chain);
+    if (many) hipLaunchKernelGGL(shares_kernel, dim3(parts), dim3(kShareThreads), 0, st, shares, h, turn, first);
+    if (done < steps) hipLaunchKernelGGL(roomy(short_step_kernel<float, false, false>), strips, threads, lds, st, g, h, turn, many, first, chain);
+    else hipLaunchKernelGGL(roomy(short_step_kernel<T, MUON, true>), strips, threads, lds, st, g, h, turn, many, first, chain);
   }
 }
 
@@ -1122,13 +1158,13 @@ void run_group(THCState* s, Group& g, const Update& h, int steps, char* work, do
     g.matrix[k].work = work;
     work += bytes_of(g.matrix[k]).work;
   }
-  const uint32_t parts = number(g, norm_parts);
-  for (int k = 0; k < g.count; ++k) g.matrix[k].norms = g.first[k];
-  if (parts) hipLaunchKernelGGL((norm_kernel<T, MUON>), dim3(parts), dim3(kBlock), 0, st, g, h, norms);
   if (is_short(g.matrix[0])) {
-    run_short<T, MUON>(s, g, h, steps, norms);
+    run_short<T, MUON>(s, g, h, steps);
     return;
   }
+  const uint32_t parts = number(g, norm_parts);
+  for (int k = 0; k < g.count; ++k) g.matrix[k].norms = g.first[k];
+  hipLaunchKernelGGL((norm_kernel<T, MUON>), dim3(parts), dim3(kBlock), 0, st, g, h, norms);
   const uint32_t tiles = number(g, tiles64);
   hipLaunchKernelGGL((split_kernel<T, MUON>), dim3(tiles), dim3(kBlock), 0, st, g, h, norms);
   Plan plan(g, num_compute_units(s));
