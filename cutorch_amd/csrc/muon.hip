@@ -186,17 +186,26 @@ struct Factor {
   __device__ __forceinline__ float operator()(float x) const { return x * first * second; }
 };
 
-struct Split {
-  _Float16 h, l;
-};
-// (The operation before it must not become one with the rounding to half: it would round once there and twice for the lower half, which now and then then
-// goes with another upper one.)
-__device__ __forceinline__ Split split(float x) {
-  asm("" : "+v"(x));
-  Split s;
-  s.h = (_Float16)x;
-  s.l = (_Float16)(x - (float)s.h);
-  return s;
+typedef _Float16 half2v __attribute__((ext_vector_type(2)));
+typedef float float2v __attribute__((ext_vector_type(2)));
+// Two elements as upper and lower halves. What is left of one is exact. (The operation before must not become one with the rounding to half: it would round
+// once there and twice for the lower half, which now and then then goes with another upper one.)
+__device__ __forceinline__ void split(float x, float y, half2v& h, half2v& l) {
+  asm("" : "+v"(x), "+v"(y));
+  h = __builtin_convertvector(float2v{x, y}, half2v);
+  l = __builtin_convertvector(float2v{__builtin_fmaf((float)h[0], -1.f, x), __builtin_fmaf((float)h[1], -1.f, y)}, half2v);
+}
+template <typename V, int N>
+__device__ __forceinline__ void split(const float (&x)[N], V& h, V& l) {
+#pragma unroll
+  for (int e = 0; e < N; e += 2) {
+    half2v a, b;
+    split(x[e], x[e + 1], a, b);
+    h[e] = a[0];
+    h[e + 1] = a[1];
+    l[e] = b[0];
+    l[e + 1] = b[1];
+  }
 }
 // Eight neighbouring elements of a plane.
 struct Eight {
@@ -205,12 +214,7 @@ struct Eight {
 __device__ __forceinline__ Eight load_eight(const char* at) { return Eight{*reinterpret_cast<const half8*>(at), *reinterpret_cast<const half8*>(at + kLower)}; }
 __device__ __forceinline__ void store_eight(char* at, const float (&v)[8]) {
   half8 h, l;
-#pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const Split s = split(v[e]);
-    h[e] = s.h;
-    l[e] = s.l;
-  }
+  split(v, h, l);
   *reinterpret_cast<half8*>(at) = h;
   *reinterpret_cast<half8*>(at + kLower) = l;
 }
@@ -648,35 +652,34 @@ __host__ __device__ inline int short_lds(int bands) { return bands * 32 * 512 + 
 struct Plane {
   char* at;
   int rowBytes;      // a multiple of 128
-  __device__ __forceinline__ int piece(int row, int k) const {
-    return row * rowBytes + ((k ^ ((rowBytes & 128) ? row >> 1 & 7 : row & 15)) << 4);
-  }
-  // of the upper half of an element; the lower one is 4 pieces on
-  __device__ __forceinline__ char* upper(int row, int column) const { return at + piece(row, (column >> 5) * 8 + (column >> 3 & 3)) + (column & 7) * 2; }
-  __device__ __forceinline__ char* lower(int row, int column) const { return at + piece(row, (column >> 5) * 8 + 4 + (column >> 3 & 3)) + (column & 7) * 2; }
-  __device__ __forceinline__ void store4(int row, int column, const float (&x)[4]) const {
+  __device__ __forceinline__ int swizzle(int row) const { return (rowBytes & 128) ? row >> 1 & 7 : row & 15; }
+  __device__ __forceinline__ char* piece(int row, int k) const { return at + row * rowBytes + ((k ^ swizzle(row)) << 4); }
+};
+// Four neighbouring elements of a plane: the lower halves' piece is the upper ones' with another bit of its number.
+struct Fours {
+  char* row;
+  int piece;      // its place in the row, without that of the four in it
+  __device__ __forceinline__ half4* upper(int at) const { return reinterpret_cast<half4*>(row + (piece ^ at)); }
+  __device__ __forceinline__ half4* lower(int at) const { return upper(at ^ 64); }
+  __device__ __forceinline__ void store(int at, const float (&x)[4]) const {
     half4 h, l;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const Split s = split(x[e]);
-      h[e] = s.h;
-      l[e] = s.l;
-    }
-    *reinterpret_cast<half4*>(upper(row, column)) = h;
-    *reinterpret_cast<half4*>(lower(row, column)) = l;
+    split(x, h, l);
+    *upper(at) = h;
+    *lower(at) = l;
   }
 };
 // 32 x 32 of P Q' over `blocks` blocks of 32 columns. Two sums side by side, and none in two products in a row (three: 3 % slower).
 __device__ __forceinline__ acc16 small_product(const Plane& P, int i0, const Plane& Q, int j0, int blocks) {
   int lane = threadIdx.x & 63;
   asm volatile("" : "+v"(lane));      // (addresses are made where they are used: kept through the steps they would be registers' spills)
-  const int rowP = i0 + (lane & 31), rowQ = j0 + (lane & 31), k0 = lane >> 5;
+  const int rowP = i0 + (lane & 31), rowQ = j0 + (lane & 31), pieceP = ((lane >> 5) ^ P.swizzle(rowP)) << 4, pieceQ = ((lane >> 5) ^ Q.swizzle(rowQ)) << 4;
+  const char *atP = P.at + rowP * P.rowBytes, *atQ = Q.at + rowQ * Q.rowBytes;
   acc16 high = {}, rest = {};
 #pragma unroll 2
   for (int k = 0; k < 2 * blocks; ++k) {
-    const int at = (k >> 1) * 8 + (k & 1) * 2 + k0;
-    const half8 ph = *reinterpret_cast<const half8*>(P.at + P.piece(rowP, at)), pl = *reinterpret_cast<const half8*>(P.at + P.piece(rowP, at + 4));
-    const half8 qh = *reinterpret_cast<const half8*>(Q.at + Q.piece(rowQ, at)), ql = *reinterpret_cast<const half8*>(Q.at + Q.piece(rowQ, at + 4));
+    const int at = (k >> 1) * 128 + (k & 1) * 32;
+    const half8 ph = *reinterpret_cast<const half8*>(atP + (pieceP ^ at)), pl = *reinterpret_cast<const half8*>(atP + (pieceP ^ at ^ 64));
+    const half8 qh = *reinterpret_cast<const half8*>(atQ + (pieceQ ^ at)), ql = *reinterpret_cast<const half8*>(atQ + (pieceQ ^ at ^ 64));
     rest = __builtin_amdgcn_mfma_f32_32x32x16_f16(ph, ql, rest, 0, 0, 0);
     high = __builtin_amdgcn_mfma_f32_32x32x16_f16(ph, qh, high, 0, 0, 0);
     rest = __builtin_amdgcn_mfma_f32_32x32x16_f16(pl, qh, rest, 0, 0, 0);
@@ -712,31 +715,44 @@ struct Strip {
     j0 = strip * kStrip;
     blocks = (min(kStrip, m.n - j0) + 31) / 32;
     lane = threadIdx.x & 63;
-    wave = threadIdx.x >> 6;
+    wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     square = Plane{lds, bands * 128};
     fresh = Plane{lds, 512};
     across = Plane{lds + bands * 32 * 512, bands * 128};
   }
-  // f(its place) for this wave's product, of `down` x `over`
+  // f(its place) for this wave's product, of `down` x `over`, up to 4 each
   template <typename F>
   __device__ __forceinline__ void each(int down, int over, F f) const {
-    if (wave < down * over) f(wave / over, wave % over);
+    const int ti = (wave * (over == 1 ? 256 : over == 2 ? 128 : over == 3 ? 86 : 64)) >> 8;
+    if (ti < down) f(ti, wave - ti * over);
+  }
+  __device__ __forceinline__ int this_lane() const {
+    int l = lane;
+    asm volatile("" : "+v"(l));
+    return l;
   }
   // f(e0, row, column) for the first of each four rows that a lane has of a product
   template <typename F>
   __device__ __forceinline__ void fours(int ti, int tj, F f) const {
-    int lane = this->lane;
-    asm volatile("" : "+v"(lane));
+    const int lane = this_lane();
 #pragma unroll
     for (int q = 0; q < 4; ++q) f(q * 4, ti * 32 + q * 8 + (lane >> 5) * 4, tj * 32 + (lane & 31));
+  }
+  // The same as the transpose's row of that column holds them, the fours 16 bytes apart, and into it.
+  __device__ __forceinline__ Fours turned(const Plane& plane, int ti, int tj) const {
+    const int lane = this_lane(), row = tj * 32 + (lane & 31);
+    return Fours{plane.at + row * plane.rowBytes + (lane >> 5) * 8, ((ti * 8) ^ plane.swizzle(row)) << 4};
+  }
+  __device__ __forceinline__ void store(const Plane& plane, int ti, int tj, const acc16& x) const {
+    const Fours at = turned(plane, ti, tj);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) at.store(q * 16, {x[q * 4], x[q * 4 + 1], x[q * 4 + 2], x[q * 4 + 3]});
   }
   // Sums as the products leave them to A.
   __device__ __forceinline__ void scaled(acc16& sums) const { sums *= kScaleA / (a.scale * a.scale); }
   // From A to B in the square.
   __device__ __forceinline__ void polynomial(acc16 sums) const {
-    each(bands, bands, [&](int ti, int tj) {
-      fours(ti, tj, [&](int e, int i, int j) { square.store4(j, i, {sums[e], sums[e + 1], sums[e + 2], sums[e + 3]}); });
-    });
+    each(bands, bands, [&](int ti, int tj) { store(square, ti, tj, sums); });
     __syncthreads();
     each(bands, bands, [&](int ti, int tj) {
       const acc16 twice = small_product(square, ti * 32, square, tj * 32, bands);
@@ -744,20 +760,20 @@ struct Strip {
       for (int e = 0; e < 16; ++e) sums[e] = __builtin_fmaf(sums[e], kB * (kScaleB / kScaleA), twice[e] * (kC * kScaleB / (kScaleA * kScaleA)));
     });
     __syncthreads();
-    each(bands, bands, [&](int ti, int tj) {
-      fours(ti, tj, [&](int e, int i, int j) { square.store4(j, i, {sums[e], sums[e + 1], sums[e + 2], sums[e + 3]}); });
-    });
+    each(bands, bands, [&](int ti, int tj) { store(square, ti, tj, sums); });
     __syncthreads();
   }
   // The next X, times its scale and `factor`.
   __device__ __forceinline__ void step(acc16& x, float factor) const {
     each(bands, blocks, [&](int ti, int tj) {
       x = small_product(square, ti * 32, across, tj * 32, bands);
-      fours(ti, tj, [&](int e, int i, int j) {
-        const half4 h = *reinterpret_cast<const half4*>(across.upper(j, i)), l = *reinterpret_cast<const half4*>(across.lower(j, i));
+      const Fours at = turned(across, ti, tj);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) x[e + k] = __builtin_fmaf((float)h[k] + (float)l[k], kA, x[e + k] * (1.f / kScaleB)) * factor;
-      });
+      for (int q = 0; q < 4; ++q) {
+        const half4 h = *at.upper(q * 16), l = *at.lower(q * 16);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) x[q * 4 + k] = __builtin_fmaf((float)h[k] + (float)l[k], kA, x[q * 4 + k] * (1.f / kScaleB)) * factor;
+      }
     });
     __syncthreads();
   }
@@ -766,9 +782,7 @@ struct Strip {
     const Plane other{across.at, bands * 128};
 #pragma unroll 1
     for (int k = 0; k < 2; ++k) {
-      each(bands, bands, [&](int ti, int tj) {
-        fours(ti, tj, [&](int e, int i, int j) { other.store4(j, i, {sums[e], sums[e + 1], sums[e + 2], sums[e + 3]}); });
-      });
+      each(bands, bands, [&](int ti, int tj) { store(other, ti, tj, sums); });
       __syncthreads();
       each(bands, bands, [&](int ti, int tj) {
         const acc16 rest = small_product(square, ti * 32, other, tj * 32, bands);
@@ -777,20 +791,21 @@ struct Strip {
       });
       __syncthreads();
     }
-    each(bands, blocks, [&](int ti, int tj) {
-      fours(ti, tj, [&](int e, int i, int j) { across.store4(j, i, {x[e], x[e + 1], x[e + 2], x[e + 3]}); });
-    });
+    each(bands, blocks, [&](int ti, int tj) { store(across, ti, tj, x); });
   }
   // X into both planes, then the strip's share of A.
   __device__ __forceinline__ void gram(const acc16& x, acc16& sums) const {
     each(bands, blocks, [&](int ti, int tj) {
-      fours(ti, tj, [&](int e, int i, int j) {
-        const float v[4] = {x[e], x[e + 1], x[e + 2], x[e + 3]};
-        across.store4(j, i, v);
-        float row[4] = {v[0], v[1], v[2], v[3]};
-        transpose4(row);
-        fresh.store4(i + (lane & 3), j & ~3, row);
-      });
+      store(across, ti, tj, x);
+      // rows, of which a lane has every eighth
+      const int lane = this_lane(), row = ti * 32 + (lane >> 5) * 4 + (lane & 3);
+      const Fours at{fresh.at + row * 512 + (lane & 4) * 2, ((tj * 8 + (lane >> 3 & 3)) ^ (row & 15)) << 4};
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        float four[4] = {x[q * 4], x[q * 4 + 1], x[q * 4 + 2], x[q * 4 + 3]};
+        transpose4(four);
+        Fours{at.row + q * 8 * 512, at.piece}.store((q & 1) * 128, four);      // (eight rows on, the swizzle has another bit)
+      }
     });
     __syncthreads();
     each(bands, bands, [&](int ti, int tj) { sums = small_product(fresh, ti * 32, fresh, tj * 32, blocks); });
@@ -827,13 +842,17 @@ struct Strip {
   }
 };
 
-// The strip's transpose and its share of A into memory.
+// The strip's transpose and its share of A into memory. Of each row 32 lanes have a piece, of which there are 32 at most.
+constexpr int kStripLoads = kStrip * 32 / kShortThreads;
 __device__ __forceinline__ void leave(const Strip& strip, const acc16& sums, char* work, uint32_t index, int turn) {
   const Matrix& a = strip.a;
-  const int pieces = strip.bands * 8, rows = min(kStrip, a.n - strip.j0);
+  const int pieces = strip.bands * 8, rows = min(kStrip, a.n - strip.j0), piece = threadIdx.x & 31;
   uint4v* to = reinterpret_cast<uint4v*>(work + (int64_t)strip.j0 * strip.bands * 128);
-  for (int k = threadIdx.x; k < rows * pieces; k += kShortThreads)
-    to[k] = *reinterpret_cast<const uint4v*>(strip.across.at + strip.across.piece(k / pieces, k % pieces));
+#pragma unroll
+  for (int q = 0; q < kStripLoads; ++q) {
+    const int row = (threadIdx.x >> 5) + q * (kShortThreads / 32);
+    if (row < rows && piece < pieces) to[row * pieces + piece] = *reinterpret_cast<const uint4v*>(strip.across.piece(row, piece));
+  }
   acc16* share = reinterpret_cast<acc16*>(work + plane_t(a) + ((int64_t)turn * strips_of(a) + index) * gram_bytes(a));
   strip.each(strip.bands, strip.bands, [&](int ti, int tj) { share[(ti * strip.bands + tj) * 64 + strip.lane] = sums; });
 }
@@ -957,13 +976,13 @@ __global__ __launch_bounds__(kShortThreads) void short_step_kernel(Group g, Upda
   const Strip strip(a, (int)p.index, lds);
   char* work = a.work + p.batch * short_bytes(a);
   // the strip's transpose is on its way while A is made
-  const int pieces = strip.bands * 8, rows = min(kStrip, a.n - strip.j0), all = kStrip * pieces;
+  const int pieces = strip.bands * 8, rows = min(kStrip, a.n - strip.j0), piece = threadIdx.x & 31;
   const uint4v* from = reinterpret_cast<const uint4v*>(work + (int64_t)strip.j0 * strip.bands * 128);
-  uint4v held[4];
+  uint4v held[kStripLoads];
 #pragma unroll
-  for (int q = 0; q < 4; ++q) {
-    const int k = threadIdx.x + q * kShortThreads;
-    held[q] = k < rows * pieces ? from[k] : uint4v{0, 0, 0, 0};
+  for (int q = 0; q < kStripLoads; ++q) {
+    const int row = (threadIdx.x >> 5) + q * (kShortThreads / 32);
+    held[q] = row < rows && piece < pieces ? from[row * pieces + piece] : uint4v{0, 0, 0, 0};
   }
   const int strips = strips_of(a);
   const int64_t bytes = gram_bytes(a);
@@ -978,18 +997,17 @@ __global__ __launch_bounds__(kShortThreads) void short_step_kernel(Group g, Upda
     norm = sqrt(norm) + (double)h.eps;
   }
   float factor = weighed ? strip_factor(norm, norms[p.index], a) : 1.f;
+  const float factors = weighed && !summed ? strip_factor(norm, norms[min(strip.lane, strips - 1)], a) : 1.f;      // of as many strips as lanes
   strip.each(strip.bands, strip.bands, [&](int ti, int tj) {
     const acc16* mine = reinterpret_cast<const acc16*>(shares) + (ti * strip.bands + tj) * 64 + strip.lane;
     for (int k = 0; k < (summed ? 1 : strips); ++k) {
-      const float f = weighed && !summed ? strip_factor(norm, norms[k], a) : 1.f;
+      const float f = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(factors), k));
       sums += mine[k * (bytes / 64)] * (f * f);
     }
   });
 #pragma unroll
-  for (int q = 0; q < 4; ++q) {
-    const int k = threadIdx.x + q * kShortThreads;
-    if (k < all) *reinterpret_cast<uint4v*>(strip.across.at + strip.across.piece(k / pieces, k % pieces)) = held[q];
-  }
+  for (int q = 0; q < kStripLoads; ++q)
+    if (piece < pieces) *reinterpret_cast<uint4v*>(strip.across.piece((threadIdx.x >> 5) + q * (kShortThreads / 32), piece)) = held[q];
   strip.scaled(sums);
 #pragma unroll 1
   for (int k = 0;;) {
