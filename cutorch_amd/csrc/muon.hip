@@ -193,7 +193,10 @@ typedef float float2v __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ void split(float x, float y, half2v& h, half2v& l) {
   asm("" : "+v"(x), "+v"(y));
   h = __builtin_convertvector(float2v{x, y}, half2v);
-  l = __builtin_convertvector(float2v{__builtin_fmaf((float)h[0], -1.f, x), __builtin_fmaf((float)h[1], -1.f, y)}, half2v);
+  float2v left;
+  asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(left[0]) : "v"(h), "v"(x));
+  asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(left[1]) : "v"(h), "v"(y));
+  l = __builtin_convertvector(left, half2v);
 }
 template <typename V, int N>
 __device__ __forceinline__ void split(const float (&x)[N], V& h, V& l) {
@@ -632,9 +635,11 @@ __global__ __launch_bounds__(256, 2) void product_kernel(Group g, Update h, Way 
 // ---------------------------------------------------------- short matrices --
 // Up to 128 rows: A and B are one tile each, and what bounds a step is how long its launches wait for memory one after another (12 matrices of 65 x 513: 17
 // launches of 9 to 17 us each). A workgroup has a strip of 128 columns of X. It adds up the strips' shares of A, makes B of it by itself,
-// takes its strip through the step and leaves the strip's share of the next A. Two steps a launch (three of halves) where it takes A along, P A P: a launch
-// costs some 8 us, a step in it 8 (12 of 65 x 513 floats 98 us with a launch for each, 82 so; of 128 x 512 121 and 106), most of them in its products'
-// reads of LDS and in splitting what they leave. One launch for all steps where X is a single strip, which makes each A from X.
+// takes its strip through the step and leaves the strip's share of the next A. Two steps
+// a launch (three of halves) where it takes A along, P A P: 12 of 65 x 513 floats took 98 us with a launch for each step and 82 so; 67 since strips
+// begin without a launch for the norm and the kernels have a third of the instructions. Of a launch's 49 thousand cycles for two steps a CU's four SIMDs have
+// vector instructions for 21 thousand, matrix ones for 10, and LDS is read or written in 13: nine waves that wait for one another at barriers.
+// One launch for all steps where X is a single strip, which makes each A from X.
 // LDS: one plane for A, then B, then the new X, a second one for the strip's transpose, both split, rows of 16-byte pieces in the order of their
 // number xor what brings sixteen rows to different banks.
 // No launch makes the norm first: a strip begins over its own norm, by a power of two, and the step that adds up the shares knows all strips' norms.
@@ -674,15 +679,21 @@ __device__ __forceinline__ acc16 small_product(const Plane& P, int i0, const Pla
   asm volatile("" : "+v"(lane));      // (addresses are made where they are used: kept through the steps they would be registers' spills)
   const int rowP = i0 + (lane & 31), rowQ = j0 + (lane & 31), pieceP = ((lane >> 5) ^ P.swizzle(rowP)) << 4, pieceQ = ((lane >> 5) ^ Q.swizzle(rowQ)) << 4;
   const char *atP = P.at + rowP * P.rowBytes, *atQ = Q.at + rowQ * Q.rowBytes;
-  acc16 high = {}, rest = {};
-#pragma unroll 2
-  for (int k = 0; k < 2 * blocks; ++k) {
-    const int at = (k >> 1) * 128 + (k & 1) * 32;
+  acc16 high, rest;
+  // (the first products take their sums' zeros as a constant)
+  auto add = [&](int at, const acc16& h, const acc16& r) {
     const half8 ph = *reinterpret_cast<const half8*>(atP + (pieceP ^ at)), pl = *reinterpret_cast<const half8*>(atP + (pieceP ^ at ^ 64));
     const half8 qh = *reinterpret_cast<const half8*>(atQ + (pieceQ ^ at)), ql = *reinterpret_cast<const half8*>(atQ + (pieceQ ^ at ^ 64));
-    rest = __builtin_amdgcn_mfma_f32_32x32x16_f16(ph, ql, rest, 0, 0, 0);
-    high = __builtin_amdgcn_mfma_f32_32x32x16_f16(ph, qh, high, 0, 0, 0);
+    rest = __builtin_amdgcn_mfma_f32_32x32x16_f16(ph, ql, r, 0, 0, 0);
+    high = __builtin_amdgcn_mfma_f32_32x32x16_f16(ph, qh, h, 0, 0, 0);
     rest = __builtin_amdgcn_mfma_f32_32x32x16_f16(pl, qh, rest, 0, 0, 0);
+  };
+  add(0, acc16{}, acc16{});
+  add(32, high, rest);
+#pragma unroll 1
+  for (int k = 1; k < blocks; ++k) {
+    add(k * 128, high, rest);
+    add(k * 128 + 32, high, rest);
   }
   return high + rest;
 }
