@@ -637,7 +637,7 @@ __global__ __launch_bounds__(256, 2) void product_kernel(Group g, Update h, Way 
 // launches of 9 to 17 us each). A workgroup has a strip of 128 columns of X. It adds up the strips' shares of A, makes B of it by itself,
 // takes its strip through the step and leaves the strip's share of the next A. Two steps
 // a launch (three of halves) where it takes A along, P A P: 12 of 65 x 513 floats took 98 us with a launch for each step and 82 so; 67 since strips
-// begin without a launch for the norm and the kernels have a third of the instructions. Of a launch's 49 thousand cycles for two steps a CU's four SIMDs have
+// begin without a launch for the norm and the kernels have 0.6 of the instructions. Of a launch's 49 thousand cycles for two steps a CU's four SIMDs have
 // vector instructions for 21 thousand, matrix ones for 10, and LDS is read or written in 13: nine waves that wait for one another at barriers.
 // One launch for all steps where X is a single strip, which makes each A from X.
 // LDS: one plane for A, then B, then the new X, a second one for the strip's transpose, both split, rows of 16-byte pieces in the order of their
