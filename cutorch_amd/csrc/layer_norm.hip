@@ -137,7 +137,7 @@ __device__ __forceinline__ void load_columns(const T* from, const Packs<V, L, P>
 }
 
 // A team of L lanes has a row in registers from its read to its write; teams go on to other rows with the weights that they hold, the next of which is
-// asked for before the one at hand is computed. Bound by memory: 16392 rows of 2048 halves 25.3 us, 5.3 TB/s.
+// asked for before the one at hand is computed. Bound by memory: 16392 rows of 2048 halves 24.6 us, 5.5 TB/s.
 template <typename T, int V, int L, int TEAMS, int P>
 __global__ __launch_bounds__(L * TEAMS) void norm_kernel(NormArgs<T> a) {
   __shared__ float lds[L > 64 ? 3 * TEAMS * (L / 64) : 1];
@@ -204,7 +204,7 @@ struct GradArgs {
 };
 
 // The same with the sums over rows of what a lane's columns add to the weights' gradients, which stay in its registers; the workgroup's teams join
-// theirs at the end. Bound by memory and, in halves, by arithmetic nearly as much: 16392 rows of 4096 halves 88 us with the joining launch, 4.6 TB/s.
+// theirs at the end. Bound by memory and, in halves, by arithmetic nearly as much: 16392 rows of 4096 halves 83 us with the joining launch, 4.8 TB/s.
 template <typename T, int V, int L, int TEAMS, int P, bool WEIGHTS, bool AHEAD>
 __global__ __launch_bounds__(L * TEAMS, 2) void norm_grad_kernel(GradArgs<T> a) {
   __shared__ float lds[L > 64 ? 5 * TEAMS * (L / 64) : 1];
@@ -501,12 +501,13 @@ void launch_norm(THCState* s, const NormArgs<T>& a) {
   const int64_t cus = num_compute_units(s), packs = (a.dim + V - 1) / V;
   auto go = [&](auto vec, auto lanes, auto teams, auto each) {
     constexpr int VV = decltype(vec)::value, L = decltype(lanes)::value, TEAMS = decltype(teams)::value, P = decltype(each)::value;
-    const int64_t groups = ((int64_t)a.rows + TEAMS - 1) / TEAMS, most = cus * std::max(1, (P == 1 ? 2048 : 1024) / (L * TEAMS));
+    const int64_t groups = ((int64_t)a.rows + TEAMS - 1) / TEAMS, most = cus * std::max(1, (P == 1 ? 2048 : packs <= 256 ? 1024 : 512) / (L * TEAMS));
     hipLaunchKernelGGL((norm_kernel<T, VV, L, TEAMS, P>), dim3((unsigned)std::min(groups, most)), dim3(L * TEAMS), 0, st, a);
   };
 #define GO(VV, L, TEAMS, P) go(integral_constant<int, VV>{}, integral_constant<int, L>{}, integral_constant<int, TEAMS>{}, integral_constant<int, P>{})
   // Two packs a lane where rows have them: half of the lanes that meet at a sum. us for 16392 rows of 2048 halves with 64 lanes of 4 packs, 128 of 2 and 256 of
-  // 1: 26.5, 25.3, 31.2; 65536 of 500 with 32 of 2 and 64 of 1 32.2, 34.4.
+  // 1: 29.2, 25.3, 26.4. Threads a CU: with 512, 1024 and 2048 16384 rows of 2048 halves 26.1, 25.1, 27.7, 65536 of 500 38.6, 30.5, 32.8; 8192 of 8192
+  // 46.4, 51.1, 48.3, 16384 of 2000 floats 44.9, 47.9, 48.6; 65536 of 64 floats 8.9, 7.9, 7.3.
   if (a.dim < V) GO(1, 8, 32, 1);
   else if (packs <= 8) GO(V, 8, 32, 1);
   else if (packs <= 16) GO(V, 16, 16, 1);
@@ -561,8 +562,8 @@ void launch_grad(THCState* s, GradArgs<T>& a, const WeightGrads<T>& to) {
 #define GO(VV, L, TEAMS, P, A, THREADS) \
   go(integral_constant<int, VV>{}, integral_constant<int, L>{}, integral_constant<int, TEAMS>{}, integral_constant<int, P>{}, integral_constant<bool, A>{}, THREADS)
   // The last number: threads a CU. More hide the two sums of a row better, and make more rows of sums that cross memory. us with 512, 768 and 1024 of
-  // them: 16384 rows of 4096 halves 90, 88, 106, of 2048 48, 50, 59, 16384 of 2000 floats 76, 80, 84; 65536 of 500 halves 63, 56, 55. The next row is
-  // asked for early where registers allow it (4096 halves 148 without, 88 with).
+  // them: 16384 rows of 4096 halves 83, 88, 103, of 2048 45, 49, 56, 16384 of 2000 floats 74, 79, 83; 65536 of 500 halves 53, 47, 47. The next row is
+  // asked for early where registers allow it (4096 halves 148 without, 88 with, in 768; two rows early 2 to 6 % slower).
   if (a.dim < V) GO(1, 8, 32, 1, true, 1024);
   else if (packs <= 8) GO(V, 8, 32, 1, true, 1024);
   else if (packs <= 16) GO(V, 16, 16, 1, true, 1024);
@@ -570,7 +571,7 @@ void launch_grad(THCState* s, GradArgs<T>& a, const WeightGrads<T>& to) {
   else if (packs <= 64) GO(V, 64, 4, 1, true, 1024);
   else if (packs <= 128) GO(V, 64, 4, 2, true, 512);
   else if (packs <= 256) GO(V, 128, 2, 2, true, 512);
-  else if (packs <= 512) GO(V, 256, 1, 2, true, V == 8 ? 768 : 512);
+  else if (packs <= 512) GO(V, 256, 1, 2, true, 512);
   else if (packs <= 1024) GO(V, 256, 1, 4, true, 512);
   else if (packs <= 2048) GO(V, 512, 1, 4, true, 512);
   else if (V == 4 && packs <= 4096) GO(V, (V == 4 ? 1024 : 512), 1, 4, (V == 8), 1024);
