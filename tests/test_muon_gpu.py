@@ -388,3 +388,34 @@ def test_one_element_a_row_of_long_matrices(thc, kind, rows, cols):
     # 10 roundings a step relative to the value, as where steps go one by one, and those of the shared products: five of an operand for each of three
     # steps more, which a following step makes at most 2.8 of (a^2 of A's relative error against the slope of its square root's)
     assert np.all(np.abs(got[at] - want) <= ((5 * 10 + 3 * 5 * 2.8) * 2.0 ** -22 + UNIT[kind] * 1.01) * np.abs(want) * 1.5), np.max(np.abs(got[at] / want - 1))
+
+
+@pytest.mark.parametrize("kind", ["float", "half"])
+@pytest.mark.parametrize("shape", [(4, 40, 300), (4, 1400, 30), (4, 130, 270), (4, 150, 160)])
+def test_not_finite_matrices_of_a_batch(thc, kind, shape):
+    rng = np.random.default_rng(sum(shape))
+    g = np.stack([_matrix(rng, shape[1], shape[2], kind) for _ in range(4)])
+    g[0, -1, -1] = np.nan
+    g[1, 0, -1] = np.inf
+    g[2] = 0
+    t = thc.Tensor.from_numpy
+    got = thc.Tensor(kind).orthogonalize(t(g)).numpy()
+    assert np.all(np.isnan(got[:2])) and np.all(got[2] == 0)
+    assert_bit_equal(got[3], thc.Tensor(kind).orthogonalize(t(g[3])).numpy())
+
+
+@pytest.mark.parametrize("kind", ["float", "half"])
+@pytest.mark.parametrize("rows,cols", [(60, 700), (700, 60), (100, 1900)])
+def test_strips_of_other_sizes(thc, kind, rows, cols):
+    """Matrices of up to 128 rows go in strips of 128 columns, each first over its own norm: strips of zeros, of tiny and of large elements."""
+    rng = np.random.default_rng(rows)
+    g = _matrix(rng, min(rows, cols), max(rows, cols), kind).astype(np.float64)
+    g[:, :128] *= 2.0 ** -9
+    g[:, 128:256] = 0
+    g[:, 256:384] *= 2.0 ** 5
+    g[:, 640:] *= 2.0 ** -14
+    g = np.ascontiguousarray(g if rows < cols else g.T).astype(NP[kind])
+    _check(thc.Tensor(kind).orthogonalize(thc.Tensor.from_numpy(g)).numpy(), g, kind)
+    if kind == "float":      # far beyond what is left of the result at all
+        g.reshape(rows, cols)[(slice(None), slice(640, None)) if rows < cols else slice(640, None)] *= np.float32(2.0 ** -110)
+        _check(thc.Tensor(kind).orthogonalize(thc.Tensor.from_numpy(g)).numpy(), g, kind)
