@@ -291,7 +291,7 @@ __global__ __launch_bounds__(kBlock) void split_kernel(Group g, Update h, const 
 // with the cores busy in 60 % of the cycles at 1.9 GHz; a library's product of halves of that size reaches 1190. A row's eight 16-byte pieces lie in the order of their number xor half the row's, so that
 // sixteen lanes that read the same piece of neighbouring rows meet all banks. (Blocks of 16 columns, four of which are on their way: 5 % slower, as
 // waves meet at twice as many barriers.)
-// Few matrices of some hundred rows would leave most CUs idle with that: they take tiles of 64 x 64, a wave's part 32 x 32, three blocks on their way. The
+// Few matrices of some hundred rows would leave most CUs idle with that: they take tiles of 64 x 64, a wave's part 32 x 32, four blocks in LDS. The
 // sums of an element are the same ones.
 constexpr int kTile = 128, kSmallTile = 64;
 __host__ __device__ inline int32_t tiles_of(int32_t n, int32_t tile) { return (n + tile - 1) / tile; }
@@ -362,52 +362,93 @@ __device__ __forceinline__ void product(const Operand& P, const Operand& Q, int3
   acc16 acc[W][W] = {};
   int32_t part = first, until = part_begin(blocks, parts, first + 1);
   const int32_t begin = part_begin(blocks, parts, first), end = part_begin(blocks, parts, last);
+  // products into the same sums lie W x W apart
+  auto products = [&](const half8 (&p)[W], const half8 (&q)[W]) {
 #pragma unroll
-  for (int k = 0; k < kStages - 1; ++k)
-    if (begin + k < end) load(begin + k, k);
-  uint32_t stage = 0;
-  for (int32_t k = begin; k < end; ++k) {
-    if (k == until) {
-      until = part_begin(blocks, parts, ++part + 1);
+    for (int i = 0; i < W; ++i)
 #pragma unroll
-      for (int q = 0; q < W * W; ++q) {
-        total[q / W][q % W] += acc[q / W][q % W];
-        acc[q / W][q % W] = acc16{};
-      }
-    }
-    // this block is there when only the later ones' loads are on their way; the one that is asked for now takes the room that was read last before
-    // the barrier
-    if (kStages > 2 && k + kStages - 2 < end) wait_loads_and_barrier<2 * U * (kStages - 2)>();
-    else wait_loads_and_barrier<0>();
-    if (k + kStages - 1 < end) load(k + kStages - 1, stage == 0 ? kStages - 1 : stage - 1);
+      for (int j = 0; j < W; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(p[i], q[j], acc[i][j], 0, 0, 0);
+  };
+  // 16 of a block's columns
+  struct Half {
+    half8 ph[W], pl[W], qh[W], ql[W];
+  };
+  auto read = [&](uint32_t stage, int s, Half& b) {
     const char *fp = lds + stage * kStageBytes + rowP, *fq = lds + stage * kStageBytes + rowQ;
-    stage = stage == kStages - 1 ? 0 : stage + 1;
-    // all of the block's operands are asked for before the first product (2 % quicker than by halves)
-    half8 ph[2][W], pl[2][W], qh[2][W], ql[2][W];
+    const int swizzle = (lane >> 1) & 7, high = ((2 * s + (lane >> 5)) ^ swizzle) * 16, low = ((4 + 2 * s + (lane >> 5)) ^ swizzle) * 16;
 #pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      const int swizzle = (lane >> 1) & 7, high = ((2 * s + (lane >> 5)) ^ swizzle) * 16, low = ((4 + 2 * s + (lane >> 5)) ^ swizzle) * 16;
-#pragma unroll
-      for (int i = 0; i < W; ++i) {
-        ph[s][i] = *reinterpret_cast<const half8*>(fp + i * 32 * kBlockBytes + high);
-        qh[s][i] = *reinterpret_cast<const half8*>(fq + i * 32 * kBlockBytes + high);
-        ql[s][i] = *reinterpret_cast<const half8*>(fq + i * 32 * kBlockBytes + low);
-        pl[s][i] = *reinterpret_cast<const half8*>(fp + i * 32 * kBlockBytes + low);
-      }
+    for (int i = 0; i < W; ++i) {
+      b.ph[i] = *reinterpret_cast<const half8*>(fp + i * 32 * kBlockBytes + high);
+      b.qh[i] = *reinterpret_cast<const half8*>(fq + i * 32 * kBlockBytes + high);
+      b.ql[i] = *reinterpret_cast<const half8*>(fq + i * 32 * kBlockBytes + low);
+      b.pl[i] = *reinterpret_cast<const half8*>(fp + i * 32 * kBlockBytes + low);
     }
-    __builtin_amdgcn_sched_barrier(0);
-    // products into the same sums lie W x W apart
-    auto products = [&](const half8 (&p)[W], const half8 (&q)[W]) {
+  };
+  auto multiply = [&](const Half& b) {
+    products(b.ph, b.qh);
+    products(b.ph, b.ql);
+    products(b.pl, b.qh);
+  };
+  auto next_part = [&](int32_t k) {
+    if (k != until) return;
+    until = part_begin(blocks, parts, ++part + 1);
 #pragma unroll
-      for (int i = 0; i < W; ++i)
-#pragma unroll
-        for (int j = 0; j < W; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(p[i], q[j], acc[i][j], 0, 0, 0);
+    for (int q = 0; q < W * W; ++q) {
+      total[q / W][q % W] += acc[q / W][q % W];
+      acc[q / W][q % W] = acc16{};
+    }
+  };
+  auto after = [](uint32_t stage) { return stage == kStages - 1 ? 0 : stage + 1; };
+  uint32_t stage = 0;
+  if constexpr (TILE == kTile) {
+    if (begin < end) load(begin, 0);
+    for (int32_t k = begin; k < end; ++k) {
+      next_part(k);
+      // this block is there; the one that is asked for now takes the room that was read last before the barrier
+      wait_loads_and_barrier<0>();
+      if (k + 1 < end) load(k + 1, after(stage));
+      // all of the block's operands are asked for before the first product (2 % quicker than by halves)
+      Half one, two;
+      read(stage, 0, one);
+      read(stage, 1, two);
+      stage = after(stage);
+      __builtin_amdgcn_sched_barrier(0);
+      multiply(one);
+      multiply(two);
+    }
+  } else {
+    // Half a block is read while the one before it is multiplied: a CU often has no other workgroup that would do so (one matrix of 1024 x 1024 267 -> 252 us; in
+    // large tiles 1 to 4 % slower, a whole block ahead 3 % slower). A block's room is free when all waves have its second half.
+    auto lds_is_here = [] {      // (known to the compiler, which otherwise waits for the reads behind those as well)
+      __builtin_amdgcn_s_waitcnt(0xc07f);
+      __builtin_amdgcn_sched_barrier(0);
     };
 #pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      products(ph[s], qh[s]);
-      products(ph[s], ql[s]);
-      products(pl[s], qh[s]);
+    for (int k = 0; k < kStages; ++k)
+      if (begin + k < end) load(begin + k, k);
+    if (begin + kStages <= end) wait_loads_and_barrier<2 * U * (kStages - 1)>();
+    else wait_loads_and_barrier<0>();
+    Half one, two;
+    read(0, 0, one);
+    for (int32_t k = begin; k < end; ++k) {
+      next_part(k);
+      lds_is_here();
+      read(stage, 1, two);
+      __builtin_amdgcn_sched_barrier(0);
+      multiply(one);
+      __builtin_amdgcn_sched_barrier(0);
+      lds_is_here();
+      if (k + 1 < end) {
+        // (of the next block's loads and those behind it, the latter may be on their way)
+        if (k + kStages <= end) wait_loads_and_barrier<2 * U * (kStages - 2)>();
+        else wait_loads_and_barrier<0>();
+        if (k + kStages < end) load(k + kStages, stage);
+        stage = after(stage);
+        read(stage, 0, one);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      multiply(two);
+      __builtin_amdgcn_sched_barrier(0);
     }
   }
 #pragma unroll
