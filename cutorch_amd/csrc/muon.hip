@@ -686,6 +686,7 @@ __global__ __launch_bounds__(256, 2) void product_kernel(Group g, Update h, Way 
 // No launch makes the norm first: a strip begins over its own norm, by a power of two, and the step that adds up the shares knows all strips' norms.
 constexpr int kShortThreads = 1024, kShort = 128, kStrip = 128;
 __host__ __device__ inline bool is_short(const Matrix& a) { return a.m <= kShort; }
+__host__ __device__ inline bool is_thin(const Matrix& a) { return a.m <= 32; }
 __host__ __device__ inline bool is_alone(const Matrix& a) { return is_short(a) && a.n <= kStrip; }
 __host__ __device__ inline int32_t strips_of(const Matrix& a) { return (a.n + kStrip - 1) / kStrip; }
 __host__ __device__ inline int32_t bands_of(const Matrix& a) { return (a.m + 31) / 32; }
@@ -715,7 +716,8 @@ struct Fours {
   }
 };
 // 32 x 32 of P Q' over `blocks` blocks of 32 columns. Two sums side by side, and none in two products in a row (three: 3 % slower).
-__device__ __forceinline__ acc16 small_product(const Plane& P, int i0, const Plane& Q, int j0, int blocks) {
+// `fine`: the lower halves' product too.
+__device__ __forceinline__ acc16 small_product(const Plane& P, int i0, const Plane& Q, int j0, int blocks, bool fine) {
   int lane = threadIdx.x & 63;
   asm volatile("" : "+v"(lane));      // (addresses are made where they are used: kept through the steps they would be registers' spills)
   const int rowP = i0 + (lane & 31), rowQ = j0 + (lane & 31), pieceP = ((lane >> 5) ^ P.swizzle(rowP)) << 4, pieceQ = ((lane >> 5) ^ Q.swizzle(rowQ)) << 4;
@@ -728,6 +730,7 @@ __device__ __forceinline__ acc16 small_product(const Plane& P, int i0, const Pla
     rest = __builtin_amdgcn_mfma_f32_32x32x16_f16(ph, ql, r, 0, 0, 0);
     high = __builtin_amdgcn_mfma_f32_32x32x16_f16(ph, qh, h, 0, 0, 0);
     rest = __builtin_amdgcn_mfma_f32_32x32x16_f16(pl, qh, rest, 0, 0, 0);
+    if (fine) rest = __builtin_amdgcn_mfma_f32_32x32x16_f16(pl, ql, rest, 0, 0, 0);
   };
   add(0, acc16{}, acc16{});
   add(32, high, rest);
@@ -807,7 +810,7 @@ struct Strip {
     each(bands, bands, [&](int ti, int tj) { store(square, ti, tj, sums); });
     __syncthreads();
     each(bands, bands, [&](int ti, int tj) {
-      const acc16 twice = small_product(square, ti * 32, square, tj * 32, bands);
+      const acc16 twice = small_product(square, ti * 32, square, tj * 32, bands, bands == 1);
 #pragma unroll
       for (int e = 0; e < 16; ++e) sums[e] = __builtin_fmaf(sums[e], kB * (kScaleB / kScaleA), twice[e] * (kC * kScaleB / (kScaleA * kScaleA)));
     });
@@ -818,7 +821,7 @@ struct Strip {
   // The next X, times its scale and `factor`.
   __device__ __forceinline__ void step(acc16& x, float factor) const {
     each(bands, blocks, [&](int ti, int tj) {
-      x = small_product(square, ti * 32, across, tj * 32, bands);
+      x = small_product(square, ti * 32, across, tj * 32, bands, bands == 1);
       const Fours at = turned(across, ti, tj);
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
@@ -837,7 +840,7 @@ struct Strip {
       each(bands, bands, [&](int ti, int tj) { store(other, ti, tj, sums); });
       __syncthreads();
       each(bands, bands, [&](int ti, int tj) {
-        const acc16 rest = small_product(square, ti * 32, other, tj * 32, bands);
+        const acc16 rest = small_product(square, ti * 32, other, tj * 32, bands, bands == 1);
 #pragma unroll
         for (int e = 0; e < 16; ++e) sums[e] = __builtin_fmaf(sums[e], kA, rest[e] * (1.f / kScaleB));
       });
@@ -860,7 +863,7 @@ struct Strip {
       }
     });
     __syncthreads();
-    each(bands, bands, [&](int ti, int tj) { sums = small_product(fresh, ti * 32, fresh, tj * 32, blocks); });
+    each(bands, bands, [&](int ti, int tj) { sums = small_product(fresh, ti * 32, fresh, tj * 32, blocks, bands == 1); });
     __syncthreads();
   }
   // Element (row, column of the strip) of a matrix that begins at element `at` of its tensor; -1: there is none.
@@ -1107,8 +1110,8 @@ constexpr int64_t kPassBytes = int64_t(2) << 30;
 struct Bytes {
   int64_t work, norms;
 };
-enum Kind { kShortOnes, kLongOnes, kOthers };      // whose launches are others
-int kind_of(const Matrix& a) { return is_short(a) ? kShortOnes : is_long(a) ? kLongOnes : kOthers; }
+enum Kind { kThinOnes, kShortOnes, kLongOnes, kOthers };      // whose launches are others
+int kind_of(const Matrix& a) { return is_thin(a) ? kThinOnes : is_short(a) ? kShortOnes : is_long(a) ? kLongOnes : kOthers; }
 int64_t each_bytes(const Matrix& a) { return is_short(a) ? short_bytes(a) : work_bytes(a); }
 Bytes bytes_of(const Matrix& a) { return Bytes{each_bytes(a) * a.batch, is_short(a) ? 0 : (int64_t)norm_parts(a) * a.batch * 8}; }
 
@@ -1178,10 +1181,15 @@ struct Plan {
 };
 
 // How many steps go with one A from X. An error of A grows with what it belongs to, up to 12 times a step where singular values are small. Two steps
-// leave what single ones do: against 64 bits after five steps, of the result's norm, singly, as 2 + 2 + 1 and by products of floats: 12 of 65 x 513 1.1e-6,
-// 1.2e-6, 1.3e-6, 2 of 256 x 1024 1.5e-6, 2.3e-6, 1.7e-6, 1024 x 4096 1.8e-6, 1.9e-6, 3.3e-6. 3 + 2 is as good where many directions share the norm (2.1e-6
+// leave what single ones do: against 64 bits after five steps, of the result's norm, singly, as 2 + 2 + 1 and by products of floats: 12 of 65 x 513 1.2e-6,
+// 1.3e-6, 1.3e-6, 300 x 700 1.7e-6, 2.5e-6, 1.9e-6, 1024 x 4096 1.8e-6, 1.9e-6, 3.3e-6. 3 + 2 is as good where many directions share the norm (2.1e-6
 // of 1024 x 4096), not where few do (3.2e-6 of 65 x 513, 6.7e-6 of 33 x 500; 4 + 1 2e-5 to 6e-5): for halves, which come with 2e-4 of their own.
-int chain_of(int done, int steps, bool halves) { return halves && done == 0 && steps % 2 && steps >= 3 ? 3 : std::min(2, steps - done); }
+// Up to 32 rows sums of floats round least, and the later pairs would show (23 x 1024 9e-7, floats 6.4e-7): two first, then singly, and all four products of
+// halves, 7e-7 (44 us instead of 39).
+int chain_of(int done, int steps, bool halves, bool thin) {
+  if (halves) return done == 0 && steps % 2 && steps >= 3 ? 3 : std::min(2, steps - done);
+  return std::min(thin && done ? 1 : 2, steps - done);
+}
 template <typename T, bool MUON>
 void run_short(THCState* s, Group& g, const Update& h, int steps) {
   hipStream_t st = current_stream(s);
@@ -1212,7 +1220,7 @@ void run_short(THCState* s, Group& g, const Update& h, int steps) {
   }
   hipLaunchKernelGGL(roomy(short_begin_kernel<T, MUON, false>), strips, threads, lds, st, g, h, steps);
   for (int done = 0, turn = 0; done < steps; turn ^= 1) {
-    const int chain = chain_of(done, steps, std::is_same_v<T, __half>);
+    const int chain = chain_of(done, steps, std::is_same_v<T, __half>, is_thin(g.matrix[0]));
     const bool first = done == 0;
     done += chain;
     if (many) hipLaunchKernelGGL(shares_kernel, dim3(parts), dim3(kShareThreads), 0, st, shares, h, turn, first);
@@ -1244,7 +1252,7 @@ void run_group(THCState* s, Group& g, const Update& h, int steps, char* work, do
     plan.gram.go<kGram, float, false>(s, h, Way{turn, 0, 0, 0, 0, 0});
     Way way{turn, 1, 0, 0, kA, 1 / kScaleB};
     if (chained) {
-      const int last = done + chain_of(done, steps, std::is_same_v<T, __half>);
+      const int last = done + chain_of(done, steps, std::is_same_v<T, __half>, false);
       int a = 0, p = 1, c = 2, q = 1;
       float scale = kScaleB;      // of Q
       plan.polynomial.go<kPolynomial, float, false>(s, h, Way{turn, a, a, p, kA, 0});
@@ -1276,7 +1284,7 @@ void run(THCState* s, std::vector<Matrix>& all, const Update& h, int steps) {
   std::stable_sort(all.begin(), all.end(), [](const Matrix& a, const Matrix& b) { return a.n != b.n ? a.n > b.n : a.m > b.m; });
   std::vector<Group> groups;
   Bytes most{0, 0};
-  for (int kind : {kShortOnes, kLongOnes, kOthers}) {
+  for (int kind : {kThinOnes, kShortOnes, kLongOnes, kOthers}) {
     Bytes sum{0, 0};
     bool open = false;
     auto add = [&](const Matrix& a) {
