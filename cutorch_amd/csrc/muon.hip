@@ -1185,7 +1185,7 @@ struct Plan {
 // 1.3e-6, 1.3e-6, 300 x 700 1.7e-6, 2.5e-6, 1.9e-6, 1024 x 4096 1.8e-6, 1.9e-6, 3.3e-6. 3 + 2 is as good where many directions share the norm (2.1e-6
 // of 1024 x 4096), not where few do (3.2e-6 of 65 x 513, 6.7e-6 of 33 x 500; 4 + 1 2e-5 to 6e-5): for halves, which come with 2e-4 of their own.
 // Up to 32 rows sums of floats round least, and the later pairs would show (23 x 1024 9e-7, floats 6.4e-7): two first, then singly, and all four products of
-// halves, 7e-7 (44 us instead of 39).
+// halves, 7e-7 (49 us instead of 39).
 int chain_of(int done, int steps, bool halves, bool thin) {
   if (halves) return done == 0 && steps % 2 && steps >= 3 ? 3 : std::min(2, steps - done);
   return std::min(thin && done ? 1 : 2, steps - done);
