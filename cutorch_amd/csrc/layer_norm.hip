@@ -198,6 +198,8 @@ struct GradArgs {
   T* dx;
   RowOffsets xo, go, dxo;
   float *weightPart, *biasPart;    // a row of sums for each workgroup; null: not wanted
+  T *weightGrad, *biasGrad;        // where the only workgroup's sums go, with those null; or null
+  int accumulate;
   uint32_t rows;
   int32_t dim;
   float eps;
@@ -318,7 +320,22 @@ __global__ __launch_bounds__(L * TEAMS, 2) void norm_grad_kernel(GradArgs<T> a) 
         lds_barrier();
       }
     }
-    if (threadIdx.x < L) {
+    if (threadIdx.x < L && gridDim.x == 1) {
+      auto write = [&](T* to, const float (&sum)[P][V]) {
+        if (!to) return;
+#pragma unroll
+        for (int p = 0; p < P; ++p) {
+#pragma unroll
+          for (int e = 0; e < V; ++e) {
+            if (e < packs.skip[p]) continue;
+            T* at = to + packs.at[p] + e;
+            *at = rounded<T>(a.accumulate ? Cvt<T>::up(*at) + sum[p][e] : sum[p][e]);
+          }
+        }
+      };
+      write(a.weightGrad, dw);
+      write(a.biasGrad, db);
+    } else if (threadIdx.x < L) {
       float *pw = a.weightPart ? a.weightPart + (int64_t)blockIdx.x * a.dim : nullptr, *pb = a.biasPart ? a.biasPart + (int64_t)blockIdx.x * a.dim : nullptr;
 #pragma unroll
       for (int p = 0; p < P; ++p) {
@@ -552,8 +569,17 @@ void launch_grad(THCState* s, GradArgs<T>& a, const WeightGrads<T>& to) {
       hipLaunchKernelGGL((norm_grad_kernel<T, VV, L, TEAMS, P, false, A>), dim3((unsigned)std::min(groups, 2 * most)), dim3(L * TEAMS), 0, st, a);
       return;
     }
-    // a workgroup's sums cross memory twice: each has two rows at least
-    const int64_t count = std::max<int64_t>(1, std::min(groups / 2, most));
+    // Few rows: one workgroup has the sums, and no launch joins them. us with a join and so: 8 rows of 2048 halves 9.0, 8.2, 16 of them 9.1, 13.0; 16 of 500 7.1,
+    // 6.8, 32 7.0, 9.4; 128 of 64 6.9, 6.5; 4 of 4096 10.4, 8.5, 6 of them 10.5, 10.9; 1 of 16384 22.8, 12.0.
+    // Else a workgroup's sums cross memory twice: each has two rows at least.
+    const int64_t count = groups <= 4 ? 1 : std::max<int64_t>(2, std::min(groups / 2, most));
+    if (count == 1) {
+      a.weightGrad = to.weight;
+      a.biasGrad = to.bias;
+      a.accumulate = to.accumulate;
+      hipLaunchKernelGGL((norm_grad_kernel<T, VV, L, TEAMS, P, true, A>), dim3(1), dim3(L * TEAMS), 0, st, a);
+      return;
+    }
     Workspace w(s, bytes(count));
     parts(count, w);
     hipLaunchKernelGGL((norm_grad_kernel<T, VV, L, TEAMS, P, true, A>), dim3((unsigned)count), dim3(L * TEAMS), 0, st, a);

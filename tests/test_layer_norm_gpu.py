@@ -275,3 +275,28 @@ def test_refusals(thc):
     with pytest.raises(ValueError):
         F("float").layer_norm(F("half"))
     assert F("float").layer_norm(F("float")).shape == ()
+
+
+@pytest.mark.parametrize("kind", ["float", "half"])
+@pytest.mark.parametrize("dim", [3, 64, 500, 513, 2048, 5000, 16384])
+def test_gradients_of_few_rows(thc, kind, dim):
+    """One workgroup's sums or several's: the weights' gradients of as many rows as either has, and a few more; added and written, one without the other."""
+    rng = np.random.default_rng(dim)
+    t = thc.Tensor.from_numpy
+    for rows in (1, 2, 4, 5, 8, 9, 16, 17, 33, 128, 129):
+        if rows * dim > 1 << 18:
+            continue
+        x, g, w = (rng.standard_normal(s).astype(NP[kind]) for s in ((rows, dim), (rows, dim), (dim,)))
+        was = rng.standard_normal(dim).astype(NP[kind])
+        X, G = x.astype(np.float64), g.astype(np.float64)
+        m, v = X.mean(1, keepdims=True), X.var(1, keepdims=True)
+        h = (X - m) / np.sqrt(v + 1e-5)
+        both = thc.Tensor(kind), t(was.copy()), t(was.copy())
+        both[0].layer_norm_grad(both[1], both[2], t(x), t(g), t(w), accumulate=True)
+        one = thc.Tensor(kind), t(was.copy())
+        one[0].layer_norm_grad(one[1], None, t(x), t(g), t(w))
+        for got, terms, begin in ((both[1], G * h, was), (both[2], G, was), (one[1], G * h, 0 * was)):
+            want = terms.sum(0) + begin.astype(np.float64)
+            # a sum of `rows` terms in float, of which each has an h that is off by up to 8 roundings of itself and of the deviations' size, and the last rounding
+            room = 2.0 ** -24 * ((rows + 16) * np.abs(terms).sum(0) + 16 * np.abs(G).sum(0) + np.abs(begin)) + 1.01 * UNIT[kind] * np.abs(want) + 2.0 ** -25
+            assert np.all(np.abs(got.numpy().astype(np.float64) - want) <= room), (rows, np.max(np.abs(got.numpy() - want) / room))
