@@ -325,28 +325,47 @@ __global__ __launch_bounds__(L * TEAMS, 2) void norm_grad_kernel(GradArgs<T> a) 
         if (!to) return;
 #pragma unroll
         for (int p = 0; p < P; ++p) {
+          T* at = to + packs.at[p];
+          auto value = [&](int e, T was) { return rounded<T>(a.accumulate ? Cvt<T>::up(was) + sum[p][e] : sum[p][e]); };
+          if (packs.skip[p] == 0) {
+            Pack<T, V> v{};
+            if (a.accumulate) v = load_pack_unaligned<false, Pack<T, V>>(at);
 #pragma unroll
-          for (int e = 0; e < V; ++e) {
-            if (e < packs.skip[p]) continue;
-            T* at = to + packs.at[p] + e;
-            *at = rounded<T>(a.accumulate ? Cvt<T>::up(*at) + sum[p][e] : sum[p][e]);
+            for (int e = 0; e < V; ++e) v.v[e] = value(e, v.v[e]);
+            store_pack_unaligned<false>(at, v);
+          } else {
+#pragma unroll
+            for (int e = 1; e < V; ++e)
+              if (e >= packs.skip[p]) at[e] = value(e, at[e]);
           }
         }
       };
       write(a.weightGrad, dw);
       write(a.biasGrad, db);
     } else if (threadIdx.x < L) {
-      float *pw = a.weightPart ? a.weightPart + (int64_t)blockIdx.x * a.dim : nullptr, *pb = a.biasPart ? a.biasPart + (int64_t)blockIdx.x * a.dim : nullptr;
+      auto leave = [&](float* part, const float (&sum)[P][V]) {
+        if (!part) return;
 #pragma unroll
-      for (int p = 0; p < P; ++p) {
+        for (int p = 0; p < P; ++p) {
+          float* at = part + (int64_t)blockIdx.x * a.dim + packs.at[p];
+          constexpr int N = V < 4 ? V : 4;
+          if (packs.skip[p] == 0) {
 #pragma unroll
-        for (int e = 0; e < V; ++e) {
-          if (e >= packs.skip[p]) {      // (of a pack that there is)
-            if (pw) pw[packs.at[p] + e] = dw[p][e];
-            if (pb) pb[packs.at[p] + e] = db[p][e];
+            for (int q = 0; q < V / N; ++q) {
+              Pack<float, N> v;
+#pragma unroll
+              for (int e = 0; e < N; ++e) v.v[e] = sum[p][q * N + e];
+              store_pack_unaligned<false>(at + q * N, v);
+            }
+          } else {
+#pragma unroll
+            for (int e = 1; e < V; ++e)
+              if (e >= packs.skip[p]) at[e] = sum[p][e];
           }
         }
-      }
+      };
+      leave(a.weightPart, dw);
+      leave(a.biasPart, db);
     }
   }
 }
