@@ -206,7 +206,7 @@ struct GradArgs {
 };
 
 // The same with the sums over rows of what a lane's columns add to the weights' gradients, which stay in its registers; the workgroup's teams join
-// theirs at the end. Bound by memory and, in halves, by arithmetic nearly as much: 16392 rows of 4096 halves 83 us with the joining launch, 4.8 TB/s.
+// theirs at the end. Bound by memory and, in halves, by arithmetic nearly as much: 16392 rows of 4096 halves 78 us with the joining launch, 5.2 TB/s.
 template <typename T, int V, int L, int TEAMS, int P, bool WEIGHTS, bool AHEAD>
 __global__ __launch_bounds__(L * TEAMS, 2) void norm_grad_kernel(GradArgs<T> a) {
   __shared__ float lds[L > 64 ? 5 * TEAMS * (L / 64) : 1];
@@ -588,10 +588,11 @@ void launch_grad(THCState* s, GradArgs<T>& a, const WeightGrads<T>& to) {
       hipLaunchKernelGGL((norm_grad_kernel<T, VV, L, TEAMS, P, false, A>), dim3((unsigned)std::min(groups, 2 * most)), dim3(L * TEAMS), 0, st, a);
       return;
     }
-    // Few rows: one workgroup has the sums, and no launch joins them. us with a join and so: 8 rows of 2048 halves 9.0, 8.2, 16 of them 9.1, 13.0; 16 of 500 7.1,
-    // 6.8, 32 7.0, 9.4; 128 of 64 6.9, 6.5; 4 of 4096 10.4, 8.5, 6 of them 10.5, 10.9; 1 of 16384 22.8, 12.0.
-    // Else a workgroup's sums cross memory twice: each has two rows at least.
-    const int64_t count = groups <= 4 ? 1 : std::max<int64_t>(2, std::min(groups / 2, most));
+    // Few rows: one workgroup has the sums, and no launch joins them. us with a join and so: 4 rows of 2048 halves 6.9, 6.0, 8 of them 7.5, 7.7; 8 of 500 6.7,
+    // 5.7, 16 7.0, 6.9; 2 of 4096 6.7, 5.1, 4 of them 7.4, 7.6; 1 of 16384 11.7, 7.4, 4 of them 14.1, 14.9.
+    // Else a workgroup's sums cross memory twice: each has two rows at least, or three. us with two, three and four: 300 rows of 4096 halves 10.5, 10.7, 11.4,
+    // 1024 19.3, 17.7, 15.3; 1500 of 513 floats 9.7, 9.3, 10.3; 600 of 8192 23.2, 20.8, 20.4; 100 of 2048 halves 8.0, 10.2, 11.1.
+    const int64_t count = groups <= 3 ? 1 : std::max<int64_t>(2, std::min(groups / (groups < 512 ? 2 : 3), most));
     if (count == 1) {
       a.weightGrad = to.weight;
       a.biasGrad = to.bias;
@@ -607,8 +608,8 @@ void launch_grad(THCState* s, GradArgs<T>& a, const WeightGrads<T>& to) {
 #define GO(VV, L, TEAMS, P, A, THREADS) \
   go(integral_constant<int, VV>{}, integral_constant<int, L>{}, integral_constant<int, TEAMS>{}, integral_constant<int, P>{}, integral_constant<bool, A>{}, THREADS)
   // The last number: threads a CU. More hide the two sums of a row better, and make more rows of sums that cross memory. us with 512, 768 and 1024 of
-  // them: 16384 rows of 4096 halves 83, 88, 103, of 2048 45, 49, 56, 16384 of 2000 floats 74, 79, 83; 65536 of 500 halves 53, 47, 47. The next row is
-  // asked for early where registers allow it (4096 halves 148 without, 88 with, in 768; two rows early 2 to 6 % slower).
+  // them: 16384 rows of 4096 halves 78, 80, 90, of 2048 42, 45, 51, 16384 of 2000 floats 74, 78, 81; 65536 of 500 halves 53, 50, 50. The next row is
+  // asked for early where registers allow it (4096 halves 148 without, 88 with, at that time in 768; two rows early 2 to 6 % slower).
   if (a.dim < V) GO(1, 8, 32, 1, true, 1024);
   else if (packs <= 8) GO(V, 8, 32, 1, true, 1024);
   else if (packs <= 16) GO(V, 16, 16, 1, true, 1024);
