@@ -573,12 +573,14 @@ __global__ __launch_bounds__(256, 2) void product_kernel(Group g, Update h, Way 
   const Operand P{from + i0 * bytesK, bytesK, rows - i0}, Q{with + j0 * bytesK, bytesK, cols - j0};
   // The sums as columns: a lane has column `lane % 32` of each 32 x 32 product, four rows in a row of each eight.
   float* sums = reinterpret_cast<float*>(lds);
+  // (four rows of a column stay side by side; eight columns on they have changed places, so that sixteen lanes that have eight columns each meet all banks)
+  auto spot = [&](int i, int j) { return sums + j * kStride + (i ^ ((j >> 3 & 15) << 2)); };
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   auto keep = [&](int down, int over, const acc16& acc) {      // 32 x 32 at these times 32
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       const int i = down * 32 + r * 8 + (lane >> 5) * 4, j = over * 32 + (lane & 31);
-      *reinterpret_cast<Pack<float, 4>*>(sums + j * kStride + i) = Pack<float, 4>{acc[r * 4], acc[r * 4 + 1], acc[r * 4 + 2], acc[r * 4 + 3]};
+      *reinterpret_cast<Pack<float, 4>*>(spot(i, j)) = Pack<float, 4>{acc[r * 4], acc[r * 4 + 1], acc[r * 4 + 2], acc[r * 4 + 3]};
     }
   };
   if constexpr (JOIN) {
@@ -619,8 +621,8 @@ __global__ __launch_bounds__(256, 2) void product_kernel(Group g, Update h, Way 
     float v[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      float sum = sums[(jt + e) * kStride + it + u];
-      if (kSymmetric && diagonal && it + u > jt + e) sum = sums[(it + u) * kStride + jt + e];
+      float sum = *spot(it + u, jt + e);
+      if (kSymmetric && diagonal && it + u > jt + e) sum = *spot(jt + e, it + u);
       if constexpr (OP == kGram) {
         v[e] = sum * (kScaleA / (a.scale * a.scale));
       } else if constexpr (OP == kProduct) {
@@ -651,7 +653,7 @@ __global__ __launch_bounds__(256, 2) void product_kernel(Group g, Update h, Way 
       if (i < rows && j < colEnd) store_eight((OP == kStep ? xn : to) + split_at(i, j, OP == kStep ? bytesN : bytesM), v);
       if (!diagonal) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) sums[(jt + e) * kStride + it + u] = v[e];
+        for (int e = 0; e < 8; ++e) *spot(it + u, jt + e) = v[e];
       }
     }
   }
@@ -665,8 +667,7 @@ __global__ __launch_bounds__(256, 2) void product_kernel(Group g, Update h, Way 
     for (int u = 0; u < kSpan; u += kRows) {
       const int32_t c = it + u;
       if (j0 + c >= cols || i >= rowEnd) continue;
-      const Pack<float, 4>* from4 = reinterpret_cast<const Pack<float, 4>*>(sums + c * kStride + jt);
-      const Pack<float, 4> low = from4[0], high = from4[1];
+      const Pack<float, 4> low = *reinterpret_cast<const Pack<float, 4>*>(spot(jt, c)), high = *reinterpret_cast<const Pack<float, 4>*>(spot(jt + 4, c));
       const float v[8] = {low.v[0], low.v[1], low.v[2], low.v[3], high.v[0], high.v[1], high.v[2], high.v[3]};
       store_eight(mirrored + split_at(j0 + c, i, bytesM), v);
     }
