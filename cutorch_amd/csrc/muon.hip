@@ -583,7 +583,22 @@ __global__ __launch_bounds__(256, 2) void product_kernel(Group g, Update h, Way 
       *reinterpret_cast<Pack<float, 4>*>(spot(i, j)) = Pack<float, 4>{acc[r * 4], acc[r * 4 + 1], acc[r * 4 + 2], acc[r * 4 + 3]};
     }
   };
+  // Rows: a thread has eight columns of every kRows-th row. What goes into the result beside the products is asked for as early as there are registers for it:
+  // before the products of small tiles, behind those of large ones.
+  constexpr int kAcross = kSpan / 8, kRows = 256 / kAcross, kSteps = kSpan / kRows;
+  constexpr bool kBased = OP == kPolynomial || OP == kStep || OP == kLast;
+  const int32_t jt = (threadIdx.x % kAcross) * 8, it = threadIdx.x / kAcross, j = j0 + jt;
+  const int32_t colEnd = (int32_t)blocks_of(cols) * kBlockK;
+  Eight beside[kBased ? kSteps : 1] = {};
+  auto ask = [&] {
+    if (!kBased || (OP != kPolynomial && way.own == 0)) return;
+    const char* base = kSymmetric ? right : flipped ? t : x;
+#pragma unroll
+    for (int u = 0; u < kSteps; ++u)
+      beside[kBased ? u : 0] = load_eight(base + split_at(min(i0 + it + u * kRows, rows - 1), min(j, colEnd - 8), kSymmetric || flipped ? bytesM : bytesN));
+  };
   if constexpr (JOIN) {
+    ask();
     // each of the four waves has one of the 2 x 2 products of 64 x 64
     constexpr int kEach = W * W * 256;
     const acc16* from16 = tail.sums + (int64_t)unit * tail.parts * kEach + (W == 2 ? wave * 256 + quarter * 64 : wave * 64) + lane;
@@ -594,6 +609,7 @@ __global__ __launch_bounds__(256, 2) void product_kernel(Group g, Update h, Way 
   } else {
     const int32_t blocks = (int32_t)(bytesK / kBlockBytes), parts = sum_parts(blocks, product_tiles(a, kSymmetric)), part = cut ? (int32_t)((unit - tail.whole) / rest) : 0;
     acc16 acc[W][W] = {};
+    if (TILE == kSmallTile && !cut) ask();
     product<TILE>(P, Q, blocks, parts, part, cut ? part + 1 : parts, lds, acc);
     if (cut) {
       acc16* to16 = tail.sums + ((int64_t)(tile - tail.whole) * tail.parts + part) * (W * W * 256) + threadIdx.x;
@@ -604,20 +620,14 @@ __global__ __launch_bounds__(256, 2) void product_kernel(Group g, Update h, Way 
     __syncthreads();
 #pragma unroll
     for (int q = 0; q < W * W; ++q) keep((wave >> 1) * W + q / W, (wave & 1) * W + q % W, acc[q / W][q % W]);
+    if (TILE != kSmallTile) ask();
   }
   __syncthreads();
-  // Rows: a thread has eight columns of every kRows-th row. (Few of these steps at a time: each of their instructions runs but a few times, and has
-  // to come from memory first.)
-  constexpr int kAcross = kSpan / 8, kRows = 256 / kAcross;
-  const int32_t jt = (threadIdx.x % kAcross) * 8, it = threadIdx.x / kAcross, j = j0 + jt;
-  const int32_t colEnd = (int32_t)blocks_of(cols) * kBlockK;
-  const char* base = kSymmetric ? right : flipped ? t : x;
-  const int64_t baseBytes = kSymmetric || flipped ? bytesM : bytesN;
-#pragma unroll 2
+  // (few of these steps at a time where registers do not ask for them all: each of their instructions runs but a few times, and has to come from memory first)
+#pragma unroll(kBased ? kSteps : 2)
   for (int u = 0; u < kSpan; u += kRows) {
     const int32_t i = i0 + it + u;
-    Eight one{};
-    if (OP != kGram && OP != kProduct && (OP == kPolynomial || way.own != 0) && i < rows && j < colEnd) one = load_eight(base + split_at(i, j, baseBytes));
+    const Eight& one = beside[kBased ? u / kRows : 0];
     float v[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
