@@ -130,6 +130,19 @@ __device__ __forceinline__ void store_values(float* at, int64_t count, const flo
   }
 }
 
+__device__ __forceinline__ void store_values(__half* at, int64_t count, const float (&v)[8]) {
+  Pack<__half, 8> t;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) t.v[e] = rounded<__half>(v[e]);
+  if (count >= 8) {
+    store_pack_unaligned<false>(at, t);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (e < count) at[e] = t.v[e];
+  }
+}
+
 // The sum of squares of a part of a matrix, in 64 bits; the optimizer's momentum on the way.
 template <typename T, bool MUON>
 __global__ __launch_bounds__(kBlock) void norm_kernel(Group g, Update h, double* parts) {
@@ -502,24 +515,6 @@ __device__ __forceinline__ void symmetric_tile_at(uint32_t index, int32_t tiles,
   }
 }
 
-template <typename T, typename F>
-__device__ __forceinline__ void eight_of(T* at, int32_t count, F f) {
-  if (count >= 8) {
-    constexpr int N = 16 / sizeof(T);
-    Pack<T, N> v[8 / N];
-#pragma unroll
-    for (int k = 0; k < 8 / N; ++k) v[k] = load_pack_unaligned<false, Pack<T, N>>(at + k * N);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) f(e, v[e / N].v[e % N]);
-#pragma unroll
-    for (int k = 0; k < 8 / N; ++k) store_pack_unaligned<false>(at + k * N, v[k]);
-  } else {
-#pragma unroll
-    for (int e = 0; e < 8; ++e)
-      if (e < count) f(e, at[e]);
-  }
-}
-
 // One of a step's products and what is made of it. Those of m x m are symmetric (their factors are polynomials of one A): tiles above the diagonal go to
 // both places. The last step's result goes to the tensor, or into the parameter. The sums pass through LDS, so that memory sees whole packs of
 // neighbouring elements in both directions.
@@ -590,7 +585,17 @@ __global__ __launch_bounds__(256, 2) void product_kernel(Group g, Update h, Way 
   const int32_t jt = (threadIdx.x % kAcross) * 8, it = threadIdx.x / kAcross, j = j0 + jt;
   const int32_t colEnd = (int32_t)blocks_of(cols) * kBlockK;
   Eight beside[kBased ? kSteps : 1] = {};
+  float was[OP == kLast && MUON ? kSteps : 1][8];      // of the parameter
+  const int64_t result = p.batch * ((int64_t)a.m * a.n) + j;
   auto ask = [&] {
+    if constexpr (OP == kLast && MUON) {
+#pragma unroll
+      for (int u = 0; u < kSteps; ++u) {
+        const int64_t at = result + (int64_t)min(i0 + it + u * kRows, rows - 1) * cols;
+        if (a.master) load_values(a.master + at, cols - j, was[u]);
+        else load_values(static_cast<const T*>(a.out) + at, cols - j, was[u]);
+      }
+    }
     if (!kBased || (OP != kPolynomial && way.own == 0)) return;
     const char* base = kSymmetric ? right : flipped ? t : x;
 #pragma unroll
@@ -646,19 +651,17 @@ __global__ __launch_bounds__(256, 2) void product_kernel(Group g, Update h, Way 
     }
     if constexpr (OP == kLast) {
       if (i >= rows || j >= cols) continue;
-      const int64_t at = p.batch * ((int64_t)a.m * a.n) + (int64_t)i * cols + j;
+      const int64_t at = result + (int64_t)i * cols;
       const float down = 1.f / a.scale;      // (a power of two)
-      T* out = static_cast<T*>(a.out) + at;
-      if constexpr (MUON) {
-        if (a.master) {
-          eight_of(a.master + at, cols - j, [&](int e, float& was) { v[e] = was = __builtin_fmaf(v[e] * down, -a.rate, was * h.keep); });
-          eight_of(out, cols - j, [&](int e, T& o) { o = rounded<T>(v[e]); });
-        } else {
-          eight_of(out, cols - j, [&](int e, T& o) { o = rounded<T>(__builtin_fmaf(v[e] * down, -a.rate, Cvt<T>::up(o) * h.keep)); });
-        }
-      } else {
-        eight_of(out, cols - j, [&](int e, T& o) { o = rounded<T>(v[e] * down); });
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        if constexpr (MUON) v[e] = __builtin_fmaf(v[e] * down, -a.rate, was[u / kRows][e] * h.keep);
+        else v[e] *= down;
       }
+      if constexpr (MUON) {
+        if (a.master) store_values(a.master + at, cols - j, v);
+      }
+      store_values(static_cast<T*>(a.out) + at, cols - j, v);
     } else {
       if (i < rows && j < colEnd) store_eight((OP == kStep ? xn : to) + split_at(i, j, OP == kStep ? bytesN : bytesM), v);
       if (!diagonal) {
