@@ -300,7 +300,8 @@ __global__ __launch_bounds__(kBlock) void split_kernel(Group g, Update h, const 
 // ----------------------------------------------------------------- products --
 // C = P Q', P and Q in the split layout: a workgroup has a tile of 128 x 128, each of its four waves 64 x 64 of that as 2 x 2 products of
 // 32 x 32. A block of 32 columns of both operands, upper and lower halves, is 32 KiB of LDS; the next one is on its way there while one is
-// multiplied, and there is room for two workgroups a CU. Bound by the matrix cores' power: 1024 tiles of 4096 columns 350 us, 1180 TFLOP/s of halves,
+// multiplied, and there is room for two workgroups a CU. Bound by the matrix cores' power: 1024 tiles of 4096 columns 354 to 364 us
+// with what becomes of them, 1150 TFLOP/s of halves,
 // with the cores busy in 60 % of the cycles at 1.9 GHz; a library's product of halves of that size reaches 1190. A row's eight 16-byte pieces lie in the order of their number xor half the row's, so that
 // sixteen lanes that read the same piece of neighbouring rows meet all banks. (Blocks of 16 columns, four of which are on their way: 5 % slower, as
 // waves meet at twice as many barriers.)
@@ -1117,9 +1118,9 @@ float scale_of(int64_t m, int64_t n) {
   return (float)(1 << e);
 }
 
-// Workspace that the matrices of one pass share: enough of them to fill the chip many times over (72 matrices of 150 M halves in passes of 0.25, 0.5, 1, 2,
-// 4 GiB: 14.7, 12.4, 11.5, 11.2, 11.2 ms).
-constexpr int64_t kPassBytes = int64_t(2) << 30;
+// Workspace that the matrices of one pass share, which are equal shares of all: enough of them to fill the chip many times over. ms in passes of up to 0.4, 0.6, 1, 2
+// and 4 GiB: 72 matrices of 150 M halves 10.0, 8.7, 8.2, 8.5, 8.4, 64 of 1000 x 1000 5.6, 5.4, 5.6, 5.3, 5.3.
+constexpr int64_t kPassBytes = int64_t(1) << 30;
 
 struct Bytes {
   int64_t work, norms;
@@ -1137,7 +1138,7 @@ double product_time(int32_t tile, double blocks, int64_t units, int64_t cus, boo
 }
 
 // One of a step's products over a group: its tiles, numbered, and which of them are cut: those of the last round of workgroups, if that saves more than
-// the joining launch costs. Large or small tiles by what they take. us with large, large and cut, small, small and cut ones: A of 256 x 256
+// the joining launch costs. Large or small tiles by what they take. us with large, large and cut, small, small and cut ones, before the latter read ahead: A of 256 x 256
 // 17, -, 8, -; of 512 x 2048 55, 23, 26, 17; of 1024 x 1024 33, 24, 16, 20; of 2048 x 8192 198, 111, 181, 133; of 4096 x 4096 235, 161, 243, 215.
 struct Launch {
   Group g;
@@ -1299,11 +1300,19 @@ void run(THCState* s, std::vector<Matrix>& all, const Update& h, int steps) {
   std::vector<Group> groups;
   Bytes most{0, 0};
   for (int kind : {kThinOnes, kShortOnes, kLongOnes, kOthers}) {
+    // passes of equal shares
+    int64_t total = 0, largest = 0;
+    for (const Matrix& a : all) {
+      if (kind_of(a) != kind) continue;
+      total += each_bytes(a) * a.batch;
+      largest = std::max(largest, each_bytes(a));
+    }
+    const int64_t share = total / (total / kPassBytes + 1) + largest;
     Bytes sum{0, 0};
     bool open = false;
     auto add = [&](const Matrix& a) {
       const Bytes b = bytes_of(a);
-      if (!open || groups.back().count == kMatrices || sum.work + b.work > kPassBytes) {
+      if (!open || groups.back().count == kMatrices || sum.work + b.work > share) {
         groups.emplace_back();
         groups.back().count = 0;
         sum = Bytes{0, 0};
@@ -1320,7 +1329,7 @@ void run(THCState* s, std::vector<Matrix>& all, const Update& h, int steps) {
       if (kind_of(a) != kind) continue;
       // a batch in pieces: by the workspace, and by what the workgroups of a launch are counted in
       const int64_t size = (int64_t)a.m * a.n;
-      const int64_t each = std::max<int64_t>(1, std::min<int64_t>(kPassBytes / each_bytes(a), 1 << 20));
+      const int64_t each = std::max<int64_t>(1, std::min<int64_t>(share / each_bytes(a), 1 << 20));
       for (int64_t first = 0; first < a.batch; first += each) {
         Matrix piece = a;
         piece.batch = (int32_t)std::min<int64_t>(each, a.batch - first);
