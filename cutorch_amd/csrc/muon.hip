@@ -1118,9 +1118,9 @@ float scale_of(int64_t m, int64_t n) {
   return (float)(1 << e);
 }
 
-// Workspace that the matrices of one pass share, which are equal shares of all: enough of them to fill the chip many times over. ms in passes of up to 0.4, 0.6, 1, 2
-// and 4 GiB: 72 matrices of 150 M halves 10.0, 8.7, 8.2, 8.5, 8.4, 64 of 1000 x 1000 5.6, 5.4, 5.6, 5.3, 5.3.
-constexpr int64_t kPassBytes = int64_t(1) << 30;
+// Workspace that the matrices of one pass share, which are equal shares of all: enough of them to fill the chip many times over. ms in passes of up to 0.4, 0.6, 1 and
+// 2 GiB: 72 matrices of 150 M halves 10.0, 8.7, 8.4, 8.2, 64 of 1000 x 1000 5.6, 5.4, 5.6, 5.3.
+constexpr int64_t kPassBytes = int64_t(2) << 30;
 
 struct Bytes {
   int64_t work, norms;

@@ -419,3 +419,19 @@ def test_strips_of_other_sizes(thc, kind, rows, cols):
     if kind == "float":      # far beyond what is left of the result at all
         g.reshape(rows, cols)[(slice(None), slice(640, None)) if rows < cols else slice(640, None)] *= np.float32(2.0 ** -110)
         _check(thc.Tensor(kind).orthogonalize(thc.Tensor.from_numpy(g)).numpy(), g, kind)
+
+
+@pytest.mark.parametrize("count,rows,cols", [(260, 600, 600), (1150, 200, 400), (1500, 100, 1000), (4000, 30, 3000)])
+def test_batches_beyond_a_pass(thc, count, rows, cols):
+    """Workspaces of more than 2 GiB in all, of each kind of matrices: the bits of one alone, for each."""
+    one = _matrix(np.random.default_rng(rows), rows, cols, "half")
+    t = thc.Tensor.from_numpy
+    want = thc.Tensor("half").orthogonalize(t(one)).numpy()
+    source, many = t(one), thc.Tensor("half").resize((count, rows, cols))
+    for i in range(count):
+        many.select(0, i).copy(source)
+    many.orthogonalize(many)
+    got = many.numpy()
+    assert_bit_equal(got[0], want)
+    assert_bit_equal(got[-1], want)
+    assert all(np.array_equal(got[0], x) for x in got)
