@@ -692,7 +692,7 @@ __global__ __launch_bounds__(256, 2) void product_kernel(Group g, Update h, Way 
 // Up to 128 rows: A and B are one tile each, and what bounds a step is how long its launches wait for memory one after another (12 matrices of 65 x 513: 17
 // launches of 9 to 17 us each). A workgroup has a strip of 128 columns of X. It adds up the strips' shares of A, makes B of it by itself,
 // takes its strip through the step and leaves the strip's share of the next A. Two steps
-// a launch (three of halves) where it takes A along, P A P: 12 of 65 x 513 floats took 98 us with a launch for each step and 82 so; 67 since strips
+// a launch (three where results are only written as halves) where it takes A along, P A P: 12 of 65 x 513 floats took 98 us with a launch for each step and 82 so; 67 since strips
 // begin without a launch for the norm and the kernels have 0.6 of the instructions. Of a launch's 49 thousand cycles for two steps a CU's four SIMDs have
 // vector instructions for 21 thousand, matrix ones for 10, and LDS is read or written in 13: nine waves that wait for one another at barriers.
 // One launch for all steps where X is a single strip, which makes each A from X.
@@ -1196,15 +1196,21 @@ struct Plan {
 };
 
 // How many steps go with one A from X. An error of A grows with what it belongs to, up to 12 times a step where singular values are small. Two steps
-// leave what single ones do: against 64 bits after five steps, of the result's norm, singly, as 2 + 2 + 1 and by products of floats: 12 of 65 x 513 1.2e-6,
-// 1.3e-6, 1.3e-6, 300 x 700 1.7e-6, 2.5e-6, 1.9e-6, 1024 x 4096 1.8e-6, 1.9e-6, 3.3e-6. 3 + 2 is as good where many directions share the norm (2.1e-6
-// of 1024 x 4096), not where few do (3.2e-6 of 65 x 513, 6.7e-6 of 33 x 500; 4 + 1 2e-5 to 6e-5): for halves, which come with 2e-4 of their own.
-// Up to 32 rows sums of floats round least, and the later pairs would show (23 x 1024 9e-7, floats 6.4e-7): two first, then singly, and all four products of
-// halves, 7e-7 (49 us instead of 39).
-int chain_of(int done, int steps, bool halves, bool thin) {
-  if (halves) return done == 0 && steps % 2 && steps >= 3 ? 3 : std::min(2, steps - done);
+// leave what single ones do. Against 64 bits after five steps, in 1e-6 of the result's norm, by products of floats, singly, as 2 + 2 + 1 (medians of
+// four; elements alike / few directions with most of the norm / singular values from 1 to 1e-3): 65 x 513 1.7 1.9 1.9 / 1.2 1.0 1.1 / 3.5 2.8 3.0,
+// 33 x 500 2.4 2.3 3.7 / 1.5 1.3 1.3 / 3.6 3.3 3.4, 300 x 700 2.2 1.9 1.9 / 1.9 1.7 2.4 / 3.4 5.4 5.2, 1024 x 4096 3.7 1.4 1.6 / 2.7 1.5 1.4 / 4.7 5.4 4.7.
+// Three steps do not where few directions share the norm (11 of 33 x 500): they are for results that are only written as halves (`rough`), which come with
+// 200 of their own, not for float copies of half parameters. (4 + 1 leaves 20 to 60.)
+// Up to 32 rows sums of floats round least, and the later pairs would show (23 x 1024 2.4 in place of 1.8 singly): two first, then singly, and all four
+// products of halves, 1.7 (49 us instead of 39).
+int chain_of(int done, int steps, bool rough, bool thin) {
+  if (rough) return done == 0 && steps % 2 && steps >= 3 ? 3 : std::min(2, steps - done);
   return std::min(thin && done ? 1 : 2, steps - done);
 }
+// (all parameters of a call have copies, or none)
+template <typename T, bool MUON>
+bool is_rough(const Group& g) { return std::is_same_v<T, __half> && !(MUON && g.matrix[0].master); }
+
 template <typename T, bool MUON>
 void run_short(THCState* s, Group& g, const Update& h, int steps) {
   hipStream_t st = current_stream(s);
@@ -1235,7 +1241,7 @@ void run_short(THCState* s, Group& g, const Update& h, int steps) {
   }
   hipLaunchKernelGGL(roomy(short_begin_kernel<T, MUON, false>), strips, threads, lds, st, g, h, steps);
   for (int done = 0, turn = 0; done < steps; turn ^= 1) {
-    const int chain = chain_of(done, steps, std::is_same_v<T, __half>, is_thin(g.matrix[0]));
+    const int chain = chain_of(done, steps, is_rough<T, MUON>(g), is_thin(g.matrix[0]));
     const bool first = done == 0;
     done += chain;
     if (many) hipLaunchKernelGGL(shares_kernel, dim3(parts), dim3(kShareThreads), 0, st, shares, h, turn, first);
@@ -1267,7 +1273,7 @@ void run_group(THCState* s, Group& g, const Update& h, int steps, char* work, do
     plan.gram.go<kGram, float, false>(s, h, Way{turn, 0, 0, 0, 0, 0});
     Way way{turn, 1, 0, 0, kA, 1 / kScaleB};
     if (chained) {
-      const int last = done + chain_of(done, steps, std::is_same_v<T, __half>, false);
+      const int last = done + chain_of(done, steps, is_rough<T, MUON>(g), false);
       int a = 0, p = 1, c = 2, q = 1;
       float scale = kScaleB;      // of Q
       plan.polynomial.go<kPolynomial, float, false>(s, h, Way{turn, a, a, p, kA, 0});
