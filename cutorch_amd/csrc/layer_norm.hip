@@ -3,9 +3,11 @@
 //   layerNorm       y = (x - m) r w + b      m = mean(x), r = 1 / sqrt(mean((x - m)^2) + eps), of each row
 //   layerNormGrad   h = (x - m) r;  dx = r (g w - mean(g w) - h mean(g w h)),  dw = sum over rows of g h,  db = sum over rows of g
 //
-// Statistics and sums are in float, outputs round once to their type. The mean is taken in two steps: m' = sum(x) / n, then what is left,
-// c = mean(x - m'), beside the squares; m = m' + c and the variance mean((x - m')^2) - c^2 lose nothing to a large offset of the row (m' as
-// a float is off by 2^-24 of the offset, which may be much of the deviation). The gradient's pass takes the statistics anew: the row is there
+// Statistics and sums are in float, outputs round once to their type. The mean is taken in two steps: m' = x0 + mean(x - x0), x0 the row's first element,
+// then what is left, c = mean(x - m'), beside the squares; m = m' + c and the variance mean((x - m')^2) - c^2 lose nothing to a large offset of the
+// row (m' as a float is off by 2^-24 of the offset, which may be much of the deviation). With x0 = 0, which takes an operation less an element, m' would
+// be off by many times that in long rows, and the variance of a row of equal elements not 0 but what its two terms round to, below 0 among others: 1 % of
+// the time in floats. Up to 8192 halves take 0 (2 to 3 %): as many equal ones sum exactly. The gradient's pass takes the statistics anew: the row is there
 // anyway, the sums of its second step travel with those of g w and g w (x - m'), and nothing is kept between the passes.
 #include <algorithm>
 #include <type_traits>
@@ -64,6 +66,12 @@ __device__ __forceinline__ float inverse_root(float v) {
   return v < 0x1p-96f ? __builtin_amdgcn_rsqf(v * 0x1p96f) * 0x1p48f : __builtin_amdgcn_rsqf(v);
 }
 
+// What sums leave of a variance, which is not below 0. (NaN stays.)
+__device__ __forceinline__ float variance(float squares, float c) {
+  const float v = __builtin_fmaf(-c, c, squares);
+  return v < 0.f ? 0.f : v;
+}
+
 // The packs of a row that a lane of a team of L has: pack p begins at element at[p], the first skip[p] of its V elements belong to the pack before
 // it (a row's last pack is moved back into the row, so that reads need no tail; V where there is no pack at all). `whole`: none is moved.
 template <int V, int L, int P>
@@ -91,6 +99,33 @@ __device__ __forceinline__ void clear_skipped(const Packs<V, L, P>& packs, float
       for (int e = 0; e < V; ++e) x[p][e] = e < packs.skip[p] ? 0.f : x[p][e];
     }
   }
+}
+
+// A row's first element as what distances are taken from, or 0.
+template <typename T, bool WANTED>
+struct First {
+  T value;
+  __device__ __forceinline__ void load(const T* row) {
+    if constexpr (WANTED) value = *row;
+  }
+  __device__ __forceinline__ float get() const { return WANTED ? Cvt<T>::up(value) : 0.f; }
+};
+template <typename T>
+constexpr bool from_first(int most) { return sizeof(T) == 4 || most > 8192; }
+// What a lane adds to the sum of the row's distances to `from`.
+template <bool FROM, int V, int L, int P>
+__device__ __forceinline__ float distances(const Packs<V, L, P>& packs, const float (&x)[P][V], float from) {
+  float d[P][V], sum = 0.f;
+#pragma unroll
+  for (int p = 0; p < P; ++p)
+#pragma unroll
+    for (int e = 0; e < V; ++e) d[p][e] = FROM ? x[p][e] - from : x[p][e];
+  clear_skipped<V, L, P>(packs, d);
+#pragma unroll
+  for (int p = 0; p < P; ++p)
+#pragma unroll
+    for (int e = 0; e < V; ++e) sum += d[p][e];
+  return sum;
 }
 
 template <typename T>
@@ -149,21 +184,24 @@ __global__ __launch_bounds__(L * TEAMS) void norm_kernel(NormArgs<T> a) {
   load_columns<T, V, P, L>(a.weight, packs, w, 1.f);
   load_columns<T, V, P, L>(a.bias, packs, b, 0.f);
   Pack<T, V> raw[P];
-  load_row<T, V, P, L>(a.x + a.xo.at(min(blockIdx.x * TEAMS + team, a.rows - 1)), packs, raw);
+  constexpr bool kFrom = from_first<T>(V * L * P);
+  First<T, kFrom> start;
+  auto load = [&](uint32_t first) {
+    const T* in = a.x + a.xo.at(min(first + team, a.rows - 1));
+    load_row<T, V, P, L>(in, packs, raw);
+    start.load(in);
+  };
+  load(blockIdx.x * TEAMS);
   for (uint32_t first = blockIdx.x * TEAMS; first < a.rows; first += gridDim.x * TEAMS) {
     const uint32_t row = min(first + team, a.rows - 1);
     float x[P][V];
     to_floats(raw, x);
+    const float x0 = start.get();
     // the next row is asked for before this one is computed
-    if (first + gridDim.x * TEAMS < a.rows) load_row<T, V, P, L>(a.x + a.xo.at(min(first + gridDim.x * TEAMS + team, a.rows - 1)), packs, raw);
-    clear_skipped<V, L, P>(packs, x);
-    float one[1] = {0.f};
-#pragma unroll
-    for (int p = 0; p < P; ++p)
-#pragma unroll
-      for (int e = 0; e < V; ++e) one[0] += x[p][e];
+    if (first + gridDim.x * TEAMS < a.rows) load(first + gridDim.x * TEAMS);
+    float one[1] = {distances<kFrom>(packs, x, x0)};
     team_sum<1, L, TEAMS>(one, lds);
-    const float m = one[0] / n;
+    const float m = kFrom ? x0 + one[0] / n : one[0] / n;
 #pragma unroll
     for (int p = 0; p < P; ++p)
 #pragma unroll
@@ -178,7 +216,7 @@ __global__ __launch_bounds__(L * TEAMS) void norm_kernel(NormArgs<T> a) {
         two[1] = __builtin_fmaf(x[p][e], x[p][e], two[1]);
       }
     team_sum<2, L, TEAMS>(two, lds + TEAMS * (L / 64));
-    const float c = two[0] * share, r = inverse_root(two[1] * share - c * c + a.eps), cr = -c * r;
+    const float c = two[0] * share, r = inverse_root(variance(two[1] * share, c) + a.eps), cr = -c * r;
     if (first + team < a.rows) {
       T* out = a.y + a.yo.at(row);
 #pragma unroll
@@ -225,10 +263,14 @@ __global__ __launch_bounds__(L * TEAMS, 2) void norm_grad_kernel(GradArgs<T> a) 
 #pragma unroll
     for (int e = 0; e < V; ++e) dw[p][e] = db[p][e] = 0.f;
   Pack<T, V> raw[P], graw[P];
+  constexpr bool kFrom = from_first<T>(V * L * P);
+  First<T, kFrom> start;
   auto load = [&](uint32_t first) {
     const uint32_t row = min(first + team, a.rows - 1);
-    load_row<T, V, P, L>(a.x + a.xo.at(row), packs, raw);
+    const T* in = a.x + a.xo.at(row);
+    load_row<T, V, P, L>(in, packs, raw);
     load_row<T, V, P, L>(a.g + a.go.at(row), packs, graw);
+    start.load(in);
   };
   if (AHEAD) load(blockIdx.x * TEAMS);
   for (uint32_t first = blockIdx.x * TEAMS; first < a.rows; first += gridDim.x * TEAMS) {
@@ -236,16 +278,12 @@ __global__ __launch_bounds__(L * TEAMS, 2) void norm_grad_kernel(GradArgs<T> a) 
     float d[P][V], g[P][V];
     to_floats(raw, d);
     to_floats(graw, g);
+    const float x0 = start.get();
     // the next row is asked for before this one is computed
     if (AHEAD && first + gridDim.x * TEAMS < a.rows) load(first + gridDim.x * TEAMS);
-    clear_skipped<V, L, P>(packs, d);
-    float one[1] = {0.f};
-#pragma unroll
-    for (int p = 0; p < P; ++p)
-#pragma unroll
-      for (int e = 0; e < V; ++e) one[0] += d[p][e];
+    float one[1] = {distances<kFrom>(packs, d, x0)};
     team_sum<1, L, TEAMS>(one, lds);
-    const float m = one[0] / n;
+    const float m = kFrom ? x0 + one[0] / n : one[0] / n;
 #pragma unroll
     for (int p = 0; p < P; ++p)
 #pragma unroll
@@ -263,7 +301,7 @@ __global__ __launch_bounds__(L * TEAMS, 2) void norm_grad_kernel(GradArgs<T> a) 
         four[3] = __builtin_fmaf(gw, d[p][e], four[3]);
       }
     team_sum<4, L, TEAMS>(four, lds + TEAMS * (L / 64));
-    const float c = four[0] * share, r = inverse_root(four[1] * share - c * c + a.eps), cr = -c * r;
+    const float c = four[0] * share, r = inverse_root(variance(four[1] * share, c) + a.eps), cr = -c * r;
     // mean(g w h) and mean(g w), times r
     const float meanH = (four[3] - c * four[2]) * r * share * r, meanG = four[2] * share * r;
     if (TEAMS > 1 && first + team >= a.rows) continue;      // (all of a wave's lanes that still sum are back together at its next row)
@@ -426,15 +464,15 @@ struct RowStats {
 template <typename T>
 __device__ __forceinline__ RowStats stats_of(const T* row, const T* g, const T* weight, int32_t dim, float eps, float* lds) {
   RowStats s{};
-  const float n = (float)dim;
+  const float n = (float)dim, x0 = Cvt<T>::up(*row);
   float one[1] = {0.f};
   over_row<T>(dim, [&](int32_t i, auto count) {
     float x[decltype(count)::value];
     load_some(row + i, x);
-    for (float v : x) one[0] += v;
+    for (float v : x) one[0] += v - x0;
   });
   team_sum<1, kLong, 1>(one, lds);
-  s.m = one[0] / n;
+  s.m = x0 + one[0] / n;
   float four[4] = {0.f, 0.f, 0.f, 0.f};
   over_row<T>(dim, [&](int32_t i, auto count) {
     constexpr int N = decltype(count)::value;
@@ -458,7 +496,7 @@ __device__ __forceinline__ RowStats stats_of(const T* row, const T* g, const T* 
   });
   team_sum<4, kLong, 1>(four, lds + kLong / 64);
   s.c = four[0] / n;
-  s.r = 1.f / sqrtf(four[1] / n - s.c * s.c + eps);
+  s.r = 1.f / sqrtf(variance(four[1] / n, s.c) + eps);
   s.meanH = (four[3] - s.c * four[2]) * s.r / n * s.r;
   s.meanG = four[2] / n * s.r;
   return s;
