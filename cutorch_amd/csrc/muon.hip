@@ -1169,10 +1169,9 @@ struct Launch {
       }
       return (tiles > last ? rounds : 0) + (cuts ? cut : whole);
     };
-    Tail large, small;
-    tile = plan(kTile, large) <= plan(kSmallTile, small) ? kTile : kSmallTile;
-    if (tile == kTile) plan(kTile, large);      // (which numbers them)
-    tail = tile == kTile ? large : small;
+    const double large = plan(kTile, tail), small = plan(kSmallTile, tail);
+    tile = large <= small ? kTile : kSmallTile;
+    plan(tile, tail);      // (which numbers the tiles)
   }
   uint32_t rest() const { return g.first[g.count] - tail.whole; }
   int64_t bytes() const { return (int64_t)rest() * tail.parts * tile * tile * 4; }
