@@ -1118,8 +1118,9 @@ float scale_of(int64_t m, int64_t n) {
   return (float)(1 << e);
 }
 
-// Workspace that the matrices of one pass share, which are equal shares of all: enough of them to fill the chip many times over. ms in passes of up to 0.4, 0.6, 1 and
-// 2 GiB: 72 matrices of 150 M halves 10.0, 8.7, 8.4, 8.2, 64 of 1000 x 1000 5.6, 5.4, 5.6, 5.3.
+// Workspace that the matrices of one pass share, which are equal shares of all: enough of them to fill the chip many times over. ms in passes of up to 0.5, 1
+// and 2 GiB, medians of four runs in turn, each within 0.3 %: 72 matrices of 150 M halves with copies 10.11, 9.12, 9.08; 36 of 75 M floats 5.28, 4.56, 4.55; 78 of 100 M halves
+// 6.68, 6.24, 6.02; 64 of 1000 x 1000 halves 5.57, 5.51, 5.15; 40 of 1024 x 4096 7.92, 6.56, 6.32; 2000 of 100 x 1000 floats 6.68, 6.74, 6.36; 300 of 600 x 600 7.15, 6.90, 7.03.
 constexpr int64_t kPassBytes = int64_t(2) << 30;
 
 struct Bytes {
@@ -1210,15 +1211,19 @@ int chain_of(int done, int steps, bool rough, bool thin) {
 template <typename T, bool MUON>
 bool is_rough(const Group& g) { return std::is_same_v<T, __half> && !(MUON && g.matrix[0].master); }
 
+// One launch for all steps, and no workspace.
+bool is_whole(const Group& g) {
+  for (int k = 0; k < g.count; ++k)
+    if (!is_alone(g.matrix[k])) return false;
+  return true;
+}
 template <typename T, bool MUON>
 void run_short(THCState* s, Group& g, const Update& h, int steps) {
   hipStream_t st = current_stream(s);
   int bands = 0, most = 0;
-  bool whole = true;
   int64_t read = 0;
   for (int k = 0; k < g.count; ++k) {
     const Matrix& a = g.matrix[k];
-    whole = whole && is_alone(a);
     bands = std::max(bands, bands_of(a));
     most = std::max(most, strips_of(a));
     read += (int64_t)a.batch * strips_of(a) * strips_of(a) * gram_bytes(a);
@@ -1234,7 +1239,7 @@ void run_short(THCState* s, Group& g, const Update& h, int steps) {
     if (lds > 65536) THC_CHECK(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, lds));
     return kernel;
   };
-  if (whole) {
+  if (is_whole(g)) {
     hipLaunchKernelGGL(roomy(short_begin_kernel<T, MUON, true>), strips, threads, lds, st, g, h, steps);
     return;
   }
@@ -1303,7 +1308,6 @@ void run(THCState* s, std::vector<Matrix>& all, const Update& h, int steps) {
   // (equal ones side by side, long sums first: what is left of a launch at its end is short)
   std::stable_sort(all.begin(), all.end(), [](const Matrix& a, const Matrix& b) { return a.n != b.n ? a.n > b.n : a.m > b.m; });
   std::vector<Group> groups;
-  Bytes most{0, 0};
   for (int kind : {kThinOnes, kShortOnes, kLongOnes, kOthers}) {
     // passes of equal shares
     int64_t total = 0, largest = 0;
@@ -1313,22 +1317,19 @@ void run(THCState* s, std::vector<Matrix>& all, const Update& h, int steps) {
       largest = std::max(largest, each_bytes(a));
     }
     const int64_t share = total / (total / kPassBytes + 1) + largest;
-    Bytes sum{0, 0};
+    int64_t sum = 0;
     bool open = false;
     auto add = [&](const Matrix& a) {
-      const Bytes b = bytes_of(a);
-      if (!open || groups.back().count == kMatrices || sum.work + b.work > share) {
+      const int64_t bytes = bytes_of(a).work;
+      if (!open || groups.back().count == kMatrices || sum + bytes > share) {
         groups.emplace_back();
         groups.back().count = 0;
-        sum = Bytes{0, 0};
+        sum = 0;
         open = true;
       }
       Group& g = groups.back();
       g.matrix[g.count++] = a;
-      sum.work += b.work;
-      sum.norms += b.norms;
-      most.work = std::max(most.work, sum.work);
-      most.norms = std::max(most.norms, sum.norms);
+      sum += bytes;
     };
     for (const Matrix& a : all) {
       if (kind_of(a) != kind) continue;
@@ -1346,10 +1347,20 @@ void run(THCState* s, std::vector<Matrix>& all, const Update& h, int steps) {
       }
     }
   }
+  Bytes most{8, 8};
   int64_t tails = 8;
-  for (const Group& g : groups)
+  for (const Group& g : groups) {
+    if (is_whole(g)) continue;
+    Bytes sum{0, 0};
+    for (int k = 0; k < g.count; ++k) {
+      const Bytes b = bytes_of(g.matrix[k]);
+      sum.work += b.work;
+      sum.norms += b.norms;
+    }
+    most = Bytes{std::max(most.work, sum.work), std::max(most.norms, sum.norms)};
     if (!is_short(g.matrix[0])) tails = std::max(tails, Plan(g, num_compute_units(s)).bytes());
-  Workspace work(s, std::max<int64_t>(8, most.work)), norms(s, std::max<int64_t>(8, most.norms)), sums(s, tails);
+  }
+  Workspace work(s, most.work), norms(s, most.norms), sums(s, tails);
   for (Group& g : groups)
     run_group<T, MUON>(s, g, h, steps, work.data(), reinterpret_cast<double*>(norms.data()), reinterpret_cast<acc16*>(sums.data()));
 }
