@@ -3,8 +3,8 @@
 //   orthogonalize   X = G / (|G| + eps);  A = X X', B = b A + c A A, X = a X + B X, `steps` times, the shorter side first
 //   muon            m = beta m + g;  u = g + beta m (or m);  p = p (1 - lr decay) - rate orthogonalize(u)
 //
-// The products run on the matrix cores in half precision, every factor as a sum of two halves (x = h + l, 22 bits): h h' + h l' + l h' is as exact
-// as a product of floats (4096 x 4096 against 64 bits after five steps: 5e-7 of the result's norm, float products 3e-6), at a third of the
+// The products run on the matrix cores in half precision, every factor as a sum of two halves (x = h + l, 22 bits where a float has 24): h h' + h l' + l h'
+// is about as exact as a product of floats (against 64 bits after five steps 0.4 to 2.5 times as far, figures at chain_of), at a third of the
 // halves' rate, where float products have a ninth of it (1190 and 126 TFLOP/s in products of that size). One half alone would leave 1e-3 to 5e-3. Sums are in float throughout, the norm's in 64 bits.
 // Singular values of X stay below 1.21 once they are at most 1 (a s + b s^3 + c s^5 on 0 ... 1.21), so no element of X, A and B leaves
 // +-1.21, +-1.46, +-2.81, nor P = a + B, P P' and P P' P'' +-a, +-a^2 and +-a^3, and each is held times a power of two that brings its usual size to

@@ -17,7 +17,7 @@ namespace {
 using std::integral_constant;
 
 // cos and sin of a position's angle, by the series around the nearest quarter of a turn: at most pi / 4 away, where terms up to the 11th
-// power leave 2e-9 (sin) and up to the 10th 2e-9 (cos).
+// power leave (pi / 4)^13 / 13! = 7e-12 (sin) and up to the 10th (pi / 4)^12 / 12! = 1.2e-10 (cos), beside a float's rounding of 6e-8.
 struct Turn {
   float c, s;
 };

@@ -691,7 +691,8 @@ THC_AMD_DECLARE_TOKEN_API(THCudaHalfTensor)
    * gradWeight and gradBias (null: not wanted) are written, or added to with  \
    * `accumulate`, in an order of sums that the sizes alone decide. gradInput  \
    * takes the input's sizes and may be the input or gradOutput; the three     \
-   * outputs may not lie on one another. weight null: ones. */                 \
+   * outputs may not lie on one another. weight null: ones. There is no        \
+   * gradient of an empty input. */                                            \
   THC_API void Tensor##_layerNormGrad(                                         \
       THCState *, Tensor *gradInput, Tensor *gradWeight, Tensor *gradBias,     \
       Tensor *input, Tensor *gradOutput, Tensor *weight, double eps,           \
@@ -713,11 +714,11 @@ THC_AMD_DECLARE_TOKEN_API(THCudaHalfTensor)
   /* Newton-Schulz steps on each matrix of the last two dims:                  \
    *   X = G / (|G| + eps);  X = a X + b (X X') X + c (X X')^2 X, `steps` times \
    * with |G| the root of the sum of squares and a, b, c = 3.4445, -4.7750,    \
-   * 2.0315, which brings singular values to 0.7 ... 1.2. Products are of     \
-   * 22-bit factors with sums in float, which leaves results in float about as\
-   * far from 64 bits as products of floats do (0.4 to 2.5 times), and off by \
-   * less than a third of their rounding in half results. self takes the      \
-   * input's sizes and may be the input. */                                   \
+   * 2.0315, which brings singular values to 0.7 ... 1.2. Products are of      \
+   * 22-bit factors with sums in float, which leaves results in float about as \
+   * far from 64 bits as products of floats do (0.4 to 2.5 times), and off by  \
+   * less than a third of their rounding in half results. self takes the       \
+   * input's sizes and may be the input. */                                    \
   THC_API void Tensor##_orthogonalize(THCState *, Tensor *self, Tensor *input, \
                                       int steps, double eps);
 THC_AMD_DECLARE_DECODER_API(THCudaTensor)
@@ -795,7 +796,8 @@ THC_API void THCudaTensor_adamW8Moments(THCState *state, int count,
  * matrix, those before them a batch of matrices of their own; vectors and
  * tables are AdamW's. Lists as there: one tensor per parameter, of its sizes,
  * the momentum in float (zeros begin a run), float copies of half parameters
- * (`master`) or null, which are as exact as float parameters. No tensor that is written may appear twice. */
+ * (`master`), which are as exact as float parameters, or null. No tensor that
+ * is written may appear twice. */
 THC_API void THCudaTensor_muon(THCState *state, int count, THCudaTensor **param,
                                THCudaTensor **grad, THCudaTensor **momentum,
                                double lr, double beta, double weightDecay,
